@@ -75,6 +75,13 @@ SIGNATURES = {
     "g9_moe_kernel_name": (ctypes.c_char_p, [_int, _int]),
     "g9_fmha_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp,
                            ctypes.c_float, _int, _int, _int, _vp]),
+    "g9_assign_slots": (_int, [_vp, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "g9_write_cache": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "g9_varlen_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp,
+                             ctypes.c_float, _int, _int, _vp]),
+    "g9_tree_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64,
+                           _i64, _i64, _vp, _vp, _vp, _vp, ctypes.c_float, _int, _vp, _sz, _vp]),
+    "g9_tree_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64]),
     "g9_workspace_size": (_sz, [_int, _i64, _i64, _i64, _int, _int]),
     "g9_workspace_init": (_int, [_vp, _sz, _vp]),
     "g9_workspace_error": (_int, [_vp, _sz, _vp, ctypes.POINTER(_int)]),

@@ -1,7 +1,7 @@
-"""Launch of the gfx950 flash-attention kernel (``g9_fmha_fwd``) from torch
-tensors: the argument checks of the reference launchers, then one call
-through the C ABI on the current stream.  No fallback: without the built
-library the call raises."""
+"""Launch of the gfx950 attention kernels from torch tensors: argument checks
+(for ``g9_fmha_fwd`` those of the reference launchers), then one call through
+the C ABI on the current stream.  No fallback: without the built library the
+call raises."""
 
 from __future__ import annotations
 
@@ -62,3 +62,81 @@ def fmha_forward(q, k, v, o, metadata, scale_on_q: bool, variant: int, lse=None)
         with torch.cuda.device(dev):
             rc = lib.g9_fmha_fwd(*args)
     _lib.check(rc, "g9_fmha_fwd")
+
+
+# --- packed and paged attention -----------------------------------------------
+
+
+def ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def strides(t):
+    """Element strides but the last dimension's."""
+    s = t.stride()
+    return (_lib.ctypes.c_int64 * (len(s) - 1))(*s[:-1])
+
+
+def gpu_of(first, *others) -> torch.device:
+    """The one GPU that holds every given tensor."""
+    dev = first.device
+    if dev.type != "cuda" or any(t is not None and t.device != dev for t in others):
+        raise ValueError(f"all tensors must be on one GPU; got {[str(t.device) for t in (first, *others) if t is not None]}")
+    return dev
+
+
+def rows_of(name, t) -> tuple[int, int, int]:
+    if t.dim() != 3 or t.stride(2) != 1:
+        raise ValueError(f"{name} must be (rows, heads, head dim) with a unit head-dim stride; got {tuple(t.shape)}, "
+                         f"strides {t.stride()}")
+    return t.shape
+
+
+def offsets_of(name, t) -> int:
+    """The number of sequences of a cu_seqlens tensor."""
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of sequences + 1 values")
+    return t.shape[0] - 1
+
+
+def int32_of(name, t, dims) -> None:
+    """Rows of contiguous int32 values."""
+    if t.dtype != torch.int32 or t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        raise ValueError(f"{name} must be a {dims}-dimensional int32 tensor with contiguous rows; got {t.dtype} "
+                         f"{tuple(t.shape)}, strides {t.stride()}")
+
+
+def heads_fit(HQ, HK, D) -> None:
+    if HK == 0 or HQ == 0 or HQ % HK:
+        raise ValueError(f"query heads {HQ} not a multiple of key/value heads {HK}")
+    if D not in HEAD_DIMS:
+        raise ValueError(f"head dim {D} unsupported: the gfx950 kernels are built for {HEAD_DIMS}")
+
+
+def dtype_of(first, *others) -> int:
+    if first.dtype not in _DTYPES or any(t.dtype != first.dtype for t in others):
+        raise ValueError(f"the tensors must share one of {list(_DTYPES)}; got {[t.dtype for t in (first, *others)]}")
+    return _DTYPES[first.dtype]
+
+
+def lse_fits(lse, HQ, T) -> None:
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (HQ, T) or not lse.is_contiguous()):
+        raise ValueError("lse must be a contiguous fp32 (query heads, rows) tensor")
+
+
+def forward_only(*tensors) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise ValueError("forward only: call it under torch.no_grad(), or detach the tensors that require a gradient")
+
+
+def call(entry: str, dev: torch.device, *args) -> None:
+    """One C call on the current stream of `dev`."""
+    fn = getattr(_lib.load(), entry)
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    if torch._C._cuda_getDevice() == dev.index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream)
+    if rc:
+        _lib.check(rc, entry)

@@ -1,8 +1,10 @@
 /*
- * gfx950_fmha.h -- C ABI of the MI355X (gfx950) flash-attention forward pass,
- * built into the same library as gfx950_gemm.h (whose status codes and
- * element types it uses).
+ * gfx950_fmha.h -- C ABI of the MI355X (gfx950) attention forward passes, built
+ * into the same library as gfx950_gemm.h (whose status codes and element types
+ * it uses): g9_fmha_fwd (below) over equal lengths, g9_varlen_fwd over packed
+ * prompts, g9_tree_fwd over a paged cache, and the cache's bookkeeping.
  *
+ * g9_fmha_fwd:
  * O = softmax(Q K^T * sm_scale) V for every (batch, query head), non-causal,
  * with grouped K/V heads: query head h reads K/V head h * HK / HQ (HQ a
  * multiple of HK; HK == HQ is plain multi-head, HK == 1 multi-query).  Q, K, V
@@ -12,6 +14,7 @@
 #ifndef GFX950_FMHA_H
 #define GFX950_FMHA_H
 
+#include <stddef.h>
 #include <stdint.h>
 
 #include "gfx950_gemm.h"
@@ -53,6 +56,97 @@ int g9_fmha_fwd(const void* q, const void* k, const void* v, void* o, float* lse
                 int64_t HK, int64_t S, int64_t D, const int64_t* q_strides, const int64_t* k_strides,
                 const int64_t* v_strides, const int64_t* o_strides, float sm_scale, int dtype, int scale_on_q,
                 int variant, void* stream);
+
+/*
+ * Packed and paged attention (no reference counterpart: its attention is
+ * non-causal over equal lengths).  Common to the entries below:
+ *
+ * - 16-bit elements (`dtype` G9_F16 or G9_BF16; g9_write_cache moves either),
+ *   head dim D 64 or 128, fp32 softmax and accumulation; query head h reads K/V
+ *   head h * HK / HQ.
+ * - Strides are in ELEMENTS with a unit head-dim stride left out: (token, head)
+ *   for packed tensors, (block, token, head) for caches.  They are multiples of
+ *   8 and not negative; base pointers are 16-byte aligned.  What is written (o,
+ *   the caches) must not overlap itself.  Offsets are 64-bit throughout.
+ * - Lengths, tables and offsets are device data, read when the kernel runs.
+ *   Whatever they hold, nothing outside the tensors is touched: negative lengths
+ *   count as 0, cu_seqlens are held inside the packed tensor, a table entry
+ *   outside [0, num_blocks) reads as zeros, and keys behind the table's width are
+ *   left out.
+ * - cu_seqlens: B + 1 ascending row offsets from 0; rows at or behind
+ *   cu_seqlens[B] belong to no sequence and their outputs stay as they were.
+ * - A query with no key it may read gives zeros, and -inf in lse.
+ * - Keys that no query may read (cache rows behind a request, unused blocks,
+ *   other sequences) have no effect, whatever they hold, NaN included.
+ * - Each call enqueues its kernels on `stream`, allocates nothing, synchronises
+ *   nothing and can be captured into a graph.
+ */
+
+/* Most requests of one g9_assign_slots call. */
+#define G9_SLOTS_MAX_REQUESTS 4096
+
+/*
+ * Where the next counts[b] tokens of each request go in a paged cache of blocks
+ * of block_size tokens.  lengths[b] tokens of request b are in the cache, their
+ * blocks in the first ceil(lengths[b] / block_size) entries of its table row.
+ *
+ * New blocks come from free_blocks[start], free_blocks[start + 1], ... in the
+ * order of the requests and of their positions (start = free_start[0], or 0
+ * where free_start is NULL) and are entered into the table; taken[0] is their
+ * number, also where it is more than the list holds.  cu_seqlens[B + 1] are the
+ * offsets of the requests' tokens in the packed batch.  For token t < T,
+ * positions[t] is its position in its request and slots[t] = block * block_size
+ * + offset, or -1 where the free list or the table's width does not reach (the
+ * table entry then becomes -1).  Rows behind the last token get position 0 and
+ * slot -1.  Nothing but new table entries depends on earlier results: the same
+ * call twice gives the same outputs.  B <= G9_SLOTS_MAX_REQUESTS.
+ */
+int g9_assign_slots(const int32_t* lengths, const int32_t* counts, int64_t B, int32_t* block_table,
+                    int64_t table_stride, int64_t width, const int32_t* free_blocks, int64_t num_free,
+                    const int32_t* free_start, int64_t block_size, int64_t T, int32_t* cu_seqlens, int64_t* slots,
+                    int64_t* positions, int32_t* taken, void* stream);
+
+/*
+ * k and v (T x HK x D) into the caches (num_blocks x block_size x HK x D) at
+ * their slots; rows whose slot lies outside the cache are skipped.  Slots must
+ * be distinct.  block_size: a power of two, 16 to 1024.
+ */
+int g9_write_cache(const void* k, const void* v, void* k_cache, void* v_cache, const int64_t* slots, int64_t T,
+                   int64_t HK, int64_t D, int64_t num_blocks, int64_t block_size, const int64_t* k_strides,
+                   const int64_t* v_strides, const int64_t* kc_strides, const int64_t* vc_strides, void* stream);
+
+/*
+ * Attention over packed sequences: q, o T x HQ x D; k, v TK x HK x D; sequence b
+ * holds the queries [cu_q[b], cu_q[b+1]) and the keys [cu_k[b], cu_k[b+1]).
+ * causal != 0 lets query i of Lq read the keys j <= i + Lk - Lq, so that a prompt
+ * whose first part is cached passes its new queries only.  lse: optional fp32
+ * HQ x T, contiguous: the natural-log log-sum-exp of each query's scaled scores.
+ */
+int g9_varlen_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* cu_q,
+                  const int32_t* cu_k, int64_t B, int64_t T, int64_t TK, int64_t HQ, int64_t HK, int64_t D,
+                  const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                  const int64_t* o_strides, float sm_scale, int dtype, int causal, void* stream);
+
+/*
+ * Attention of drafted tokens over a paged cache: request b brings the queries
+ * [cu_q[b], cu_q[b+1]), its nodes; its table row (B x width, int32) names the
+ * blocks of its lengths[b] context tokens and, at the positions behind them, of
+ * its nodes (whose K and V rows are in the cache already).  Node i reads every
+ * context token and the nodes j whose bit j % 64 is set in word j / 64 of row
+ * cu_q[b] + i of tree_mask (T x words, int64); without a mask the nodes j <= i.
+ * One node per request without a mask is plain decoding.  lse as g9_varlen_fwd.
+ *
+ * workspace: g9_tree_workspace_size bytes, 16-byte aligned, contents arbitrary;
+ * it holds partial results between the call's kernels, so calls that can run
+ * at the same time need one each.
+ */
+int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cache, void* o, float* lse,
+                const int32_t* block_table, int64_t table_stride, int64_t width, const int32_t* lengths,
+                const int32_t* cu_q, const int64_t* tree_mask, int64_t words, int64_t B, int64_t T, int64_t HQ,
+                int64_t HK, int64_t D, int64_t num_blocks, int64_t block_size, const int64_t* q_strides,
+                const int64_t* kc_strides, const int64_t* vc_strides, const int64_t* o_strides, float sm_scale,
+                int dtype, void* workspace, size_t workspace_bytes, void* stream);
+size_t g9_tree_workspace_size(int64_t B, int64_t T, int64_t HQ, int64_t HK, int64_t D);
 
 #ifdef __cplusplus
 }
