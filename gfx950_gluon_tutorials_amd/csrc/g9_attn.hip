@@ -2,9 +2,11 @@
 // bookkeeping (declared in include/gfx950_fmha.h).
 #include "../../include/gfx950_fmha.h"
 #include "g9_attn.hpp"
+#include "g9_attn_host.hpp"
 
 using namespace g9;
 using namespace g9::at;
+using namespace g9::host;
 
 namespace {
 
@@ -282,53 +284,12 @@ __global__ __launch_bounds__(256) void g9_attn_rows(AttnParams p) {
     p.lse[(long long)h * p.T + t] = l == 0.f ? -__builtin_inff() : (m + __builtin_log2f(l)) * kLn2;
 }
 
-// --- host side ----------------------------------------------------------------
-
-bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-
-int launched(hipError_t e) { return e == hipSuccess ? G9_OK : G9_ERR_HIP; }
-
-// Strides in elements: 16-byte steps, none negative.
-bool steps(const int64_t* s, int n) {
-  for (int i = 0; i < n; ++i)
-    if (s[i] < 0 || s[i] % 8 || s[i] > (int64_t(1) << 40)) return false;
-  return true;
-}
-// Whether the rows of D elements at these steps are apart: what is written
-// must not overlap.
-bool apart(const int64_t* size, const int64_t* stride, int n, int64_t D) {
-  int order[3] = {0, 1, 2};
-  for (int i = 0; i < n; ++i)
-    for (int j = i + 1; j < n; ++j)
-      if (stride[order[j]] < stride[order[i]]) {
-        const int x = order[i];
-        order[i] = order[j], order[j] = x;
-      }
-  int64_t reach = D;  // elements that the inner dimensions span
-  for (int i = 0; i < n; ++i) {
-    const int d = order[i];
-    if (size[d] <= 1) continue;
-    if (stride[d] < reach) return false;
-    reach += stride[d] * (size[d] - 1);
-  }
-  return true;
-}
-int log2_of(int64_t x) {
-  int n = 0;
-  while ((int64_t(1) << n) < x) ++n;
-  return n;
-}
-bool block_size_ok(int64_t s) { return s >= 16 && s <= 1024 && (s & (s - 1)) == 0; }
-bool scale_ok(float s) { return s > 0.f && s <= 3.4028234663852886e38f; }
-constexpr int64_t kMaxRows = 0x7fffffff - 4096;
-
-template <bool PAGED>
 const void* rows_kernel(int dtype, int64_t D) {
   if (dtype == G9_BF16)
-    return D == 128 ? reinterpret_cast<const void*>(g9_attn_rows<true, 128, PAGED>)
-                    : reinterpret_cast<const void*>(g9_attn_rows<true, 64, PAGED>);
-  return D == 128 ? reinterpret_cast<const void*>(g9_attn_rows<false, 128, PAGED>)
-                  : reinterpret_cast<const void*>(g9_attn_rows<false, 64, PAGED>);
+    return D == 128 ? reinterpret_cast<const void*>(g9_attn_rows<true, 128, true>)
+                    : reinterpret_cast<const void*>(g9_attn_rows<true, 64, true>);
+  return D == 128 ? reinterpret_cast<const void*>(g9_attn_rows<false, 128, true>)
+                  : reinterpret_cast<const void*>(g9_attn_rows<false, 64, true>);
 }
 
 }  // namespace
@@ -404,42 +365,6 @@ int g9_write_cache(const void* k, const void* v, void* k_cache, void* v_cache, c
                                   dim3(256), args, 0, reinterpret_cast<hipStream_t>(stream)));
 }
 
-int g9_varlen_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* cu_q,
-                  const int32_t* cu_k, int64_t B, int64_t T, int64_t TK, int64_t HQ, int64_t HK, int64_t D,
-                  const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
-                  const int64_t* o_strides, float sm_scale, int dtype, int causal, void* stream) {
-  if (dtype != G9_F16 && dtype != G9_BF16) return G9_ERR_DTYPE;
-  if (B < 0 || B > kMaxRows || T < 0 || T > kMaxRows || TK < 0 || TK > kMaxRows || HQ <= 0 || HQ > 65536 || HK <= 0 ||
-      HQ % HK || (D != 64 && D != 128) || !scale_ok(sm_scale))
-    return G9_ERR_SHAPE;
-  if (!q_strides || !k_strides || !v_strides || !o_strides) return G9_ERR_LAYOUT;
-  if (!steps(q_strides, 2) || !steps(k_strides, 2) || !steps(v_strides, 2) || !steps(o_strides, 2))
-    return G9_ERR_LAYOUT;
-  const int64_t size[2] = {T, HQ};
-  if (!apart(size, o_strides, 2, D)) return G9_ERR_LAYOUT;
-  if (B == 0 || T == 0) return G9_OK;
-  if (!q || !o || (TK && (!k || !v)) || !cu_q || !cu_k) return G9_ERR_LAYOUT;
-  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || ((uintptr_t)lse & 3)) return G9_ERR_LAYOUT;
-  AttnParams p{};
-  p.q = static_cast<const char*>(q);
-  p.k = static_cast<const char*>(k);
-  p.v = static_cast<const char*>(v);
-  p.o = static_cast<char*>(o);
-  p.lse = lse;
-  p.cu_q = cu_q;
-  p.cu_k = cu_k;
-  p.q_t = q_strides[0] * 2, p.q_h = q_strides[1] * 2, p.o_t = o_strides[0] * 2, p.o_h = o_strides[1] * 2;
-  p.k_t = k_strides[0] * 2, p.k_h = k_strides[1] * 2, p.v_t = v_strides[0] * 2, p.v_h = v_strides[1] * 2;
-  p.B = (int)B, p.T = (int)T, p.TK = (int)TK, p.HQ = (int)HQ, p.HK = (int)HK;
-  p.causal = causal != 0;
-  p.scale_log2 = sm_scale * kLog2e;
-  const int64_t waves = T * HQ;
-  if ((waves + 3) / 4 > INT32_MAX) return G9_ERR_SHAPE;
-  void* args[] = {&p};
-  return launched(hipLaunchKernel(rows_kernel<false>(dtype, D), dim3((unsigned)((waves + 3) / 4)), dim3(256), args, 0,
-                                  reinterpret_cast<hipStream_t>(stream)));
-}
-
 int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cache, void* o, float* lse,
                 const int32_t* block_table, int64_t table_stride, int64_t width, const int32_t* lengths,
                 const int32_t* cu_q, const int64_t* tree_mask, int64_t words, int64_t B, int64_t T, int64_t HQ,
@@ -488,7 +413,7 @@ int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cache, void* o
   const int64_t waves = T * HQ;
   if ((waves + 3) / 4 > INT32_MAX) return G9_ERR_SHAPE;
   void* args[] = {&p};
-  return launched(hipLaunchKernel(rows_kernel<true>(dtype, D), dim3((unsigned)((waves + 3) / 4)), dim3(256), args, 0,
+  return launched(hipLaunchKernel(rows_kernel(dtype, D), dim3((unsigned)((waves + 3) / 4)), dim3(256), args, 0,
                                   reinterpret_cast<hipStream_t>(stream)));
 }
 
