@@ -1,11 +1,10 @@
-// Attention over packed sequences and over a paged cache, and the cache's
-// bookkeeping (declared in include/gfx950_fmha.h).
+// The paged cache's bookkeeping: block tables and slot maps, and rows into the
+// cache (declared in include/gfx950_fmha.h).
 #include "../../include/gfx950_fmha.h"
-#include "g9_attn.hpp"
 #include "g9_attn_host.hpp"
+#include "g9_common.hpp"
 
 using namespace g9;
-using namespace g9::at;
 using namespace g9::host;
 
 namespace {
@@ -154,144 +153,6 @@ __global__ __launch_bounds__(256) void g9_cache_write(WriteParams p) {
   }
 }
 
-// --- attention, one wave per query row and head -------------------------------
-
-struct AttnParams {
-  const char* q;
-  const char* k;
-  const char* v;
-  char* o;
-  float* lse;                                      // [HQ][T], or null
-  const int* cu_q;
-  const int* cu_k;                                 // packed keys
-  long long q_t, q_h, o_t, o_h;                    // token / head strides, bytes
-  long long k_b, k_t, k_h, v_b, v_t, v_h;          // (block,) token, head strides, bytes
-  const int* table;                                // paged keys
-  const int* lengths;
-  const unsigned long long* mask;
-  long long table_stride, num_blocks;
-  int width, shift, words;
-  int B, T, TK, HQ, HK, causal;
-  float scale_log2;
-};
-
-// One pass with a running maximum m and sum l (log2 units): 64 keys at a
-// time, lane i scoring key i; then each lane sums its HD / 64 columns of P V
-// over the keys that the row may read.  Keys that it may not read are never
-// multiplied, whatever their rows hold.
-template <bool BF16, int HD, bool PAGED>
-__global__ __launch_bounds__(256) void g9_attn_rows(AttnParams p) {
-  __shared__ float qs[4][HD];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const long long item = (long long)blockIdx.x * 4 + wave;
-  const int t = (int)(item / p.HQ), h = (int)(item - (long long)t * p.HQ);
-  if (t >= p.T) return;
-  const int b = sequence_of(p.cu_q, p.B, t);
-  if (b >= p.B) return;
-  const Span sq = span_of(p.cu_q, b, p.T);
-  const int i = t - sq.first;
-  if (i < 0) return;
-  const int hk = (int)((long long)h * p.HK / p.HQ);
-  const char* kb = p.k + hk * p.k_h;
-  const char* vb = p.v + hk * p.v_h;
-  int keys, first = 0, context = 0;
-  if constexpr (PAGED) {
-    context = max(p.lengths[b], 0);
-    keys = (int)min((long long)context + sq.rows, (long long)p.width << p.shift);
-  } else {
-    const Span sk = span_of(p.cu_k, b, p.TK);
-    first = sk.first;
-    keys = sk.rows;
-    if (p.causal) keys = min(keys, max(i + 1 + sk.rows - sq.rows, 0));
-  }
-  const char* qrow = p.q + t * p.q_t + h * p.q_h;
-  if (lane < HD / 2) {
-    const f32x2 x = unpack2<BF16>(reinterpret_cast<const u32*>(qrow)[lane]);
-    qs[wave][2 * lane] = x.x * p.scale_log2;
-    qs[wave][2 * lane + 1] = x.y * p.scale_log2;
-  }
-  constexpr int kCols = HD / 64;
-  float m = -__builtin_inff(), l = 0.f, acc[kCols] = {};
-  for (int j0 = 0; j0 < keys; j0 += 64) {
-    const int j = j0 + lane;
-    bool reads = j < keys;
-    long long ko = -1, vo = -1;  // the key's rows; -1: a page outside the cache, read as zeros
-    if constexpr (PAGED) {
-      if (reads && j >= context) {
-        const int n = j - context;
-        if (p.mask)
-          reads = n < 64 * p.words && ((p.mask[(long long)t * p.words + n / 64] >> (n & 63)) & 1);
-        else
-          reads = n <= i;
-      }
-      if (reads) {
-        const int page = p.table[b * p.table_stride + (j >> p.shift)];
-        if (page >= 0 && page < p.num_blocks) {
-          const int off = j & ((1 << p.shift) - 1);
-          ko = page * p.k_b + off * p.k_t;
-          vo = page * p.v_b + off * p.v_t;
-        }
-      }
-    } else if (reads) {
-      ko = (long long)(first + j) * p.k_t;
-      vo = (long long)(first + j) * p.v_t;
-    }
-    float s = 0.f;
-    if (ko >= 0) {
-      const u32x4* row = reinterpret_cast<const u32x4*>(kb + ko);
-      for (int c = 0; c < HD / 8; ++c) {
-        const u32x4 w = row[c];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const f32x2 x = unpack2<BF16>(w[e]);
-          s = __builtin_fmaf(x.x, qs[wave][8 * c + 2 * e], s);
-          s = __builtin_fmaf(x.y, qs[wave][8 * c + 2 * e + 1], s);
-        }
-      }
-    }
-    if (!reads) s = -__builtin_inff();
-    const float top = fmaxf(m, wave_max(s));
-    const float base = top == -__builtin_inff() ? 0.f : top;
-    const float alpha = __builtin_amdgcn_exp2f(m - base);
-    const float pj = reads ? __builtin_amdgcn_exp2f(s - base) : 0.f;
-    l = l * alpha + wave_sum(pj);
-#pragma unroll
-    for (int c = 0; c < kCols; ++c) acc[c] *= alpha;
-    m = top;
-    const unsigned long long who = __builtin_amdgcn_ballot_w64(reads);
-    for (int n = 0; n < 64; ++n) {
-      if (!((who >> n) & 1)) continue;
-      const float w = __shfl(pj, n, 64);
-      const long long off = __shfl(vo, n, 64);
-      if (off < 0) continue;
-      if constexpr (kCols == 2) {
-        const f32x2 x = unpack2<BF16>(reinterpret_cast<const u32*>(vb + off)[lane]);
-        acc[0] = __builtin_fmaf(w, x.x, acc[0]);
-        acc[1] = __builtin_fmaf(w, x.y, acc[1]);
-      } else {
-        const u32 x = reinterpret_cast<const uint16_t*>(vb + off)[lane];
-        acc[0] = __builtin_fmaf(w, unpack2<BF16>(x).x, acc[0]);
-      }
-    }
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  char* orow = p.o + t * p.o_t + h * p.o_h;
-  if constexpr (kCols == 2)
-    reinterpret_cast<u32*>(orow)[lane] = pack2<BF16>(acc[0] * inv, acc[1] * inv);
-  else
-    reinterpret_cast<uint16_t*>(orow)[lane] = (uint16_t)pack2<BF16>(acc[0] * inv, 0.f);
-  if (p.lse && lane == 0)
-    p.lse[(long long)h * p.T + t] = l == 0.f ? -__builtin_inff() : (m + __builtin_log2f(l)) * kLn2;
-}
-
-const void* rows_kernel(int dtype, int64_t D) {
-  if (dtype == G9_BF16)
-    return D == 128 ? reinterpret_cast<const void*>(g9_attn_rows<true, 128, true>)
-                    : reinterpret_cast<const void*>(g9_attn_rows<true, 64, true>);
-  return D == 128 ? reinterpret_cast<const void*>(g9_attn_rows<false, 128, true>)
-                  : reinterpret_cast<const void*>(g9_attn_rows<false, 64, true>);
-}
-
 }  // namespace
 
 extern "C" {
@@ -363,63 +224,6 @@ int g9_write_cache(const void* k, const void* v, void* k_cache, void* v_cache, c
   void* args[] = {&p};
   return launched(hipLaunchKernel(reinterpret_cast<const void*>(g9_cache_write), dim3((unsigned)((T + 3) / 4)),
                                   dim3(256), args, 0, reinterpret_cast<hipStream_t>(stream)));
-}
-
-int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cache, void* o, float* lse,
-                const int32_t* block_table, int64_t table_stride, int64_t width, const int32_t* lengths,
-                const int32_t* cu_q, const int64_t* tree_mask, int64_t words, int64_t B, int64_t T, int64_t HQ,
-                int64_t HK, int64_t D, int64_t num_blocks, int64_t block_size, const int64_t* q_strides,
-                const int64_t* kc_strides, const int64_t* vc_strides, const int64_t* o_strides, float sm_scale,
-                int dtype, void* workspace, size_t workspace_bytes, void* stream) {
-  if (dtype != G9_F16 && dtype != G9_BF16) return G9_ERR_DTYPE;
-  if (B < 0 || B > kMaxRows || T < 0 || T > kMaxRows || HQ <= 0 || HQ > 65536 || HK <= 0 || HQ % HK ||
-      (D != 64 && D != 128) || !scale_ok(sm_scale) || num_blocks < 0 || num_blocks > kMaxRows || width < 0 ||
-      width > kMaxRows || !block_size_ok(block_size) || width * block_size > kMaxRows || words < 0 || words > 1024 ||
-      (tree_mask && words == 0))
-    return G9_ERR_SHAPE;
-  if (!q_strides || !kc_strides || !vc_strides || !o_strides) return G9_ERR_LAYOUT;
-  if (!steps(q_strides, 2) || !steps(kc_strides, 3) || !steps(vc_strides, 3) || !steps(o_strides, 2))
-    return G9_ERR_LAYOUT;
-  const int64_t size[2] = {T, HQ};
-  if (!apart(size, o_strides, 2, D) || (B > 1 && table_stride < width)) return G9_ERR_LAYOUT;
-  if (B == 0 || T == 0) return G9_OK;
-  if (!q || !o || !lengths || !cu_q || (width && !block_table) || (num_blocks && (!k_cache || !v_cache)))
-    return G9_ERR_LAYOUT;
-  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(o) || ((uintptr_t)lse & 3) ||
-      ((uintptr_t)tree_mask & 7))
-    return G9_ERR_LAYOUT;
-  (void)workspace, (void)workspace_bytes;
-  AttnParams p{};
-  p.q = static_cast<const char*>(q);
-  p.k = static_cast<const char*>(k_cache);
-  p.v = static_cast<const char*>(v_cache);
-  p.o = static_cast<char*>(o);
-  p.lse = lse;
-  p.cu_q = cu_q;
-  p.q_t = q_strides[0] * 2, p.q_h = q_strides[1] * 2, p.o_t = o_strides[0] * 2, p.o_h = o_strides[1] * 2;
-  p.k_b = kc_strides[0] * 2, p.k_t = kc_strides[1] * 2, p.k_h = kc_strides[2] * 2;
-  p.v_b = vc_strides[0] * 2, p.v_t = vc_strides[1] * 2, p.v_h = vc_strides[2] * 2;
-  p.table = block_table;
-  p.table_stride = table_stride;
-  p.lengths = lengths;
-  p.mask = reinterpret_cast<const unsigned long long*>(tree_mask);
-  p.words = (int)words;
-  p.width = (int)width;
-  p.num_blocks = num_blocks;
-  p.shift = log2_of(block_size);
-  p.B = (int)B, p.T = (int)T, p.HQ = (int)HQ, p.HK = (int)HK;
-  p.causal = 1;
-  p.scale_log2 = sm_scale * kLog2e;
-  const int64_t waves = T * HQ;
-  if ((waves + 3) / 4 > INT32_MAX) return G9_ERR_SHAPE;
-  void* args[] = {&p};
-  return launched(hipLaunchKernel(rows_kernel(dtype, D), dim3((unsigned)((waves + 3) / 4)), dim3(256), args, 0,
-                                  reinterpret_cast<hipStream_t>(stream)));
-}
-
-size_t g9_tree_workspace_size(int64_t B, int64_t T, int64_t HQ, int64_t HK, int64_t D) {
-  (void)B, (void)T, (void)HQ, (void)HK, (void)D;
-  return 0;
 }
 
 }  // extern "C"

@@ -1,0 +1,689 @@
+// Attention of drafted tokens over a paged cache (g9_tree_fwd,
+// include/gfx950_fmha.h); one node per request is plain decoding.
+//
+// Bound by reading the cache: every K and V row of the batch once, a few
+// products per value.  So the kernel is a stream.  The work is a line of tiles:
+// for each request, K/V head and block of 32 query rows (all query heads of
+// the K/V head and all nodes, node-major) the tiles of 4096 / D keys from first
+// to last.  The line is cut into equal parts, one per wave of a grid that fills
+// the chip once: requests of any lengths load every CU alike, and a single long
+// request is spread over all of them.  A wave keeps its own tiles in LDS (two
+// stages of 8 KB of K and 8 KB of V, filled by LDS-DMA), so no wave ever waits
+// for another one: there is no barrier in the loop.
+//
+// Per tile a wave computes S^T = K Q^T and O^T += V^T P^T with 32x32x16 MFMAs in
+// the register layouts that g9_fmha.hip describes: the scores are the second
+// product's operand as they stand, V is read by transposing LDS reads.  Blocks
+// of 32 rows are half empty where a request brings fewer, which costs nothing:
+// the matrix unit is idle most of the time.
+//
+// A block of rows whose tiles lie in one wave's part is finished there.  Else
+// each wave writes its unnormalized sum, maximum and weight to the workspace and
+// g9_tree_join, launched behind, joins them in the order of the keys: the result
+// depends on no timing.
+#include "../../include/gfx950_fmha.h"
+#include "g9_attn_host.hpp"
+#include "g9_fmha_pipe.hpp"
+
+namespace g9 {
+namespace tree {
+
+using namespace fa;
+
+constexpr int kWgs = 256;             // one workgroup per CU
+constexpr int kWavesWg = 4;
+constexpr int kWorkers = kWgs * kWavesWg;
+constexpr int kBlock = 32;            // query rows of a block
+
+struct Params {
+  const char* q;
+  const char* kc;
+  const char* vc;
+  char* o;
+  float* lse;                                      // [HQ][T], or null
+  const int* table;
+  const int* lengths;
+  const int* cu;
+  const unsigned long long* mask;                  // or null: a chain
+  float* part;                                     // partial sums [2 kWorkers][32][D], then (m, l) pairs
+  unsigned long long* first;                       // [B + 1]: first tile of each request on the line
+  long long q_t, q_h, o_t, o_h;                    // token / head strides, bytes
+  long long k_b, k_h, v_b, v_h;                    // block / head strides, bytes
+  long long table_stride;
+  u32 k_t, v_t;                                    // token strides, bytes
+  int num_blocks, width, shift, words;
+  int B, T, HQ, HK, group;
+  float scale_log2;
+};
+
+// One request: its query rows, context, keys, blocks of query rows, tiles.
+struct Req {
+  int q0, n, context, keys, blocks, tiles;
+};
+template <int HD>
+G9_DEV Req request(const Params& p, int b) {
+  Req r;
+  r.q0 = min(max(p.cu[b], 0), p.T);
+  r.n = min(max(p.cu[b + 1], r.q0), p.T) - r.q0;
+  r.context = max(p.lengths[b], 0);
+  r.keys = (int)min((long long)r.context + r.n, (long long)p.width << p.shift);
+  r.blocks = (int)(((long long)r.n * p.group + kBlock - 1) / (kBlock));
+  constexpr int kKeys = 4096 / HD;
+  r.tiles = max((r.keys + kKeys - 1) / kKeys, 1);
+  return r;
+}
+G9_DEV unsigned long long tiles_of(const Params& p, const Req& r) {
+  return (unsigned long long)r.blocks * (unsigned)p.HK * (unsigned)r.tiles;
+}
+// Worker w of W takes the tiles [w n / W, (w + 1) n / W) of a line of n; W is at
+// most n, so that no part in between is empty.
+G9_DEV unsigned workers(unsigned long long n) { return n < kWorkers ? (unsigned)n : kWorkers; }
+G9_DEV unsigned long long part_begin(unsigned w, unsigned long long n) { return w * n / workers(n); }
+G9_DEV unsigned worker_of(unsigned long long tile, unsigned long long n) {
+  return (unsigned)(((tile + 1) * workers(n) - 1) / n);
+}
+
+// A place on the line.
+struct Place {
+  Req r;
+  int b, hk, block, tile;
+};
+
+template <class V>
+G9_DEV V uniform(V x) {
+  if constexpr (sizeof(V) == 8) {
+    const unsigned long long u = (unsigned long long)x;
+    const u32 lo = (u32)__builtin_amdgcn_readfirstlane((int)u), hi = (u32)__builtin_amdgcn_readfirstlane((int)(u >> 32));
+    return (V)((unsigned long long)hi << 32 | lo);
+  } else {
+    return (V)__builtin_amdgcn_readfirstlane((int)x);
+  }
+}
+
+template <bool BF16, int HD>
+struct Wave {
+  static constexpr int kKeys = 4096 / HD;          // keys per tile
+  static constexpr int kNB = kKeys / 32;           // 32-key score blocks
+  static constexpr int kNS = HD / 16;              // QK steps of 16 head-dim values
+  static constexpr int kKS = kKeys / 16;           // PV steps of 16 keys
+  static constexpr int kND = HD / 32;              // PV blocks of 32 head-dim values
+  static constexpr int kRow = HD * 2;              // bytes of a row
+  static constexpr int kRows = 1024 / kRow;        // rows of one DMA
+  static constexpr int kPieces = kKeys / 16;       // 16-row pieces: never across a page
+  static constexpr int kDmas = 8;                  // per tile and operand
+  static constexpr int kStage = 16384, kV = 8192;  // a stage; V behind K
+  static constexpr int kScratch = kBlock * kKeys * 2;  // P of one tile, 16 bit
+  static constexpr int kWaveLds = 2 * kStage + kScratch;
+
+  const Params& p;
+  int lane, h, col;  // lane, lane / 32, lane % 32
+  u32 lds;           // this wave's LDS
+  char* scratch;
+  u32 voffk[4], voffv[1];
+  u32 ak, av;        // LDS read bases in a stage (K, V)
+  u32x4 qf[kNS];
+  f32x16 o[kND];
+  float m, l;
+  int node;          // the node of this lane's query row, -1 where there is none
+
+  G9_DEV explicit Wave(const Params& pp) : p(pp) {}
+
+  // LDS layout of a tile: rows of kRow bytes, their 16-byte chunks permuted
+  // within the row so that a read of one chunk from 16 rows (K), or of 64 bytes
+  // from 4 rows (V), touches every bank once.  Chunk c of row r is at slot c ^
+  // swz(r).  An LDS-DMA writes lane i's 16 bytes at 16 i, so lane i fetches the
+  // chunk that belongs there; a wave's DMA reads whole rows.
+  static G9_DEV int swz_k(int r) { return HD == 128 ? r & 15 : (r >> 1) & 7; }
+  static G9_DEV int swz_v(int r) { return HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); }
+
+  G9_DEV void init(char* smem, int wave) {
+    lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
+    lds = (u32)(uintptr_t)to_lds(smem) + wave * kWaveLds;
+    scratch = smem + wave * kWaveLds + 2 * kStage;
+    constexpr int kPer = kRow / 16;  // chunks of a row
+    const int r = lane / kPer, slot = lane % kPer;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) voffk[j] = r * p.k_t + 16 * (slot ^ swz_k(kRows * j + r));
+    voffv[0] = r * p.v_t + 16 * (slot ^ swz_v(r));
+    const int jj = lane & 15;
+    ak = lds + col * kRow;
+    av = lds + kV + vrow() * kRow + 8 * (jj & 1);
+  }
+  // V's transposing reads: 16 lanes cover 4 rows and 16 values; lane jj of them
+  // addresses row jj / 4, values 4 (jj % 4).
+  G9_DEV int vrow() const { return 4 * h + ((lane & 15) >> 2); }
+
+  // The 16-row pieces' pages of a tile; -1: none.
+  G9_DEV void pages(const Place& at, int (&pg)[kPieces]) const {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int k = at.tile * kKeys + 16 * i;
+      pg[i] = k < at.r.keys ? p.table[at.b * p.table_stride + (k >> p.shift)] : -1;
+    }
+  }
+  G9_DEV void fill(const Place& at, const int (&pg)[kPieces], int stage) const {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int k = at.tile * kKeys + 16 * i, off = k & ((1 << p.shift) - 1);
+      const bool in = (u32)pg[i] < (u32)p.num_blocks;
+      const int rows = in ? min(max(at.r.keys - k, 0), 16) : 0;
+      const long long page = in ? pg[i] : 0;
+      const rsrc_t rk = make_rsrc(uniform(p.kc + page * p.k_b + at.hk * p.k_h + (unsigned long long)off * p.k_t),
+                                  uniform((u32)rows * p.k_t));
+      const rsrc_t rv = make_rsrc(uniform(p.vc + page * p.v_b + at.hk * p.v_h + (unsigned long long)off * p.v_t),
+                                  uniform((u32)rows * p.v_t));
+#pragma unroll
+      for (int jj = 0; jj < 16 / kRows; ++jj) {
+        const int j = i * (16 / kRows) + jj;
+        dma16_untracked(rk, lds + stage * kStage + j * 1024, voffk[j & (HD == 128 ? 3 : 1)], jj * kRows * p.k_t);
+        dma16_untracked(rv, lds + stage * kStage + kV + j * 1024, voffv[0], jj * kRows * p.v_t);
+      }
+    }
+  }
+
+  G9_DEV void begin(const Place& at) {
+    const int row = at.block * kBlock + col;
+    const int nd = row / p.group, hd = row - nd * p.group;
+    const bool in = nd < at.r.n;
+    node = in ? nd : -1;
+    const char* qrow = p.q + (long long)(at.r.q0 + (in ? nd : 0)) * p.q_t + (long long)(at.hk * p.group + (in ? hd : 0)) * p.q_h;
+#pragma unroll
+    for (int s = 0; s < kNS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(qrow + (16 * s + 8 * h) * 2);
+    // Finite, so that a row that has read nothing yet has weights 2^(-inf - m) =
+    // 0 and a sum of 0, not NaN.
+    m = -3.0e38f, l = 0.f;
+#pragma unroll
+    for (int d = 0; d < kND; ++d) o[d] = f32x16{};
+    // Waited for here: the compiler does not count the DMAs in flight, and a wait
+    // of its own at the first use would be one in every tile.
+    waitcnt<0, 0>();
+  }
+
+  // Bit i: the row reads key i of the tile.
+  G9_DEV unsigned long long reads(const Place& at) const {
+    const int k0 = at.tile * kKeys;
+    const int n0 = max(k0 - at.r.context, -4096);  // the tile's first node, negative in the context
+    unsigned long long w;
+    if (!p.mask) {
+      const int c = node + 1 - n0;  // keys up to the row's own
+      w = c >= 64 ? ~0ull : c <= 0 ? 0 : (1ull << c) - 1;
+    } else {
+      const unsigned long long* row = p.mask + (long long)(at.r.q0 + max(node, 0)) * p.words;
+      const int first = max(n0, 0) >> 6, sh = max(n0, 0) & 63;
+      const unsigned long long a = first < p.words ? row[first] : 0, b = first + 1 < p.words ? row[first + 1] : 0;
+      w = sh ? a >> sh | b << (64 - sh) : a;
+      if (n0 < 0) w = n0 <= -64 ? ~0ull : w << -n0 | ((1ull << -n0) - 1);
+    }
+    const int left = at.r.keys - k0;
+    if (left < 64) w &= left <= 0 ? 0 : (1ull << left) - 1;
+    return w;
+  }
+
+  template <bool TAIL>
+  G9_DEV void tile(const Place& at, int stage) {
+    f32x16 sc[kNB];
+#pragma unroll
+    for (int s = 0; s < kNS; ++s)
+#pragma unroll
+      for (int b = 0; b < kNB; ++b) {
+        const u32x4 kf = *(const G9_LDS u32x4*)(uintptr_t)(ak + stage * kStage + 32 * b * kRow +
+                                                           16 * ((2 * s + h) ^ swz_k(col)));
+        sc[b] = mfma<BF16>(kf, qf[s], s ? sc[b] : f32x16{});
+      }
+    if constexpr (TAIL) {
+      const unsigned long long w = reads(at);
+#pragma unroll
+      for (int b = 0; b < kNB; ++b) {
+        const u32 bits = (u32)(w >> (32 * b)) >> (4 * h);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float x = sc[b][i];
+          sc[b][i] = bits >> (8 * (i / 4) + i % 4) & 1 ? x : -__builtin_inff();
+        }
+      }
+    }
+    float top = sc[0][0];
+#pragma unroll
+    for (int b = 0; b < kNB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, sc[b][i]);
+    top = xhalf(top, [](float x, float y) { return __builtin_fmaxf(x, y); });
+    const float m_new = __builtin_fmaxf(m, top * p.scale_log2);
+    const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+    m = m_new;
+    float sum[4] = {};
+    u32x4 pf[kKS];
+#pragma unroll
+    for (int b = 0; b < kNB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i], p.scale_log2, -m_new));
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i + 1], p.scale_log2, -m_new));
+        sum[i / 2 % 2 * 2] += x, sum[i / 2 % 2 * 2 + 1] += y;
+        pf[2 * b + i / 8][i % 8 / 2] = pack2<BF16>(x, y);
+      }
+    l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.f)) {
+#pragma unroll
+      for (int d = 0; d < kND; ++d) o[d] *= alpha;
+    }
+    u32x4 vf[kKS][kND];
+#pragma unroll
+    for (int k = 0; k < kKS; ++k)
+#pragma unroll
+      for (int d = 0; d < kND; ++d) {
+        // Rows vrow and vrow + 8 of the step: swz_v of both is the same.
+        const u32 a = av + stage * kStage + 16 * k * kRow +
+                      16 * ((4 * d + 2 * (lane >> 4 & 1) + ((lane & 3) >> 1)) ^ swz_v(vrow()));
+        const u32x2 lo = tr_read(a), hi = tr_read(a + 8 * kRow);
+        vf[k][d] = u32x4{lo.x, lo.y, hi.x, hi.y};
+      }
+    if constexpr (TAIL) guard(at, stage, vf, pf);
+#pragma unroll
+    for (int k = 0; k < kKS; ++k)
+#pragma unroll
+      for (int d = 0; d < kND; ++d) o[d] = mfma<BF16>(vf[k][d], pf[k], o[d]);
+  }
+
+  // Tiles that hold nodes: a weight of 0 does not keep an infinite or NaN value
+  // out of the product.  Such values (rare) are taken out of the registers, and
+  // added on the vector unit to the rows that read their key.
+  G9_DEV void guard(const Place& at, int stage, u32x4 (&vf)[kKS][kND], const u32x4 (&pf)[kKS]) {
+    typedef unsigned short h2 __attribute__((ext_vector_type(2)));
+    constexpr u32 kExp = BF16 ? 0x7f80u : 0x7c00u;
+    h2 top = {0, 0};
+#pragma unroll
+    for (int k = 0; k < kKS; ++k)
+#pragma unroll
+      for (int d = 0; d < kND; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          top = __builtin_elementwise_max(top, __builtin_bit_cast(h2, vf[k][d][e] & 0x7fff7fffu));
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(top.x >= kExp || top.y >= kExp) == 0, 1)) return;
+#pragma unroll
+    for (int k = 0; k < kKS; ++k)
+#pragma unroll
+      for (int d = 0; d < kND; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          u32 x = vf[k][d][e];
+          if ((x & kExp) == kExp) x &= 0xffff0000u;
+          if (((x >> 16) & kExp) == kExp) x &= 0xffffu;
+          pin(x);  // one compare at a time: their masks would not fit the scalar registers
+          vf[k][d][e] = x;
+        }
+    // P in LDS: row of the query, column of the key.
+    uint16_t* const row = reinterpret_cast<uint16_t*>(scratch) + col * kKeys;
+#pragma unroll
+    for (int k = 0; k < kKS; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<u32*>(row + 16 * k + 8 * (e >> 1) + 4 * h + 2 * (e & 1)) = pf[k][e];
+    const unsigned long long w = reads(at);
+    waitcnt<63, 0>();
+#pragma unroll 1
+    for (int key = 0; key < kKeys; ++key) {
+      if (!((w >> key) & 1)) continue;
+      const float wt = unpack2<BF16>(row[key]).x;
+      const u32 vr = lds + stage * kStage + kV + key * kRow;
+#pragma unroll
+      for (int d = 0; d < kND; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const u32x2 x = *(const G9_LDS u32x2*)(uintptr_t)(vr + 16 * ((4 * d + r) ^ swz_v(key)) + 8 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            u32 y = (e & 1 ? x[e / 2] >> 16 : x[e / 2]) & 0xffffu;
+            if ((y & kExp) != kExp) y = 0;
+            o[d][4 * r + e] += wt * unpack2<BF16>(y).x;
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+  }
+
+  // The rows' results, or their sums to slot `slot` of the workspace.
+  G9_DEV void end(const Place& at, int slot) {
+    const float lt = xhalf(l, [](float x, float y) { return x + y; });
+    if (node < 0) return;
+    if (slot >= 0) {
+      float* const sum = p.part + ((size_t)slot * kBlock + col) * HD;
+#pragma unroll
+      for (int d = 0; d < kND; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          *reinterpret_cast<f32x4*>(sum + 32 * d + 8 * r + 4 * h) =
+              f32x4{o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]};
+      if (h == 0) {
+        float* const ml = p.part + (size_t)2 * kWorkers * kBlock * HD + ((size_t)slot * kBlock + col) * 2;
+        ml[0] = m, ml[1] = lt;
+      }
+      return;
+    }
+    const int hq = at.hk * p.group + at.block * kBlock + col - node * p.group;
+    const long long tok = at.r.q0 + node;
+    // By its bits: comparisons here may take NaN for a number.
+    const bool none = (__float_as_uint(lt) << 1) == 0;
+    const float inv = none ? 0.f : 1.f / lt;
+    char* const orow = p.o + tok * p.o_t + hq * p.o_h;
+#pragma unroll
+    for (int d = 0; d < kND; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *reinterpret_cast<u32x2*>(orow + (32 * d + 8 * r + 4 * h) * 2) =
+            u32x2{pack2<BF16>(o[d][4 * r] * inv, o[d][4 * r + 1] * inv),
+                  pack2<BF16>(o[d][4 * r + 2] * inv, o[d][4 * r + 3] * inv)};
+    if (p.lse && h == 0) p.lse[(long long)hq * p.T + tok] = none ? -__builtin_inff() : (m + __builtin_log2f(lt)) * kLn2;
+  }
+};
+
+template <class X>
+G9_DEV void scalar(X& r) {
+  r.r.q0 = uniform(r.r.q0), r.r.n = uniform(r.r.n), r.r.context = uniform(r.r.context), r.r.keys = uniform(r.r.keys);
+  r.r.blocks = uniform(r.r.blocks), r.r.tiles = uniform(r.r.tiles);
+  r.b = uniform(r.b), r.hk = uniform(r.hk), r.block = uniform(r.block), r.tile = uniform(r.tile);
+}
+
+template <bool BF16, int HD>
+G9_DEV void run(const Params& p, char* smem) {
+  using W = Wave<BF16, HD>;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // Consecutive workgroups go round the 8 XCDs; consecutive parts of the line
+  // stay on one, whose L2 then serves the rows' blocks that share keys.
+  const unsigned wg = (blockIdx.x & 7) * (kWgs / 8) + (blockIdx.x >> 3);
+  const unsigned worker = wg * kWavesWg + wave;
+
+  // The requests' first tiles (in LDS, and from one workgroup in the workspace
+  // for the kernel that joins the parts).
+  unsigned long long* const first = reinterpret_cast<unsigned long long*>(smem);  // [B + 1], then the waves' sums
+  constexpr int kThreadsWg = 64 * kWavesWg;
+  unsigned long long* const sums = first + p.B + 1;
+  const int run_len = (p.B + kThreadsWg - 1) / kThreadsWg;
+  const int b0 = min(tid * run_len, p.B), b1 = min(b0 + run_len, p.B);
+  unsigned long long mine = 0;
+  for (int b = b0; b < b1; ++b) mine += tiles_of(p, request<HD>(p, b));
+  unsigned long long before = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const unsigned long long x = __shfl_up(before, d, 64);
+    if (lane >= d) before += x;
+  }
+  if (lane == 63) sums[wave] = before;
+  __syncthreads();
+  before -= mine;
+  unsigned long long total = 0;
+  for (int w = 0; w < kWavesWg; ++w) {
+    if (w < wave) before += sums[w];
+    total += sums[w];
+  }
+  for (int b = b0; b < b1; ++b) {
+    first[b] = before;
+    if (wg == 0) p.first[b] = before;
+    before += tiles_of(p, request<HD>(p, b));
+  }
+  if (tid == 0) {
+    first[p.B] = total;
+    if (wg == 0) p.first[p.B] = total;
+  }
+  __syncthreads();
+  total = uniform(total);
+  unsigned long long begin = 0;
+  int count = 0;
+  if (worker < workers(total)) {
+    begin = uniform(part_begin(worker, total));
+    count = uniform((int)(part_begin(worker + 1, total) - begin));
+  }
+  Place cur;
+  if (count > 0) {
+    // The last request that begins at or before the part (empty ones begin
+    // where the next one does).
+    int lo = 0, hi = p.B;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (first[mid] <= begin)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    cur.b = uniform(lo);
+    cur.r = request<HD>(p, cur.b);
+    const unsigned long long in = uniform(begin - first[lo]);
+    const unsigned long long unit = in / (unsigned)cur.r.tiles;
+    cur.tile = (int)(in - unit * (unsigned)cur.r.tiles);
+    cur.hk = (int)(unit / (unsigned)cur.r.blocks);
+    cur.block = (int)(unit - (unsigned long long)cur.hk * cur.r.blocks);
+    scalar(cur);
+  }
+  __syncthreads();  // first[] is read: the stages take its place
+  if (count <= 0) return;
+
+  W w(p);
+  w.init(smem, wave);
+  const auto next = [&](const Place& a) {
+    Place n = a;
+    if (++n.tile < n.r.tiles) return n;
+    n.tile = 0;
+    if (++n.block < n.r.blocks) return n;
+    n.block = 0;
+    if (++n.hk < p.HK) return n;
+    n.hk = 0;
+    do {
+      n.b = min(n.b + 1, p.B - 1);
+      n.r = request<HD>(p, n.b);
+    } while (n.r.blocks == 0 && n.b < p.B - 1);
+    scalar(n);
+    return n;
+  };
+  int pg[W::kPieces];
+  w.pages(cur, pg);
+  w.fill(cur, pg, 0);
+  Place nxt = cur;
+  if (count > 1) {
+    nxt = next(cur);
+    w.pages(nxt, pg);
+  }
+  bool fresh = true, from_start = cur.tile == 0;
+  for (int i = 0; i < count; ++i) {
+    // The stage that tile i + 1 takes was last read for tile i - 1.
+    waitcnt<63, 0>();
+    __builtin_amdgcn_sched_barrier(0);
+    Place aft = nxt;
+    if (i + 1 < count) {
+      w.fill(nxt, pg, (i + 1) & 1);
+      if (i + 2 < count) {
+        aft = next(nxt);
+        w.pages(aft, pg);
+      }
+      if (fresh) w.begin(cur);
+      waitcnt<2 * W::kDmas, 15>();
+    } else {
+      if (fresh) w.begin(cur);
+      waitcnt<0, 15>();
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    const bool tail = (cur.tile + 1) * W::kKeys > min(cur.r.context, cur.r.keys);
+    if (tail)
+      w.template tile<true>(cur, i & 1);
+    else
+      w.template tile<false>(cur, i & 1);
+    const bool last = cur.tile + 1 == cur.r.tiles;
+    fresh = last;
+    if (last || i + 1 == count) {
+      // Slot 0 of the worker: a block that another worker began; slot 1: one
+      // that the next worker goes on with.
+      w.end(cur, last && from_start ? -1 : (int)(2 * worker + (from_start ? 1 : 0)));
+      from_start = true;
+    }
+    cur = nxt;
+    nxt = aft;
+  }
+}
+
+// Joins the parts of query row (token t, head hq): with m the largest of their
+// maxima, sum of 2^(m_i - m) O_i over the sum of 2^(m_i - m) l_i, in the order of
+// the keys.  One workgroup per row; its threads hold HD / 4 columns by kLanes
+// parts.
+template <bool BF16, int HD>
+G9_DEV void join(const Params& p, float* lds) {
+  constexpr int kCols = HD / 4, kParts = 256 / kCols;
+  const int t = blockIdx.x / p.HQ, hq = blockIdx.x - t * p.HQ;
+  const int tid = threadIdx.x, c = tid % kCols, s = tid / kCols;
+  // The request of row t.
+  int lo = 0, hi = p.B;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (p.cu[mid + 1] <= t)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  if (lo >= p.B) return;
+  const Req r = request<HD>(p, lo);
+  const int nd = t - r.q0, hk = hq / p.group;
+  if (nd < 0 || nd >= r.n) return;
+  const int row = nd * p.group + hq - hk * p.group;
+  const int block = row / (kBlock), in = row - block * kBlock;
+  const unsigned long long total = p.first[p.B];
+  const unsigned long long u0 = p.first[lo] + ((unsigned long long)hk * r.blocks + block) * r.tiles;
+  const unsigned w0 = worker_of(u0, total), w1 = worker_of(u0 + r.tiles - 1, total);
+  if (w0 == w1) return;  // finished by its wave
+  const float* const ml = p.part + (size_t)2 * kWorkers * kBlock * HD;
+  // Worker w0 has it in slot 1 unless it began the block before its part.
+  const auto at = [&](unsigned w) {
+    const unsigned slot = 2 * w + (w == w0 && part_begin(w0, total) <= u0 ? 1 : 0);
+    return (size_t)slot * kBlock + in;
+  };
+  const unsigned n = w1 - w0 + 1;
+  float top = -3.0e38f;
+  for (unsigned i = tid; i < n; i += 256) top = __builtin_fmaxf(top, ml[at(w0 + i) * 2]);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, d, 64));
+  if ((tid & 63) == 0) lds[tid >> 6] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = __builtin_fmaxf(top, lds[i]);
+  f32x4 sum = {};
+  float l = 0.f;
+  for (unsigned i = s; i < n; i += kParts) {
+    const size_t a = at(w0 + i);
+    const float f = __builtin_amdgcn_exp2f(ml[a * 2] - top);
+    l += f * ml[a * 2 + 1];
+    sum += f * *reinterpret_cast<const f32x4*>(p.part + a * HD + 4 * c);
+  }
+  __syncthreads();
+  float* const mine = lds + (s * kCols + c) * 5;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) mine[e] = sum[e];
+  mine[4] = l;
+  __syncthreads();
+  if (tid >= kCols) return;
+  for (int i = 1; i < kParts; ++i) {
+    const float* const other = lds + (i * kCols + c) * 5;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] += other[e];
+    l += other[4];
+  }
+  const bool none = (__float_as_uint(l) << 1) == 0;
+  const float inv = none ? 0.f : 1.f / l;
+  *reinterpret_cast<u32x2*>(p.o + t * p.o_t + hq * p.o_h + c * 8) =
+      u32x2{pack2<BF16>(sum[0] * inv, sum[1] * inv), pack2<BF16>(sum[2] * inv, sum[3] * inv)};
+  if (p.lse && c == 0) p.lse[(long long)hq * p.T + t] = none ? -__builtin_inff() : (top + __builtin_log2f(l)) * kLn2;
+}
+
+}  // namespace tree
+}  // namespace g9
+
+using namespace g9;
+using namespace g9::host;
+
+#define G9_TREE_KERNEL(NAME, BF16, HD)                                                                    \
+  extern "C" __global__ __launch_bounds__(64 * tree::kWavesWg) __attribute__((amdgpu_waves_per_eu(1, 1))) void \
+  g9_tree_##NAME(tree::Params p) {                                                                            \
+    __shared__ __attribute__((aligned(1024))) char smem[tree::kWavesWg * tree::Wave<BF16, HD>::kWaveLds];  \
+    tree::run<BF16, HD>(p, smem);                                                                         \
+  }                                                                                                           \
+  extern "C" __global__ __launch_bounds__(256) void g9_tree_join_##NAME(tree::Params p) {                     \
+    __shared__ float lds[256 * 5];                                                                            \
+    tree::join<BF16, HD>(p, lds);                                                                         \
+  }
+G9_TREE_KERNEL(bf16, true, 128)
+G9_TREE_KERNEL(f16, false, 128)
+G9_TREE_KERNEL(bf16_d64, true, 64)
+G9_TREE_KERNEL(f16_d64, false, 64)
+
+namespace {
+
+size_t part_floats(int64_t D) { return (size_t)2 * tree::kWorkers * tree::kBlock * (D + 2); }
+
+#define G9_TREE_FNS(WHAT)                                                                       \
+  {{reinterpret_cast<const void*>(WHAT##f16), reinterpret_cast<const void*>(WHAT##bf16)},       \
+   {reinterpret_cast<const void*>(WHAT##f16_d64), reinterpret_cast<const void*>(WHAT##bf16_d64)}}
+// [head dim 64][bf16]
+const void* const kRun[2][2] = G9_TREE_FNS(g9_tree_);
+const void* const kJoin[2][2] = G9_TREE_FNS(g9_tree_join_);
+
+}  // namespace
+
+extern "C" size_t g9_tree_workspace_size(int64_t B, int64_t T, int64_t HQ, int64_t HK, int64_t D) {
+  if (B <= 0 || T <= 0 || HQ <= 0 || HK <= 0 || HQ % HK || D <= 0) return 0;
+  return part_floats(D) * 4 + (size_t)(B + 1) * 8;
+}
+
+extern "C" int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cache, void* o, float* lse,
+                const int32_t* block_table, int64_t table_stride, int64_t width, const int32_t* lengths,
+                const int32_t* cu_q, const int64_t* tree_mask, int64_t words, int64_t B, int64_t T, int64_t HQ,
+                int64_t HK, int64_t D, int64_t num_blocks, int64_t block_size, const int64_t* q_strides,
+                const int64_t* kc_strides, const int64_t* vc_strides, const int64_t* o_strides, float sm_scale,
+                int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  if (dtype != G9_F16 && dtype != G9_BF16) return G9_ERR_DTYPE;
+  if (B < 0 || B > G9_TREE_MAX_REQUESTS || T < 0 || T > kMaxRows || HQ <= 0 || HQ > 65536 || HK <= 0 || HQ % HK ||
+      (D != 64 && D != 128) || !scale_ok(sm_scale) || num_blocks < 0 || num_blocks > kMaxRows || width < 0 ||
+      width > kMaxRows || !block_size_ok(block_size) || width * block_size > kMaxRows || words < 0 || words > 1024 ||
+      (tree_mask && words == 0))
+    return G9_ERR_SHAPE;
+  if (!q_strides || !kc_strides || !vc_strides || !o_strides) return G9_ERR_LAYOUT;
+  if (!steps(q_strides, 2) || !steps(kc_strides, 3) || !steps(vc_strides, 3) || !steps(o_strides, 2))
+    return G9_ERR_LAYOUT;
+  const int64_t size[2] = {T, HQ};
+  if (!apart(size, o_strides, 2, D) || (B > 1 && table_stride < width)) return G9_ERR_LAYOUT;
+  // A 16-row piece of a page lies within a descriptor's range, its rows apart.
+  for (const int64_t* st : {kc_strides, vc_strides})
+    if (st[1] < D || st[1] * 2 * 16 >= (int64_t(1) << 31)) return G9_ERR_LAYOUT;
+  if (T * HQ > INT32_MAX) return G9_ERR_SHAPE;
+  if (B == 0 || T == 0) return G9_OK;
+  if (!q || !o || !lengths || !cu_q || (width && !block_table) || (num_blocks && (!k_cache || !v_cache)))
+    return G9_ERR_LAYOUT;
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(o) || ((uintptr_t)lse & 3) ||
+      ((uintptr_t)tree_mask & 7))
+    return G9_ERR_LAYOUT;
+  const int64_t group = HQ / HK;
+  const size_t floats = part_floats(D);
+  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < floats * 4 + (size_t)(B + 1) * 8)
+    return G9_ERR_WORKSPACE;
+  tree::Params p{};
+  p.q = static_cast<const char*>(q);
+  p.kc = static_cast<const char*>(k_cache);
+  p.vc = static_cast<const char*>(v_cache);
+  p.o = static_cast<char*>(o);
+  p.lse = lse;
+  p.table = block_table;
+  p.lengths = lengths;
+  p.cu = cu_q;
+  p.mask = reinterpret_cast<const unsigned long long*>(tree_mask);
+  p.part = static_cast<float*>(workspace);
+  p.first = reinterpret_cast<unsigned long long*>(p.part + floats);
+  p.q_t = q_strides[0] * 2, p.q_h = q_strides[1] * 2, p.o_t = o_strides[0] * 2, p.o_h = o_strides[1] * 2;
+  p.k_b = kc_strides[0] * 2, p.k_h = kc_strides[2] * 2, p.v_b = vc_strides[0] * 2, p.v_h = vc_strides[2] * 2;
+  p.k_t = (u32)(kc_strides[1] * 2), p.v_t = (u32)(vc_strides[1] * 2);
+  p.table_stride = table_stride;
+  p.num_blocks = (int)num_blocks, p.width = (int)width, p.shift = log2_of(block_size), p.words = (int)words;
+  p.B = (int)B, p.T = (int)T, p.HQ = (int)HQ, p.HK = (int)HK, p.group = (int)group;
+  p.scale_log2 = sm_scale * fa::kLog2e;
+  void* args[] = {&p};
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (hipLaunchKernel(kRun[D == 64][dtype == G9_BF16], dim3(tree::kWgs), dim3(64 * tree::kWavesWg), args, 0, st) !=
+      hipSuccess)
+    return G9_ERR_HIP;
+  return launched(hipLaunchKernel(kJoin[D == 64][dtype == G9_BF16], dim3((unsigned)(T * HQ)), dim3(256), args, 0, st));
+}

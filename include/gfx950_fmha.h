@@ -82,8 +82,9 @@ int g9_fmha_fwd(const void* q, const void* k, const void* v, void* o, float* lse
  *   nothing and can be captured into a graph.
  */
 
-/* Most requests of one g9_assign_slots call. */
+/* Most requests of one g9_assign_slots call, of one g9_tree_fwd call. */
 #define G9_SLOTS_MAX_REQUESTS 4096
+#define G9_TREE_MAX_REQUESTS 8192
 
 /*
  * Where the next counts[b] tokens of each request go in a paged cache of blocks
