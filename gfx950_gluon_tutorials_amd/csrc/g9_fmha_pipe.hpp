@@ -73,6 +73,15 @@ G9_DEV void dma16_untracked(rsrc_t r, u32 lds, u32 voff, u32 soff) {
   asm volatile("buffer_load_dwordx4 %1, %2, %3 offen lds" : : "{m0}"(lds), "v"(voff), "s"(r), "s"(soff) : "memory");
 }
 
+// The same with a descriptor or offset that the vector unit may just have
+// written (v_readfirstlane, or v_readlane where the compiler keeps scalar
+// registers in vector lanes): a vector-memory instruction may read such a
+// register five wait states later at the earliest, and the compiler, which sees
+// to that for its own instructions, does not look into assembly.
+G9_DEV void dma16_fresh(rsrc_t r, u32 lds, u32 voff, u32 soff) {
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "{m0}"(lds), "v"(voff), "s"(r), "s"(soff) : "memory");
+}
+
 // Pins a value to this point of the program: the compiler can neither move
 // its computation past the statement nor sink it toward its uses.
 G9_DEV void pin(float& x) { asm volatile("" : "+v"(x)); }
@@ -164,13 +173,34 @@ constexpr int sum16(const int (&a)[16]) {
 // per-cluster costs (barriers, the row-max chain, waits) over the same MFMA
 // work.  A tile's scores are kNB blocks of 32 keys (Sc).
 //
-// VAR: keys of one packed sequence, of which each query may read the first
-// `lim` (its causal limit).  Tiles that reach past the wave's smallest limit
-// (`wlim`) are masked by comparing key indexes with lim.  Tile addresses are
-// 64-bit: a descriptor per tile whose range ends with the sequence, so rows
-// behind it read as zeros.
-template <class Params, bool BF16, bool LAZY, bool SOQ, int HD, bool VAR = false>
-struct Pipe {
+// KIND says where the keys are and which of them a query reads:
+//   kEqual   all of p.S rows.
+//   kPacked  `keys` rows of one packed sequence, of which each query reads the
+//            first `lim` (its causal limit).  Tiles that reach past the wave's
+//            smallest limit (`wlim`) are masked by comparing key indexes with
+//            lim.  Tile addresses are 64-bit: a descriptor per tile whose range
+//            ends with the sequence, so rows behind it read as zeros.
+//   kPaged   the tiles from t0 on of a paged request, up to `keys` rows.  A DMA
+//            covers four 16-byte chunks of 16 rows, which never cross a page, with
+//            a descriptor of its own; in LDS, rows go by 16 and chunks of 256
+//            bytes, V's rows permuted within a chunk so that the transposing reads
+//            of four chunks touch every bank once.  Which keys from `wlim` on
+//            (the request's nodes) a query reads is p's to say (p.reads).
+enum Kind { kEqual, kPacked, kPaged };
+template <class Params, Kind KIND>
+struct Where {};
+// The request's table row and first tile; the pages of this wave's rows of the
+// next K tile and of the next V tile to ask for; V's second read base; the
+// query's row in the mask.
+template <class Params>
+struct Where<Params, kPaged> {
+  const int* table;
+  int t0, pgk, pgv;
+  u32 avh;
+  typename Params::Row row;
+};
+template <class Params, bool BF16, bool LAZY, bool SOQ, int HD, Kind KIND = kEqual>
+struct Pipe : Where<Params, KIND> {
   static_assert(HD == 64 || HD == 128, "head dim 64 or 128");
   static constexpr int kBN = 8192 / HD;        // keys per tile
   static constexpr int kNB = kBN / 32;         // 32-key score blocks per tile
@@ -182,7 +212,9 @@ struct Pipe {
   static constexpr int kRH = kBN / 64;         // 64-row halves of a chunk column (one DMA each)
   static constexpr int kDW = kNC * kRH / kWaves;  // DMAs per wave per operand and tile
   static constexpr int kPitchK = kBN * 16;     // bytes between K chunk columns
-  static constexpr int kPitchV = kBN * 16 + 64;  // bytes between V chunk columns (pad: distinct banks)
+  // Bytes between V chunk columns (pad: distinct banks).
+  static constexpr int kPitchV = kBN * 16 + (KIND == kPaged ? 0 : 64);
+  static constexpr int kGroup = kNC * 256;     // kPaged: 16 rows
   static constexpr int kTileK = kNC * kPitchK;  // one K tile in LDS
   static constexpr int kTileV = kNC * kPitchV;  // one V tile in LDS
   static constexpr int kLdsV = 2 * kTileK;     // V buffers after the two K buffers
@@ -205,7 +237,7 @@ struct Pipe {
   u32x4 kv[kNF];  // K_t (kv[kNB s + blk]: step s of 16 head-dim values, key block blk) or V_t (kv[kND t + d])
   f32x16 o[kND];  // O^T, head-dim block d
   float m, l, alpha;
-  // VAR only: first key's rows, keys of the sequence, limits, scratch for P.
+  // Not kEqual: first key's rows (kPaged: of the cache), keys, limits, scratch for P.
   const char *kp, *vp;
   int keys, lim, wlim;
   char* pscratch;
@@ -215,7 +247,7 @@ struct Pipe {
 
   // DMA q = kDW w + i of wave w covers chunk column q / kRH, rows 64 (q % kRH)
   // .. +63 of a tile: lane i fetches row 64 (q % kRH) + i.
-  // The rows of a tile that the sequence has (VAR).
+  // kPacked: the rows of a tile that the sequence has.
   G9_DEV rsrc_t tile_rows(const char* base, int tile, u32 ld) const {
     const int left = min(max(keys - tile * kBN, 0), kBN);
     const unsigned long long at = (unsigned long long)base + (unsigned long long)(u32)(tile * kBN) * ld;
@@ -224,38 +256,68 @@ struct Pipe {
     return make_rsrc(reinterpret_cast<const void*>((unsigned long long)hi << 32 | lo),
                      (u32)__builtin_amdgcn_readfirstlane((int)((u32)left * ld)));
   }
+  G9_DEV int first_tile() const {
+    if constexpr (KIND == kPaged) return this->t0;
+    return 0;
+  }
+  // The V rows 8 below those at a.
+  G9_DEV u32 second(u32 a) const {
+    if constexpr (KIND == kPaged) return a + (this->avh - av);
+    return a + 128;
+  }
+  // kPaged: this wave's 16 rows of a tile, and which of their DMAs are its.
+  G9_DEV int my_key(int tile) const { return (this->t0 + tile) * kBN + 16 * (wave * kDW / (kNC / 4)); }
+  G9_DEV int page_of(int tile) const {
+    const int k = my_key(tile);
+    return k < keys ? this->table[k >> p.shift] : -1;
+  }
+  G9_DEV void dma_paged(const char* base, int tile, int page, u32 lds, u32 voff, long long step, u32 ld) const {
+    const int k = my_key(tile), off = k & ((1 << p.shift) - 1);
+    const bool in = (u32)page < (u32)p.num_blocks;
+    const int rows = in ? min(max(keys - k, 0), 16) : 0;
+    const unsigned long long at = (unsigned long long)base + (in ? page : 0) * step + (unsigned long long)off * ld;
+    const u32 lo = (u32)__builtin_amdgcn_readfirstlane((int)at), hi = (u32)__builtin_amdgcn_readfirstlane((int)(at >> 32));
+    const rsrc_t r4 = make_rsrc(reinterpret_cast<const void*>((unsigned long long)hi << 32 | lo),
+                                (u32)__builtin_amdgcn_readfirstlane((int)((u32)rows * ld)));
+#pragma unroll
+    for (int i = 0; i < kDW; ++i) dma16_fresh(r4, lds + (kDW * wave + i) * 1024, voff, ((kDW * wave + i) % (kNC / 4)) * 64);
+  }
   G9_DEV void dma_k(int tile, int buf) {
-    if constexpr (VAR) {
+    if constexpr (KIND == kPaged) {
+      dma_paged(kp, tile, this->pgk, lds0 + buf * kTileK, voffk, p.k_b, p.k_t);
+    } else if constexpr (KIND == kPacked) {
       const rsrc_t r4 = tile_rows(kp, tile, p.ldk);
 #pragma unroll
       for (int i = 0; i < kDW; ++i) {
         const int q = kDW * wave + i, c = q / kRH, r = q % kRH;
-        dma16_untracked(r4, lds0 + buf * kTileK + c * kPitchK + r * 1024, voffk, 64 * r * p.ldk + c * 16);
+        dma16_fresh(r4, lds0 + buf * kTileK + c * kPitchK + r * 1024, voffk, 64 * r * p.ldk + c * 16);
       }
-      return;
-    }
+    } else {
 #pragma unroll
-    for (int i = 0; i < kDW; ++i) {
-      const int q = kDW * wave + i, c = q / kRH, r = q % kRH;
-      dma16_untracked(rk, lds0 + buf * kTileK + c * kPitchK + r * 1024, voffk,
-                      ((u32)tile * kBN + 64 * r) * p.ldk + c * 16);
+      for (int i = 0; i < kDW; ++i) {
+        const int q = kDW * wave + i, c = q / kRH, r = q % kRH;
+        dma16_untracked(rk, lds0 + buf * kTileK + c * kPitchK + r * 1024, voffk,
+                        ((u32)tile * kBN + 64 * r) * p.ldk + c * 16);
+      }
     }
   }
   G9_DEV void dma_v(int tile, int buf) {
-    if constexpr (VAR) {
+    if constexpr (KIND == kPaged) {
+      dma_paged(vp, tile, this->pgv, lds0 + kLdsV + buf * kTileV, voffv, p.v_b, p.v_t);
+    } else if constexpr (KIND == kPacked) {
       const rsrc_t r4 = tile_rows(vp, tile, p.ldv);
 #pragma unroll
       for (int i = 0; i < kDW; ++i) {
         const int q = kDW * wave + i, c = q / kRH, r = q % kRH;
-        dma16_untracked(r4, lds0 + kLdsV + buf * kTileV + c * kPitchV + r * 1024, voffv, 64 * r * p.ldv + c * 16);
+        dma16_fresh(r4, lds0 + kLdsV + buf * kTileV + c * kPitchV + r * 1024, voffv, 64 * r * p.ldv + c * 16);
       }
-      return;
-    }
+    } else {
 #pragma unroll
-    for (int i = 0; i < kDW; ++i) {
-      const int q = kDW * wave + i, c = q / kRH, r = q % kRH;
-      dma16_untracked(rv, lds0 + kLdsV + buf * kTileV + c * kPitchV + r * 1024, voffv,
-                      ((u32)tile * kBN + 64 * r) * p.ldv + c * 16);
+      for (int i = 0; i < kDW; ++i) {
+        const int q = kDW * wave + i, c = q / kRH, r = q % kRH;
+        dma16_untracked(rv, lds0 + kLdsV + buf * kTileV + c * kPitchV + r * 1024, voffv,
+                        ((u32)tile * kBN + 64 * r) * p.ldv + c * 16);
+      }
     }
   }
   template <int BUF>
@@ -264,7 +326,8 @@ struct Pipe {
     for (int s = 0; s < kNS; ++s)
 #pragma unroll
       for (int blk = 0; blk < kNB; ++blk)
-        kv[kNB * s + blk] = *(const G9_LDS u32x4*)(uintptr_t)(ak + BUF * kTileK + 2 * s * kPitchK + blk * 512);
+        kv[kNB * s + blk] = *(const G9_LDS u32x4*)(uintptr_t)(
+            KIND == kPaged ? ak + BUF * kTileK + 512 * s + 2 * blk * kGroup : ak + BUF * kTileK + 2 * s * kPitchK + blk * 512);
   }
   template <int BUF>
   G9_DEV void read_v() {
@@ -272,9 +335,9 @@ struct Pipe {
     for (int t = 0; t < kKS; ++t)
 #pragma unroll
       for (int d = 0; d < kND; ++d) {
-        const u32 a = av + BUF * kTileV + 4 * d * kPitchV + 256 * t;
+        const u32 a = KIND == kPaged ? av + BUF * kTileV + 1024 * d + t * kGroup : av + BUF * kTileV + 4 * d * kPitchV + 256 * t;
         const u32x2 lo = tr_read(a);
-        const u32x2 hi = tr_read(a + 128);
+        const u32x2 hi = tr_read(second(a));
         kv[kND * t + d] = u32x4{lo.x, lo.y, hi.x, hi.y};
       }
   }
@@ -315,19 +378,37 @@ struct Pipe {
       if (blk >= from) S.b[blk] = f32x16{} - __builtin_inff();
   }
 
-  // VAR: key 32 blk + 8 (i / 4) + 4 h + i % 4 of the tile scores -inf unless it
-  // is below the query's limit; rel = lim - first key of the tile - 4 h.
-  G9_DEV void mask_limit(Sc& S, int rel) const {
+  // Masked tiles: key 32 blk + 8 (i / 4) + 4 h + i % 4 of the tile scores -inf
+  // unless the query reads it.
+  G9_DEV void mask_tile(Sc& S, int tile) const {
+    const int h = (int)((threadIdx.x & 63) >> 5);
+    if constexpr (KIND == kPacked) {
+      const int rel = lim - tile * kBN - 4 * h;
 #pragma unroll
-    for (int blk = 0; blk < kNB; ++blk)
+      for (int blk = 0; blk < kNB; ++blk)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float x = S.b[blk][i];
-        S.b[blk][i] = 32 * blk + 8 * (i / 4) + i % 4 < rel ? x : -__builtin_inff();
+        for (int i = 0; i < 16; ++i) {
+          const float x = S.b[blk][i];
+          S.b[blk][i] = 32 * blk + 8 * (i / 4) + i % 4 < rel ? x : -__builtin_inff();
+        }
+    } else {
+#pragma unroll
+      for (int half = 0; half < kRH; ++half) {
+        const unsigned long long w = p.reads(this->row, (this->t0 + tile) * kBN + 64 * half, keys);
+#pragma unroll
+        for (int blk = 2 * half; blk < 2 * half + 2; ++blk) {
+          const u32 bits = (u32)(w >> (32 * (blk & 1))) >> (4 * h);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float x = S.b[blk][i];
+            S.b[blk][i] = bits >> (8 * (i / 4) + i % 4) & 1 ? x : -__builtin_inff();
+          }
+        }
       }
+    }
   }
-  G9_DEV bool masked(int tile) const { return (tile + 1) * kBN > wlim; }
-  // VAR, masked tiles: a weight of 0 does not keep an infinite or NaN value out
+  G9_DEV bool masked(int tile) const { return (first_tile() + tile + 1) * kBN > wlim; }
+  // Masked tiles: a weight of 0 does not keep an infinite or NaN value out
   // of the product.  Such values (rare: one packed maximum over V's registers
   // finds them) are taken out of the registers, and added on the vector unit to
   // the rows that may read their key.  V_tile is in buffer BUF and in kv, P_tile
@@ -355,26 +436,33 @@ struct Pipe {
       }
     // P in LDS: row of the query, column of the key.
     const int lane = threadIdx.x & 63, h = lane >> 5;
-    uint16_t* const row = reinterpret_cast<uint16_t*>(pscratch) + (lane & 31) * kBN;
+    uint16_t* const prow = reinterpret_cast<uint16_t*>(pscratch) + (lane & 31) * kBN;
 #pragma unroll
     for (int blk = 0; blk < kNB; ++blk)
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
         const u32 w = __float_as_uint(S.b[blk][8 * (i / 8) + (i % 8) / 2]);
-        *reinterpret_cast<u32*>(row + 32 * blk + 8 * (i / 4) + 4 * h + i % 4) = w;
+        *reinterpret_cast<u32*>(prow + 32 * blk + 8 * (i / 4) + 4 * h + i % 4) = w;
       }
     waitcnt<63, 0>();
-    const int mine = min(lim - tile * kBN, kBN), most = min(keys - tile * kBN, kBN);
+    const int first = (first_tile() + tile) * kBN, most = min(keys - first, kBN);
+    unsigned long long who = 0;
 #pragma unroll 1
     for (int key = 0; key < most; ++key) {
-      if (key >= mine) continue;
-      const float w = unpack2<BF16>(row[key]).x;
-      const u32 a = lds0 + kLdsV + BUF * kTileV + key * 16 + 8 * h;
+      if constexpr (KIND == kPaged) {
+        if (key % 64 == 0) who = p.reads(this->row, first + key, keys);
+        if (!((who >> (key & 63)) & 1)) continue;
+      } else {
+        if (first + key >= lim) continue;
+      }
+      const float w = unpack2<BF16>(prow[key]).x;
+      const u32 a = lds0 + kLdsV + BUF * kTileV + 8 * h + (KIND == kPaged ? (key >> 4) * kGroup : key * 16);
 #pragma unroll
       for (int d = 0; d < kND; ++d)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const u32x2 x = *(const G9_LDS u32x2*)(uintptr_t)(a + (4 * d + r) * kPitchV);
+          const u32x2 x = *(const G9_LDS u32x2*)(uintptr_t)(
+              a + (KIND == kPaged ? (4 * d + r) * 256 + ((key & 15) ^ (4 * r)) * 16 : (4 * d + r) * kPitchV));
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             u32 y = (e & 1 ? x[e / 2] >> 16 : x[e / 2]) & 0xffffu;
@@ -568,10 +656,10 @@ struct Pipe {
     if (j + 2 < nte) waitcnt<kDW, 15>();  // K_{j+2} landed (V_{j+1} may be in flight)
     if (j + 3 < nte) dma_k(j + 3, PAR ^ 1);
     if constexpr (NEXT) {
-      if constexpr (VAR) {
+      if constexpr (KIND != kEqual) {
         if (masked(j + 1)) {
           asm volatile("");
-          mask_limit(n, lim - (j + 1) * kBN - 4 * (int)((threadIdx.x & 63) >> 5));
+          mask_tile(n, j + 1);
         }
       } else if (j + 1 >= nfull) {  // past the end (a branch, not selects in every step)
         asm volatile("");
@@ -582,10 +670,8 @@ struct Pipe {
       pin(alpha);
     }
     waitcnt<63, 0>();
-    if constexpr (VAR)
-#ifndef NOGUARD
+    if constexpr (KIND != kEqual)
       if (masked(j)) guard_v<PAR>(c, j);
-#endif
     barrier();
     // D2(j)
     __builtin_amdgcn_s_setprio(0);
@@ -611,6 +697,10 @@ struct Pipe {
       rescale();
     }
     if (j + 2 < nte) dma_v(j + 2, PAR);
+    if constexpr (KIND == kPaged) {
+      this->pgv = this->pgk;  // tile j + 3's V is asked for next, tile j + 4's K
+      this->pgk = page_of(j + 4);
+    }
     waitcnt<63, 0>();
     barrier();
   }

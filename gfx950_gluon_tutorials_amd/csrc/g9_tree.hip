@@ -30,10 +30,7 @@ namespace tree {
 
 using namespace fa;
 
-constexpr int kWgs = 256;             // one workgroup per CU
-constexpr int kWavesWg = 4;
-constexpr int kWorkers = kWgs * kWavesWg;
-constexpr int kBlock = 32;            // query rows of a block
+constexpr int kWgs = 256;  // one workgroup per CU
 
 struct Params {
   const char* q;
@@ -45,7 +42,7 @@ struct Params {
   const int* lengths;
   const int* cu;
   const unsigned long long* mask;                  // or null: a chain
-  float* part;                                     // partial sums [2 kWorkers][32][D], then (m, l) pairs
+  float* part;                                     // sums [2 kWorkers][kBlock][D], then (m, l) pairs
   unsigned long long* first;                       // [B + 1]: first tile of each request on the line
   long long q_t, q_h, o_t, o_h;                    // token / head strides, bytes
   long long k_b, k_h, v_b, v_h;                    // block / head strides, bytes
@@ -54,35 +51,35 @@ struct Params {
   int num_blocks, width, shift, words;
   int B, T, HQ, HK, group;
   float scale_log2;
+
+  // A query row: its node (-1: no row), its request's context, its mask.
+  struct Row {
+    int node, context;
+    const unsigned long long* mask;
+  };
+  // Bit i: the row reads key k0 + i of `keys`.
+  G9_DEV unsigned long long reads(const Row& r, int k0, int keys) const {
+    const int n0 = max(k0 - r.context, -4096);  // key k0's node, negative in the context
+    unsigned long long w;
+    if (!mask) {
+      const int c = r.node + 1 - n0;  // keys up to the row's own
+      w = c >= 64 ? ~0ull : c <= 0 ? 0 : (1ull << c) - 1;
+    } else {
+      const int first = max(n0, 0) >> 6, sh = max(n0, 0) & 63;
+      const unsigned long long a = first < words ? r.mask[first] : 0, b = first + 1 < words ? r.mask[first + 1] : 0;
+      w = sh ? a >> sh | b << (64 - sh) : a;
+      if (n0 < 0) w = n0 <= -64 ? ~0ull : w << -n0 | ((1ull << -n0) - 1);
+    }
+    const int left = keys - k0;
+    if (left < 64) w &= left <= 0 ? 0 : (1ull << left) - 1;
+    return w;
+  }
 };
 
 // One request: its query rows, context, keys, blocks of query rows, tiles.
 struct Req {
   int q0, n, context, keys, blocks, tiles;
 };
-template <int HD>
-G9_DEV Req request(const Params& p, int b) {
-  Req r;
-  r.q0 = min(max(p.cu[b], 0), p.T);
-  r.n = min(max(p.cu[b + 1], r.q0), p.T) - r.q0;
-  r.context = max(p.lengths[b], 0);
-  r.keys = (int)min((long long)r.context + r.n, (long long)p.width << p.shift);
-  r.blocks = (int)(((long long)r.n * p.group + kBlock - 1) / (kBlock));
-  constexpr int kKeys = 4096 / HD;
-  r.tiles = max((r.keys + kKeys - 1) / kKeys, 1);
-  return r;
-}
-G9_DEV unsigned long long tiles_of(const Params& p, const Req& r) {
-  return (unsigned long long)r.blocks * (unsigned)p.HK * (unsigned)r.tiles;
-}
-// Worker w of W takes the tiles [w n / W, (w + 1) n / W) of a line of n; W is at
-// most n, so that no part in between is empty.
-G9_DEV unsigned workers(unsigned long long n) { return n < kWorkers ? (unsigned)n : kWorkers; }
-G9_DEV unsigned long long part_begin(unsigned w, unsigned long long n) { return w * n / workers(n); }
-G9_DEV unsigned worker_of(unsigned long long tile, unsigned long long n) {
-  return (unsigned)(((tile + 1) * workers(n) - 1) / n);
-}
-
 // A place on the line.
 struct Place {
   Req r;
@@ -99,10 +96,178 @@ G9_DEV V uniform(V x) {
     return (V)__builtin_amdgcn_readfirstlane((int)x);
   }
 }
+G9_DEV void make_uniform(Place& a) {
+  for (int* x : {&a.r.q0, &a.r.n, &a.r.context, &a.r.keys, &a.r.blocks, &a.r.tiles, &a.b, &a.hk, &a.block, &a.tile})
+    *x = uniform(*x);
+}
+
+// The line of tiles: KEYS keys a tile, blocks of BLOCK query rows, WORKERS parts.
+template <int KEYS, int BLOCK, int WORKERS>
+struct Line {
+  static constexpr int kKeys = KEYS, kBlock = BLOCK, kWorkers = WORKERS;
+
+  static G9_DEV Req request(const Params& p, int b) {
+    Req r;
+    r.q0 = min(max(p.cu[b], 0), p.T);
+    r.n = min(max(p.cu[b + 1], r.q0), p.T) - r.q0;
+    r.context = max(p.lengths[b], 0);
+    r.keys = (int)min((long long)r.context + r.n, (long long)p.width << p.shift);
+    r.blocks = (int)(((long long)r.n * p.group + kBlock - 1) / kBlock);
+    r.tiles = max((r.keys + kKeys - 1) / kKeys, 1);
+    return r;
+  }
+  static G9_DEV unsigned long long tiles_of(const Params& p, const Req& r) {
+    return (unsigned long long)r.blocks * (unsigned)p.HK * (unsigned)r.tiles;
+  }
+  // Worker w of W takes the tiles [w n / W, (w + 1) n / W) of a line of n; W is at
+  // most n, so that no part in between is empty.
+  static G9_DEV unsigned workers(unsigned long long n) { return n < kWorkers ? (unsigned)n : kWorkers; }
+  static G9_DEV unsigned long long part_begin(unsigned w, unsigned long long n) { return w * n / workers(n); }
+  static G9_DEV unsigned worker_of(unsigned long long tile, unsigned long long n) {
+    return (unsigned)(((tile + 1) * workers(n) - 1) / n);
+  }
+
+  // Where this worker's part begins, and its tiles.  The workgroup sums the
+  // requests' tiles into LDS (first[B + 1]); workgroup 0 leaves them in the
+  // workspace for the kernel that joins the parts.
+  template <int THREADS>
+  static G9_DEV int locate(const Params& p, char* smem, unsigned worker, bool publish, Place& at) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    unsigned long long* const first = reinterpret_cast<unsigned long long*>(smem);  // then the waves' sums
+    unsigned long long* const sums = first + p.B + 1;
+    const int run = (p.B + THREADS - 1) / THREADS;
+    const int b0 = min(tid * run, p.B), b1 = min(b0 + run, p.B);
+    unsigned long long mine = 0;
+    for (int b = b0; b < b1; ++b) mine += tiles_of(p, request(p, b));
+    unsigned long long before = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const unsigned long long x = __shfl_up(before, d, 64);
+      if (lane >= d) before += x;
+    }
+    if (lane == 63) sums[wave] = before;
+    __syncthreads();
+    before -= mine;
+    unsigned long long total = 0;
+    for (int w = 0; w < THREADS / 64; ++w) {
+      if (w < wave) before += sums[w];
+      total += sums[w];
+    }
+    for (int b = b0; b < b1; ++b) {
+      first[b] = before;
+      if (publish) p.first[b] = before;
+      before += tiles_of(p, request(p, b));
+    }
+    if (tid == 0) {
+      first[p.B] = total;
+      if (publish) p.first[p.B] = total;
+    }
+    __syncthreads();
+    total = uniform(total);
+    int count = 0;
+    if (worker < workers(total)) {
+      const unsigned long long begin = uniform(part_begin(worker, total));
+      count = uniform((int)(part_begin(worker + 1, total) - begin));
+      // The last request that begins at or before the part (empty ones begin
+      // where the next one does).
+      int lo = 0, hi = p.B;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first[mid] <= begin)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      at.b = uniform(lo);
+      at.r = request(p, at.b);
+      const unsigned long long in = uniform(begin - first[lo]);
+      const unsigned long long unit = in / (unsigned)at.r.tiles;
+      at.tile = (int)(in - unit * (unsigned)at.r.tiles);
+      at.hk = (int)(unit / (unsigned)at.r.blocks);
+      at.block = (int)(unit - (unsigned long long)at.hk * at.r.blocks);
+      make_uniform(at);
+    }
+    __syncthreads();  // first[] is read: what comes next takes its place
+    return count;
+  }
+  // The first tile of the block behind `a`'s (there is one).
+  static G9_DEV Place next_block(const Params& p, const Place& a) {
+    Place n = a;
+    n.tile = 0;
+    if (++n.block < n.r.blocks) return n;
+    n.block = 0;
+    if (++n.hk < p.HK) return n;
+    n.hk = 0;
+    do {
+      n.b = min(n.b + 1, p.B - 1);
+      n.r = request(p, n.b);
+    } while (n.r.blocks == 0 && n.b < p.B - 1);
+    make_uniform(n);
+    return n;
+  }
+};
+// A wave's own tiles of up to 8 KB, or a workgroup's of 16 KB.
+template <int HD>
+using Narrow = Line<4096 / HD, 32, 4 * kWgs>;
+template <int HD>
+using Wide = Line<8192 / HD, 256, kWgs>;
+
+// A lane's query row of the block.
+template <class L>
+G9_DEV Params::Row row_of(const Params& p, const Place& at, int row) {
+  const int nd = (at.block * L::kBlock + row) / p.group;
+  const bool in = nd < at.r.n;
+  return {in ? nd : -1, at.r.context, p.mask ? p.mask + (long long)(at.r.q0 + (in ? nd : 0)) * p.words : nullptr};
+}
+template <class L>
+G9_DEV const char* query_of(const Params& p, const Place& at, int row, int node) {
+  const int hd = at.block * L::kBlock + row - max(node, 0) * p.group;
+  return p.q + (long long)(at.r.q0 + max(node, 0)) * p.q_t + (long long)(at.hk * p.group + (node < 0 ? 0 : hd)) * p.q_h;
+}
+// The row's results, or its sum to slot `slot` of the workspace.  o, m, l as the
+// 32x32 layout leaves them: lane half h has the values 8 r + 4 h + 0..3 of every
+// 32, l is its half of the weight.
+template <bool BF16, int HD, class L>
+G9_DEV void finish(const Params& p, const Place& at, int slot, int row, int node, const f32x16 (&o)[HD / 32], float m,
+                   float l) {
+  const int h = (threadIdx.x & 63) >> 5;
+  const float lt = xhalf(l, [](float x, float y) { return x + y; });
+  if (node < 0) return;
+  if (slot >= 0) {
+    float* const sum = p.part + ((size_t)slot * L::kBlock + row) * HD;
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *reinterpret_cast<f32x4*>(sum + 32 * d + 8 * r + 4 * h) =
+            f32x4{o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]};
+    if (h == 0) {
+      float* const ml = p.part + (size_t)2 * L::kWorkers * L::kBlock * HD + ((size_t)slot * L::kBlock + row) * 2;
+      ml[0] = m, ml[1] = lt;
+    }
+    return;
+  }
+  const int hq = at.hk * p.group + at.block * L::kBlock + row - node * p.group;
+  const long long tok = at.r.q0 + node;
+  // By its bits: comparisons here may take NaN for a number.
+  const bool none = (__float_as_uint(lt) << 1) == 0;
+  const float inv = none ? 0.f : 1.f / lt;
+  char* const orow = p.o + tok * p.o_t + hq * p.o_h;
+#pragma unroll
+  for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      *reinterpret_cast<u32x2*>(orow + (32 * d + 8 * r + 4 * h) * 2) =
+          u32x2{pack2<BF16>(o[d][4 * r] * inv, o[d][4 * r + 1] * inv),
+                pack2<BF16>(o[d][4 * r + 2] * inv, o[d][4 * r + 3] * inv)};
+  if (p.lse && h == 0) p.lse[(long long)hq * p.T + tok] = none ? -__builtin_inff() : (m + __builtin_log2f(lt)) * kLn2;
+}
 
 template <bool BF16, int HD>
 struct Wave {
-  static constexpr int kKeys = 4096 / HD;          // keys per tile
+  using L = Narrow<HD>;
+  static constexpr int kKeys = L::kKeys;           // keys per tile
+  static constexpr int kBlock = L::kBlock;
   static constexpr int kNB = kKeys / 32;           // 32-key score blocks
   static constexpr int kNS = HD / 16;              // QK steps of 16 head-dim values
   static constexpr int kKS = kKeys / 16;           // PV steps of 16 keys
@@ -124,7 +289,7 @@ struct Wave {
   u32x4 qf[kNS];
   f32x16 o[kND];
   float m, l;
-  int node;          // the node of this lane's query row, -1 where there is none
+  Params::Row row;   // this lane's query
 
   G9_DEV explicit Wave(const Params& pp) : p(pp) {}
 
@@ -175,18 +340,15 @@ struct Wave {
 #pragma unroll
       for (int jj = 0; jj < 16 / kRows; ++jj) {
         const int j = i * (16 / kRows) + jj;
-        dma16_untracked(rk, lds + stage * kStage + j * 1024, voffk[j & (HD == 128 ? 3 : 1)], jj * kRows * p.k_t);
-        dma16_untracked(rv, lds + stage * kStage + kV + j * 1024, voffv[0], jj * kRows * p.v_t);
+        dma16_fresh(rk, lds + stage * kStage + j * 1024, voffk[j & (HD == 128 ? 3 : 1)], jj * kRows * p.k_t);
+        dma16_fresh(rv, lds + stage * kStage + kV + j * 1024, voffv[0], jj * kRows * p.v_t);
       }
     }
   }
 
   G9_DEV void begin(const Place& at) {
-    const int row = at.block * kBlock + col;
-    const int nd = row / p.group, hd = row - nd * p.group;
-    const bool in = nd < at.r.n;
-    node = in ? nd : -1;
-    const char* qrow = p.q + (long long)(at.r.q0 + (in ? nd : 0)) * p.q_t + (long long)(at.hk * p.group + (in ? hd : 0)) * p.q_h;
+    row = row_of<L>(p, at, col);
+    const char* const qrow = query_of<L>(p, at, col, row.node);
 #pragma unroll
     for (int s = 0; s < kNS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(qrow + (16 * s + 8 * h) * 2);
     // Finite, so that a row that has read nothing yet has weights 2^(-inf - m) =
@@ -197,26 +359,6 @@ struct Wave {
     // Waited for here: the compiler does not count the DMAs in flight, and a wait
     // of its own at the first use would be one in every tile.
     waitcnt<0, 0>();
-  }
-
-  // Bit i: the row reads key i of the tile.
-  G9_DEV unsigned long long reads(const Place& at) const {
-    const int k0 = at.tile * kKeys;
-    const int n0 = max(k0 - at.r.context, -4096);  // the tile's first node, negative in the context
-    unsigned long long w;
-    if (!p.mask) {
-      const int c = node + 1 - n0;  // keys up to the row's own
-      w = c >= 64 ? ~0ull : c <= 0 ? 0 : (1ull << c) - 1;
-    } else {
-      const unsigned long long* row = p.mask + (long long)(at.r.q0 + max(node, 0)) * p.words;
-      const int first = max(n0, 0) >> 6, sh = max(n0, 0) & 63;
-      const unsigned long long a = first < p.words ? row[first] : 0, b = first + 1 < p.words ? row[first + 1] : 0;
-      w = sh ? a >> sh | b << (64 - sh) : a;
-      if (n0 < 0) w = n0 <= -64 ? ~0ull : w << -n0 | ((1ull << -n0) - 1);
-    }
-    const int left = at.r.keys - k0;
-    if (left < 64) w &= left <= 0 ? 0 : (1ull << left) - 1;
-    return w;
   }
 
   template <bool TAIL>
@@ -231,7 +373,7 @@ struct Wave {
         sc[b] = mfma<BF16>(kf, qf[s], s ? sc[b] : f32x16{});
       }
     if constexpr (TAIL) {
-      const unsigned long long w = reads(at);
+      const unsigned long long w = p.reads(row, at.tile * kKeys, at.r.keys);
 #pragma unroll
       for (int b = 0; b < kNB; ++b) {
         const u32 bits = (u32)(w >> (32 * b)) >> (4 * h);
@@ -313,18 +455,18 @@ struct Wave {
           vf[k][d][e] = x;
         }
     // P in LDS: row of the query, column of the key.
-    uint16_t* const row = reinterpret_cast<uint16_t*>(scratch) + col * kKeys;
+    uint16_t* const prow = reinterpret_cast<uint16_t*>(scratch) + col * kKeys;
 #pragma unroll
     for (int k = 0; k < kKS; ++k)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        *reinterpret_cast<u32*>(row + 16 * k + 8 * (e >> 1) + 4 * h + 2 * (e & 1)) = pf[k][e];
-    const unsigned long long w = reads(at);
+        *reinterpret_cast<u32*>(prow + 16 * k + 8 * (e >> 1) + 4 * h + 2 * (e & 1)) = pf[k][e];
+    const unsigned long long w = p.reads(row, at.tile * kKeys, at.r.keys);
     waitcnt<63, 0>();
 #pragma unroll 1
     for (int key = 0; key < kKeys; ++key) {
       if (!((w >> key) & 1)) continue;
-      const float wt = unpack2<BF16>(row[key]).x;
+      const float wt = unpack2<BF16>(prow[key]).x;
       const u32 vr = lds + stage * kStage + kV + key * kRow;
 #pragma unroll
       for (int d = 0; d < kND; ++d)
@@ -341,138 +483,28 @@ struct Wave {
         }
     }
   }
-
-  // The rows' results, or their sums to slot `slot` of the workspace.
-  G9_DEV void end(const Place& at, int slot) {
-    const float lt = xhalf(l, [](float x, float y) { return x + y; });
-    if (node < 0) return;
-    if (slot >= 0) {
-      float* const sum = p.part + ((size_t)slot * kBlock + col) * HD;
-#pragma unroll
-      for (int d = 0; d < kND; ++d)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          *reinterpret_cast<f32x4*>(sum + 32 * d + 8 * r + 4 * h) =
-              f32x4{o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]};
-      if (h == 0) {
-        float* const ml = p.part + (size_t)2 * kWorkers * kBlock * HD + ((size_t)slot * kBlock + col) * 2;
-        ml[0] = m, ml[1] = lt;
-      }
-      return;
-    }
-    const int hq = at.hk * p.group + at.block * kBlock + col - node * p.group;
-    const long long tok = at.r.q0 + node;
-    // By its bits: comparisons here may take NaN for a number.
-    const bool none = (__float_as_uint(lt) << 1) == 0;
-    const float inv = none ? 0.f : 1.f / lt;
-    char* const orow = p.o + tok * p.o_t + hq * p.o_h;
-#pragma unroll
-    for (int d = 0; d < kND; ++d)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        *reinterpret_cast<u32x2*>(orow + (32 * d + 8 * r + 4 * h) * 2) =
-            u32x2{pack2<BF16>(o[d][4 * r] * inv, o[d][4 * r + 1] * inv),
-                  pack2<BF16>(o[d][4 * r + 2] * inv, o[d][4 * r + 3] * inv)};
-    if (p.lse && h == 0) p.lse[(long long)hq * p.T + tok] = none ? -__builtin_inff() : (m + __builtin_log2f(lt)) * kLn2;
-  }
 };
 
-template <class X>
-G9_DEV void scalar(X& r) {
-  r.r.q0 = uniform(r.r.q0), r.r.n = uniform(r.r.n), r.r.context = uniform(r.r.context), r.r.keys = uniform(r.r.keys);
-  r.r.blocks = uniform(r.r.blocks), r.r.tiles = uniform(r.r.tiles);
-  r.b = uniform(r.b), r.hk = uniform(r.hk), r.block = uniform(r.block), r.tile = uniform(r.tile);
-}
+// Consecutive workgroups go round the 8 XCDs; consecutive parts of the line stay
+// on one, whose L2 then serves the blocks of rows that share keys.
+G9_DEV unsigned my_part() { return (blockIdx.x & 7) * (kWgs / 8) + (blockIdx.x >> 3); }
 
 template <bool BF16, int HD>
-G9_DEV void run(const Params& p, char* smem) {
+G9_DEV void narrow(const Params& p, char* smem) {
   using W = Wave<BF16, HD>;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // Consecutive workgroups go round the 8 XCDs; consecutive parts of the line
-  // stay on one, whose L2 then serves the rows' blocks that share keys.
-  const unsigned wg = (blockIdx.x & 7) * (kWgs / 8) + (blockIdx.x >> 3);
-  const unsigned worker = wg * kWavesWg + wave;
-
-  // The requests' first tiles (in LDS, and from one workgroup in the workspace
-  // for the kernel that joins the parts).
-  unsigned long long* const first = reinterpret_cast<unsigned long long*>(smem);  // [B + 1], then the waves' sums
-  constexpr int kThreadsWg = 64 * kWavesWg;
-  unsigned long long* const sums = first + p.B + 1;
-  const int run_len = (p.B + kThreadsWg - 1) / kThreadsWg;
-  const int b0 = min(tid * run_len, p.B), b1 = min(b0 + run_len, p.B);
-  unsigned long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += tiles_of(p, request<HD>(p, b));
-  unsigned long long before = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const unsigned long long x = __shfl_up(before, d, 64);
-    if (lane >= d) before += x;
-  }
-  if (lane == 63) sums[wave] = before;
-  __syncthreads();
-  before -= mine;
-  unsigned long long total = 0;
-  for (int w = 0; w < kWavesWg; ++w) {
-    if (w < wave) before += sums[w];
-    total += sums[w];
-  }
-  for (int b = b0; b < b1; ++b) {
-    first[b] = before;
-    if (wg == 0) p.first[b] = before;
-    before += tiles_of(p, request<HD>(p, b));
-  }
-  if (tid == 0) {
-    first[p.B] = total;
-    if (wg == 0) p.first[p.B] = total;
-  }
-  __syncthreads();
-  total = uniform(total);
-  unsigned long long begin = 0;
-  int count = 0;
-  if (worker < workers(total)) {
-    begin = uniform(part_begin(worker, total));
-    count = uniform((int)(part_begin(worker + 1, total) - begin));
-  }
+  using L = Narrow<HD>;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned worker = my_part() * 4 + wave;
   Place cur;
-  if (count > 0) {
-    // The last request that begins at or before the part (empty ones begin
-    // where the next one does).
-    int lo = 0, hi = p.B;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (first[mid] <= begin)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    cur.b = uniform(lo);
-    cur.r = request<HD>(p, cur.b);
-    const unsigned long long in = uniform(begin - first[lo]);
-    const unsigned long long unit = in / (unsigned)cur.r.tiles;
-    cur.tile = (int)(in - unit * (unsigned)cur.r.tiles);
-    cur.hk = (int)(unit / (unsigned)cur.r.blocks);
-    cur.block = (int)(unit - (unsigned long long)cur.hk * cur.r.blocks);
-    scalar(cur);
-  }
-  __syncthreads();  // first[] is read: the stages take its place
+  const int count = L::template locate<256>(p, smem, worker, my_part() == 0, cur);
   if (count <= 0) return;
 
   W w(p);
   w.init(smem, wave);
   const auto next = [&](const Place& a) {
+    if (a.tile + 1 == a.r.tiles) return L::next_block(p, a);
     Place n = a;
-    if (++n.tile < n.r.tiles) return n;
-    n.tile = 0;
-    if (++n.block < n.r.blocks) return n;
-    n.block = 0;
-    if (++n.hk < p.HK) return n;
-    n.hk = 0;
-    do {
-      n.b = min(n.b + 1, p.B - 1);
-      n.r = request<HD>(p, n.b);
-    } while (n.r.blocks == 0 && n.b < p.B - 1);
-    scalar(n);
+    ++n.tile;
     return n;
   };
   int pg[W::kPieces];
@@ -512,7 +544,8 @@ G9_DEV void run(const Params& p, char* smem) {
     if (last || i + 1 == count) {
       // Slot 0 of the worker: a block that another worker began; slot 1: one
       // that the next worker goes on with.
-      w.end(cur, last && from_start ? -1 : (int)(2 * worker + (from_start ? 1 : 0)));
+      finish<BF16, HD, L>(p, cur, last && from_start ? -1 : (int)(2 * worker + (from_start ? 1 : 0)), w.col, w.row.node,
+                          w.o, w.m, w.l);
       from_start = true;
     }
     cur = nxt;
@@ -520,11 +553,107 @@ G9_DEV void run(const Params& p, char* smem) {
   }
 }
 
+// Many query rows: a workgroup's 8 waves, 32 rows each, share every tile, on the
+// pipeline of g9_fmha_pipe.hpp.
+template <bool BF16, int HD>
+struct WidePipe {
+  using T = Pipe<Params, BF16, true, false, HD, kPaged>;
+  static constexpr int kLds = T::kLdsBytes + kWaves * T::kScratchBytes;
+};
+
+template <bool BF16, int HD>
+G9_DEV void wide(const Params& p, char* smem) {
+  using L = Wide<HD>;
+  using PipeT = typename WidePipe<BF16, HD>::T;
+  static_assert(PipeT::kBN == L::kKeys && kBlockM == L::kBlock);
+  const unsigned worker = my_part();
+  Place cur;
+  int count = L::template locate<kThreads>(p, smem, worker, worker == 0, cur);
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
+  PipeT P(p);
+  P.wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  P.lds0 = (u32)(uintptr_t)to_lds(smem);
+  P.pscratch = smem + PipeT::kLdsBytes + P.wave * PipeT::kScratchBytes;
+  P.sc = p.scale_log2;
+  // A DMA's lane i fetches chunk i / 16 of row i % 16 (V: of row i % 16 ^ 4 (chunk
+  // % 4), see Kind).
+  P.voffk = (u32)(lane & 15) * p.k_t + (lane >> 4) * 16;
+  P.voffv = (u32)((lane & 15) ^ (4 * (lane >> 4))) * p.v_t + (lane >> 4) * 16;
+  P.ak = P.lds0 + ((lane & 31) >> 4) * PipeT::kGroup + h * 256 + (lane & 15) * 16;
+  {
+    const int c = 2 * (lane >> 4 & 1) + ((lane & 3) >> 1);  // chunk, of every four
+    P.av = P.lds0 + PipeT::kLdsV + c * 256 + ((4 * h + ((lane & 15) >> 2)) ^ (4 * c)) * 16 + 8 * (lane & 1);
+    P.avh = P.av ^ 128;
+  }
+  const bool lag = P.wave >= 4;
+  const int row = P.wave * 32 + (lane & 31);
+  while (count > 0) {
+    const int seg = min(count, cur.r.tiles - cur.tile);
+    P.keys = min(cur.r.keys, (cur.tile + seg) * PipeT::kBN);
+    P.wlim = min(cur.r.context, P.keys);
+    P.t0 = cur.tile;
+    P.table = p.table + cur.b * p.table_stride;
+    P.row = row_of<L>(p, cur, row);
+    P.nte = max((seg + 1) & ~1, 2);
+    P.kp = p.kc + cur.hk * p.k_h;
+    P.vp = p.vc + cur.hk * p.v_h;
+    const int nte = P.nte;
+    const char* const qrow = query_of<L>(p, cur, row, P.row.node);
+#pragma unroll
+    for (int s = 0; s < PipeT::kNS; ++s) P.qf[s] = *reinterpret_cast<const u32x4*>(qrow + (16 * s + 8 * h) * 2);
+    // The prologue of g9_fmha.hip's kernel.
+    P.pgk = P.pgv = P.page_of(0);
+    P.dma_k(0, 0);
+    P.dma_v(0, 0);
+    P.pgk = P.page_of(1);
+    P.dma_k(1, 1);
+#pragma unroll
+    for (int d = 0; d < PipeT::kND; ++d) P.o[d] = f32x16{};
+    P.m = -3.0e38f;
+    P.l = 0.f;
+    P.pgv = P.pgk;
+    P.pgk = P.page_of(2);
+    waitcnt<0, 0>();
+    barrier();
+    P.template read_k<0>();
+    typename PipeT::Sc sa, sb;
+    P.qk(sa);
+    waitcnt<63, 0>();
+    barrier();  // every wave has read K_0: its buffer takes K_2
+    if (nte > 2) P.dma_k(2, 0);
+    P.dma_v(1, 1);
+    P.pgv = P.pgk;
+    P.pgk = P.page_of(3);
+    if (P.masked(0)) P.mask_tile(sa, 0);
+    P.vec0(sa);
+    P.vec1(sa);
+    P.l *= P.alpha;
+    P.template read_k<1>();
+    waitcnt<63, 0>();
+    if (lag) barrier();
+    int j = 0;
+    for (; j + 2 < nte; j += 2) {
+      P.template step<0, true>(j, sa, sb);
+      P.template step<1, true>(j + 1, sb, sa);
+    }
+    P.template step<0, true>(j, sa, sb);
+    P.template step<1, false>(j + 1, sb, sa);
+    __builtin_amdgcn_s_setprio(0);
+    if (!lag) barrier();
+    const bool from_start = cur.tile == 0, last = cur.tile + seg == cur.r.tiles;
+    finish<BF16, HD, L>(p, cur, last && from_start ? -1 : (int)(2 * worker + (from_start ? 1 : 0)), row, P.row.node, P.o,
+                        P.m, P.l);
+    count -= seg;
+    if (count > 0) cur = L::next_block(p, cur);
+    barrier();  // the stages are read: the next block's tiles take them
+  }
+}
+
 // Joins the parts of query row (token t, head hq): with m the largest of their
 // maxima, sum of 2^(m_i - m) O_i over the sum of 2^(m_i - m) l_i, in the order of
 // the keys.  One workgroup per row; its threads hold HD / 4 columns by kLanes
 // parts.
-template <bool BF16, int HD>
+template <bool BF16, int HD, class L>
 G9_DEV void join(const Params& p, float* lds) {
   constexpr int kCols = HD / 4, kParts = 256 / kCols;
   const int t = blockIdx.x / p.HQ, hq = blockIdx.x - t * p.HQ;
@@ -539,20 +668,20 @@ G9_DEV void join(const Params& p, float* lds) {
       hi = mid;
   }
   if (lo >= p.B) return;
-  const Req r = request<HD>(p, lo);
+  const Req r = L::request(p, lo);
   const int nd = t - r.q0, hk = hq / p.group;
   if (nd < 0 || nd >= r.n) return;
   const int row = nd * p.group + hq - hk * p.group;
-  const int block = row / (kBlock), in = row - block * kBlock;
+  const int block = row / L::kBlock, in = row - block * L::kBlock;
   const unsigned long long total = p.first[p.B];
   const unsigned long long u0 = p.first[lo] + ((unsigned long long)hk * r.blocks + block) * r.tiles;
-  const unsigned w0 = worker_of(u0, total), w1 = worker_of(u0 + r.tiles - 1, total);
-  if (w0 == w1) return;  // finished by its wave
-  const float* const ml = p.part + (size_t)2 * kWorkers * kBlock * HD;
+  const unsigned w0 = L::worker_of(u0, total), w1 = L::worker_of(u0 + r.tiles - 1, total);
+  if (w0 == w1) return;  // finished by its worker
+  const float* const ml = p.part + (size_t)2 * L::kWorkers * L::kBlock * HD;
   // Worker w0 has it in slot 1 unless it began the block before its part.
   const auto at = [&](unsigned w) {
-    const unsigned slot = 2 * w + (w == w0 && part_begin(w0, total) <= u0 ? 1 : 0);
-    return (size_t)slot * kBlock + in;
+    const unsigned slot = 2 * w + (w == w0 && L::part_begin(w0, total) <= u0 ? 1 : 0);
+    return (size_t)slot * L::kBlock + in;
   };
   const unsigned n = w1 - w0 + 1;
   float top = -3.0e38f;
@@ -597,15 +726,24 @@ G9_DEV void join(const Params& p, float* lds) {
 using namespace g9;
 using namespace g9::host;
 
-#define G9_TREE_KERNEL(NAME, BF16, HD)                                                                    \
-  extern "C" __global__ __launch_bounds__(64 * tree::kWavesWg) __attribute__((amdgpu_waves_per_eu(1, 1))) void \
+#define G9_TREE_KERNEL(NAME, BF16, HD)                                                                        \
+  extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void                \
   g9_tree_##NAME(tree::Params p) {                                                                            \
-    __shared__ __attribute__((aligned(1024))) char smem[tree::kWavesWg * tree::Wave<BF16, HD>::kWaveLds];  \
-    tree::run<BF16, HD>(p, smem);                                                                         \
+    __shared__ __attribute__((aligned(1024))) char smem[4 * tree::Wave<BF16, HD>::kWaveLds];                   \
+    tree::narrow<BF16, HD>(p, smem);                                                                          \
+  }                                                                                                           \
+  extern "C" __global__ __launch_bounds__(fa::kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void       \
+  g9_tree_wide_##NAME(tree::Params p) {                                                                       \
+    __shared__ __attribute__((aligned(1024))) char smem[tree::WidePipe<BF16, HD>::kLds];                       \
+    tree::wide<BF16, HD>(p, smem);                                                                            \
   }                                                                                                           \
   extern "C" __global__ __launch_bounds__(256) void g9_tree_join_##NAME(tree::Params p) {                     \
     __shared__ float lds[256 * 5];                                                                            \
-    tree::join<BF16, HD>(p, lds);                                                                         \
+    tree::join<BF16, HD, tree::Narrow<HD>>(p, lds);                                                           \
+  }                                                                                                           \
+  extern "C" __global__ __launch_bounds__(256) void g9_tree_join_wide_##NAME(tree::Params p) {                \
+    __shared__ float lds[256 * 5];                                                                            \
+    tree::join<BF16, HD, tree::Wide<HD>>(p, lds);                                                             \
   }
 G9_TREE_KERNEL(bf16, true, 128)
 G9_TREE_KERNEL(f16, false, 128)
@@ -614,20 +752,24 @@ G9_TREE_KERNEL(f16_d64, false, 64)
 
 namespace {
 
-size_t part_floats(int64_t D) { return (size_t)2 * tree::kWorkers * tree::kBlock * (D + 2); }
+// Whether the workgroup's form takes a batch: by the rows that its requests
+// bring on average to one K/V head.
+bool wide_form(int64_t B, int64_t T, int64_t group) { return (T + B - 1) / B * group > 64; }
+// Both forms keep 2 x 1024 x 32 or 2 x 256 x 256 rows' sums.
+size_t part_floats(bool wide, int64_t D) { return (size_t)2 * (wide ? 256 * 256 : 1024 * 32) * (D + 2); }
 
 #define G9_TREE_FNS(WHAT)                                                                       \
   {{reinterpret_cast<const void*>(WHAT##f16), reinterpret_cast<const void*>(WHAT##bf16)},       \
    {reinterpret_cast<const void*>(WHAT##f16_d64), reinterpret_cast<const void*>(WHAT##bf16_d64)}}
-// [head dim 64][bf16]
-const void* const kRun[2][2] = G9_TREE_FNS(g9_tree_);
-const void* const kJoin[2][2] = G9_TREE_FNS(g9_tree_join_);
+// [wide][head dim 64][bf16]
+const void* const kRun[2][2][2] = {G9_TREE_FNS(g9_tree_), G9_TREE_FNS(g9_tree_wide_)};
+const void* const kJoin[2][2][2] = {G9_TREE_FNS(g9_tree_join_), G9_TREE_FNS(g9_tree_join_wide_)};
 
 }  // namespace
 
 extern "C" size_t g9_tree_workspace_size(int64_t B, int64_t T, int64_t HQ, int64_t HK, int64_t D) {
   if (B <= 0 || T <= 0 || HQ <= 0 || HK <= 0 || HQ % HK || D <= 0) return 0;
-  return part_floats(D) * 4 + (size_t)(B + 1) * 8;
+  return part_floats(wide_form(B, T, HQ / HK), D) * 4 + (size_t)(B + 1) * 8;
 }
 
 extern "C" int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cache, void* o, float* lse,
@@ -658,7 +800,8 @@ extern "C" int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cac
       ((uintptr_t)tree_mask & 7))
     return G9_ERR_LAYOUT;
   const int64_t group = HQ / HK;
-  const size_t floats = part_floats(D);
+  const bool wide = wide_form(B, T, group);
+  const size_t floats = part_floats(wide, D);
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < floats * 4 + (size_t)(B + 1) * 8)
     return G9_ERR_WORKSPACE;
   tree::Params p{};
@@ -682,8 +825,9 @@ extern "C" int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cac
   p.scale_log2 = sm_scale * fa::kLog2e;
   void* args[] = {&p};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (hipLaunchKernel(kRun[D == 64][dtype == G9_BF16], dim3(tree::kWgs), dim3(64 * tree::kWavesWg), args, 0, st) !=
-      hipSuccess)
+  if (hipLaunchKernel(kRun[wide][D == 64][dtype == G9_BF16], dim3(tree::kWgs), dim3(wide ? fa::kThreads : 256), args, 0,
+                      st) != hipSuccess)
     return G9_ERR_HIP;
-  return launched(hipLaunchKernel(kJoin[D == 64][dtype == G9_BF16], dim3((unsigned)(T * HQ)), dim3(256), args, 0, st));
+  return launched(hipLaunchKernel(kJoin[wide][D == 64][dtype == G9_BF16], dim3((unsigned)(T * HQ)), dim3(256), args, 0,
+                                  st));
 }

@@ -151,7 +151,7 @@ G9_DEV bool find_tile(const VarParams& p, int rank, int* lds, Tile& t) {
 
 template <bool BF16, int HD>
 struct VarPipe {
-  using T = Pipe<VarParams, BF16, true, false, HD, true>;
+  using T = Pipe<VarParams, BF16, true, false, HD, kPacked>;
   static constexpr int kLds = T::kLdsBytes + kWaves * T::kScratchBytes;
 };
 
@@ -224,7 +224,7 @@ G9_DEV void varlen_fwd(const VarParams& p, char* smem) {
   barrier();  // every wave has read K_0: its buffer takes K_2
   if (nte > 2) P.dma_k(2, 0);
   P.dma_v(1, 1);
-  if (P.masked(0)) P.mask_limit(sa, P.lim - 4 * h);
+  if (P.masked(0)) P.mask_tile(sa, 0);
   P.vec0(sa);
   P.vec1(sa);
   P.l *= P.alpha;
