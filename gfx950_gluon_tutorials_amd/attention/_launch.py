@@ -71,10 +71,13 @@ def ptr(t):
     return t.data_ptr() if t is not None else None
 
 
+def array(*values):
+    return (_lib.ctypes.c_int64 * len(values))(*values)
+
+
 def strides(t):
     """Element strides but the last dimension's."""
-    s = t.stride()
-    return (_lib.ctypes.c_int64 * (len(s) - 1))(*s[:-1])
+    return array(*t.stride()[:-1])
 
 
 def gpu_of(first, *others) -> torch.device:
@@ -125,8 +128,31 @@ def lse_fits(lse, HQ, T) -> None:
 
 
 def forward_only(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise ValueError("forward only: call it under torch.no_grad(), or detach the tensors that require a gradient")
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("forward only: call it under torch.no_grad(), or detach the tensors that require a gradient")
+
+
+# What a call's arguments are but for their addresses and contents, to the
+# arguments of the C call that follow from it: a call of the same kind as an
+# earlier one is not checked again (half of its host time otherwise).
+_plans: dict = {}
+
+
+def sig(t):
+    return (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def planned(key):
+    return _plans.get(key)
+
+
+def keep(key, dev, plan):
+    if dev.type == "cuda":
+        if len(_plans) >= 4096:
+            _plans.clear()
+        _plans[key] = plan
+    return plan
 
 
 def call(entry: str, dev: torch.device, *args) -> None:

@@ -17,7 +17,7 @@ import torch
 
 from .. import _lib
 from . import _launch
-from ._launch import ptr, strides
+from ._launch import ptr, sig, strides
 
 MAX_REQUESTS = 4096  # of one assign_slots call (G9_SLOTS_MAX_REQUESTS)
 
@@ -47,6 +47,22 @@ def assign_slots(lengths: torch.Tensor, counts: torch.Tensor, block_table: torch
     slot -1 and position 0.  A token for which the free list or the table's width
     does not reach gets slot -1 (``taken`` above what the list holds says so).
     At most ``MAX_REQUESTS`` requests."""
+    key = ("slots", block_size, num_tokens, sig(lengths), sig(counts), sig(block_table), sig(free_blocks),
+           free_start is not None and sig(free_start))
+    dev, B, args = _launch.planned(key) or _plan_slots(key, lengths, counts, block_table, free_blocks, block_size,
+                                                       num_tokens, free_start)
+    longs = torch.empty((2, num_tokens), dtype=torch.int64, device=dev)
+    ints = torch.empty(B + 2, dtype=torch.int32, device=dev)
+    slots, positions = longs.unbind(0)
+    cu, taken = ints.split_with_sizes((B + 1, 1))
+    at, cu_at = longs.data_ptr(), ints.data_ptr()
+    _launch.call("g9_assign_slots", dev, lengths.data_ptr(), counts.data_ptr(), B, block_table.data_ptr(), *args[:2],
+                 free_blocks.data_ptr(), args[2], ptr(free_start), block_size, num_tokens, cu_at, at, at + 8 * num_tokens,
+                 cu_at + 4 * (B + 1))
+    return Slots(cu, slots, positions, taken)
+
+
+def _plan_slots(key, lengths, counts, block_table, free_blocks, block_size, num_tokens, free_start):
     dev = _launch.gpu_of(lengths, counts, block_table, free_blocks, free_start)
     for name, t, n in (("lengths", lengths, 1), ("counts", counts, 1), ("block_table", block_table, 2),
                        ("free_blocks", free_blocks, 1)):
@@ -56,17 +72,13 @@ def assign_slots(lengths: torch.Tensor, counts: torch.Tensor, block_table: torch
         raise ValueError(f"lengths, counts and block_table hold {B}, {counts.shape[0]} and {block_table.shape[0]} requests")
     if B > MAX_REQUESTS:
         raise ValueError(f"{B} requests; at most {MAX_REQUESTS} in one call")
+    if num_tokens < 0:
+        raise ValueError(f"num_tokens is {num_tokens}")
     if free_start is not None:
         _launch.int32_of("free_start", free_start, 1)
         if free_start.shape[0] != 1:
             raise ValueError("free_start must hold one value")
-    ints = torch.empty(B + 2, dtype=torch.int32, device=dev)
-    longs = torch.empty((2, num_tokens), dtype=torch.int64, device=dev)
-    out = Slots(ints[: B + 1], longs[0], longs[1], ints[B + 1 :])
-    _launch.call("g9_assign_slots", dev, ptr(lengths), ptr(counts), B, ptr(block_table), block_table.stride(0),
-                 block_table.shape[1], ptr(free_blocks), free_blocks.shape[0], ptr(free_start), block_size, num_tokens,
-                 ptr(out.cu_seqlens), ptr(out.slots), ptr(out.positions), ptr(out.taken))
-    return out
+    return _launch.keep(key, dev, (dev, B, (block_table.stride(0), block_table.shape[1], free_blocks.shape[0])))
 
 
 def _cache_of(k_cache, v_cache):
@@ -85,6 +97,14 @@ def write_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
     must be distinct (two rows of one slot may leave a mixture of both there).
 
     fp16 or bf16, head dim 64 or 128; block_size a power of two from 16 to 1024."""
+    key = ("write", sig(k), sig(v), sig(k_cache), sig(v_cache), sig(slots))
+    dev, rest = _launch.planned(key) or _plan_write(key, k, v, k_cache, v_cache, slots)
+    _launch.forward_only(k, v, k_cache, v_cache)
+    _launch.call("g9_write_cache", dev, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                 slots.data_ptr(), *rest)
+
+
+def _plan_write(key, k, v, k_cache, v_cache, slots):
     dev = _launch.gpu_of(k, v, k_cache, v_cache, slots)
     T, HK, D = _launch.rows_of("k", k)
     _launch.rows_of("v", v)
@@ -94,9 +114,8 @@ def write_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
     if slots.dtype != torch.int64 or slots.dim() != 1 or slots.shape[0] != T or not slots.is_contiguous():
         raise ValueError(f"slots must be {T} contiguous int64 values")
     _launch.dtype_of(k, v, k_cache, v_cache)
-    _launch.forward_only(k, v, k_cache, v_cache)
-    _launch.call("g9_write_cache", dev, ptr(k), ptr(v), ptr(k_cache), ptr(v_cache), ptr(slots), T, HK, D, blocks, size,
-                 strides(k), strides(v), strides(k_cache), strides(v_cache))
+    return _launch.keep(key, dev, (dev, (T, HK, D, blocks, size, strides(k), strides(v), strides(k_cache),
+                                         strides(v_cache))))
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -120,6 +139,21 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     behind the last request are left as they were, a row that reads nothing gives
     zeros.  ``lse`` as in ``varlen_attention``.  Asynchronous on the current
     stream; forward only."""
+    key = ("tree", sm_scale, sig(q), sig(k_cache), sig(v_cache), sig(block_table), sig(lengths), sig(cu_seqlens),
+           tree_mask is not None and sig(tree_mask), o is not None and sig(o), lse is not None and sig(lse))
+    dev, need, table, words, rest = _launch.planned(key) or _plan_tree(
+        key, q, k_cache, v_cache, block_table, lengths, cu_seqlens, tree_mask, o, lse, sm_scale)
+    _launch.forward_only(q, k_cache, v_cache)
+    if o is None:
+        o = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _launch.call("g9_tree_fwd", dev, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), ptr(lse),
+                 block_table.data_ptr(), *table, lengths.data_ptr(), cu_seqlens.data_ptr(), ptr(tree_mask), words, *rest,
+                 ws.data_ptr(), need)
+    return o
+
+
+def _plan_tree(key, q, k_cache, v_cache, block_table, lengths, cu_seqlens, tree_mask, o, lse, sm_scale):
     dev = _launch.gpu_of(q, k_cache, v_cache, block_table, lengths, cu_seqlens, tree_mask, o, lse)
     T, HQ, D = _launch.rows_of("q", q)
     blocks, size, HK, dim = _cache_of(k_cache, v_cache)
@@ -138,17 +172,14 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         if tree_mask.shape[0] != T or words == 0:
             raise ValueError(f"tree_mask {tuple(tree_mask.shape)} does not fit {T} rows")
     _launch.heads_fit(HQ, HK, D)
-    if o is None:
-        o = torch.empty((T, HQ, D), dtype=q.dtype, device=dev)
-    elif o.shape != q.shape:
-        raise ValueError(f"o is {tuple(o.shape)}, q {tuple(q.shape)}")
-    dtype = _launch.dtype_of(q, k_cache, v_cache, o)
+    if o is not None:
+        _launch.rows_of("o", o)
+        if o.shape != q.shape:
+            raise ValueError(f"o is {tuple(o.shape)}, q {tuple(q.shape)}")
+    dtype = _launch.dtype_of(q, k_cache, v_cache, *([o] if o is not None else []))
     _launch.lse_fits(lse, HQ, T)
-    _launch.forward_only(q, k_cache, v_cache)
-    need = _lib.load().g9_tree_workspace_size(B, T, HQ, HK, D)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _launch.call("g9_tree_fwd", dev, ptr(q), ptr(k_cache), ptr(v_cache), ptr(o), ptr(lse), ptr(block_table),
-                 block_table.stride(0), block_table.shape[1], ptr(lengths), ptr(cu_seqlens), ptr(tree_mask), words, B, T,
-                 HQ, HK, D, blocks, size, strides(q), strides(k_cache), strides(v_cache), strides(o),
-                 D**-0.5 if sm_scale is None else float(sm_scale), dtype, ptr(ws), need)
-    return o
+    os = _launch.array(HQ * D, D) if o is None else strides(o)
+    return _launch.keep(key, dev, (
+        dev, _lib.load().g9_tree_workspace_size(B, T, HQ, HK, D), (block_table.stride(0), block_table.shape[1]), words,
+        (B, T, HQ, HK, D, blocks, size, strides(q), strides(k_cache), strides(v_cache), os,
+         D**-0.5 if sm_scale is None else float(sm_scale), dtype)))

@@ -8,7 +8,7 @@ from __future__ import annotations
 import torch
 
 from . import _launch
-from ._launch import ptr, strides
+from ._launch import ptr, sig, strides
 
 
 def varlen_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -29,27 +29,38 @@ def varlen_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     sequence are left as they were.  ``lse``, if given, is a contiguous fp32
     (HQ, T) tensor that receives each query's natural-log log-sum-exp.
     Asynchronous on the current stream; forward only."""
+    key = ("varlen", causal, sm_scale, sig(q), sig(k), sig(v), sig(cu_seqlens), cu_seqlens_k is not None and sig(cu_seqlens_k),
+           o is not None and sig(o), lse is not None and sig(lse))
+    dev, rest = _launch.planned(key) or _plan(key, q, k, v, cu_seqlens, cu_seqlens_k, o, lse, causal, sm_scale)
+    _launch.forward_only(q, k, v)
+    if o is None:
+        o = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    cu = cu_seqlens.data_ptr()
+    _launch.call("g9_varlen_fwd", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), ptr(lse), cu,
+                 cu if cu_seqlens_k is None else cu_seqlens_k.data_ptr(), *rest)
+    return o
+
+
+def _plan(key, q, k, v, cu_seqlens, cu_seqlens_k, o, lse, causal, sm_scale):
+    """The checks, and the C call's arguments behind the pointers."""
     dev = _launch.gpu_of(q, k, v, cu_seqlens, cu_seqlens_k, o, lse)
     T, HQ, D = _launch.rows_of("q", q)
     TK, HK, _ = _launch.rows_of("k", k)
+    _launch.rows_of("v", v)
     if k.shape != v.shape or k.shape[2] != D:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not fit")
-    if cu_seqlens_k is None:
-        if TK != T:
-            raise ValueError(f"{TK} keys for {T} queries need cu_seqlens_k")
-        cu_seqlens_k = cu_seqlens
+    if cu_seqlens_k is None and TK != T:
+        raise ValueError(f"{TK} keys for {T} queries need cu_seqlens_k")
     B = _launch.offsets_of("cu_seqlens", cu_seqlens)
-    if _launch.offsets_of("cu_seqlens_k", cu_seqlens_k) != B:
+    if cu_seqlens_k is not None and _launch.offsets_of("cu_seqlens_k", cu_seqlens_k) != B:
         raise ValueError("cu_seqlens and cu_seqlens_k hold different numbers of sequences")
     _launch.heads_fit(HQ, HK, D)
-    if o is None:
-        o = torch.empty((T, HQ, D), dtype=q.dtype, device=dev)
-    elif o.shape != q.shape:
-        raise ValueError(f"o is {tuple(o.shape)}, q {tuple(q.shape)}")
-    dtype = _launch.dtype_of(q, k, v, o)
+    if o is not None:
+        _launch.rows_of("o", o)
+        if o.shape != q.shape:
+            raise ValueError(f"o is {tuple(o.shape)}, q {tuple(q.shape)}")
+    dtype = _launch.dtype_of(q, k, v, *([o] if o is not None else []))
     _launch.lse_fits(lse, HQ, T)
-    _launch.forward_only(q, k, v)
-    _launch.call("g9_varlen_fwd", dev, ptr(q), ptr(k), ptr(v), ptr(o), ptr(lse), ptr(cu_seqlens), ptr(cu_seqlens_k),
-                 B, T, TK, HQ, HK, D, strides(q), strides(k), strides(v), strides(o),
-                 D**-0.5 if sm_scale is None else float(sm_scale), dtype, 1 if causal else 0)
-    return o
+    os = _launch.array(HQ * D, D) if o is None else strides(o)
+    return _launch.keep(key, dev, (dev, (B, T, TK, HQ, HK, D, strides(q), strides(k), strides(v), os,
+                                         D**-0.5 if sm_scale is None else float(sm_scale), dtype, 1 if causal else 0)))

@@ -185,17 +185,22 @@ constexpr int sum16(const int (&a)[16]) {
 //            a descriptor of its own; in LDS, rows go by 16 and chunks of 256
 //            bytes, V's rows permuted within a chunk so that the transposing reads
 //            of four chunks touch every bank once.  Which keys from `wlim` on
-//            (the request's nodes) a query reads is p's to say (p.reads).
+//            (the request's nodes) a query reads is p's to say (p.reads).  Four
+//            tiles of K and of V are in LDS instead of two: the tiles come from
+//            HBM, not from an L2 that other workgroups have filled, and 32 KB in
+//            flight per CU carry 2.3 TB/s.
 enum Kind { kEqual, kPacked, kPaged };
 template <class Params, Kind KIND>
 struct Where {};
-// The request's table row and first tile; the pages of this wave's rows of the
-// next K tile and of the next V tile to ask for; V's second read base; the
-// query's row in the mask.
+// The request's table row and first tile; the pages of this wave's rows of 64
+// tiles, one per lane, and of the next K tile and the next V tile to ask for
+// (a scalar load per tile would be waited for in every tile's last cluster:
+// 3.3 us a tile instead of 1.4); V's second read base; the query's row in the
+// mask.
 template <class Params>
 struct Where<Params, kPaged> {
   const int* table;
-  int t0, pgk, pgv;
+  int t0, held, pgk, pgv;
   u32 avh;
   typename Params::Row row;
 };
@@ -217,8 +222,9 @@ struct Pipe : Where<Params, KIND> {
   static constexpr int kGroup = kNC * 256;     // kPaged: 16 rows
   static constexpr int kTileK = kNC * kPitchK;  // one K tile in LDS
   static constexpr int kTileV = kNC * kPitchV;  // one V tile in LDS
-  static constexpr int kLdsV = 2 * kTileK;     // V buffers after the two K buffers
-  static constexpr int kLdsBytes = 2 * kTileK + 2 * kTileV;
+  static constexpr int kBufs = KIND == kPaged ? 4 : 2;  // tiles of K and of V in LDS
+  static constexpr int kLdsV = kBufs * kTileK;  // V buffers after the K buffers
+  static constexpr int kLdsBytes = kBufs * (kTileK + kTileV);
   static constexpr int kE1 = HD == 128 ? G9_FMHA_VEC1_EXPS : G9_FMHA_VEC1_EXPS_64;
   static constexpr int kVN1 = HD == 128 ? G9_FMHA_VN1 : G9_FMHA_VN1_64;
   static constexpr int kVN2 = HD == 128 ? G9_FMHA_VN2 : G9_FMHA_VN2_64;
@@ -241,7 +247,7 @@ struct Pipe : Where<Params, KIND> {
   const char *kp, *vp;
   int keys, lim, wlim;
   char* pscratch;
-  static constexpr int kScratchBytes = kBN * 32 * 2;  // per wave: P of one tile, 16 bit
+  static constexpr int kScratchBytes = 64 * 32 * 2;  // per wave: P of 64 keys, 16 bit
 
   G9_DEV explicit Pipe(const Params& pp) : p(pp) {}
 
@@ -267,10 +273,12 @@ struct Pipe : Where<Params, KIND> {
   }
   // kPaged: this wave's 16 rows of a tile, and which of their DMAs are its.
   G9_DEV int my_key(int tile) const { return (this->t0 + tile) * kBN + 16 * (wave * kDW / (kNC / 4)); }
-  G9_DEV int page_of(int tile) const {
-    const int k = my_key(tile);
-    return k < keys ? this->table[k >> p.shift] : -1;
+  G9_DEV void hold_pages(int tile) {
+    const int k = my_key(tile + (int)(threadIdx.x & 63));
+    this->held = k < keys ? this->table[k >> p.shift] : -1;
+    waitcnt<0, 15>();  // here, not at the first use: see dma16_untracked
   }
+  G9_DEV int page_of(int tile) const { return __builtin_amdgcn_readlane(this->held, tile & 63); }
   G9_DEV void dma_paged(const char* base, int tile, int page, u32 lds, u32 voff, long long step, u32 ld) const {
     const int k = my_key(tile), off = k & ((1 << p.shift) - 1);
     const bool in = (u32)page < (u32)p.num_blocks;
@@ -320,22 +328,25 @@ struct Pipe : Where<Params, KIND> {
       }
     }
   }
+  // BUF < 0: buffer `buf` (kPaged).
   template <int BUF>
-  G9_DEV void read_k() {
+  G9_DEV void read_k(int buf = 0) {
+    const u32 ak_buf = BUF < 0 ? ak + buf * kTileK : ak;
 #pragma unroll
     for (int s = 0; s < kNS; ++s)
 #pragma unroll
       for (int blk = 0; blk < kNB; ++blk)
         kv[kNB * s + blk] = *(const G9_LDS u32x4*)(uintptr_t)(
-            KIND == kPaged ? ak + BUF * kTileK + 512 * s + 2 * blk * kGroup : ak + BUF * kTileK + 2 * s * kPitchK + blk * 512);
+            KIND == kPaged ? ak_buf + 512 * s + 2 * blk * kGroup : ak + BUF * kTileK + 2 * s * kPitchK + blk * 512);
   }
   template <int BUF>
-  G9_DEV void read_v() {
+  G9_DEV void read_v(int buf = 0) {
+    const u32 av_buf = BUF < 0 ? av + buf * kTileV : av;
 #pragma unroll
     for (int t = 0; t < kKS; ++t)
 #pragma unroll
       for (int d = 0; d < kND; ++d) {
-        const u32 a = KIND == kPaged ? av + BUF * kTileV + 1024 * d + t * kGroup : av + BUF * kTileV + 4 * d * kPitchV + 256 * t;
+        const u32 a = KIND == kPaged ? av_buf + 1024 * d + t * kGroup : av + BUF * kTileV + 4 * d * kPitchV + 256 * t;
         const u32x2 lo = tr_read(a);
         const u32x2 hi = tr_read(second(a));
         kv[kND * t + d] = u32x4{lo.x, lo.y, hi.x, hi.y};
@@ -411,10 +422,9 @@ struct Pipe : Where<Params, KIND> {
   // Masked tiles: a weight of 0 does not keep an infinite or NaN value out
   // of the product.  Such values (rare: one packed maximum over V's registers
   // finds them) are taken out of the registers, and added on the vector unit to
-  // the rows that may read their key.  V_tile is in buffer BUF and in kv, P_tile
+  // the rows that may read their key.  V_tile is in buffer `buf` and in kv, P_tile
   // in S as vec2 left it.
-  template <int BUF>
-  G9_DEV void guard_v(const Sc& S, int tile) {
+  G9_DEV void guard_v(const Sc& S, int tile, int buf) {
     typedef unsigned short h2 __attribute__((ext_vector_type(2)));
     constexpr u32 kExp = BF16 ? 0x7f80u : 0x7c00u;
     h2 top = {0, 0};
@@ -434,43 +444,47 @@ struct Pipe : Where<Params, KIND> {
         pin(x);  // one compare at a time: their masks would not fit the scalar registers
         kv[f][e] = x;
       }
-    // P in LDS: row of the query, column of the key.
+    // 64 keys at a time: P in LDS, row of the query, column of the key.
     const int lane = threadIdx.x & 63, h = lane >> 5;
-    uint16_t* const prow = reinterpret_cast<uint16_t*>(pscratch) + (lane & 31) * kBN;
+    uint16_t* const prow = reinterpret_cast<uint16_t*>(pscratch) + (lane & 31) * 64;
+    const int first = (first_tile() + tile) * kBN;
 #pragma unroll
-    for (int blk = 0; blk < kNB; ++blk)
+    for (int half = 0; half < kRH; ++half) {
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        const u32 w = __float_as_uint(S.b[blk][8 * (i / 8) + (i % 8) / 2]);
-        *reinterpret_cast<u32*>(prow + 32 * blk + 8 * (i / 4) + 4 * h + i % 4) = w;
-      }
-    waitcnt<63, 0>();
-    const int first = (first_tile() + tile) * kBN, most = min(keys - first, kBN);
-    unsigned long long who = 0;
-#pragma unroll 1
-    for (int key = 0; key < most; ++key) {
-      if constexpr (KIND == kPaged) {
-        if (key % 64 == 0) who = p.reads(this->row, first + key, keys);
-        if (!((who >> (key & 63)) & 1)) continue;
-      } else {
-        if (first + key >= lim) continue;
-      }
-      const float w = unpack2<BF16>(prow[key]).x;
-      const u32 a = lds0 + kLdsV + BUF * kTileV + 8 * h + (KIND == kPaged ? (key >> 4) * kGroup : key * 16);
+      for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
-      for (int d = 0; d < kND; ++d)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const u32x2 x = *(const G9_LDS u32x2*)(uintptr_t)(
-              a + (KIND == kPaged ? (4 * d + r) * 256 + ((key & 15) ^ (4 * r)) * 16 : (4 * d + r) * kPitchV));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            u32 y = (e & 1 ? x[e / 2] >> 16 : x[e / 2]) & 0xffffu;
-            if ((y & kExp) != kExp) y = 0;
-            o[d][4 * r + e] += w * unpack2<BF16>(y).x;
-          }
-          __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < 16; i += 2) {
+          const u32 w = __float_as_uint(S.b[2 * half + blk][8 * (i / 8) + (i % 8) / 2]);
+          *reinterpret_cast<u32*>(prow + 32 * blk + 8 * (i / 4) + 4 * h + i % 4) = w;
         }
+      waitcnt<63, 0>();
+      const int from = first + 64 * half;
+      unsigned long long who = 0;
+      if constexpr (KIND == kPaged)
+        who = p.reads(this->row, from, keys);
+      else
+        who = lim - from >= 64 ? ~0ull : lim - from <= 0 ? 0 : (1ull << (lim - from)) - 1;
+#pragma unroll 1
+      for (int key = 0; key < 64; ++key) {
+        if (!((who >> key) & 1)) continue;
+        const float w = unpack2<BF16>(prow[key]).x;
+        const int kt = 64 * half + key;
+        const u32 a = lds0 + kLdsV + buf * kTileV + 8 * h + (KIND == kPaged ? (kt >> 4) * kGroup : kt * 16);
+#pragma unroll
+        for (int d = 0; d < kND; ++d)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const u32x2 x = *(const G9_LDS u32x2*)(uintptr_t)(
+                a + (KIND == kPaged ? (4 * d + r) * 256 + ((key & 15) ^ (4 * r)) * 16 : (4 * d + r) * kPitchV));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              u32 y = (e & 1 ? x[e / 2] >> 16 : x[e / 2]) & 0xffffu;
+              if ((y & kExp) != kExp) y = 0;
+              o[d][4 * r + e] += w * unpack2<BF16>(y).x;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+      }
     }
   }
 
@@ -652,9 +666,18 @@ struct Pipe : Where<Params, KIND> {
     barrier();
     // M1(j): V_j was waited for at the end of M2(j-1) (or the prologue).
     __builtin_amdgcn_s_setprio(1);
-    read_v<PAR>();
-    if (j + 2 < nte) waitcnt<kDW, 15>();  // K_{j+2} landed (V_{j+1} may be in flight)
-    if (j + 3 < nte) dma_k(j + 3, PAR ^ 1);
+    if constexpr (KIND == kPaged) {
+      read_v<-1>(j & 3);
+      if (j + 4 < nte)
+        waitcnt<5 * kDW, 15>();  // K_{j+2} landed; V_{j+1}, K_{j+3}, V_{j+2}, K_{j+4}, V_{j+3} may be in flight
+      else
+        waitcnt<0, 15>();
+      if (j + 5 < nte) dma_k(j + 5, (j + 1) & 3);
+    } else {
+      read_v<PAR>();
+      if (j + 2 < nte) waitcnt<kDW, 15>();  // K_{j+2} landed (V_{j+1} may be in flight)
+      if (j + 3 < nte) dma_k(j + 3, PAR ^ 1);
+    }
     if constexpr (NEXT) {
       if constexpr (KIND != kEqual) {
         if (masked(j + 1)) {
@@ -671,7 +694,7 @@ struct Pipe : Where<Params, KIND> {
     }
     waitcnt<63, 0>();
     if constexpr (KIND != kEqual)
-      if (masked(j)) guard_v<PAR>(c, j);
+      if (masked(j)) guard_v(c, j, KIND == kPaged ? j & 3 : PAR);
     barrier();
     // D2(j)
     __builtin_amdgcn_s_setprio(0);
@@ -689,17 +712,28 @@ struct Pipe : Where<Params, KIND> {
     // M2(j)
     __builtin_amdgcn_s_setprio(1);
     if constexpr (NEXT) {
-      read_k<PAR>();
-      if (j + 3 < nte)
-        waitcnt<kDW, 15>();  // V_{j+1} landed (K_{j+3} may be in flight)
-      else
-        waitcnt<0, 15>();
+      if constexpr (KIND == kPaged) {
+        read_k<-1>((j + 2) & 3);
+        if (j + 5 < nte)
+          waitcnt<5 * kDW, 15>();  // V_{j+1} landed; K_{j+3}, V_{j+2}, K_{j+4}, V_{j+3}, K_{j+5} may be in flight
+        else
+          waitcnt<0, 15>();
+      } else {
+        read_k<PAR>();
+        if (j + 3 < nte)
+          waitcnt<kDW, 15>();  // V_{j+1} landed (K_{j+3} may be in flight)
+        else
+          waitcnt<0, 15>();
+      }
       rescale();
     }
-    if (j + 2 < nte) dma_v(j + 2, PAR);
     if constexpr (KIND == kPaged) {
-      this->pgv = this->pgk;  // tile j + 3's V is asked for next, tile j + 4's K
-      this->pgk = page_of(j + 4);
+      if (j + 4 < nte) dma_v(j + 4, j & 3);
+      this->pgv = this->pgk;  // tile j + 5's V is asked for next, tile j + 6's K
+      if (((j + 6) & 63) == 0) hold_pages(j + 6);
+      this->pgk = page_of(j + 6);
+    } else {
+      if (j + 2 < nte) dma_v(j + 2, PAR);
     }
     waitcnt<63, 0>();
     barrier();

@@ -44,6 +44,7 @@ struct Params {
   const unsigned long long* mask;                  // or null: a chain
   float* part;                                     // sums [2 kWorkers][kBlock][D], then (m, l) pairs
   unsigned long long* first;                       // [B + 1]: first tile of each request on the line
+  struct Start* start;                             // [kWorkers]: where each part begins
   long long q_t, q_h, o_t, o_h;                    // token / head strides, bytes
   long long k_b, k_h, v_b, v_h;                    // block / head strides, bytes
   long long table_stride;
@@ -85,6 +86,16 @@ struct Place {
   Req r;
   int b, hk, block, tile;
 };
+// The beginning of a worker's part, for the kernel that joins the parts.
+struct alignas(32) Start {
+  int q0, n, hk, block, tile, tiles;
+  u32 total_lo, total_hi;
+};
+
+// x / y with the 32-bit division where it holds them.
+G9_DEV unsigned long long quotient(unsigned long long x, unsigned long long y) {
+  return (x | y) >> 32 ? x / y : (unsigned long long)((u32)x / (u32)y);
+}
 
 template <class V>
 G9_DEV V uniform(V x) {
@@ -122,9 +133,9 @@ struct Line {
   // Worker w of W takes the tiles [w n / W, (w + 1) n / W) of a line of n; W is at
   // most n, so that no part in between is empty.
   static G9_DEV unsigned workers(unsigned long long n) { return n < kWorkers ? (unsigned)n : kWorkers; }
-  static G9_DEV unsigned long long part_begin(unsigned w, unsigned long long n) { return w * n / workers(n); }
+  static G9_DEV unsigned long long part_begin(unsigned w, unsigned long long n) { return quotient(w * n, workers(n)); }
   static G9_DEV unsigned worker_of(unsigned long long tile, unsigned long long n) {
-    return (unsigned)(((tile + 1) * workers(n) - 1) / n);
+    return (unsigned)quotient((tile + 1) * workers(n) - 1, n);
   }
 
   // Where this worker's part begins, and its tiles.  The workgroup sums the
@@ -181,11 +192,13 @@ struct Line {
       at.b = uniform(lo);
       at.r = request(p, at.b);
       const unsigned long long in = uniform(begin - first[lo]);
-      const unsigned long long unit = in / (unsigned)at.r.tiles;
+      const unsigned long long unit = quotient(in, (unsigned)at.r.tiles);
       at.tile = (int)(in - unit * (unsigned)at.r.tiles);
-      at.hk = (int)(unit / (unsigned)at.r.blocks);
+      at.hk = (int)quotient(unit, (unsigned)at.r.blocks);
       at.block = (int)(unit - (unsigned long long)at.hk * at.r.blocks);
       make_uniform(at);
+      if (THREADS == 64 * (kWorkers / kWgs) ? lane == 0 : tid == 0)
+        p.start[worker] = {at.r.q0, at.r.n, at.hk, at.block, at.tile, at.r.tiles, (u32)total, (u32)(total >> 32)};
     }
     __syncthreads();  // first[] is read: what comes next takes its place
     return count;
@@ -601,34 +614,48 @@ G9_DEV void wide(const Params& p, char* smem) {
     const char* const qrow = query_of<L>(p, cur, row, P.row.node);
 #pragma unroll
     for (int s = 0; s < PipeT::kNS; ++s) P.qf[s] = *reinterpret_cast<const u32x4*>(qrow + (16 * s + 8 * h) * 2);
-    // The prologue of g9_fmha.hip's kernel.
-    P.pgk = P.pgv = P.page_of(0);
-    P.dma_k(0, 0);
-    P.dma_v(0, 0);
-    P.pgk = P.page_of(1);
-    P.dma_k(1, 1);
+    // The prologue of g9_fmha.hip's kernel, with more tiles asked for.
+    P.hold_pages(0);
+    int pg[6];
+#pragma unroll
+    for (int i = 0; i < 6; ++i) pg[i] = P.page_of(i);
+    const auto ask_k = [&](int tile, int page) {
+      P.pgk = page;
+      P.dma_k(tile, tile & 3);
+    };
+    const auto ask_v = [&](int tile, int page) {
+      P.pgv = page;
+      P.dma_v(tile, tile & 3);
+    };
+    ask_k(0, pg[0]);
+    ask_v(0, pg[0]);
+    ask_k(1, pg[1]);
 #pragma unroll
     for (int d = 0; d < PipeT::kND; ++d) P.o[d] = f32x16{};
     P.m = -3.0e38f;
     P.l = 0.f;
-    P.pgv = P.pgk;
-    P.pgk = P.page_of(2);
     waitcnt<0, 0>();
     barrier();
-    P.template read_k<0>();
+    if (nte > 2) ask_k(2, pg[2]);
+    ask_v(1, pg[1]);
+    if (nte > 2) {
+      ask_k(3, pg[3]);
+      ask_v(2, pg[2]);
+    }
+    P.template read_k<-1>(0);
     typename PipeT::Sc sa, sb;
     P.qk(sa);
     waitcnt<63, 0>();
-    barrier();  // every wave has read K_0: its buffer takes K_2
-    if (nte > 2) P.dma_k(2, 0);
-    P.dma_v(1, 1);
-    P.pgv = P.pgk;
-    P.pgk = P.page_of(3);
+    barrier();  // every wave has read K_0: its buffer takes K_4
+    if (nte > 4) ask_k(4, pg[4]);
+    if (nte > 2) ask_v(3, pg[3]);
+    P.pgv = pg[4];
+    P.pgk = pg[5];
     if (P.masked(0)) P.mask_tile(sa, 0);
     P.vec0(sa);
     P.vec1(sa);
     P.l *= P.alpha;
-    P.template read_k<1>();
+    P.template read_k<-1>(1);
     waitcnt<63, 0>();
     if (lag) barrier();
     int j = 0;
@@ -649,23 +676,77 @@ G9_DEV void wide(const Params& p, char* smem) {
   }
 }
 
-// Joins the parts of query row (token t, head hq): with m the largest of their
-// maxima, sum of 2^(m_i - m) O_i over the sum of 2^(m_i - m) l_i, in the order of
-// the keys.  One workgroup per row; its threads hold HD / 4 columns by kLanes
-// parts.
+// The joined row: with m the largest of the parts' maxima, the sum of 2^(m_i - m)
+// O_i over the sum of 2^(m_i - m) l_i, in the order of the keys.
+template <bool BF16>
+G9_DEV void store4(const Params& p, long long tok, int hq, int c, f32x4 sum, float m, float l) {
+  const bool none = (__float_as_uint(l) << 1) == 0;
+  const float inv = none ? 0.f : 1.f / l;
+  *reinterpret_cast<u32x2*>(p.o + tok * p.o_t + hq * p.o_h + c * 8) =
+      u32x2{pack2<BF16>(sum[0] * inv, sum[1] * inv), pack2<BF16>(sum[2] * inv, sum[3] * inv)};
+  if (p.lse && c == 0) p.lse[(long long)hq * p.T + tok] = none ? -__builtin_inff() : (m + __builtin_log2f(l)) * kLn2;
+}
+
+// Joins the block that worker blockIdx.x + 1's part begins in the middle of, if
+// that worker is the second of the block's (each split block has one such); 32
+// rows a workgroup.  The parts of a block are few here: every thread sums its
+// four columns of four rows over all of them.
 template <bool BF16, int HD, class L>
-G9_DEV void join(const Params& p, float* lds) {
-  constexpr int kCols = HD / 4, kParts = 256 / kCols;
+G9_DEV void join(const Params& p) {
+  const unsigned w = blockIdx.x + 1;
+  const Start st = p.start[w];
+  const unsigned long long total = (unsigned long long)st.total_hi << 32 | st.total_lo;
+  // Workers behind the line's last have left no start: the line's own length
+  // says how many there are.
+  if (w >= L::workers(p.first[p.B]) || st.tile == 0) return;
+  const unsigned long long u0 = L::part_begin(w, total) - (unsigned)st.tile;
+  const unsigned w0 = L::worker_of(u0, total);
+  if (w0 != w - 1) return;
+  const unsigned n = L::worker_of(u0 + st.tiles - 1, total) - w0 + 1;
+  // Worker w0 has it in slot 1 unless it began the block before its part; the
+  // others in slot 0.
+  const size_t head = (size_t)2 * w0 + (L::part_begin(w0, total) <= u0 ? 1 : 0);
+  const float* const ml = p.part + (size_t)2 * L::kWorkers * L::kBlock * HD;
+  constexpr int kCols = HD / 4, kRowsAtOnce = 256 / kCols;
+  const int c = threadIdx.x % kCols;
+#pragma unroll
+  for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
+    const int in = blockIdx.y * 32 + i * kRowsAtOnce + threadIdx.x / kCols;
+    const long long row = (long long)st.block * L::kBlock + in;
+    if (row >= (long long)st.n * p.group) break;
+    f32x4 sum = {};
+    float m = -3.0e38f, l = 0.f;
+    for (unsigned k = 0; k < n; ++k) {
+      const size_t a = (k ? (size_t)2 * (w0 + k) : head) * L::kBlock + in;
+      const float mk = ml[a * 2], lk = ml[a * 2 + 1];
+      const f32x4 x = *reinterpret_cast<const f32x4*>(p.part + a * HD + 4 * c);
+      const float m_new = __builtin_fmaxf(m, mk), f = __builtin_amdgcn_exp2f(m - m_new), g = __builtin_amdgcn_exp2f(mk - m_new);
+      l = l * f + lk * g;
+      sum = sum * f + x * g;
+      m = m_new;
+    }
+    const int nd = (int)(row / p.group);
+    store4<BF16>(p, st.q0 + nd, st.hk * p.group + (int)(row - (long long)nd * p.group), c, sum, m, l);
+  }
+}
+
+// The same for a few query rows whose blocks are cut into many parts: one
+// workgroup per row (token t, head hq), its threads HD / 4 columns by kParts
+// parts.
+constexpr int kDeepThreads = 1024;
+template <bool BF16, int HD, class L>
+G9_DEV void join_deep(const Params& p, float* lds) {
+  constexpr int kCols = HD / 4, kParts = kDeepThreads / kCols;
   const int t = blockIdx.x / p.HQ, hq = blockIdx.x - t * p.HQ;
-  const int tid = threadIdx.x, c = tid % kCols, s = tid / kCols;
-  // The request of row t.
+  const int tid = threadIdx.x, lane = tid & 63, c = tid % kCols, s = tid / kCols;
+  // The request of row t: the number of sequence ends at or before it, 64
+  // candidates at a time.
   int lo = 0, hi = p.B;
   while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (p.cu[mid + 1] <= t)
-      lo = mid + 1;
-    else
-      hi = mid;
+    const int step = (hi - lo + 63) / 64, at = lo + (lane + 1) * step - 1;
+    const int full = __popcll(__builtin_amdgcn_ballot_w64(at < hi && p.cu[at + 1] <= t));
+    lo += full * step;
+    hi = min(hi, lo + step - 1);
   }
   if (lo >= p.B) return;
   const Req r = L::request(p, lo);
@@ -675,27 +756,23 @@ G9_DEV void join(const Params& p, float* lds) {
   const int block = row / L::kBlock, in = row - block * L::kBlock;
   const unsigned long long total = p.first[p.B];
   const unsigned long long u0 = p.first[lo] + ((unsigned long long)hk * r.blocks + block) * r.tiles;
-  const unsigned w0 = L::worker_of(u0, total), w1 = L::worker_of(u0 + r.tiles - 1, total);
-  if (w0 == w1) return;  // finished by its worker
+  const unsigned w0 = L::worker_of(u0, total), n = L::worker_of(u0 + r.tiles - 1, total) - w0 + 1;
+  if (n == 1) return;  // finished by its worker
   const float* const ml = p.part + (size_t)2 * L::kWorkers * L::kBlock * HD;
-  // Worker w0 has it in slot 1 unless it began the block before its part.
-  const auto at = [&](unsigned w) {
-    const unsigned slot = 2 * w + (w == w0 && L::part_begin(w0, total) <= u0 ? 1 : 0);
-    return (size_t)slot * L::kBlock + in;
-  };
-  const unsigned n = w1 - w0 + 1;
+  const size_t head = (size_t)2 * w0 + (L::part_begin(w0, total) <= u0 ? 1 : 0);
+  const auto at = [&](unsigned k) { return (k ? (size_t)2 * (w0 + k) : head) * L::kBlock + in; };
   float top = -3.0e38f;
-  for (unsigned i = tid; i < n; i += 256) top = __builtin_fmaxf(top, ml[at(w0 + i) * 2]);
+  for (unsigned k = tid; k < n; k += kDeepThreads) top = __builtin_fmaxf(top, ml[at(k) * 2]);
 #pragma unroll
   for (int d = 32; d; d >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, d, 64));
-  if ((tid & 63) == 0) lds[tid >> 6] = top;
+  if (lane == 0) lds[tid >> 6] = top;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) top = __builtin_fmaxf(top, lds[i]);
+  for (int i = 0; i < kDeepThreads / 64; ++i) top = __builtin_fmaxf(top, lds[i]);
   f32x4 sum = {};
   float l = 0.f;
-  for (unsigned i = s; i < n; i += kParts) {
-    const size_t a = at(w0 + i);
+  for (unsigned k = s; k < n; k += kParts) {
+    const size_t a = at(k);
     const float f = __builtin_amdgcn_exp2f(ml[a * 2] - top);
     l += f * ml[a * 2 + 1];
     sum += f * *reinterpret_cast<const f32x4*>(p.part + a * HD + 4 * c);
@@ -713,11 +790,7 @@ G9_DEV void join(const Params& p, float* lds) {
     for (int e = 0; e < 4; ++e) sum[e] += other[e];
     l += other[4];
   }
-  const bool none = (__float_as_uint(l) << 1) == 0;
-  const float inv = none ? 0.f : 1.f / l;
-  *reinterpret_cast<u32x2*>(p.o + t * p.o_t + hq * p.o_h + c * 8) =
-      u32x2{pack2<BF16>(sum[0] * inv, sum[1] * inv), pack2<BF16>(sum[2] * inv, sum[3] * inv)};
-  if (p.lse && c == 0) p.lse[(long long)hq * p.T + t] = none ? -__builtin_inff() : (top + __builtin_log2f(l)) * kLn2;
+  store4<BF16>(p, t, hq, c, sum, top, l);
 }
 
 }  // namespace tree
@@ -738,12 +811,14 @@ using namespace g9::host;
     tree::wide<BF16, HD>(p, smem);                                                                            \
   }                                                                                                           \
   extern "C" __global__ __launch_bounds__(256) void g9_tree_join_##NAME(tree::Params p) {                     \
-    __shared__ float lds[256 * 5];                                                                            \
-    tree::join<BF16, HD, tree::Narrow<HD>>(p, lds);                                                           \
+    tree::join<BF16, HD, tree::Narrow<HD>>(p);                                                                \
   }                                                                                                           \
   extern "C" __global__ __launch_bounds__(256) void g9_tree_join_wide_##NAME(tree::Params p) {                \
-    __shared__ float lds[256 * 5];                                                                            \
-    tree::join<BF16, HD, tree::Wide<HD>>(p, lds);                                                             \
+    tree::join<BF16, HD, tree::Wide<HD>>(p);                                                                  \
+  }                                                                                                           \
+  extern "C" __global__ __launch_bounds__(tree::kDeepThreads) void g9_tree_join_deep_##NAME(tree::Params p) { \
+    __shared__ float lds[tree::kDeepThreads * 5];                                                             \
+    tree::join_deep<BF16, HD, tree::Narrow<HD>>(p, lds);                                                      \
   }
 G9_TREE_KERNEL(bf16, true, 128)
 G9_TREE_KERNEL(f16, false, 128)
@@ -764,12 +839,30 @@ size_t part_floats(bool wide, int64_t D) { return (size_t)2 * (wide ? 256 * 256 
 // [wide][head dim 64][bf16]
 const void* const kRun[2][2][2] = {G9_TREE_FNS(g9_tree_), G9_TREE_FNS(g9_tree_wide_)};
 const void* const kJoin[2][2][2] = {G9_TREE_FNS(g9_tree_join_), G9_TREE_FNS(g9_tree_join_wide_)};
+const void* const kJoinDeep[2][2] = G9_TREE_FNS(g9_tree_join_deep_);
+// Up to this many rows (tokens by query heads) of the waves' form a block may be
+// cut into more than 32 parts, and a workgroup per row joins them faster than
+// one per block.
+constexpr int64_t kDeepRows = 1024;
+
+// The workspace: sums, first[], start[].
+struct Space {
+  size_t floats, first, start, bytes;
+};
+Space space_of(bool wide, int64_t B, int64_t D) {
+  Space s;
+  s.floats = part_floats(wide, D);
+  s.first = s.floats * 4;
+  s.start = (s.first + (size_t)(B + 1) * 8 + 31) / 32 * 32;
+  s.bytes = s.start + 1024 * sizeof(tree::Start);
+  return s;
+}
 
 }  // namespace
 
 extern "C" size_t g9_tree_workspace_size(int64_t B, int64_t T, int64_t HQ, int64_t HK, int64_t D) {
   if (B <= 0 || T <= 0 || HQ <= 0 || HK <= 0 || HQ % HK || D <= 0) return 0;
-  return part_floats(wide_form(B, T, HQ / HK), D) * 4 + (size_t)(B + 1) * 8;
+  return space_of(wide_form(B, T, HQ / HK), B, D).bytes;
 }
 
 extern "C" int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cache, void* o, float* lse,
@@ -801,9 +894,8 @@ extern "C" int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cac
     return G9_ERR_LAYOUT;
   const int64_t group = HQ / HK;
   const bool wide = wide_form(B, T, group);
-  const size_t floats = part_floats(wide, D);
-  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < floats * 4 + (size_t)(B + 1) * 8)
-    return G9_ERR_WORKSPACE;
+  const Space sp = space_of(wide, B, D);
+  if (!workspace || ((uintptr_t)workspace & 31) || workspace_bytes < sp.bytes) return G9_ERR_WORKSPACE;
   tree::Params p{};
   p.q = static_cast<const char*>(q);
   p.kc = static_cast<const char*>(k_cache);
@@ -815,7 +907,8 @@ extern "C" int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cac
   p.cu = cu_q;
   p.mask = reinterpret_cast<const unsigned long long*>(tree_mask);
   p.part = static_cast<float*>(workspace);
-  p.first = reinterpret_cast<unsigned long long*>(p.part + floats);
+  p.first = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + sp.first);
+  p.start = reinterpret_cast<tree::Start*>(static_cast<char*>(workspace) + sp.start);
   p.q_t = q_strides[0] * 2, p.q_h = q_strides[1] * 2, p.o_t = o_strides[0] * 2, p.o_h = o_strides[1] * 2;
   p.k_b = kc_strides[0] * 2, p.k_h = kc_strides[2] * 2, p.v_b = vc_strides[0] * 2, p.v_h = vc_strides[2] * 2;
   p.k_t = (u32)(kc_strides[1] * 2), p.v_t = (u32)(vc_strides[1] * 2);
@@ -828,6 +921,8 @@ extern "C" int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cac
   if (hipLaunchKernel(kRun[wide][D == 64][dtype == G9_BF16], dim3(tree::kWgs), dim3(wide ? fa::kThreads : 256), args, 0,
                       st) != hipSuccess)
     return G9_ERR_HIP;
-  return launched(hipLaunchKernel(kJoin[wide][D == 64][dtype == G9_BF16], dim3((unsigned)(T * HQ)), dim3(256), args, 0,
-                                  st));
+  const int d64 = D == 64, bf16 = dtype == G9_BF16;
+  if (!wide && T * HQ <= kDeepRows)
+    return launched(hipLaunchKernel(kJoinDeep[d64][bf16], dim3((unsigned)(T * HQ)), dim3(tree::kDeepThreads), args, 0, st));
+  return launched(hipLaunchKernel(kJoin[wide][d64][bf16], dim3(wide ? 255 : 1023, wide ? 8 : 1), dim3(256), args, 0, st));
 }

@@ -137,7 +137,7 @@ int g9_varlen_fwd(const void* q, const void* k, const void* v, void* o, float* l
  * cu_q[b] + i of tree_mask (T x words, int64); without a mask the nodes j <= i.
  * One node per request without a mask is plain decoding.  lse as g9_varlen_fwd.
  *
- * workspace: g9_tree_workspace_size bytes, 16-byte aligned, contents arbitrary;
+ * workspace: g9_tree_workspace_size bytes, 32-byte aligned, contents arbitrary;
  * it holds partial results between the call's kernels, so calls that can run
  * at the same time need one each.
  */
