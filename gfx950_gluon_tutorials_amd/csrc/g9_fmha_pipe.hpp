@@ -181,10 +181,12 @@ constexpr int sum16(const int (&a)[16]) {
 //            lim.  Tile addresses are 64-bit: a descriptor per tile whose range
 //            ends with the sequence, so rows behind it read as zeros.
 //   kPaged   the tiles from t0 on of a paged request, up to `keys` rows.  A DMA
-//            covers four 16-byte chunks of 16 rows, which never cross a page, with
-//            a descriptor of its own; in LDS, rows go by 16 and chunks of 256
-//            bytes, V's rows permuted within a chunk so that the transposing reads
-//            of four chunks touch every bank once.  Which keys from `wlim` on
+//            covers eight 16-byte chunks of 8 rows (whole 128-byte lines: with 64
+//            bytes of 16 rows HBM gave 3.6 TB/s), which never cross a page.  In
+//            LDS, rows go by 8 and chunks of 128 bytes; the groups of K are a
+//            chunk further apart and V's rows permuted within a chunk, so that
+//            K's reads of 16 rows and V's transposing reads of four chunks touch
+//            every bank once.  Which keys from `wlim` on
 //            (the request's nodes) a query reads is p's to say (p.reads).  Four
 //            tiles of K and of V are in LDS instead of two: the tiles come from
 //            HBM, not from an L2 that other workgroups have filled, and 32 KB in
@@ -195,13 +197,11 @@ struct Where {};
 // The request's table row and first tile; the pages of this wave's rows of 64
 // tiles, one per lane, and of the next K tile and the next V tile to ask for
 // (a scalar load per tile would be waited for in every tile's last cluster:
-// 3.3 us a tile instead of 1.4); V's second read base; the query's row in the
-// mask.
+// 3.3 us a tile instead of 1.4); the query's row in the mask.
 template <class Params>
 struct Where<Params, kPaged> {
   const int* table;
   int t0, held, pgk, pgv;
-  u32 avh;
   typename Params::Row row;
 };
 template <class Params, bool BF16, bool LAZY, bool SOQ, int HD, Kind KIND = kEqual>
@@ -219,8 +219,8 @@ struct Pipe : Where<Params, KIND> {
   static constexpr int kPitchK = kBN * 16;     // bytes between K chunk columns
   // Bytes between V chunk columns (pad: distinct banks).
   static constexpr int kPitchV = kBN * 16 + (KIND == kPaged ? 0 : 64);
-  static constexpr int kGroup = kNC * 256;     // kPaged: 16 rows
-  static constexpr int kTileK = kNC * kPitchK;  // one K tile in LDS
+  static constexpr int kGroupV = kNC * 128, kGroupK = kGroupV + 128;  // kPaged: 8 rows
+  static constexpr int kTileK = KIND == kPaged ? kBN / 8 * kGroupK : kNC * kPitchK;  // one K tile in LDS
   static constexpr int kTileV = kNC * kPitchV;  // one V tile in LDS
   static constexpr int kBufs = KIND == kPaged ? 4 : 2;  // tiles of K and of V in LDS
   static constexpr int kLdsV = kBufs * kTileK;  // V buffers after the K buffers
@@ -247,7 +247,7 @@ struct Pipe : Where<Params, KIND> {
   const char *kp, *vp;
   int keys, lim, wlim;
   char* pscratch;
-  static constexpr int kScratchBytes = 64 * 32 * 2;  // per wave: P of 64 keys, 16 bit
+  static constexpr int kScratchBytes = 32 * 32 * 2;  // per wave: P of 32 keys, 16 bit
 
   G9_DEV explicit Pipe(const Params& pp) : p(pp) {}
 
@@ -268,31 +268,33 @@ struct Pipe : Where<Params, KIND> {
   }
   // The V rows 8 below those at a.
   G9_DEV u32 second(u32 a) const {
-    if constexpr (KIND == kPaged) return a + (this->avh - av);
-    return a + 128;
+    return KIND == kPaged ? a + kGroupV : a + 128;
   }
-  // kPaged: this wave's 16 rows of a tile, and which of their DMAs are its.
-  G9_DEV int my_key(int tile) const { return (this->t0 + tile) * kBN + 16 * (wave * kDW / (kNC / 4)); }
+  // kPaged: this wave's rows of a tile, 8 by 256 bytes or 16 by 128.
+  static constexpr int kMine = kBN / kWaves;
+  G9_DEV int my_key(int tile) const { return (this->t0 + tile) * kBN + kMine * wave; }
   G9_DEV void hold_pages(int tile) {
     const int k = my_key(tile + (int)(threadIdx.x & 63));
     this->held = k < keys ? this->table[k >> p.shift] : -1;
     waitcnt<0, 15>();  // here, not at the first use: see dma16_untracked
   }
   G9_DEV int page_of(int tile) const { return __builtin_amdgcn_readlane(this->held, tile & 63); }
-  G9_DEV void dma_paged(const char* base, int tile, int page, u32 lds, u32 voff, long long step, u32 ld) const {
+  G9_DEV void dma_paged(const char* base, int tile, int page, u32 lds, u32 step_lds, u32 voff, long long step,
+                        u32 ld) const {
     const int k = my_key(tile), off = k & ((1 << p.shift) - 1);
     const bool in = (u32)page < (u32)p.num_blocks;
-    const int rows = in ? min(max(keys - k, 0), 16) : 0;
+    const int rows = in ? min(max(keys - k, 0), kMine) : 0;
     const unsigned long long at = (unsigned long long)base + (in ? page : 0) * step + (unsigned long long)off * ld;
     const u32 lo = (u32)__builtin_amdgcn_readfirstlane((int)at), hi = (u32)__builtin_amdgcn_readfirstlane((int)(at >> 32));
     const rsrc_t r4 = make_rsrc(reinterpret_cast<const void*>((unsigned long long)hi << 32 | lo),
                                 (u32)__builtin_amdgcn_readfirstlane((int)((u32)rows * ld)));
 #pragma unroll
-    for (int i = 0; i < kDW; ++i) dma16_fresh(r4, lds + (kDW * wave + i) * 1024, voff, ((kDW * wave + i) % (kNC / 4)) * 64);
+    for (int i = 0; i < kDW; ++i) dma16_fresh(r4, lds + i * step_lds, voff, HD == 128 ? i * 128 : i * 8 * ld);
   }
   G9_DEV void dma_k(int tile, int buf) {
     if constexpr (KIND == kPaged) {
-      dma_paged(kp, tile, this->pgk, lds0 + buf * kTileK, voffk, p.k_b, p.k_t);
+      dma_paged(kp, tile, this->pgk, lds0 + buf * kTileK + kMine / 8 * wave * kGroupK, HD == 128 ? 1024 : kGroupK, voffk,
+                p.k_b, p.k_t);
     } else if constexpr (KIND == kPacked) {
       const rsrc_t r4 = tile_rows(kp, tile, p.ldk);
 #pragma unroll
@@ -311,7 +313,7 @@ struct Pipe : Where<Params, KIND> {
   }
   G9_DEV void dma_v(int tile, int buf) {
     if constexpr (KIND == kPaged) {
-      dma_paged(vp, tile, this->pgv, lds0 + kLdsV + buf * kTileV, voffv, p.v_b, p.v_t);
+      dma_paged(vp, tile, this->pgv, lds0 + kLdsV + buf * kTileV + kMine / 8 * wave * kGroupV, 1024, voffv, p.v_b, p.v_t);
     } else if constexpr (KIND == kPacked) {
       const rsrc_t r4 = tile_rows(vp, tile, p.ldv);
 #pragma unroll
@@ -337,7 +339,7 @@ struct Pipe : Where<Params, KIND> {
 #pragma unroll
       for (int blk = 0; blk < kNB; ++blk)
         kv[kNB * s + blk] = *(const G9_LDS u32x4*)(uintptr_t)(
-            KIND == kPaged ? ak_buf + 512 * s + 2 * blk * kGroup : ak + BUF * kTileK + 2 * s * kPitchK + blk * 512);
+            KIND == kPaged ? ak_buf + 256 * s + 4 * blk * kGroupK : ak + BUF * kTileK + 2 * s * kPitchK + blk * 512);
   }
   template <int BUF>
   G9_DEV void read_v(int buf = 0) {
@@ -346,7 +348,7 @@ struct Pipe : Where<Params, KIND> {
     for (int t = 0; t < kKS; ++t)
 #pragma unroll
       for (int d = 0; d < kND; ++d) {
-        const u32 a = KIND == kPaged ? av_buf + 1024 * d + t * kGroup : av + BUF * kTileV + 4 * d * kPitchV + 256 * t;
+        const u32 a = KIND == kPaged ? av_buf + 512 * d + 2 * t * kGroupV : av + BUF * kTileV + 4 * d * kPitchV + 256 * t;
         const u32x2 lo = tr_read(a);
         const u32x2 hi = tr_read(second(a));
         kv[kND * t + d] = u32x4{lo.x, lo.y, hi.x, hi.y};
@@ -444,38 +446,36 @@ struct Pipe : Where<Params, KIND> {
         pin(x);  // one compare at a time: their masks would not fit the scalar registers
         kv[f][e] = x;
       }
-    // 64 keys at a time: P in LDS, row of the query, column of the key.
+    // 32 keys at a time: P in LDS, row of the query, column of the key.
     const int lane = threadIdx.x & 63, h = lane >> 5;
-    uint16_t* const prow = reinterpret_cast<uint16_t*>(pscratch) + (lane & 31) * 64;
+    uint16_t* const prow = reinterpret_cast<uint16_t*>(pscratch) + (lane & 31) * 32;
     const int first = (first_tile() + tile) * kBN;
 #pragma unroll
-    for (int half = 0; half < kRH; ++half) {
+    for (int blk = 0; blk < kNB; ++blk) {
 #pragma unroll
-      for (int blk = 0; blk < 2; ++blk)
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const u32 w = __float_as_uint(S.b[2 * half + blk][8 * (i / 8) + (i % 8) / 2]);
-          *reinterpret_cast<u32*>(prow + 32 * blk + 8 * (i / 4) + 4 * h + i % 4) = w;
-        }
+      for (int i = 0; i < 16; i += 2) {
+        const u32 w = __float_as_uint(S.b[blk][8 * (i / 8) + (i % 8) / 2]);
+        *reinterpret_cast<u32*>(prow + 8 * (i / 4) + 4 * h + i % 4) = w;
+      }
       waitcnt<63, 0>();
-      const int from = first + 64 * half;
+      const int from = first + 32 * blk;
       unsigned long long who = 0;
       if constexpr (KIND == kPaged)
         who = p.reads(this->row, from, keys);
       else
         who = lim - from >= 64 ? ~0ull : lim - from <= 0 ? 0 : (1ull << (lim - from)) - 1;
 #pragma unroll 1
-      for (int key = 0; key < 64; ++key) {
+      for (int key = 0; key < 32; ++key) {
         if (!((who >> key) & 1)) continue;
         const float w = unpack2<BF16>(prow[key]).x;
-        const int kt = 64 * half + key;
-        const u32 a = lds0 + kLdsV + buf * kTileV + 8 * h + (KIND == kPaged ? (kt >> 4) * kGroup : kt * 16);
+        const int kt = 32 * blk + key;
+        const u32 a = lds0 + kLdsV + buf * kTileV + 8 * h + (KIND == kPaged ? (kt >> 3) * kGroupV : kt * 16);
 #pragma unroll
         for (int d = 0; d < kND; ++d)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const u32x2 x = *(const G9_LDS u32x2*)(uintptr_t)(
-                a + (KIND == kPaged ? (4 * d + r) * 256 + ((key & 15) ^ (4 * r)) * 16 : (4 * d + r) * kPitchV));
+                a + (KIND == kPaged ? (4 * d + r) * 128 + ((key & 7) ^ (4 * (r >> 1))) * 16 : (4 * d + r) * kPitchV));
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               u32 y = (e & 1 ? x[e / 2] >> 16 : x[e / 2]) & 0xffffu;

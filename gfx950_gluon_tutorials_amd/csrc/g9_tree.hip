@@ -220,8 +220,8 @@ struct Line {
   }
 };
 // A wave's own tiles of up to 8 KB, or a workgroup's of 16 KB.
-template <int HD>
-using Narrow = Line<4096 / HD, 32, 4 * kWgs>;
+template <int HD, int NQ>
+using Narrow = Line<4096 / HD, 32 * NQ, 4 * kWgs>;
 template <int HD>
 using Wide = Line<8192 / HD, 256, kWgs>;
 
@@ -276,11 +276,11 @@ G9_DEV void finish(const Params& p, const Place& at, int slot, int row, int node
   if (p.lse && h == 0) p.lse[(long long)hq * p.T + tok] = none ? -__builtin_inff() : (m + __builtin_log2f(lt)) * kLn2;
 }
 
-template <bool BF16, int HD>
+// NQ groups of 32 query rows, which share every K and V register read from LDS.
+template <bool BF16, int HD, int NQ>
 struct Wave {
-  using L = Narrow<HD>;
+  using L = Narrow<HD, NQ>;
   static constexpr int kKeys = L::kKeys;           // keys per tile
-  static constexpr int kBlock = L::kBlock;
   static constexpr int kNB = kKeys / 32;           // 32-key score blocks
   static constexpr int kNS = HD / 16;              // QK steps of 16 head-dim values
   static constexpr int kKS = kKeys / 16;           // PV steps of 16 keys
@@ -290,7 +290,7 @@ struct Wave {
   static constexpr int kPieces = kKeys / 16;       // 16-row pieces: never across a page
   static constexpr int kDmas = 8;                  // per tile and operand
   static constexpr int kStage = 16384, kV = 8192;  // a stage; V behind K
-  static constexpr int kScratch = kBlock * kKeys * 2;  // P of one tile, 16 bit
+  static constexpr int kScratch = 32 * kKeys * 2;  // P of one tile and 32 rows, 16 bit
   static constexpr int kWaveLds = 2 * kStage + kScratch;
 
   const Params& p;
@@ -299,10 +299,10 @@ struct Wave {
   char* scratch;
   u32 voffk[4], voffv[1];
   u32 ak, av;        // LDS read bases in a stage (K, V)
-  u32x4 qf[kNS];
-  f32x16 o[kND];
-  float m, l;
-  Params::Row row;   // this lane's query
+  u32x4 qf[NQ][kNS];
+  f32x16 o[NQ][kND];
+  float m[NQ], l[NQ];
+  Params::Row row[NQ];  // this lane's queries
 
   G9_DEV explicit Wave(const Params& pp) : p(pp) {}
 
@@ -360,69 +360,75 @@ struct Wave {
   }
 
   G9_DEV void begin(const Place& at) {
-    row = row_of<L>(p, at, col);
-    const char* const qrow = query_of<L>(p, at, col, row.node);
 #pragma unroll
-    for (int s = 0; s < kNS; ++s) qf[s] = *reinterpret_cast<const u32x4*>(qrow + (16 * s + 8 * h) * 2);
-    // Finite, so that a row that has read nothing yet has weights 2^(-inf - m) =
-    // 0 and a sum of 0, not NaN.
-    m = -3.0e38f, l = 0.f;
+    for (int t = 0; t < NQ; ++t) {
+      row[t] = row_of<L>(p, at, 32 * t + col);
+      const char* const qrow = query_of<L>(p, at, 32 * t + col, row[t].node);
 #pragma unroll
-    for (int d = 0; d < kND; ++d) o[d] = f32x16{};
+      for (int s = 0; s < kNS; ++s) qf[t][s] = *reinterpret_cast<const u32x4*>(qrow + (16 * s + 8 * h) * 2);
+      // Finite, so that a row that has read nothing yet has weights 2^(-inf - m) =
+      // 0 and a sum of 0, not NaN.
+      m[t] = -3.0e38f, l[t] = 0.f;
+#pragma unroll
+      for (int d = 0; d < kND; ++d) o[t][d] = f32x16{};
+    }
     // Waited for here: the compiler does not count the DMAs in flight, and a wait
     // of its own at the first use would be one in every tile.
     waitcnt<0, 0>();
   }
 
-  template <bool TAIL>
-  G9_DEV void tile(const Place& at, int stage) {
-    f32x16 sc[kNB];
+  G9_DEV void tile(const Place& at, int stage, bool tail) {
+    f32x16 sc[NQ][kNB];
 #pragma unroll
     for (int s = 0; s < kNS; ++s)
 #pragma unroll
       for (int b = 0; b < kNB; ++b) {
         const u32x4 kf = *(const G9_LDS u32x4*)(uintptr_t)(ak + stage * kStage + 32 * b * kRow +
                                                            16 * ((2 * s + h) ^ swz_k(col)));
-        sc[b] = mfma<BF16>(kf, qf[s], s ? sc[b] : f32x16{});
+#pragma unroll
+        for (int t = 0; t < NQ; ++t) sc[t][b] = mfma<BF16>(kf, qf[t][s], s ? sc[t][b] : f32x16{});
       }
-    if constexpr (TAIL) {
-      const unsigned long long w = p.reads(row, at.tile * kKeys, at.r.keys);
+    u32x4 pf[NQ][kKS];
 #pragma unroll
-      for (int b = 0; b < kNB; ++b) {
-        const u32 bits = (u32)(w >> (32 * b)) >> (4 * h);
+    for (int t = 0; t < NQ; ++t) {
+      if (tail) {
+        const unsigned long long w = p.reads(row[t], at.tile * kKeys, at.r.keys);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float x = sc[b][i];
-          sc[b][i] = bits >> (8 * (i / 4) + i % 4) & 1 ? x : -__builtin_inff();
+        for (int b = 0; b < kNB; ++b) {
+          const u32 bits = (u32)(w >> (32 * b)) >> (4 * h);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float x = sc[t][b][i];
+            sc[t][b][i] = bits >> (8 * (i / 4) + i % 4) & 1 ? x : -__builtin_inff();
+          }
         }
       }
-    }
-    float top = sc[0][0];
+      float top = sc[t][0][0];
 #pragma unroll
-    for (int b = 0; b < kNB; ++b)
+      for (int b = 0; b < kNB; ++b)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, sc[b][i]);
-    top = xhalf(top, [](float x, float y) { return __builtin_fmaxf(x, y); });
-    const float m_new = __builtin_fmaxf(m, top * p.scale_log2);
-    const float alpha = __builtin_amdgcn_exp2f(m - m_new);
-    m = m_new;
-    float sum[4] = {};
-    u32x4 pf[kKS];
+        for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, sc[t][b][i]);
+      top = xhalf(top, [](float x, float y) { return __builtin_fmaxf(x, y); });
+      const float m_new = __builtin_fmaxf(m[t], top * p.scale_log2);
+      const float alpha = __builtin_amdgcn_exp2f(m[t] - m_new);
+      m[t] = m_new;
+      float sum[4] = {};
 #pragma unroll
-    for (int b = 0; b < kNB; ++b)
+      for (int b = 0; b < kNB; ++b)
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i], p.scale_log2, -m_new));
-        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i + 1], p.scale_log2, -m_new));
-        sum[i / 2 % 2 * 2] += x, sum[i / 2 % 2 * 2 + 1] += y;
-        pf[2 * b + i / 8][i % 8 / 2] = pack2<BF16>(x, y);
+        for (int i = 0; i < 16; i += 2) {
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][b][i], p.scale_log2, -m_new));
+          const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][b][i + 1], p.scale_log2, -m_new));
+          sum[i / 2 % 2 * 2] += x, sum[i / 2 % 2 * 2 + 1] += y;
+          pf[t][2 * b + i / 8][i % 8 / 2] = pack2<BF16>(x, y);
+        }
+      l[t] = l[t] * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+      if (__builtin_amdgcn_ballot_w64(alpha != 1.f)) {
+#pragma unroll
+        for (int d = 0; d < kND; ++d) o[t][d] *= alpha;
       }
-    l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-    if (__builtin_amdgcn_ballot_w64(alpha != 1.f)) {
-#pragma unroll
-      for (int d = 0; d < kND; ++d) o[d] *= alpha;
     }
-    u32x4 vf[kKS][kND];
+    if (tail) guard(at, stage, pf);
 #pragma unroll
     for (int k = 0; k < kKS; ++k)
 #pragma unroll
@@ -431,70 +437,69 @@ struct Wave {
         const u32 a = av + stage * kStage + 16 * k * kRow +
                       16 * ((4 * d + 2 * (lane >> 4 & 1) + ((lane & 3) >> 1)) ^ swz_v(vrow()));
         const u32x2 lo = tr_read(a), hi = tr_read(a + 8 * kRow);
-        vf[k][d] = u32x4{lo.x, lo.y, hi.x, hi.y};
+        const u32x4 vf = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+        for (int t = 0; t < NQ; ++t) o[t][d] = mfma<BF16>(vf, pf[t][k], o[t][d]);
       }
-    if constexpr (TAIL) guard(at, stage, vf, pf);
-#pragma unroll
-    for (int k = 0; k < kKS; ++k)
-#pragma unroll
-      for (int d = 0; d < kND; ++d) o[d] = mfma<BF16>(vf[k][d], pf[k], o[d]);
   }
 
   // Tiles that hold nodes: a weight of 0 does not keep an infinite or NaN value
-  // out of the product.  Such values (rare) are taken out of the registers, and
-  // added on the vector unit to the rows that read their key.
-  G9_DEV void guard(const Place& at, int stage, u32x4 (&vf)[kKS][kND], const u32x4 (&pf)[kKS]) {
+  // out of the product.  Such values (rare) are added on the vector unit to the
+  // rows that read their key, and then taken out of the tile.
+  G9_DEV void guard(const Place& at, int stage, const u32x4 (&pf)[NQ][kKS]) {
     typedef unsigned short h2 __attribute__((ext_vector_type(2)));
     constexpr u32 kExp = BF16 ? 0x7f80u : 0x7c00u;
+    G9_LDS u32x4* const mine = (G9_LDS u32x4*)(uintptr_t)(lds + stage * kStage + kV + lane * 16);
     h2 top = {0, 0};
 #pragma unroll
-    for (int k = 0; k < kKS; ++k)
+    for (int j = 0; j < 8; ++j) {
+      const u32x4 x = mine[64 * j];
 #pragma unroll
-      for (int d = 0; d < kND; ++d)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          top = __builtin_elementwise_max(top, __builtin_bit_cast(h2, vf[k][d][e] & 0x7fff7fffu));
+      for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(h2, x[e] & 0x7fff7fffu));
+    }
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(top.x >= kExp || top.y >= kExp) == 0, 1)) return;
-#pragma unroll
-    for (int k = 0; k < kKS; ++k)
-#pragma unroll
-      for (int d = 0; d < kND; ++d)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          u32 x = vf[k][d][e];
-          if ((x & kExp) == kExp) x &= 0xffff0000u;
-          if (((x >> 16) & kExp) == kExp) x &= 0xffffu;
-          pin(x);  // one compare at a time: their masks would not fit the scalar registers
-          vf[k][d][e] = x;
-        }
-    // P in LDS: row of the query, column of the key.
+    // P in LDS, 32 rows at a time: row of the query, column of the key.
     uint16_t* const prow = reinterpret_cast<uint16_t*>(scratch) + col * kKeys;
 #pragma unroll
-    for (int k = 0; k < kKS; ++k)
+    for (int t = 0; t < NQ; ++t) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        *reinterpret_cast<u32*>(prow + 16 * k + 8 * (e >> 1) + 4 * h + 2 * (e & 1)) = pf[k][e];
-    const unsigned long long w = p.reads(row, at.tile * kKeys, at.r.keys);
-    waitcnt<63, 0>();
+      for (int k = 0; k < kKS; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<u32*>(prow + 16 * k + 8 * (e >> 1) + 4 * h + 2 * (e & 1)) = pf[t][k][e];
+      const unsigned long long w = p.reads(row[t], at.tile * kKeys, at.r.keys);
+      waitcnt<63, 0>();
 #pragma unroll 1
-    for (int key = 0; key < kKeys; ++key) {
-      if (!((w >> key) & 1)) continue;
-      const float wt = unpack2<BF16>(prow[key]).x;
-      const u32 vr = lds + stage * kStage + kV + key * kRow;
+      for (int key = 0; key < kKeys; ++key) {
+        if (!((w >> key) & 1)) continue;
+        const float wt = unpack2<BF16>(prow[key]).x;
+        const u32 vr = lds + stage * kStage + kV + key * kRow;
 #pragma unroll
-      for (int d = 0; d < kND; ++d)
+        for (int d = 0; d < kND; ++d)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const u32x2 x = *(const G9_LDS u32x2*)(uintptr_t)(vr + 16 * ((4 * d + r) ^ swz_v(key)) + 8 * h);
+          for (int r = 0; r < 4; ++r) {
+            const u32x2 x = *(const G9_LDS u32x2*)(uintptr_t)(vr + 16 * ((4 * d + r) ^ swz_v(key)) + 8 * h);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            u32 y = (e & 1 ? x[e / 2] >> 16 : x[e / 2]) & 0xffffu;
-            if ((y & kExp) != kExp) y = 0;
-            o[d][4 * r + e] += wt * unpack2<BF16>(y).x;
+            for (int e = 0; e < 4; ++e) {
+              u32 y = (e & 1 ? x[e / 2] >> 16 : x[e / 2]) & 0xffffu;
+              if ((y & kExp) != kExp) y = 0;
+              o[t][d][4 * r + e] += wt * unpack2<BF16>(y).x;
+            }
+            __builtin_amdgcn_sched_barrier(0);
           }
-          __builtin_amdgcn_sched_barrier(0);
-        }
+      }
     }
+#pragma unroll 1
+    for (int j = 0; j < 8; ++j) {
+      u32x4 x = mine[64 * j];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if ((x[e] & kExp) == kExp) x[e] &= 0xffff0000u;
+        if (((x[e] >> 16) & kExp) == kExp) x[e] &= 0xffffu;
+      }
+      mine[64 * j] = x;
+    }
+    waitcnt<63, 0>();
   }
 };
 
@@ -502,10 +507,10 @@ struct Wave {
 // on one, whose L2 then serves the blocks of rows that share keys.
 G9_DEV unsigned my_part() { return (blockIdx.x & 7) * (kWgs / 8) + (blockIdx.x >> 3); }
 
-template <bool BF16, int HD>
+template <bool BF16, int HD, int NQ>
 G9_DEV void narrow(const Params& p, char* smem) {
-  using W = Wave<BF16, HD>;
-  using L = Narrow<HD>;
+  using W = Wave<BF16, HD, NQ>;
+  using L = Narrow<HD, NQ>;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned worker = my_part() * 4 + wave;
   Place cur;
@@ -548,17 +553,16 @@ G9_DEV void narrow(const Params& p, char* smem) {
     }
     __builtin_amdgcn_sched_barrier(0);
     const bool tail = (cur.tile + 1) * W::kKeys > min(cur.r.context, cur.r.keys);
-    if (tail)
-      w.template tile<true>(cur, i & 1);
-    else
-      w.template tile<false>(cur, i & 1);
+    w.tile(cur, i & 1, tail);
     const bool last = cur.tile + 1 == cur.r.tiles;
     fresh = last;
     if (last || i + 1 == count) {
       // Slot 0 of the worker: a block that another worker began; slot 1: one
       // that the next worker goes on with.
-      finish<BF16, HD, L>(p, cur, last && from_start ? -1 : (int)(2 * worker + (from_start ? 1 : 0)), w.col, w.row.node,
-                          w.o, w.m, w.l);
+#pragma unroll
+      for (int t = 0; t < NQ; ++t)
+        finish<BF16, HD, L>(p, cur, last && from_start ? -1 : (int)(2 * worker + (from_start ? 1 : 0)), 32 * t + w.col,
+                            w.row[t].node, w.o[t], w.m[t], w.l[t]);
       from_start = true;
     }
     cur = nxt;
@@ -588,15 +592,14 @@ G9_DEV void wide(const Params& p, char* smem) {
   P.lds0 = (u32)(uintptr_t)to_lds(smem);
   P.pscratch = smem + PipeT::kLdsBytes + P.wave * PipeT::kScratchBytes;
   P.sc = p.scale_log2;
-  // A DMA's lane i fetches chunk i / 16 of row i % 16 (V: of row i % 16 ^ 4 (chunk
-  // % 4), see Kind).
-  P.voffk = (u32)(lane & 15) * p.k_t + (lane >> 4) * 16;
-  P.voffv = (u32)((lane & 15) ^ (4 * (lane >> 4))) * p.v_t + (lane >> 4) * 16;
-  P.ak = P.lds0 + ((lane & 31) >> 4) * PipeT::kGroup + h * 256 + (lane & 15) * 16;
+  // A DMA's lane i fetches chunk i / 8 of row i % 8 (V: of row i % 8 ^ 4 (chunk /
+  // 2 % 2), see Kind).
+  P.voffk = (u32)(lane & 7) * p.k_t + (lane >> 3) * 16;
+  P.voffv = (u32)((lane & 7) ^ (4 * (lane >> 4 & 1))) * p.v_t + (lane >> 3) * 16;
+  P.ak = P.lds0 + ((lane & 31) >> 3) * PipeT::kGroupK + h * 128 + (lane & 7) * 16;
   {
-    const int c = 2 * (lane >> 4 & 1) + ((lane & 3) >> 1);  // chunk, of every four
-    P.av = P.lds0 + PipeT::kLdsV + c * 256 + ((4 * h + ((lane & 15) >> 2)) ^ (4 * c)) * 16 + 8 * (lane & 1);
-    P.avh = P.av ^ 128;
+    const int G = lane >> 4 & 1, jj = lane & 15;
+    P.av = P.lds0 + PipeT::kLdsV + (2 * G + ((jj & 3) >> 1)) * 128 + ((4 * h + (jj >> 2)) ^ (4 * G)) * 16 + 8 * (jj & 1);
   }
   const bool lag = P.wave >= 4;
   const int row = P.wave * 32 + (lane & 31);
@@ -709,21 +712,33 @@ G9_DEV void join(const Params& p) {
   const float* const ml = p.part + (size_t)2 * L::kWorkers * L::kBlock * HD;
   constexpr int kCols = HD / 4, kRowsAtOnce = 256 / kCols;
   const int c = threadIdx.x % kCols;
-#pragma unroll
+#pragma unroll 1
   for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
     const int in = blockIdx.y * 32 + i * kRowsAtOnce + threadIdx.x / kCols;
     const long long row = (long long)st.block * L::kBlock + in;
     if (row >= (long long)st.n * p.group) break;
     f32x4 sum = {};
     float m = -3.0e38f, l = 0.f;
-    for (unsigned k = 0; k < n; ++k) {
-      const size_t a = (k ? (size_t)2 * (w0 + k) : head) * L::kBlock + in;
-      const float mk = ml[a * 2], lk = ml[a * 2 + 1];
-      const f32x4 x = *reinterpret_cast<const f32x4*>(p.part + a * HD + 4 * c);
-      const float m_new = __builtin_fmaxf(m, mk), f = __builtin_amdgcn_exp2f(m - m_new), g = __builtin_amdgcn_exp2f(mk - m_new);
-      l = l * f + lk * g;
-      sum = sum * f + x * g;
-      m = m_new;
+    constexpr unsigned kAtOnce = 8;  // parts asked for together
+    for (unsigned k0 = 0; k0 < n; k0 += kAtOnce) {
+      float mk[kAtOnce], lk[kAtOnce];
+      f32x4 x[kAtOnce];
+#pragma unroll
+      for (unsigned e = 0; e < kAtOnce; ++e) {
+        const unsigned k = min(k0 + e, n - 1);
+        const size_t a = (k ? (size_t)2 * (w0 + k) : head) * L::kBlock + in;
+        mk[e] = ml[a * 2], lk[e] = ml[a * 2 + 1];
+        x[e] = *reinterpret_cast<const f32x4*>(p.part + a * HD + 4 * c);
+      }
+#pragma unroll
+      for (unsigned e = 0; e < kAtOnce; ++e) {
+        if (k0 + e >= n) break;
+        const float m_new = __builtin_fmaxf(m, mk[e]);
+        const float f = __builtin_amdgcn_exp2f(m - m_new), g = __builtin_amdgcn_exp2f(mk[e] - m_new);
+        l = l * f + lk[e] * g;
+        sum = sum * f + x[e] * g;
+        m = m_new;
+      }
     }
     const int nd = (int)(row / p.group);
     store4<BF16>(p, st.q0 + nd, st.hk * p.group + (int)(row - (long long)nd * p.group), c, sum, m, l);
@@ -799,59 +814,73 @@ G9_DEV void join_deep(const Params& p, float* lds) {
 using namespace g9;
 using namespace g9::host;
 
-#define G9_TREE_KERNEL(NAME, BF16, HD)                                                                        \
+#define G9_TREE_NARROW(NAME, BF16, HD, NQ)                                                                    \
   extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void                \
   g9_tree_##NAME(tree::Params p) {                                                                            \
-    __shared__ __attribute__((aligned(1024))) char smem[4 * tree::Wave<BF16, HD>::kWaveLds];                   \
-    tree::narrow<BF16, HD>(p, smem);                                                                          \
+    __shared__ __attribute__((aligned(1024))) char smem[4 * tree::Wave<BF16, HD, NQ>::kWaveLds];               \
+    tree::narrow<BF16, HD, NQ>(p, smem);                                                                      \
   }                                                                                                           \
+  extern "C" __global__ __launch_bounds__(256) void g9_tree_join_##NAME(tree::Params p) {                     \
+    tree::join<BF16, HD, tree::Narrow<HD, NQ>>(p);                                                            \
+  }                                                                                                           \
+  extern "C" __global__ __launch_bounds__(tree::kDeepThreads) void g9_tree_join_deep_##NAME(tree::Params p) { \
+    __shared__ float lds[tree::kDeepThreads * 5];                                                             \
+    tree::join_deep<BF16, HD, tree::Narrow<HD, NQ>>(p, lds);                                                  \
+  }
+#define G9_TREE_WIDE(NAME, BF16, HD)                                                                          \
   extern "C" __global__ __launch_bounds__(fa::kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void       \
-  g9_tree_wide_##NAME(tree::Params p) {                                                                       \
+  g9_tree_##NAME(tree::Params p) {                                                                            \
     __shared__ __attribute__((aligned(1024))) char smem[tree::WidePipe<BF16, HD>::kLds];                       \
     tree::wide<BF16, HD>(p, smem);                                                                            \
   }                                                                                                           \
   extern "C" __global__ __launch_bounds__(256) void g9_tree_join_##NAME(tree::Params p) {                     \
-    tree::join<BF16, HD, tree::Narrow<HD>>(p);                                                                \
-  }                                                                                                           \
-  extern "C" __global__ __launch_bounds__(256) void g9_tree_join_wide_##NAME(tree::Params p) {                \
     tree::join<BF16, HD, tree::Wide<HD>>(p);                                                                  \
-  }                                                                                                           \
-  extern "C" __global__ __launch_bounds__(tree::kDeepThreads) void g9_tree_join_deep_##NAME(tree::Params p) { \
-    __shared__ float lds[tree::kDeepThreads * 5];                                                             \
-    tree::join_deep<BF16, HD, tree::Narrow<HD>>(p, lds);                                                      \
   }
-G9_TREE_KERNEL(bf16, true, 128)
-G9_TREE_KERNEL(f16, false, 128)
-G9_TREE_KERNEL(bf16_d64, true, 64)
-G9_TREE_KERNEL(f16_d64, false, 64)
+#define G9_TREE_KERNELS(NAME, BF16, HD)      \
+  G9_TREE_NARROW(NAME##_q32, BF16, HD, 1)    \
+  G9_TREE_NARROW(NAME##_q64, BF16, HD, 2)    \
+  G9_TREE_WIDE(NAME##_q256, BF16, HD)
+G9_TREE_KERNELS(bf16, true, 128)
+G9_TREE_KERNELS(f16, false, 128)
+G9_TREE_KERNELS(bf16_d64, true, 64)
+G9_TREE_KERNELS(f16_d64, false, 64)
+
+#ifndef G9_WIDE_ROWS
+#define G9_WIDE_ROWS 64
+#endif
 
 namespace {
 
-// Whether the workgroup's form takes a batch: by the rows that its requests
-// bring on average to one K/V head.
-bool wide_form(int64_t B, int64_t T, int64_t group) { return (T + B - 1) / B * group > 64; }
-// Both forms keep 2 x 1024 x 32 or 2 x 256 x 256 rows' sums.
-size_t part_floats(bool wide, int64_t D) { return (size_t)2 * (wide ? 256 * 256 : 1024 * 32) * (D + 2); }
+// Query rows of a block, by the rows that the requests of a batch bring on
+// average to one K/V head.
+enum { Q32, Q64, Q256 };
+int form_of(int64_t B, int64_t T, int64_t group) {
+  const int64_t rows = (T + B - 1) / B * group;
+  return rows <= 32 ? Q32 : rows <= G9_WIDE_ROWS ? Q64 : Q256;
+}
+// The sums of 2 x 1024 blocks of 32 or 64 rows, or of 2 x 256 of 256.
+size_t part_floats(int form, int64_t D) { return (size_t)2 * (form == Q32 ? 1024 * 32 : 1024 * 64) * (D + 2); }
 
-#define G9_TREE_FNS(WHAT)                                                                       \
-  {{reinterpret_cast<const void*>(WHAT##f16), reinterpret_cast<const void*>(WHAT##bf16)},       \
-   {reinterpret_cast<const void*>(WHAT##f16_d64), reinterpret_cast<const void*>(WHAT##bf16_d64)}}
-// [wide][head dim 64][bf16]
-const void* const kRun[2][2][2] = {G9_TREE_FNS(g9_tree_), G9_TREE_FNS(g9_tree_wide_)};
-const void* const kJoin[2][2][2] = {G9_TREE_FNS(g9_tree_join_), G9_TREE_FNS(g9_tree_join_wide_)};
-const void* const kJoinDeep[2][2] = G9_TREE_FNS(g9_tree_join_deep_);
+#define G9_TREE_FNS(WHAT, Q)                                                                          \
+  {{reinterpret_cast<const void*>(WHAT##f16_##Q), reinterpret_cast<const void*>(WHAT##bf16_##Q)},     \
+   {reinterpret_cast<const void*>(WHAT##f16_d64_##Q), reinterpret_cast<const void*>(WHAT##bf16_d64_##Q)}}
+// [form][head dim 64][bf16]
+const void* const kRun[3][2][2] = {G9_TREE_FNS(g9_tree_, q32), G9_TREE_FNS(g9_tree_, q64), G9_TREE_FNS(g9_tree_, q256)};
+const void* const kJoin[3][2][2] = {G9_TREE_FNS(g9_tree_join_, q32), G9_TREE_FNS(g9_tree_join_, q64),
+                                    G9_TREE_FNS(g9_tree_join_, q256)};
+const void* const kJoinDeep[2][2][2] = {G9_TREE_FNS(g9_tree_join_deep_, q32), G9_TREE_FNS(g9_tree_join_deep_, q64)};
 // Up to this many rows (tokens by query heads) of the waves' form a block may be
 // cut into more than 32 parts, and a workgroup per row joins them faster than
 // one per block.
-constexpr int64_t kDeepRows = 1024;
+constexpr int64_t kDeepRows = 256;
 
 // The workspace: sums, first[], start[].
 struct Space {
   size_t floats, first, start, bytes;
 };
-Space space_of(bool wide, int64_t B, int64_t D) {
+Space space_of(int form, int64_t B, int64_t D) {
   Space s;
-  s.floats = part_floats(wide, D);
+  s.floats = part_floats(form, D);
   s.first = s.floats * 4;
   s.start = (s.first + (size_t)(B + 1) * 8 + 31) / 32 * 32;
   s.bytes = s.start + 1024 * sizeof(tree::Start);
@@ -862,7 +891,7 @@ Space space_of(bool wide, int64_t B, int64_t D) {
 
 extern "C" size_t g9_tree_workspace_size(int64_t B, int64_t T, int64_t HQ, int64_t HK, int64_t D) {
   if (B <= 0 || T <= 0 || HQ <= 0 || HK <= 0 || HQ % HK || D <= 0) return 0;
-  return space_of(wide_form(B, T, HQ / HK), B, D).bytes;
+  return space_of(form_of(B, T, HQ / HK), B, D).bytes;
 }
 
 extern "C" int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cache, void* o, float* lse,
@@ -893,8 +922,8 @@ extern "C" int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cac
       ((uintptr_t)tree_mask & 7))
     return G9_ERR_LAYOUT;
   const int64_t group = HQ / HK;
-  const bool wide = wide_form(B, T, group);
-  const Space sp = space_of(wide, B, D);
+  const int form = form_of(B, T, group);
+  const Space sp = space_of(form, B, D);
   if (!workspace || ((uintptr_t)workspace & 31) || workspace_bytes < sp.bytes) return G9_ERR_WORKSPACE;
   tree::Params p{};
   p.q = static_cast<const char*>(q);
@@ -918,11 +947,13 @@ extern "C" int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cac
   p.scale_log2 = sm_scale * fa::kLog2e;
   void* args[] = {&p};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (hipLaunchKernel(kRun[wide][D == 64][dtype == G9_BF16], dim3(tree::kWgs), dim3(wide ? fa::kThreads : 256), args, 0,
-                      st) != hipSuccess)
-    return G9_ERR_HIP;
   const int d64 = D == 64, bf16 = dtype == G9_BF16;
-  if (!wide && T * HQ <= kDeepRows)
-    return launched(hipLaunchKernel(kJoinDeep[d64][bf16], dim3((unsigned)(T * HQ)), dim3(tree::kDeepThreads), args, 0, st));
-  return launched(hipLaunchKernel(kJoin[wide][d64][bf16], dim3(wide ? 255 : 1023, wide ? 8 : 1), dim3(256), args, 0, st));
+  if (hipLaunchKernel(kRun[form][d64][bf16], dim3(tree::kWgs), dim3(form == Q256 ? fa::kThreads : 256), args, 0, st) !=
+      hipSuccess)
+    return G9_ERR_HIP;
+  if (form != Q256 && T * HQ <= kDeepRows)
+    return launched(hipLaunchKernel(kJoinDeep[form][d64][bf16], dim3((unsigned)(T * HQ)), dim3(tree::kDeepThreads), args, 0,
+                                    st));
+  const dim3 grid = form == Q256 ? dim3(255, 8) : dim3(1023, form == Q64 ? 2 : 1);
+  return launched(hipLaunchKernel(kJoin[form][d64][bf16], grid, dim3(256), args, 0, st));
 }
