@@ -43,7 +43,6 @@ struct Params {
   const int* cu;
   const unsigned long long* mask;                  // or null: a chain
   float* part;                                     // sums [2 kWorkers][kBlock][D], then (m, l) pairs
-  unsigned long long* first;                       // [B + 1]: first tile of each request on the line
   struct Start* start;                             // [kWorkers]: where each part begins
   long long q_t, q_h, o_t, o_h;                    // token / head strides, bytes
   long long k_b, k_h, v_b, v_h;                    // block / head strides, bytes
@@ -53,10 +52,9 @@ struct Params {
   int B, T, HQ, HK, group;
   float scale_log2;
 
-  // A query row: its node (-1: no row), its request's context, its mask.
+  // A query row: its node (-1: no row), its request's context and first query.
   struct Row {
-    int node, context;
-    const unsigned long long* mask;
+    int node, context, q0;
   };
   // Bit i: the row reads key k0 + i of `keys`.
   G9_DEV unsigned long long reads(const Row& r, int k0, int keys) const {
@@ -67,7 +65,8 @@ struct Params {
       w = c >= 64 ? ~0ull : c <= 0 ? 0 : (1ull << c) - 1;
     } else {
       const int first = max(n0, 0) >> 6, sh = max(n0, 0) & 63;
-      const unsigned long long a = first < words ? r.mask[first] : 0, b = first + 1 < words ? r.mask[first + 1] : 0;
+      const unsigned long long* const m = mask + (long long)(r.q0 + max(r.node, 0)) * words + first;
+      const unsigned long long a = first < words ? m[0] : 0, b = first + 1 < words ? m[1] : 0;
       w = sh ? a >> sh | b << (64 - sh) : a;
       if (n0 < 0) w = n0 <= -64 ? ~0ull : w << -n0 | ((1ull << -n0) - 1);
     }
@@ -139,10 +138,9 @@ struct Line {
   }
 
   // Where this worker's part begins, and its tiles.  The workgroup sums the
-  // requests' tiles into LDS (first[B + 1]); workgroup 0 leaves them in the
-  // workspace for the kernel that joins the parts.
+  // requests' tiles into LDS (first[B + 1]).
   template <int THREADS>
-  static G9_DEV int locate(const Params& p, char* smem, unsigned worker, bool publish, Place& at) {
+  static G9_DEV int locate(const Params& p, char* smem, unsigned worker, Place& at) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     unsigned long long* const first = reinterpret_cast<unsigned long long*>(smem);  // then the waves' sums
     unsigned long long* const sums = first + p.B + 1;
@@ -166,13 +164,9 @@ struct Line {
     }
     for (int b = b0; b < b1; ++b) {
       first[b] = before;
-      if (publish) p.first[b] = before;
       before += tiles_of(p, request(p, b));
     }
-    if (tid == 0) {
-      first[p.B] = total;
-      if (publish) p.first[p.B] = total;
-    }
+    if (tid == 0) first[p.B] = total;
     __syncthreads();
     total = uniform(total);
     int count = 0;
@@ -197,9 +191,10 @@ struct Line {
       at.hk = (int)quotient(unit, (unsigned)at.r.blocks);
       at.block = (int)(unit - (unsigned long long)at.hk * at.r.blocks);
       make_uniform(at);
-      if (THREADS == 64 * (kWorkers / kWgs) ? lane == 0 : tid == 0)
-        p.start[worker] = {at.r.q0, at.r.n, at.hk, at.block, at.tile, at.r.tiles, (u32)total, (u32)(total >> 32)};
     }
+    // Worker 0 says how long the line is, also where it is empty.
+    if ((worker == 0 || count > 0) && (THREADS == 64 * (kWorkers / kWgs) ? lane == 0 : tid == 0))
+      p.start[worker] = {at.r.q0, at.r.n, at.hk, at.block, at.tile, at.r.tiles, (u32)total, (u32)(total >> 32)};
     __syncthreads();  // first[] is read: what comes next takes its place
     return count;
   }
@@ -230,7 +225,7 @@ template <class L>
 G9_DEV Params::Row row_of(const Params& p, const Place& at, int row) {
   const int nd = (at.block * L::kBlock + row) / p.group;
   const bool in = nd < at.r.n;
-  return {in ? nd : -1, at.r.context, p.mask ? p.mask + (long long)(at.r.q0 + (in ? nd : 0)) * p.words : nullptr};
+  return {in ? nd : -1, at.r.context, at.r.q0};
 }
 template <class L>
 G9_DEV const char* query_of(const Params& p, const Place& at, int row, int node) {
@@ -302,7 +297,7 @@ struct Wave {
   u32x4 qf[NQ][kNS];
   f32x16 o[NQ][kND];
   float m[NQ], l[NQ];
-  Params::Row row[NQ];  // this lane's queries
+  int node[NQ];      // of this lane's queries, -1 where there is none
 
   G9_DEV explicit Wave(const Params& pp) : p(pp) {}
 
@@ -323,13 +318,14 @@ struct Wave {
 #pragma unroll
     for (int j = 0; j < 4; ++j) voffk[j] = r * p.k_t + 16 * (slot ^ swz_k(kRows * j + r));
     voffv[0] = r * p.v_t + 16 * (slot ^ swz_v(r));
-    const int jj = lane & 15;
-    ak = lds + col * kRow;
-    av = lds + kV + vrow() * kRow + 8 * (jj & 1);
+    // K: row col, chunk 2 s + h.  V's transposing reads: 16 lanes cover 4 rows and
+    // 16 values; lane jj of them addresses row jj / 4 and values 4 (jj % 4) of
+    // chunk 4 d + 2 (lane / 16 % 2) + jj / 2 % 2.  Steps and blocks come in by XOR
+    // (of whole bit fields: the rows are aligned to their size).
+    const int jj = lane & 15, r4 = 4 * h + (jj >> 2);
+    ak = lds + col * kRow + 16 * (h ^ swz_k(col));
+    av = lds + kV + r4 * kRow + 16 * ((2 * (lane >> 4 & 1) + ((jj & 3) >> 1)) ^ swz_v(r4)) + 8 * (jj & 1);
   }
-  // V's transposing reads: 16 lanes cover 4 rows and 16 values; lane jj of them
-  // addresses row jj / 4, values 4 (jj % 4).
-  G9_DEV int vrow() const { return 4 * h + ((lane & 15) >> 2); }
 
   // The 16-row pieces' pages of a tile; -1: none.
   G9_DEV void pages(const Place& at, int (&pg)[kPieces]) const {
@@ -362,8 +358,8 @@ struct Wave {
   G9_DEV void begin(const Place& at) {
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
-      row[t] = row_of<L>(p, at, 32 * t + col);
-      const char* const qrow = query_of<L>(p, at, 32 * t + col, row[t].node);
+      node[t] = row_of<L>(p, at, 32 * t + col).node;
+      const char* const qrow = query_of<L>(p, at, 32 * t + col, node[t]);
 #pragma unroll
       for (int s = 0; s < kNS; ++s) qf[t][s] = *reinterpret_cast<const u32x4*>(qrow + (16 * s + 8 * h) * 2);
       // Finite, so that a row that has read nothing yet has weights 2^(-inf - m) =
@@ -379,12 +375,12 @@ struct Wave {
 
   G9_DEV void tile(const Place& at, int stage, bool tail) {
     f32x16 sc[NQ][kNB];
+    const u32 ak_s = ak + stage * kStage, av_s = av + stage * kStage;
 #pragma unroll
     for (int s = 0; s < kNS; ++s)
 #pragma unroll
       for (int b = 0; b < kNB; ++b) {
-        const u32x4 kf = *(const G9_LDS u32x4*)(uintptr_t)(ak + stage * kStage + 32 * b * kRow +
-                                                           16 * ((2 * s + h) ^ swz_k(col)));
+        const u32x4 kf = *(const G9_LDS u32x4*)(uintptr_t)((ak_s ^ (32 * s)) + 32 * b * kRow);
 #pragma unroll
         for (int t = 0; t < NQ; ++t) sc[t][b] = mfma<BF16>(kf, qf[t][s], s ? sc[t][b] : f32x16{});
       }
@@ -392,7 +388,7 @@ struct Wave {
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
       if (tail) {
-        const unsigned long long w = p.reads(row[t], at.tile * kKeys, at.r.keys);
+        const unsigned long long w = p.reads({node[t], at.r.context, at.r.q0}, at.tile * kKeys, at.r.keys);
 #pragma unroll
         for (int b = 0; b < kNB; ++b) {
           const u32 bits = (u32)(w >> (32 * b)) >> (4 * h);
@@ -433,9 +429,8 @@ struct Wave {
     for (int k = 0; k < kKS; ++k)
 #pragma unroll
       for (int d = 0; d < kND; ++d) {
-        // Rows vrow and vrow + 8 of the step: swz_v of both is the same.
-        const u32 a = av + stage * kStage + 16 * k * kRow +
-                      16 * ((4 * d + 2 * (lane >> 4 & 1) + ((lane & 3) >> 1)) ^ swz_v(vrow()));
+        // And the rows 8 below: their chunks are permuted alike.
+        const u32 a = (av_s ^ (64 * d)) + 16 * k * kRow;
         const u32x2 lo = tr_read(a), hi = tr_read(a + 8 * kRow);
         const u32x4 vf = {lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
@@ -467,7 +462,7 @@ struct Wave {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           *reinterpret_cast<u32*>(prow + 16 * k + 8 * (e >> 1) + 4 * h + 2 * (e & 1)) = pf[t][k][e];
-      const unsigned long long w = p.reads(row[t], at.tile * kKeys, at.r.keys);
+      const unsigned long long w = p.reads({node[t], at.r.context, at.r.q0}, at.tile * kKeys, at.r.keys);
       waitcnt<63, 0>();
 #pragma unroll 1
       for (int key = 0; key < kKeys; ++key) {
@@ -513,8 +508,8 @@ G9_DEV void narrow(const Params& p, char* smem) {
   using L = Narrow<HD, NQ>;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned worker = my_part() * 4 + wave;
-  Place cur;
-  const int count = L::template locate<256>(p, smem, worker, my_part() == 0, cur);
+  Place cur{};
+  const int count = L::template locate<256>(p, smem, worker, cur);
   if (count <= 0) return;
 
   W w(p);
@@ -562,7 +557,7 @@ G9_DEV void narrow(const Params& p, char* smem) {
 #pragma unroll
       for (int t = 0; t < NQ; ++t)
         finish<BF16, HD, L>(p, cur, last && from_start ? -1 : (int)(2 * worker + (from_start ? 1 : 0)), 32 * t + w.col,
-                            w.row[t].node, w.o[t], w.m[t], w.l[t]);
+                            w.node[t], w.o[t], w.m[t], w.l[t]);
       from_start = true;
     }
     cur = nxt;
@@ -584,8 +579,8 @@ G9_DEV void wide(const Params& p, char* smem) {
   using PipeT = typename WidePipe<BF16, HD>::T;
   static_assert(PipeT::kBN == L::kKeys && kBlockM == L::kBlock);
   const unsigned worker = my_part();
-  Place cur;
-  int count = L::template locate<kThreads>(p, smem, worker, worker == 0, cur);
+  Place cur{};
+  int count = L::template locate<kThreads>(p, smem, worker, cur);
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   PipeT P(p);
   P.wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -690,122 +685,94 @@ G9_DEV void store4(const Params& p, long long tok, int hq, int c, f32x4 sum, flo
   if (p.lse && c == 0) p.lse[(long long)hq * p.T + tok] = none ? -__builtin_inff() : (m + __builtin_log2f(l)) * kLn2;
 }
 
-// Joins the block that worker blockIdx.x + 1's part begins in the middle of, if
-// that worker is the second of the block's (each split block has one such); 32
-// rows a workgroup.  The parts of a block are few here: every thread sums its
-// four columns of four rows over all of them.
+// Joins the blocks that are cut.  A block of n parts has the n - 1 workers whose
+// parts begin within it, and with each of them a workgroup here (blockIdx.x + 1):
+// they (and gridDim.y times as many) share its rows, so that a workgroup's work
+// is a fraction of a part, however many parts a long request's blocks have.
+constexpr int kJoinThreads = 512;
 template <bool BF16, int HD, class L>
-G9_DEV void join(const Params& p) {
+G9_DEV void join(const Params& p, float* lds) {
   const unsigned w = blockIdx.x + 1;
+  const Start zero = p.start[0];
+  const unsigned long long total = (unsigned long long)zero.total_hi << 32 | zero.total_lo;
+  if (w >= L::workers(total)) return;
   const Start st = p.start[w];
-  const unsigned long long total = (unsigned long long)st.total_hi << 32 | st.total_lo;
-  // Workers behind the line's last have left no start: the line's own length
-  // says how many there are.
-  if (w >= L::workers(p.first[p.B]) || st.tile == 0) return;
+  if (st.tile == 0) return;
   const unsigned long long u0 = L::part_begin(w, total) - (unsigned)st.tile;
-  const unsigned w0 = L::worker_of(u0, total);
-  if (w0 != w - 1) return;
-  const unsigned n = L::worker_of(u0 + st.tiles - 1, total) - w0 + 1;
-  // Worker w0 has it in slot 1 unless it began the block before its part; the
+  const unsigned w0 = L::worker_of(u0, total), n = L::worker_of(u0 + st.tiles - 1, total) - w0 + 1;
+  // Worker w0 has the block in slot 1 unless it began it before its part; the
   // others in slot 0.
   const size_t head = (size_t)2 * w0 + (L::part_begin(w0, total) <= u0 ? 1 : 0);
   const float* const ml = p.part + (size_t)2 * L::kWorkers * L::kBlock * HD;
-  constexpr int kCols = HD / 4, kRowsAtOnce = 256 / kCols;
-  const int c = threadIdx.x % kCols;
-#pragma unroll 1
-  for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
-    const int in = blockIdx.y * 32 + i * kRowsAtOnce + threadIdx.x / kCols;
-    const long long row = (long long)st.block * L::kBlock + in;
-    if (row >= (long long)st.n * p.group) break;
-    f32x4 sum = {};
-    float m = -3.0e38f, l = 0.f;
-    constexpr unsigned kAtOnce = 8;  // parts asked for together
-    for (unsigned k0 = 0; k0 < n; k0 += kAtOnce) {
+  const int row0 = st.block * L::kBlock;
+  const u32 rows = (u32)min((long long)st.n * p.group - row0, (long long)L::kBlock);
+  const u32 share = (w - w0 - 1) * gridDim.y + blockIdx.y, shares = (n - 1) * gridDim.y;
+  const u32 from = share * rows / shares, to = (share + 1) * rows / shares;
+  constexpr unsigned kCols = HD / 4, kLanes = kJoinThreads / kCols;
+  const unsigned c = threadIdx.x % kCols, lane = threadIdx.x / kCols;
+  f32x4 sum;
+  float m, l;
+  const auto clear = [&] { sum = f32x4{}, m = -3.0e38f, l = 0.f; };
+  const auto add = [&](f32x4 x, float mk, float lk) {
+    const float m_new = __builtin_fmaxf(m, mk);
+    const float f = __builtin_amdgcn_exp2f(m - m_new), g = __builtin_amdgcn_exp2f(mk - m_new);
+    l = l * f + lk * g;
+    sum = sum * f + x * g;
+    m = m_new;
+  };
+  // Adds the row's parts k0, k0 + step, ..., kAtOnce of them asked for together.
+  const auto add_parts = [&]<unsigned kAtOnce>(unsigned in, unsigned k0, unsigned step) {
+    for (unsigned k = k0; k < n; k += kAtOnce * step) {
       float mk[kAtOnce], lk[kAtOnce];
       f32x4 x[kAtOnce];
 #pragma unroll
       for (unsigned e = 0; e < kAtOnce; ++e) {
-        const unsigned k = min(k0 + e, n - 1);
-        const size_t a = (k ? (size_t)2 * (w0 + k) : head) * L::kBlock + in;
+        const unsigned i = min(k + e * step, n - 1);
+        const size_t a = (i ? (size_t)2 * (w0 + i) : head) * L::kBlock + in;
         mk[e] = ml[a * 2], lk[e] = ml[a * 2 + 1];
         x[e] = *reinterpret_cast<const f32x4*>(p.part + a * HD + 4 * c);
       }
 #pragma unroll
-      for (unsigned e = 0; e < kAtOnce; ++e) {
-        if (k0 + e >= n) break;
-        const float m_new = __builtin_fmaxf(m, mk[e]);
-        const float f = __builtin_amdgcn_exp2f(m - m_new), g = __builtin_amdgcn_exp2f(mk[e] - m_new);
-        l = l * f + lk[e] * g;
-        sum = sum * f + x[e] * g;
-        m = m_new;
-      }
+      for (unsigned e = 0; e < kAtOnce; ++e)
+        if (k + e * step < n) add(x[e], mk[e], lk[e]);
     }
-    const int nd = (int)(row / p.group);
-    store4<BF16>(p, st.q0 + nd, st.hk * p.group + (int)(row - (long long)nd * p.group), c, sum, m, l);
+  };
+  const auto store = [&](unsigned in) {
+    const int row = row0 + (int)in, nd = row / p.group;
+    store4<BF16>(p, st.q0 + nd, st.hk * p.group + row - nd * p.group, c, sum, m, l);
+  };
+  // Round trips to memory: a row per 16-byte column group of threads, its parts
+  // eight at a time, or the threads sharing a row's parts, and the row's join in
+  // LDS behind them.
+  const u32 r = to - from;
+  if ((r + kLanes - 1) / kLanes * ((n + 7) / 8) <= 2 * r) {
+    for (unsigned in = from + lane; in < to; in += kLanes) {
+      clear();
+      if (n <= 3)
+        add_parts.template operator()<3>(in, 0, 1);
+      else
+        add_parts.template operator()<8>(in, 0, 1);
+      store(in);
+    }
+    return;
   }
-}
-
-// The same for a few query rows whose blocks are cut into many parts: one
-// workgroup per row (token t, head hq), its threads HD / 4 columns by kParts
-// parts.
-constexpr int kDeepThreads = 1024;
-template <bool BF16, int HD, class L>
-G9_DEV void join_deep(const Params& p, float* lds) {
-  constexpr int kCols = HD / 4, kParts = kDeepThreads / kCols;
-  const int t = blockIdx.x / p.HQ, hq = blockIdx.x - t * p.HQ;
-  const int tid = threadIdx.x, lane = tid & 63, c = tid % kCols, s = tid / kCols;
-  // The request of row t: the number of sequence ends at or before it, 64
-  // candidates at a time.
-  int lo = 0, hi = p.B;
-  while (lo < hi) {
-    const int step = (hi - lo + 63) / 64, at = lo + (lane + 1) * step - 1;
-    const int full = __popcll(__builtin_amdgcn_ballot_w64(at < hi && p.cu[at + 1] <= t));
-    lo += full * step;
-    hi = min(hi, lo + step - 1);
+  for (unsigned in = from; in < to; ++in) {
+    clear();
+    add_parts.template operator()<8>(in, lane, kLanes);
+    float* const mine = lds + threadIdx.x * 7;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) mine[e] = sum[e];
+    mine[4] = m, mine[5] = l;
+    __syncthreads();
+    if (lane == 0) {
+      for (unsigned i = 1; i < kLanes; ++i) {
+        const float* const o = lds + (i * kCols + c) * 7;
+        add(f32x4{o[0], o[1], o[2], o[3]}, o[4], o[5]);
+      }
+      store(in);
+    }
+    __syncthreads();
   }
-  if (lo >= p.B) return;
-  const Req r = L::request(p, lo);
-  const int nd = t - r.q0, hk = hq / p.group;
-  if (nd < 0 || nd >= r.n) return;
-  const int row = nd * p.group + hq - hk * p.group;
-  const int block = row / L::kBlock, in = row - block * L::kBlock;
-  const unsigned long long total = p.first[p.B];
-  const unsigned long long u0 = p.first[lo] + ((unsigned long long)hk * r.blocks + block) * r.tiles;
-  const unsigned w0 = L::worker_of(u0, total), n = L::worker_of(u0 + r.tiles - 1, total) - w0 + 1;
-  if (n == 1) return;  // finished by its worker
-  const float* const ml = p.part + (size_t)2 * L::kWorkers * L::kBlock * HD;
-  const size_t head = (size_t)2 * w0 + (L::part_begin(w0, total) <= u0 ? 1 : 0);
-  const auto at = [&](unsigned k) { return (k ? (size_t)2 * (w0 + k) : head) * L::kBlock + in; };
-  float top = -3.0e38f;
-  for (unsigned k = tid; k < n; k += kDeepThreads) top = __builtin_fmaxf(top, ml[at(k) * 2]);
-#pragma unroll
-  for (int d = 32; d; d >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, d, 64));
-  if (lane == 0) lds[tid >> 6] = top;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kDeepThreads / 64; ++i) top = __builtin_fmaxf(top, lds[i]);
-  f32x4 sum = {};
-  float l = 0.f;
-  for (unsigned k = s; k < n; k += kParts) {
-    const size_t a = at(k);
-    const float f = __builtin_amdgcn_exp2f(ml[a * 2] - top);
-    l += f * ml[a * 2 + 1];
-    sum += f * *reinterpret_cast<const f32x4*>(p.part + a * HD + 4 * c);
-  }
-  __syncthreads();
-  float* const mine = lds + (s * kCols + c) * 5;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) mine[e] = sum[e];
-  mine[4] = l;
-  __syncthreads();
-  if (tid >= kCols) return;
-  for (int i = 1; i < kParts; ++i) {
-    const float* const other = lds + (i * kCols + c) * 5;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sum[e] += other[e];
-    l += other[4];
-  }
-  store4<BF16>(p, t, hq, c, sum, top, l);
 }
 
 }  // namespace tree
@@ -820,12 +787,9 @@ using namespace g9::host;
     __shared__ __attribute__((aligned(1024))) char smem[4 * tree::Wave<BF16, HD, NQ>::kWaveLds];               \
     tree::narrow<BF16, HD, NQ>(p, smem);                                                                      \
   }                                                                                                           \
-  extern "C" __global__ __launch_bounds__(256) void g9_tree_join_##NAME(tree::Params p) {                     \
-    tree::join<BF16, HD, tree::Narrow<HD, NQ>>(p);                                                            \
-  }                                                                                                           \
-  extern "C" __global__ __launch_bounds__(tree::kDeepThreads) void g9_tree_join_deep_##NAME(tree::Params p) { \
-    __shared__ float lds[tree::kDeepThreads * 5];                                                             \
-    tree::join_deep<BF16, HD, tree::Narrow<HD, NQ>>(p, lds);                                                  \
+  extern "C" __global__ __launch_bounds__(tree::kJoinThreads) void g9_tree_join_##NAME(tree::Params p) {      \
+    __shared__ float lds[tree::kJoinThreads * 7];                                                             \
+    tree::join<BF16, HD, tree::Narrow<HD, NQ>>(p, lds);                                                       \
   }
 #define G9_TREE_WIDE(NAME, BF16, HD)                                                                          \
   extern "C" __global__ __launch_bounds__(fa::kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void       \
@@ -833,65 +797,57 @@ using namespace g9::host;
     __shared__ __attribute__((aligned(1024))) char smem[tree::WidePipe<BF16, HD>::kLds];                       \
     tree::wide<BF16, HD>(p, smem);                                                                            \
   }                                                                                                           \
-  extern "C" __global__ __launch_bounds__(256) void g9_tree_join_##NAME(tree::Params p) {                     \
-    tree::join<BF16, HD, tree::Wide<HD>>(p);                                                                  \
+  extern "C" __global__ __launch_bounds__(tree::kJoinThreads) void g9_tree_join_##NAME(tree::Params p) {      \
+    __shared__ float lds[tree::kJoinThreads * 7];                                                             \
+    tree::join<BF16, HD, tree::Wide<HD>>(p, lds);                                                             \
   }
-#define G9_TREE_KERNELS(NAME, BF16, HD)      \
-  G9_TREE_NARROW(NAME##_q32, BF16, HD, 1)    \
-  G9_TREE_NARROW(NAME##_q64, BF16, HD, 2)    \
-  G9_TREE_WIDE(NAME##_q256, BF16, HD)
-G9_TREE_KERNELS(bf16, true, 128)
-G9_TREE_KERNELS(f16, false, 128)
-G9_TREE_KERNELS(bf16_d64, true, 64)
-G9_TREE_KERNELS(f16_d64, false, 64)
-
-#ifndef G9_WIDE_ROWS
-#define G9_WIDE_ROWS 64
-#endif
+G9_TREE_NARROW(bf16_q32, true, 128, 1)
+G9_TREE_NARROW(f16_q32, false, 128, 1)
+G9_TREE_NARROW(bf16_d64_q32, true, 64, 1)
+G9_TREE_NARROW(f16_d64_q32, false, 64, 1)
+G9_TREE_NARROW(bf16_d64_q64, true, 64, 2)
+G9_TREE_NARROW(f16_d64_q64, false, 64, 2)
+G9_TREE_WIDE(bf16_q256, true, 128)
+G9_TREE_WIDE(f16_q256, false, 128)
+G9_TREE_WIDE(bf16_d64_q256, true, 64)
+G9_TREE_WIDE(f16_d64_q256, false, 64)
 
 namespace {
 
 // Query rows of a block, by the rows that the requests of a batch bring on
-// average to one K/V head.
+// average to one K/V head.  Measured (us, without the joins), 8 K/V heads, one
+// MI355X: head dim 128, 16 x 6000 tokens: 40 rows 101 in blocks of 256 against
+// 119 of 64, 128 rows 138 and 203; so 64 is not built.  Head dim 64, whose
+// blocks of 256 spill: 40 rows 58 of 64 and 96 of 256, 128 rows 99 and 99, 256
+// rows 173 and 112.
 enum { Q32, Q64, Q256 };
-int form_of(int64_t B, int64_t T, int64_t group) {
+int form_of(int64_t B, int64_t T, int64_t group, int64_t D) {
   const int64_t rows = (T + B - 1) / B * group;
-  return rows <= 32 ? Q32 : rows <= G9_WIDE_ROWS ? Q64 : Q256;
+  return rows <= 32 ? Q32 : D == 64 && rows <= 128 ? Q64 : Q256;
 }
 // The sums of 2 x 1024 blocks of 32 or 64 rows, or of 2 x 256 of 256.
 size_t part_floats(int form, int64_t D) { return (size_t)2 * (form == Q32 ? 1024 * 32 : 1024 * 64) * (D + 2); }
 
-#define G9_TREE_FNS(WHAT, Q)                                                                          \
-  {{reinterpret_cast<const void*>(WHAT##f16_##Q), reinterpret_cast<const void*>(WHAT##bf16_##Q)},     \
-   {reinterpret_cast<const void*>(WHAT##f16_d64_##Q), reinterpret_cast<const void*>(WHAT##bf16_d64_##Q)}}
+#define G9_TREE_FN(WHAT, Q) {reinterpret_cast<const void*>(WHAT##f16_##Q), reinterpret_cast<const void*>(WHAT##bf16_##Q)}
+#define G9_TREE_FN64(WHAT, Q) \
+  {reinterpret_cast<const void*>(WHAT##f16_d64_##Q), reinterpret_cast<const void*>(WHAT##bf16_d64_##Q)}
 // [form][head dim 64][bf16]
-const void* const kRun[3][2][2] = {G9_TREE_FNS(g9_tree_, q32), G9_TREE_FNS(g9_tree_, q64), G9_TREE_FNS(g9_tree_, q256)};
-const void* const kJoin[3][2][2] = {G9_TREE_FNS(g9_tree_join_, q32), G9_TREE_FNS(g9_tree_join_, q64),
-                                    G9_TREE_FNS(g9_tree_join_, q256)};
-const void* const kJoinDeep[2][2][2] = {G9_TREE_FNS(g9_tree_join_deep_, q32), G9_TREE_FNS(g9_tree_join_deep_, q64)};
-// Up to this many rows (tokens by query heads) of the waves' form a block may be
-// cut into more than 32 parts, and a workgroup per row joins them faster than
-// one per block.
-constexpr int64_t kDeepRows = 256;
+const void* const kRun[3][2][2] = {{G9_TREE_FN(g9_tree_, q32), G9_TREE_FN64(g9_tree_, q32)},
+                                   {{nullptr, nullptr}, G9_TREE_FN64(g9_tree_, q64)},
+                                   {G9_TREE_FN(g9_tree_, q256), G9_TREE_FN64(g9_tree_, q256)}};
+const void* const kJoin[3][2][2] = {{G9_TREE_FN(g9_tree_join_, q32), G9_TREE_FN64(g9_tree_join_, q32)},
+                                    {{nullptr, nullptr}, G9_TREE_FN64(g9_tree_join_, q64)},
+                                    {G9_TREE_FN(g9_tree_join_, q256), G9_TREE_FN64(g9_tree_join_, q256)}};
 
-// The workspace: sums, first[], start[].
-struct Space {
-  size_t floats, first, start, bytes;
-};
-Space space_of(int form, int64_t B, int64_t D) {
-  Space s;
-  s.floats = part_floats(form, D);
-  s.first = s.floats * 4;
-  s.start = (s.first + (size_t)(B + 1) * 8 + 31) / 32 * 32;
-  s.bytes = s.start + 1024 * sizeof(tree::Start);
-  return s;
-}
+// The workspace: sums, then start[].
+size_t start_at(int form, int64_t D) { return (part_floats(form, D) * 4 + 31) / 32 * 32; }
+size_t workspace_of(int form, int64_t D) { return start_at(form, D) + 1024 * sizeof(tree::Start); }
 
 }  // namespace
 
 extern "C" size_t g9_tree_workspace_size(int64_t B, int64_t T, int64_t HQ, int64_t HK, int64_t D) {
   if (B <= 0 || T <= 0 || HQ <= 0 || HK <= 0 || HQ % HK || D <= 0) return 0;
-  return space_of(form_of(B, T, HQ / HK), B, D).bytes;
+  return workspace_of(form_of(B, T, HQ / HK, D), D);
 }
 
 extern "C" int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cache, void* o, float* lse,
@@ -922,9 +878,8 @@ extern "C" int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cac
       ((uintptr_t)tree_mask & 7))
     return G9_ERR_LAYOUT;
   const int64_t group = HQ / HK;
-  const int form = form_of(B, T, group);
-  const Space sp = space_of(form, B, D);
-  if (!workspace || ((uintptr_t)workspace & 31) || workspace_bytes < sp.bytes) return G9_ERR_WORKSPACE;
+  const int form = form_of(B, T, group, D);
+  if (!workspace || ((uintptr_t)workspace & 31) || workspace_bytes < workspace_of(form, D)) return G9_ERR_WORKSPACE;
   tree::Params p{};
   p.q = static_cast<const char*>(q);
   p.kc = static_cast<const char*>(k_cache);
@@ -936,8 +891,7 @@ extern "C" int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cac
   p.cu = cu_q;
   p.mask = reinterpret_cast<const unsigned long long*>(tree_mask);
   p.part = static_cast<float*>(workspace);
-  p.first = reinterpret_cast<unsigned long long*>(static_cast<char*>(workspace) + sp.first);
-  p.start = reinterpret_cast<tree::Start*>(static_cast<char*>(workspace) + sp.start);
+  p.start = reinterpret_cast<tree::Start*>(static_cast<char*>(workspace) + start_at(form, D));
   p.q_t = q_strides[0] * 2, p.q_h = q_strides[1] * 2, p.o_t = o_strides[0] * 2, p.o_h = o_strides[1] * 2;
   p.k_b = kc_strides[0] * 2, p.k_h = kc_strides[2] * 2, p.v_b = vc_strides[0] * 2, p.v_h = vc_strides[2] * 2;
   p.k_t = (u32)(kc_strides[1] * 2), p.v_t = (u32)(vc_strides[1] * 2);
@@ -951,9 +905,6 @@ extern "C" int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cac
   if (hipLaunchKernel(kRun[form][d64][bf16], dim3(tree::kWgs), dim3(form == Q256 ? fa::kThreads : 256), args, 0, st) !=
       hipSuccess)
     return G9_ERR_HIP;
-  if (form != Q256 && T * HQ <= kDeepRows)
-    return launched(hipLaunchKernel(kJoinDeep[form][d64][bf16], dim3((unsigned)(T * HQ)), dim3(tree::kDeepThreads), args, 0,
-                                    st));
-  const dim3 grid = form == Q256 ? dim3(255, 8) : dim3(1023, form == Q64 ? 2 : 1);
-  return launched(hipLaunchKernel(kJoin[form][d64][bf16], grid, dim3(256), args, 0, st));
+  return launched(hipLaunchKernel(kJoin[form][d64][bf16], dim3(form == Q256 ? 255 : 1023, form == Q256 ? 4 : 1),
+                                  dim3(tree::kJoinThreads), args, 0, st));
 }
