@@ -34,7 +34,7 @@ SOURCES = ["g9_capi.hip", "g9_tile.hip", "g9_quant.hip", "g9_fmha.hip", "g9_varl
 # their exponentials are NaN).
 SOURCE_FLAGS = {s: ["-fno-honor-nans"] for s in ("g9_fmha.hip", "g9_varlen.hip", "g9_tree.hip")}
 HEADERS = ["g9_common.hpp", "g9_gemm.hpp", "g9_tile.hpp", "g9_tile_pick.hpp",
-           "g9_fmha_pipe.hpp", "g9_attn_host.hpp"]
+           "g9_fmha_pipe.hpp", "g9_wave.hpp", "g9_attn_host.hpp"]
 
 # -packed-fp32-ops: keep the compiler from forming v_pk_*_f32, whose results
 # have been unreliable on the target machines.

@@ -11,11 +11,8 @@
 // stages of 8 KB of K and 8 KB of V, filled by LDS-DMA), so no wave ever waits
 // for another one: there is no barrier in the loop.
 //
-// Per tile a wave computes S^T = K Q^T and O^T += V^T P^T with 32x32x16 MFMAs in
-// the register layouts that g9_fmha.hip describes: the scores are the second
-// product's operand as they stand, V is read by transposing LDS reads.  Blocks
-// of 32 rows are half empty where a request brings fewer, which costs nothing:
-// the matrix unit is idle most of the time.
+// Blocks of 32 rows are half empty where a request brings fewer, which costs
+// nothing: the matrix unit is idle most of the time (g9_wave.hpp has the tile).
 //
 // A block of rows whose tiles lie in one wave's part is finished there.  Else
 // each wave writes its unnormalized sum, maximum and weight to the workspace and
@@ -23,7 +20,7 @@
 // depends on no timing.
 #include "../../include/gfx950_fmha.h"
 #include "g9_attn_host.hpp"
-#include "g9_fmha_pipe.hpp"
+#include "g9_wave.hpp"
 
 namespace g9 {
 namespace tree {
@@ -96,16 +93,6 @@ G9_DEV unsigned long long quotient(unsigned long long x, unsigned long long y) {
   return (x | y) >> 32 ? x / y : (unsigned long long)((u32)x / (u32)y);
 }
 
-template <class V>
-G9_DEV V uniform(V x) {
-  if constexpr (sizeof(V) == 8) {
-    const unsigned long long u = (unsigned long long)x;
-    const u32 lo = (u32)__builtin_amdgcn_readfirstlane((int)u), hi = (u32)__builtin_amdgcn_readfirstlane((int)(u >> 32));
-    return (V)((unsigned long long)hi << 32 | lo);
-  } else {
-    return (V)__builtin_amdgcn_readfirstlane((int)x);
-  }
-}
 G9_DEV void make_uniform(Place& a) {
   for (int* x : {&a.r.q0, &a.r.n, &a.r.context, &a.r.keys, &a.r.blocks, &a.r.tiles, &a.b, &a.hk, &a.block, &a.tile})
     *x = uniform(*x);
@@ -271,240 +258,48 @@ G9_DEV void finish(const Params& p, const Place& at, int slot, int row, int node
   if (p.lse && h == 0) p.lse[(long long)hq * p.T + tok] = none ? -__builtin_inff() : (m + __builtin_log2f(lt)) * kLn2;
 }
 
-// NQ groups of 32 query rows, which share every K and V register read from LDS.
-template <bool BF16, int HD, int NQ>
-struct Wave {
-  using L = Narrow<HD, NQ>;
-  static constexpr int kKeys = L::kKeys;           // keys per tile
-  static constexpr int kNB = kKeys / 32;           // 32-key score blocks
-  static constexpr int kNS = HD / 16;              // QK steps of 16 head-dim values
-  static constexpr int kKS = kKeys / 16;           // PV steps of 16 keys
-  static constexpr int kND = HD / 32;              // PV blocks of 32 head-dim values
-  static constexpr int kRow = HD * 2;              // bytes of a row
-  static constexpr int kRows = 1024 / kRow;        // rows of one DMA
-  static constexpr int kPieces = kKeys / 16;       // 16-row pieces: never across a page
-  static constexpr int kDmas = 8;                  // per tile and operand
-  static constexpr int kStage = 16384, kV = 8192;  // a stage; V behind K
-  static constexpr int kScratch = 32 * kKeys * 2;  // P of one tile and 32 rows, 16 bit
-  static constexpr int kWaveLds = 2 * kStage + kScratch;
-
-  const Params& p;
-  int lane, h, col;  // lane, lane / 32, lane % 32
-  u32 lds;           // this wave's LDS
-  char* scratch;
-  u32 voffk[4], voffv[1];
-  u32 ak, av;        // LDS read bases in a stage (K, V)
-  u32x4 qf[NQ][kNS];
-  f32x16 o[NQ][kND];
-  float m[NQ], l[NQ];
-  int node[NQ];      // of this lane's queries, -1 where there is none
-
-  G9_DEV explicit Wave(const Params& pp) : p(pp) {}
-
-  // LDS layout of a tile: rows of kRow bytes, their 16-byte chunks permuted
-  // within the row so that a read of one chunk from 16 rows (K), or of 64 bytes
-  // from 4 rows (V), touches every bank once.  Chunk c of row r is at slot c ^
-  // swz(r).  An LDS-DMA writes lane i's 16 bytes at 16 i, so lane i fetches the
-  // chunk that belongs there; a wave's DMA reads whole rows.
-  static G9_DEV int swz_k(int r) { return HD == 128 ? r & 15 : (r >> 1) & 7; }
-  static G9_DEV int swz_v(int r) { return HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); }
-
-  G9_DEV void init(char* smem, int wave) {
-    lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
-    lds = (u32)(uintptr_t)to_lds(smem) + wave * kWaveLds;
-    scratch = smem + wave * kWaveLds + 2 * kStage;
-    constexpr int kPer = kRow / 16;  // chunks of a row
-    const int r = lane / kPer, slot = lane % kPer;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) voffk[j] = r * p.k_t + 16 * (slot ^ swz_k(kRows * j + r));
-    voffv[0] = r * p.v_t + 16 * (slot ^ swz_v(r));
-    // K: row col, chunk 2 s + h.  V's transposing reads: 16 lanes cover 4 rows and
-    // 16 values; lane jj of them addresses row jj / 4 and values 4 (jj % 4) of
-    // chunk 4 d + 2 (lane / 16 % 2) + jj / 2 % 2.  Steps and blocks come in by XOR
-    // (of whole bit fields: the rows are aligned to their size).
-    const int jj = lane & 15, r4 = 4 * h + (jj >> 2);
-    ak = lds + col * kRow + 16 * (h ^ swz_k(col));
-    av = lds + kV + r4 * kRow + 16 * ((2 * (lane >> 4 & 1) + ((jj & 3) >> 1)) ^ swz_v(r4)) + 8 * (jj & 1);
-  }
-
-  // The 16-row pieces' pages of a tile; -1: none.
-  G9_DEV void pages(const Place& at, int (&pg)[kPieces]) const {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int k = at.tile * kKeys + 16 * i;
-      pg[i] = k < at.r.keys ? p.table[at.b * p.table_stride + (k >> p.shift)] : -1;
-    }
-  }
-  G9_DEV void fill(const Place& at, const int (&pg)[kPieces], int stage) const {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int k = at.tile * kKeys + 16 * i, off = k & ((1 << p.shift) - 1);
-      const bool in = (u32)pg[i] < (u32)p.num_blocks;
-      const int rows = in ? min(max(at.r.keys - k, 0), 16) : 0;
-      const long long page = in ? pg[i] : 0;
-      const rsrc_t rk = make_rsrc(uniform(p.kc + page * p.k_b + at.hk * p.k_h + (unsigned long long)off * p.k_t),
-                                  uniform((u32)rows * p.k_t));
-      const rsrc_t rv = make_rsrc(uniform(p.vc + page * p.v_b + at.hk * p.v_h + (unsigned long long)off * p.v_t),
-                                  uniform((u32)rows * p.v_t));
-#pragma unroll
-      for (int jj = 0; jj < 16 / kRows; ++jj) {
-        const int j = i * (16 / kRows) + jj;
-        dma16_fresh(rk, lds + stage * kStage + j * 1024, voffk[j & (HD == 128 ? 3 : 1)], jj * kRows * p.k_t);
-        dma16_fresh(rv, lds + stage * kStage + kV + j * 1024, voffv[0], jj * kRows * p.v_t);
-      }
-    }
-  }
-
-  G9_DEV void begin(const Place& at) {
-#pragma unroll
-    for (int t = 0; t < NQ; ++t) {
-      node[t] = row_of<L>(p, at, 32 * t + col).node;
-      const char* const qrow = query_of<L>(p, at, 32 * t + col, node[t]);
-#pragma unroll
-      for (int s = 0; s < kNS; ++s) qf[t][s] = *reinterpret_cast<const u32x4*>(qrow + (16 * s + 8 * h) * 2);
-      // Finite, so that a row that has read nothing yet has weights 2^(-inf - m) =
-      // 0 and a sum of 0, not NaN.
-      m[t] = -3.0e38f, l[t] = 0.f;
-#pragma unroll
-      for (int d = 0; d < kND; ++d) o[t][d] = f32x16{};
-    }
-    // Waited for here: the compiler does not count the DMAs in flight, and a wait
-    // of its own at the first use would be one in every tile.
-    waitcnt<0, 0>();
-  }
-
-  G9_DEV void tile(const Place& at, int stage, bool tail) {
-    f32x16 sc[NQ][kNB];
-    const u32 ak_s = ak + stage * kStage, av_s = av + stage * kStage;
-#pragma unroll
-    for (int s = 0; s < kNS; ++s)
-#pragma unroll
-      for (int b = 0; b < kNB; ++b) {
-        const u32x4 kf = *(const G9_LDS u32x4*)(uintptr_t)((ak_s ^ (32 * s)) + 32 * b * kRow);
-#pragma unroll
-        for (int t = 0; t < NQ; ++t) sc[t][b] = mfma<BF16>(kf, qf[t][s], s ? sc[t][b] : f32x16{});
-      }
-    u32x4 pf[NQ][kKS];
-#pragma unroll
-    for (int t = 0; t < NQ; ++t) {
-      if (tail) {
-        const unsigned long long w = p.reads({node[t], at.r.context, at.r.q0}, at.tile * kKeys, at.r.keys);
-#pragma unroll
-        for (int b = 0; b < kNB; ++b) {
-          const u32 bits = (u32)(w >> (32 * b)) >> (4 * h);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float x = sc[t][b][i];
-            sc[t][b][i] = bits >> (8 * (i / 4) + i % 4) & 1 ? x : -__builtin_inff();
-          }
-        }
-      }
-      float top = sc[t][0][0];
-#pragma unroll
-      for (int b = 0; b < kNB; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, sc[t][b][i]);
-      top = xhalf(top, [](float x, float y) { return __builtin_fmaxf(x, y); });
-      const float m_new = __builtin_fmaxf(m[t], top * p.scale_log2);
-      const float alpha = __builtin_amdgcn_exp2f(m[t] - m_new);
-      m[t] = m_new;
-      float sum[4] = {};
-#pragma unroll
-      for (int b = 0; b < kNB; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][b][i], p.scale_log2, -m_new));
-          const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][b][i + 1], p.scale_log2, -m_new));
-          sum[i / 2 % 2 * 2] += x, sum[i / 2 % 2 * 2 + 1] += y;
-          pf[t][2 * b + i / 8][i % 8 / 2] = pack2<BF16>(x, y);
-        }
-      l[t] = l[t] * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-      if (__builtin_amdgcn_ballot_w64(alpha != 1.f)) {
-#pragma unroll
-        for (int d = 0; d < kND; ++d) o[t][d] *= alpha;
-      }
-    }
-    if (tail) guard(at, stage, pf);
-#pragma unroll
-    for (int k = 0; k < kKS; ++k)
-#pragma unroll
-      for (int d = 0; d < kND; ++d) {
-        // And the rows 8 below: their chunks are permuted alike.
-        const u32 a = (av_s ^ (64 * d)) + 16 * k * kRow;
-        const u32x2 lo = tr_read(a), hi = tr_read(a + 8 * kRow);
-        const u32x4 vf = {lo.x, lo.y, hi.x, hi.y};
-#pragma unroll
-        for (int t = 0; t < NQ; ++t) o[t][d] = mfma<BF16>(vf, pf[t][k], o[t][d]);
-      }
-  }
-
-  // Tiles that hold nodes: a weight of 0 does not keep an infinite or NaN value
-  // out of the product.  Such values (rare) are added on the vector unit to the
-  // rows that read their key, and then taken out of the tile.
-  G9_DEV void guard(const Place& at, int stage, const u32x4 (&pf)[NQ][kKS]) {
-    typedef unsigned short h2 __attribute__((ext_vector_type(2)));
-    constexpr u32 kExp = BF16 ? 0x7f80u : 0x7c00u;
-    G9_LDS u32x4* const mine = (G9_LDS u32x4*)(uintptr_t)(lds + stage * kStage + kV + lane * 16);
-    h2 top = {0, 0};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const u32x4 x = mine[64 * j];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(h2, x[e] & 0x7fff7fffu));
-    }
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(top.x >= kExp || top.y >= kExp) == 0, 1)) return;
-    // P in LDS, 32 rows at a time: row of the query, column of the key.
-    uint16_t* const prow = reinterpret_cast<uint16_t*>(scratch) + col * kKeys;
-#pragma unroll
-    for (int t = 0; t < NQ; ++t) {
-#pragma unroll
-      for (int k = 0; k < kKS; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          *reinterpret_cast<u32*>(prow + 16 * k + 8 * (e >> 1) + 4 * h + 2 * (e & 1)) = pf[t][k][e];
-      const unsigned long long w = p.reads({node[t], at.r.context, at.r.q0}, at.tile * kKeys, at.r.keys);
-      waitcnt<63, 0>();
-#pragma unroll 1
-      for (int key = 0; key < kKeys; ++key) {
-        if (!((w >> key) & 1)) continue;
-        const float wt = unpack2<BF16>(prow[key]).x;
-        const u32 vr = lds + stage * kStage + kV + key * kRow;
-#pragma unroll
-        for (int d = 0; d < kND; ++d)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const u32x2 x = *(const G9_LDS u32x2*)(uintptr_t)(vr + 16 * ((4 * d + r) ^ swz_v(key)) + 8 * h);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              u32 y = (e & 1 ? x[e / 2] >> 16 : x[e / 2]) & 0xffffu;
-              if ((y & kExp) != kExp) y = 0;
-              o[t][d][4 * r + e] += wt * unpack2<BF16>(y).x;
-            }
-            __builtin_amdgcn_sched_barrier(0);
-          }
-      }
-    }
-#pragma unroll 1
-    for (int j = 0; j < 8; ++j) {
-      u32x4 x = mine[64 * j];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if ((x[e] & kExp) == kExp) x[e] &= 0xffff0000u;
-        if (((x[e] >> 16) & kExp) == kExp) x[e] &= 0xffffu;
-      }
-      mine[64 * j] = x;
-    }
-    waitcnt<63, 0>();
-  }
-};
-
 // Consecutive workgroups go round the 8 XCDs; consecutive parts of the line stay
 // on one, whose L2 then serves the blocks of rows that share keys.
 G9_DEV unsigned my_part() { return (blockIdx.x & 7) * (kWgs / 8) + (blockIdx.x >> 3); }
 
+// The 16-row pieces' pages of a tile; -1: none.
+template <class W>
+G9_DEV void pages_of(const Params& p, const Place& at, int (&pg)[W::kPieces]) {
+#pragma unroll
+  for (int i = 0; i < W::kPieces; ++i) {
+    const int k = at.tile * W::kKeys + 16 * i;
+    pg[i] = k < at.r.keys ? p.table[at.b * p.table_stride + (k >> p.shift)] : -1;
+  }
+}
+template <class W>
+G9_DEV void fill(const Params& p, const W& w, const Place& at, const int (&pg)[W::kPieces], int stage) {
+#pragma unroll
+  for (int i = 0; i < W::kPieces; ++i) {
+    const int k = at.tile * W::kKeys + 16 * i, off = k & ((1 << p.shift) - 1);
+    const bool in = (u32)pg[i] < (u32)p.num_blocks;
+    const int rows = in ? min(max(at.r.keys - k, 0), 16) : 0;
+    const long long page = in ? pg[i] : 0;
+    w.fill_piece(i, stage, p.kc + page * p.k_b + at.hk * p.k_h + (unsigned long long)off * p.k_t,
+                 p.vc + page * p.v_b + at.hk * p.v_h + (unsigned long long)off * p.v_t, rows, p.k_t, p.v_t);
+  }
+}
+template <class W, class L, int NQ>
+G9_DEV void begin(const Params& p, W& w, const Place& at) {
+#pragma unroll
+  for (int t = 0; t < NQ; ++t) {
+    w.node[t] = row_of<L>(p, at, 32 * t + w.col).node;
+    w.load_q(t, query_of<L>(p, at, 32 * t + w.col, w.node[t]));
+  }
+  w.clear();
+  w.context = at.r.context, w.q0 = at.r.q0, w.keys = at.r.keys;
+  // Waited for here: the compiler does not count the DMAs in flight, and a wait
+  // of its own at the first use would be one in every tile.
+  waitcnt<0, 0>();
+}
+
 template <bool BF16, int HD, int NQ>
 G9_DEV void narrow(const Params& p, char* smem) {
-  using W = Wave<BF16, HD, NQ>;
+  using W = Wave<Params, BF16, HD, NQ>;
   using L = Narrow<HD, NQ>;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned worker = my_part() * 4 + wave;
@@ -513,7 +308,7 @@ G9_DEV void narrow(const Params& p, char* smem) {
   if (count <= 0) return;
 
   W w(p);
-  w.init(smem, wave);
+  w.init(smem, wave, p.k_t, p.v_t);
   const auto next = [&](const Place& a) {
     if (a.tile + 1 == a.r.tiles) return L::next_block(p, a);
     Place n = a;
@@ -521,12 +316,12 @@ G9_DEV void narrow(const Params& p, char* smem) {
     return n;
   };
   int pg[W::kPieces];
-  w.pages(cur, pg);
-  w.fill(cur, pg, 0);
+  pages_of<W>(p, cur, pg);
+  fill(p, w, cur, pg, 0);
   Place nxt = cur;
   if (count > 1) {
     nxt = next(cur);
-    w.pages(nxt, pg);
+    pages_of<W>(p, nxt, pg);
   }
   bool fresh = true, from_start = cur.tile == 0;
   for (int i = 0; i < count; ++i) {
@@ -535,20 +330,20 @@ G9_DEV void narrow(const Params& p, char* smem) {
     __builtin_amdgcn_sched_barrier(0);
     Place aft = nxt;
     if (i + 1 < count) {
-      w.fill(nxt, pg, (i + 1) & 1);
+      fill(p, w, nxt, pg, (i + 1) & 1);
       if (i + 2 < count) {
         aft = next(nxt);
-        w.pages(aft, pg);
+        pages_of<W>(p, aft, pg);
       }
-      if (fresh) w.begin(cur);
+      if (fresh) begin<W, L, NQ>(p, w, cur);
       waitcnt<2 * W::kDmas, 15>();
     } else {
-      if (fresh) w.begin(cur);
+      if (fresh) begin<W, L, NQ>(p, w, cur);
       waitcnt<0, 15>();
     }
     __builtin_amdgcn_sched_barrier(0);
     const bool tail = (cur.tile + 1) * W::kKeys > min(cur.r.context, cur.r.keys);
-    w.tile(cur, i & 1, tail);
+    w.tile(cur.tile * W::kKeys, i & 1, tail);
     const bool last = cur.tile + 1 == cur.r.tiles;
     fresh = last;
     if (last || i + 1 == count) {
@@ -689,7 +484,8 @@ G9_DEV void store4(const Params& p, long long tok, int hq, int c, f32x4 sum, flo
 // parts begin within it, and with each of them a workgroup here (blockIdx.x + 1):
 // they (and gridDim.y times as many) share its rows, so that a workgroup's work
 // is a fraction of a part, however many parts a long request's blocks have.
-constexpr int kJoinThreads = 512;
+template <int HD>
+constexpr int kJoinThreads = 4 * HD;
 template <bool BF16, int HD, class L>
 G9_DEV void join(const Params& p, float* lds) {
   const unsigned w = blockIdx.x + 1;
@@ -708,7 +504,7 @@ G9_DEV void join(const Params& p, float* lds) {
   const u32 rows = (u32)min((long long)st.n * p.group - row0, (long long)L::kBlock);
   const u32 share = (w - w0 - 1) * gridDim.y + blockIdx.y, shares = (n - 1) * gridDim.y;
   const u32 from = share * rows / shares, to = (share + 1) * rows / shares;
-  constexpr unsigned kCols = HD / 4, kLanes = kJoinThreads / kCols;
+  constexpr unsigned kCols = HD / 4, kLanes = kJoinThreads<HD> / kCols;
   const unsigned c = threadIdx.x % kCols, lane = threadIdx.x / kCols;
   f32x4 sum;
   float m, l;
@@ -784,11 +580,11 @@ using namespace g9::host;
 #define G9_TREE_NARROW(NAME, BF16, HD, NQ)                                                                    \
   extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void                \
   g9_tree_##NAME(tree::Params p) {                                                                            \
-    __shared__ __attribute__((aligned(1024))) char smem[4 * tree::Wave<BF16, HD, NQ>::kWaveLds];               \
+    __shared__ __attribute__((aligned(1024))) char smem[4 * fa::Wave<tree::Params, BF16, HD, NQ>::kWaveLds];               \
     tree::narrow<BF16, HD, NQ>(p, smem);                                                                      \
   }                                                                                                           \
-  extern "C" __global__ __launch_bounds__(tree::kJoinThreads) void g9_tree_join_##NAME(tree::Params p) {      \
-    __shared__ float lds[tree::kJoinThreads * 7];                                                             \
+  extern "C" __global__ __launch_bounds__(tree::kJoinThreads<HD>) void g9_tree_join_##NAME(tree::Params p) {  \
+    __shared__ float lds[tree::kJoinThreads<HD> * 7];                                                         \
     tree::join<BF16, HD, tree::Narrow<HD, NQ>>(p, lds);                                                       \
   }
 #define G9_TREE_WIDE(NAME, BF16, HD)                                                                          \
@@ -797,8 +593,8 @@ using namespace g9::host;
     __shared__ __attribute__((aligned(1024))) char smem[tree::WidePipe<BF16, HD>::kLds];                       \
     tree::wide<BF16, HD>(p, smem);                                                                            \
   }                                                                                                           \
-  extern "C" __global__ __launch_bounds__(tree::kJoinThreads) void g9_tree_join_##NAME(tree::Params p) {      \
-    __shared__ float lds[tree::kJoinThreads * 7];                                                             \
+  extern "C" __global__ __launch_bounds__(tree::kJoinThreads<HD>) void g9_tree_join_##NAME(tree::Params p) {  \
+    __shared__ float lds[tree::kJoinThreads<HD> * 7];                                                         \
     tree::join<BF16, HD, tree::Wide<HD>>(p, lds);                                                             \
   }
 G9_TREE_NARROW(bf16_q32, true, 128, 1)
@@ -906,5 +702,5 @@ extern "C" int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cac
       hipSuccess)
     return G9_ERR_HIP;
   return launched(hipLaunchKernel(kJoin[form][d64][bf16], dim3(form == Q256 ? 255 : 1023, form == Q256 ? 4 : 1),
-                                  dim3(tree::kJoinThreads), args, 0, st));
+                                  dim3(unsigned(4 * D)), args, 0, st));
 }
