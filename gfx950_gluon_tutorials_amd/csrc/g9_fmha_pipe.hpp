@@ -639,6 +639,46 @@ struct Pipe : Where<Params, KIND> {
     }
   }
 
+  // Not kEqual: V_{j+1} landed, for a wave that has no more use for it.
+  G9_DEV void wait_v(int j) const {
+    if (j + 1 >= nte) return;
+    if (KIND == kPaged ? j + 5 < nte : j + 3 < nte)
+      waitcnt<(KIND == kPaged ? 5 : 1) * kDW, 15>();
+    else
+      waitcnt<0, 15>();
+  }
+  // kPaged: M2(j)'s DMA, and the pages of the next ones.
+  G9_DEV void ask_v(int j) {
+    if (j + 4 < nte) dma_v(j + 4, j & 3);
+    this->pgv = this->pgk;  // tile j + 5's V is asked for next, tile j + 6's K
+    if (((j + 6) & 63) == 0) hold_pages(j + 6);
+    this->pgk = page_of(j + 6);
+  }
+  // Not kEqual: iteration j of a wave none of whose rows reads tile j or one
+  // behind it: its share of the DMAs and the barriers.
+  G9_DEV void idle(int j) {
+    barrier();
+    if constexpr (KIND == kPaged) {
+      if (j + 4 < nte)
+        waitcnt<5 * kDW, 15>();
+      else
+        waitcnt<0, 15>();
+      if (j + 5 < nte) dma_k(j + 5, (j + 1) & 3);
+    } else {
+      if (j + 2 < nte) waitcnt<kDW, 15>();
+      if (j + 3 < nte) dma_k(j + 3, (j & 1) ^ 1);
+    }
+    barrier();
+    barrier();
+    wait_v(j);
+    if constexpr (KIND == kPaged) {
+      ask_v(j);
+    } else {
+      if (j + 2 < nte) dma_v(j + 2, j & 1);
+    }
+    barrier();
+  }
+
   // One loop iteration; PAR = j & 1 fixes the LDS buffers; c holds tile j's
   // scores after vec1, n receives tile j+1's; NEXT: tile j+1 exists.  The
   // loop runs over an even number of tiles nte: when nt is odd the last tile
@@ -727,11 +767,10 @@ struct Pipe : Where<Params, KIND> {
       }
       rescale();
     }
+    // Not kEqual: a wave's last tile need not be the workgroup's.
+    if constexpr (KIND != kEqual && !NEXT) wait_v(j);
     if constexpr (KIND == kPaged) {
-      if (j + 4 < nte) dma_v(j + 4, j & 3);
-      this->pgv = this->pgk;  // tile j + 5's V is asked for next, tile j + 6's K
-      if (((j + 6) & 63) == 0) hold_pages(j + 6);
-      this->pgk = page_of(j + 6);
+      ask_v(j);
     } else {
       if (j + 2 < nte) dma_v(j + 2, PAR);
     }

@@ -451,14 +451,17 @@ G9_DEV void wide(const Params& p, char* smem) {
     P.template read_k<-1>(1);
     waitcnt<63, 0>();
     if (lag) barrier();
+    // A wave without query rows leaves the tiles to the others.
+    const int own = (cur.block * L::kBlock + P.wave * 32) / p.group < cur.r.n ? nte : 2;
     int j = 0;
-    for (; j + 2 < nte; j += 2) {
+    for (; j + 2 < own; j += 2) {
       P.template step<0, true>(j, sa, sb);
       P.template step<1, true>(j + 1, sb, sa);
     }
     P.template step<0, true>(j, sa, sb);
     P.template step<1, false>(j + 1, sb, sa);
     __builtin_amdgcn_s_setprio(0);
+    for (j += 2; j < nte; ++j) P.idle(j);
     if (!lag) barrier();
     const bool from_start = cur.tile == 0, last = cur.tile + seg == cur.r.tiles;
     finish<BF16, HD, L>(p, cur, last && from_start ? -1 : (int)(2 * worker + (from_start ? 1 : 0)), row, P.row.node, P.o,

@@ -254,14 +254,20 @@ G9_DEV void varlen_fwd(const VarParams& p, char* smem) {
 
   const bool lag = wave >= 4;
   if (lag) barrier();
+  // The tiles that a row of this wave reads, rounded up to even; the others are
+  // left to the waves behind it (12% of a 256-query prompt's tiles, and most of a
+  // short last block's).
+  const int w0 = t.mb * kBlockM + wave * 32;
+  const int own = w0 < t.lq ? min(max(((limit(w0 + 31) + PipeT::kBN - 1) / PipeT::kBN + 1) & ~1, 2), nte) : 2;
   int j = 0;
-  for (; j + 2 < nte; j += 2) {
+  for (; j + 2 < own; j += 2) {
     P.template step<0, true>(j, sa, sb);
     P.template step<1, true>(j + 1, sb, sa);
   }
   P.template step<0, true>(j, sa, sb);
   P.template step<1, false>(j + 1, sb, sa);
   __builtin_amdgcn_s_setprio(0);
+  for (j += 2; j < nte; ++j) P.idle(j);
   if (!lag) barrier();
 
   const float lt = xhalf(P.l, [](float x, float y) { return x + y; });
