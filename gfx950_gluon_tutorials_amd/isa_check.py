@@ -28,6 +28,11 @@ no instruction may read or write it while it is pending.  Compiler-generated
 LDS reads satisfy this by construction; the scan proves it for the inline
 ones.
 
+A third scan covers the LDS-DMAs that are inline assembly: a scalar register
+that the vector unit wrote (``v_readfirstlane``, ``v_readlane``, a compare) may
+be read by a vector-memory instruction ``VMEM_AFTER_VALU_SGPR`` wait states later
+at the earliest.
+
 Usage: ``python -m gfx950_gluon_tutorials_amd.isa_check file.s`` (exit status 1
 on violations), or ``check_text(asm) -> list of violations``.
 """
@@ -52,6 +57,9 @@ READ_AFTER_MFMA = {
 }
 DEFAULT_READ_AFTER_MFMA = 20
 MFMA_AFTER_VALU = 2
+# Wait states between a VALU write of a scalar register and a vector-memory
+# instruction that reads it (descriptor, offset, M0).
+VMEM_AFTER_VALU_SGPR = 5
 
 _REG = re.compile(r"\b([vas])(?:\[(\d+):(\d+)\]|(\d+)\b)")
 _LABEL = re.compile(r"^([.\w]+):")
@@ -241,6 +249,42 @@ def _lds_step(state: dict, ins: Instr, violations: list, func: str):
                 state[r] = (0, ins.line)
 
 
+_SCALAR = re.compile(r"\b(vcc|m0)(?:_lo|_hi)?\b")
+
+
+def _sregs(ops: str) -> set[tuple[str, int]]:
+    return _regs(ops, "s") | {(m.group(1), 0) for m in _SCALAR.finditer(ops)}
+
+
+def _sgpr_step(state: dict, ins: Instr, violations: list, func: str):
+    """Advances the scalar registers that the VALU wrote over one instruction.
+
+    state maps a register to (remaining wait states, line of the write)."""
+    parts = ins.text.split(None, 1)
+    operands = parts[1].split(",") if len(parts) > 1 else []
+    if ins.mnemonic.startswith(("buffer_", "global_", "scratch_", "flat_")):
+        reads = _sregs(parts[1] if len(parts) > 1 else "")
+        if re.search(r"\blds\b", ins.text):
+            reads.add(("m0", 0))
+        for r in sorted(reads):
+            if r in state:
+                violations.append(f"{func}: line {ins.line + 1}: '{ins.text}' reads {r[0]}{r[1]} {state[r][0]} wait "
+                                  f"state(s) too soon after the VALU write at line {state[r][1] + 1}")
+                break
+    for r in list(state):
+        rem = state[r][0] - ins.waits
+        if rem <= 0:
+            del state[r]
+        else:
+            state[r] = (rem, state[r][1])
+    if ins.mnemonic.startswith("s_"):
+        for r in _sregs(operands[0]) if operands else ():
+            state.pop(r, None)  # written again, by the scalar unit
+    elif ins.mnemonic.startswith("v_") and operands:
+        for r in _sregs(operands[0]):
+            state[r] = (VMEM_AFTER_VALU_SGPR, ins.line)
+
+
 def _merge_lds(a: dict, b: dict) -> dict:
     out = dict(a)
     for r, ent in b.items():
@@ -282,7 +326,8 @@ def _fixpoint(name: str, blocks, step, merge) -> list[str]:
 
 def check_function(name: str, lines: list[str]) -> list[str]:
     blocks = _blocks(lines)
-    return _fixpoint(name, blocks, _step, _merge) + _fixpoint(name, blocks, _lds_step, _merge_lds)
+    return _fixpoint(name, blocks, _step, _merge) + _fixpoint(
+        name, blocks, _lds_step, _merge_lds) + _fixpoint(name, blocks, _sgpr_step, _merge)
 
 
 def check_text(asm: str) -> list[str]:
