@@ -127,10 +127,15 @@ def lse_fits(lse, HQ, T) -> None:
         raise ValueError("lse must be a contiguous fp32 (query heads, rows) tensor")
 
 
-def forward_only(*tensors) -> None:
+def plain(*tensors) -> None:
+    """Refuses what the kernels would silently lose: a gradient, a pending negation."""
     for t in tensors:
+        if t is None:
+            continue
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError("forward only: call it under torch.no_grad(), or detach the tensors that require a gradient")
+        if t.is_neg():
+            raise ValueError("a lazily negated view: call resolve_neg() first")
 
 
 # What a call's arguments are but for their addresses and contents, to the

@@ -47,6 +47,7 @@ def assign_slots(lengths: torch.Tensor, counts: torch.Tensor, block_table: torch
     slot -1 and position 0.  A token for which the free list or the table's width
     does not reach gets slot -1 (``taken`` above what the list holds says so).
     At most ``MAX_REQUESTS`` requests."""
+    block_size, num_tokens = int(block_size), int(num_tokens)
     key = ("slots", block_size, num_tokens, sig(lengths), sig(counts), sig(block_table), sig(free_blocks),
            free_start is not None and sig(free_start))
     dev, B, args = _launch.planned(key) or _plan_slots(key, lengths, counts, block_table, free_blocks, block_size,
@@ -99,7 +100,7 @@ def write_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
     fp16 or bf16, head dim 64 or 128; block_size a power of two from 16 to 1024."""
     key = ("write", sig(k), sig(v), sig(k_cache), sig(v_cache), sig(slots))
     dev, rest = _launch.planned(key) or _plan_write(key, k, v, k_cache, v_cache, slots)
-    _launch.forward_only(k, v, k_cache, v_cache)
+    _launch.plain(k, v, k_cache, v_cache)
     _launch.call("g9_write_cache", dev, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                  slots.data_ptr(), *rest)
 
@@ -139,11 +140,12 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     behind the last request are left as they were, a row that reads nothing gives
     zeros.  ``lse`` as in ``varlen_attention``.  Asynchronous on the current
     stream; forward only."""
+    sm_scale = None if sm_scale is None else float(sm_scale)
     key = ("tree", sm_scale, sig(q), sig(k_cache), sig(v_cache), sig(block_table), sig(lengths), sig(cu_seqlens),
            tree_mask is not None and sig(tree_mask), o is not None and sig(o), lse is not None and sig(lse))
     dev, need, table, words, rest = _launch.planned(key) or _plan_tree(
         key, q, k_cache, v_cache, block_table, lengths, cu_seqlens, tree_mask, o, lse, sm_scale)
-    _launch.forward_only(q, k_cache, v_cache)
+    _launch.plain(q, k_cache, v_cache, o)
     if o is None:
         o = torch.empty(q.shape, dtype=q.dtype, device=dev)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
@@ -182,4 +184,4 @@ def _plan_tree(key, q, k_cache, v_cache, block_table, lengths, cu_seqlens, tree_
     return _launch.keep(key, dev, (
         dev, _lib.load().g9_tree_workspace_size(B, T, HQ, HK, D), (block_table.stride(0), block_table.shape[1]), words,
         (B, T, HQ, HK, D, blocks, size, strides(q), strides(k_cache), strides(v_cache), os,
-         D**-0.5 if sm_scale is None else float(sm_scale), dtype)))
+         D**-0.5 if sm_scale is None else sm_scale, dtype)))

@@ -29,10 +29,11 @@ def varlen_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     sequence are left as they were.  ``lse``, if given, is a contiguous fp32
     (HQ, T) tensor that receives each query's natural-log log-sum-exp.
     Asynchronous on the current stream; forward only."""
+    sm_scale = None if sm_scale is None else float(sm_scale)
     key = ("varlen", causal, sm_scale, sig(q), sig(k), sig(v), sig(cu_seqlens), cu_seqlens_k is not None and sig(cu_seqlens_k),
            o is not None and sig(o), lse is not None and sig(lse))
     dev, rest = _launch.planned(key) or _plan(key, q, k, v, cu_seqlens, cu_seqlens_k, o, lse, causal, sm_scale)
-    _launch.forward_only(q, k, v)
+    _launch.plain(q, k, v, o)
     if o is None:
         o = torch.empty(q.shape, dtype=q.dtype, device=dev)
     cu = cu_seqlens.data_ptr()
@@ -63,4 +64,4 @@ def _plan(key, q, k, v, cu_seqlens, cu_seqlens_k, o, lse, causal, sm_scale):
     _launch.lse_fits(lse, HQ, T)
     os = _launch.array(HQ * D, D) if o is None else strides(o)
     return _launch.keep(key, dev, (dev, (B, T, TK, HQ, HK, D, strides(q), strides(k), strides(v), os,
-                                         D**-0.5 if sm_scale is None else float(sm_scale), dtype, 1 if causal else 0)))
+                                         D**-0.5 if sm_scale is None else sm_scale, dtype, 1 if causal else 0)))

@@ -658,7 +658,7 @@ extern "C" int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cac
   if (dtype != G9_F16 && dtype != G9_BF16) return G9_ERR_DTYPE;
   if (B < 0 || B > G9_TREE_MAX_REQUESTS || T < 0 || T > kMaxRows || HQ <= 0 || HQ > 65536 || HK <= 0 || HQ % HK ||
       (D != 64 && D != 128) || !scale_ok(sm_scale) || num_blocks < 0 || num_blocks > kMaxRows || width < 0 ||
-      width > kMaxRows || !block_size_ok(block_size) || width * block_size > kMaxRows || words < 0 || words > 1024 ||
+      width > kMaxRows || !block_size_ok(block_size) || width * block_size > (int64_t(1) << 30) || words < 0 || words > 1024 ||
       (tree_mask && words == 0))
     return G9_ERR_SHAPE;
   if (!q_strides || !kc_strides || !vc_strides || !o_strides) return G9_ERR_LAYOUT;

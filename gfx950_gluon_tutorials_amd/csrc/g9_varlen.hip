@@ -68,7 +68,7 @@ G9_DEV Cost cost_of(const VarParams& p, int b, int per) {
   if (b >= p.B) return {0, 0};
   const int q0 = min(max(p.cu_q[b], 0), p.T), lq = min(max(p.cu_q[b + 1], q0), p.T) - q0;
   const int k0 = min(max(p.cu_k[b], 0), p.TK), lk = min(max(p.cu_k[b + 1], k0), p.TK) - k0;
-  const auto blocks = [&](int x) { return (int)(((long long)x * per + BLOCK - 1) / BLOCK); };
+  const auto blocks = [&](int x) { return (int)min(((long long)x * per + BLOCK - 1) / BLOCK, 1ll << 28); };
   const int n = blocks(lq);
   return {n, n + blocks(p.causal ? max(lk - lq, 0) : lk)};
 }

@@ -73,8 +73,8 @@ int g9_fmha_fwd(const void* q, const void* k, const void* v, void* o, float* lse
  *   count as 0, cu_seqlens are held inside the packed tensor, a table entry
  *   outside [0, num_blocks) reads as zeros, and keys behind the table's width are
  *   left out.
- * - cu_seqlens: B + 1 ascending row offsets from 0; rows at or behind
- *   cu_seqlens[B] belong to no sequence and their outputs stay as they were.
+ * - cu_seqlens: B + 1 ascending row offsets; rows before cu_seqlens[0] and from
+ *   cu_seqlens[B] on belong to no sequence and their outputs stay as they were.
  * - A query with no key it may read gives zeros, and -inf in lse.
  * - Keys that no query may read (cache rows behind a request, unused blocks,
  *   other sequences) have no effect, whatever they hold, NaN included.
@@ -136,6 +136,9 @@ int g9_varlen_fwd(const void* q, const void* k, const void* v, void* o, float* l
  * context token and the nodes j whose bit j % 64 is set in word j / 64 of row
  * cu_q[b] + i of tree_mask (T x words, int64); without a mask the nodes j <= i.
  * One node per request without a mask is plain decoding.  lse as g9_varlen_fwd.
+ *
+ * B <= G9_TREE_MAX_REQUESTS; width * block_size <= 2^30; the caches' tokens at
+ * least D elements apart.
  *
  * workspace: g9_tree_workspace_size bytes, 32-byte aligned, contents arbitrary;
  * it holds partial results between the call's kernels, so calls that can run
