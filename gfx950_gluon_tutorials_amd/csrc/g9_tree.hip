@@ -580,8 +580,11 @@ G9_DEV void join(const Params& p, float* lds) {
 using namespace g9;
 using namespace g9::host;
 
+// The bound of 512 threads (256 are launched) keeps the kernels to 256 registers a
+// lane, all of the vector file: with more the products' results go to the
+// accumulation file, and a third of a tile's instructions moves them back.
 #define G9_TREE_NARROW(NAME, BF16, HD, NQ)                                                                    \
-  extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void                \
+  extern "C" __global__ __launch_bounds__(512) void                                                           \
   g9_tree_##NAME(tree::Params p) {                                                                            \
     __shared__ __attribute__((aligned(1024))) char smem[4 * fa::Wave<tree::Params, BF16, HD, NQ>::kWaveLds];               \
     tree::narrow<BF16, HD, NQ>(p, smem);                                                                      \
