@@ -494,9 +494,8 @@ G9_DEV void join(const Params& p, float* lds) {
   const unsigned w = blockIdx.x + 1;
   const Start zero = p.start[0];
   const unsigned long long total = (unsigned long long)zero.total_hi << 32 | zero.total_lo;
-  if (w >= L::workers(total)) return;
-  const Start st = p.start[w];
-  if (st.tile == 0) return;
+  const Start st = p.start[w];  // asked for together with worker 0's
+  if (w >= L::workers(total) || st.tile == 0) return;
   const unsigned long long u0 = L::part_begin(w, total) - (unsigned)st.tile;
   const unsigned w0 = L::worker_of(u0, total), n = L::worker_of(u0 + st.tiles - 1, total) - w0 + 1;
   // Worker w0 has the block in slot 1 unless it began it before its part; the
