@@ -140,7 +140,7 @@ def plain(*tensors) -> None:
 
 # What a call's arguments are but for their addresses and contents, to the
 # arguments of the C call that follow from it: a call of the same kind as an
-# earlier one is not checked again (half of its host time otherwise).
+# earlier one is not checked again (decoding's host time is 6.9 us instead of 10.6).
 _plans: dict = {}
 
 

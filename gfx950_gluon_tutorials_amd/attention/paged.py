@@ -145,7 +145,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
            tree_mask is not None and sig(tree_mask), o is not None and sig(o), lse is not None and sig(lse))
     dev, need, table, words, rest = _launch.planned(key) or _plan_tree(
         key, q, k_cache, v_cache, block_table, lengths, cu_seqlens, tree_mask, o, lse, sm_scale)
-    _launch.plain(q, k_cache, v_cache, o)
+    _launch.plain(q, k_cache, v_cache, o, lse)
     if o is None:
         o = torch.empty(q.shape, dtype=q.dtype, device=dev)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)

@@ -29,11 +29,11 @@ def varlen_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     sequence are left as they were.  ``lse``, if given, is a contiguous fp32
     (HQ, T) tensor that receives each query's natural-log log-sum-exp.
     Asynchronous on the current stream; forward only."""
-    sm_scale = None if sm_scale is None else float(sm_scale)
+    causal, sm_scale = bool(causal), None if sm_scale is None else float(sm_scale)
     key = ("varlen", causal, sm_scale, sig(q), sig(k), sig(v), sig(cu_seqlens), cu_seqlens_k is not None and sig(cu_seqlens_k),
            o is not None and sig(o), lse is not None and sig(lse))
     dev, rest = _launch.planned(key) or _plan(key, q, k, v, cu_seqlens, cu_seqlens_k, o, lse, causal, sm_scale)
-    _launch.plain(q, k, v, o)
+    _launch.plain(q, k, v, o, lse)
     if o is None:
         o = torch.empty(q.shape, dtype=q.dtype, device=dev)
     cu = cu_seqlens.data_ptr()

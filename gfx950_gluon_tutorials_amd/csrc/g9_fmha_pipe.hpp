@@ -181,23 +181,22 @@ constexpr int sum16(const int (&a)[16]) {
 //            lim.  Tile addresses are 64-bit: a descriptor per tile whose range
 //            ends with the sequence, so rows behind it read as zeros.
 //   kPaged   the tiles from t0 on of a paged request, up to `keys` rows.  A DMA
-//            covers eight 16-byte chunks of 8 rows (whole 128-byte lines: with 64
-//            bytes of 16 rows HBM gave 3.6 TB/s), which never cross a page.  In
+//            covers eight 16-byte chunks of 8 rows, whole 128-byte lines, which never
+//            cross a page.  In
 //            LDS, rows go by 8 and chunks of 128 bytes; the groups of K are a
 //            chunk further apart and V's rows permuted within a chunk, so that
 //            K's reads of 16 rows and V's transposing reads of four chunks touch
 //            every bank once.  Which keys from `wlim` on
 //            (the request's nodes) a query reads is p's to say (p.reads).  Four
 //            tiles of K and of V are in LDS instead of two: the tiles come from
-//            HBM, not from an L2 that other workgroups have filled, and 32 KB in
-//            flight per CU carry 2.3 TB/s.
+//            HBM, not from an L2 that other workgroups have filled.
 enum Kind { kEqual, kPacked, kPaged };
 template <class Params, Kind KIND>
 struct Where {};
 // The request's table row and first tile; the pages of this wave's rows of 64
 // tiles, one per lane, and of the next K tile and the next V tile to ask for
 // (a scalar load per tile would be waited for in every tile's last cluster:
-// 3.3 us a tile instead of 1.4); the query's row in the mask.
+// 3.3 us a tile instead of 2.4); the query's row in the mask.
 template <class Params>
 struct Where<Params, kPaged> {
   const int* table;

@@ -139,7 +139,8 @@ struct WriteParams {
 extern "C" __global__ __launch_bounds__(256) void g9_cache_write(WriteParams p) {
   const int n = p.HK << p.chunks_log2, sub = threadIdx.x & 63;
   const int in = p.tokens > 1 ? sub / n : 0, lane = sub - in * n;
-  const long long at = ((long long)blockIdx.x * 4 + (threadIdx.x >> 6)) * p.tokens + in;
+  const long long wg = (long long)blockIdx.y * gridDim.x + blockIdx.x;
+  const long long at = (wg * 4 + (threadIdx.x >> 6)) * p.tokens + in;
   if (at >= p.T || in >= p.tokens) return;
   const int t = (int)at;
   const long long slot = p.slots[t];
@@ -228,10 +229,12 @@ int g9_write_cache(const void* k, const void* v, void* k_cache, void* v_cache, c
   p.chunks_log2 = log2_of(D / 8);
   const int64_t chunks = HK * D / 8, per = chunks < 64 ? 64 / chunks : 1;
   p.tokens = (int)per;
+  // A dimension of a launch has fewer than 2^32 threads.
+  const int64_t wgs = (T + 4 * per - 1) / (4 * per), row = wgs < (1 << 22) ? wgs : 1 << 22;
   void* args[] = {&p};
   return launched(hipLaunchKernel(reinterpret_cast<const void*>(g9_cache_write),
-                                  dim3((unsigned)((T + 4 * per - 1) / (4 * per))),
-                                  dim3(256), args, 0, reinterpret_cast<hipStream_t>(stream)));
+                                  dim3((unsigned)row, (unsigned)((wgs + row - 1) / row)), dim3(256), args, 0,
+                                  reinterpret_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

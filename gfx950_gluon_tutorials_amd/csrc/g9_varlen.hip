@@ -158,7 +158,8 @@ G9_DEV bool find_tile(const VarParams& p, int rank, int per, int* lds, Tile& t) 
     seq = lds[(THREADS / 64)];
     __syncthreads();
   }
-  seq = __builtin_amdgcn_readfirstlane(seq);
+  // Held inside whatever the offsets say (sums of more than 2^31 tiles wrap).
+  seq = min(max(__builtin_amdgcn_readfirstlane(seq), 0), p.B - 1);
   cost = __builtin_amdgcn_readfirstlane(cost);
   const Cost s = cost_of<BLOCK>(p, seq, per);
   t.mb = s.n - 1 - (s.top - cost);
@@ -167,7 +168,7 @@ G9_DEV bool find_tile(const VarParams& p, int rank, int per, int* lds, Tile& t) 
   t.k0 = min(max(p.cu_k[seq], 0), p.TK);
   t.lk = min(max(p.cu_k[seq + 1], t.k0), p.TK) - t.k0;
   for (int* x : {&t.mb, &t.q0, &t.lq, &t.k0, &t.lk}) *x = __builtin_amdgcn_readfirstlane(*x);
-  return true;
+  return (u32)t.mb < (u32)s.n;
 }
 
 template <bool BF16, int HD>
@@ -255,8 +256,8 @@ G9_DEV void varlen_fwd(const VarParams& p, char* smem) {
   const bool lag = wave >= 4;
   if (lag) barrier();
   // The tiles that a row of this wave reads, rounded up to even; the others are
-  // left to the waves behind it (12% of a 256-query prompt's tiles, and most of a
-  // short last block's).
+  // left to the waves behind it (a quarter of a 256-query prompt's tiles, and most of
+  // a short last block's).
   const int w0 = t.mb * kBlockM + wave * 32;
   const int own = w0 < t.lq ? min(max(((limit(w0 + 31) + PipeT::kBN - 1) / PipeT::kBN + 1) & ~1, 2), nte) : 2;
   int j = 0;
@@ -468,7 +469,7 @@ extern "C" int g9_varlen_fwd(const void* q, const void* k, const void* v, void* 
   // At most T / 256 whole tiles and a partial one per sequence.
   const int64_t tiles = T / fa::kBlockM + (B < T ? B : T);
   const int64_t grid = 8 * group * ((tiles * HK + 7) / 8);
-  if (grid > INT32_MAX) return G9_ERR_SHAPE;
+  if (grid * fa::kThreads > UINT32_MAX) return G9_ERR_SHAPE;  // the threads of a launch
   static const void* const kFns[2][2] = {
       {reinterpret_cast<const void*>(g9_varlen_f16), reinterpret_cast<const void*>(g9_varlen_bf16)},
       {reinterpret_cast<const void*>(g9_varlen_f16_d64), reinterpret_cast<const void*>(g9_varlen_bf16_d64)}};

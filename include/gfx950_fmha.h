@@ -122,6 +122,7 @@ int g9_write_cache(const void* k, const void* v, void* k_cache, void* v_cache, c
  * causal != 0 lets query i of Lq read the keys j <= i + Lk - Lq, so that a prompt
  * whose first part is cached passes its new queries only.  lse: optional fp32
  * HQ x T, contiguous: the natural-log log-sum-exp of each query's scaled scores.
+ * (T / 256 + min(B, T)) x HQ below 2^23.
  */
 int g9_varlen_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* cu_q,
                   const int32_t* cu_k, int64_t B, int64_t T, int64_t TK, int64_t HQ, int64_t HK, int64_t D,

@@ -190,6 +190,7 @@ VARLEN = dict(q=FAKE, k=FAKE, v=FAKE, o=FAKE, lse=None, cu_q=FAKE, cu_k=FAKE, B=
     (dict(T=-1), _lib.G9_ERR_SHAPE),
     (dict(T=2**31), _lib.G9_ERR_SHAPE),
     (dict(TK=2**31), _lib.G9_ERR_SHAPE),
+    (dict(B=2**21, T=2**21), _lib.G9_ERR_SHAPE),  # workgroups of a launch
     (dict(scale=0.0), _lib.G9_ERR_SHAPE),
     (dict(scale=-1.0), _lib.G9_ERR_SHAPE),
     (dict(scale=float("nan")), _lib.G9_ERR_SHAPE),

@@ -304,6 +304,27 @@ def test_a_scale_tensor_is_taken_by_value(gpu):
     assert torch.equal(b, varlen_attention(q, q, q, cu, sm_scale=float(s))) and not torch.equal(a, b)
 
 
+def test_a_causal_flag_tensor_is_taken_by_value(gpu):
+    q = torch.randn(4, 1, 64, device=gpu).half()
+    cu = _i32([0, 4], gpu)
+    flag = torch.tensor(True)
+    a = varlen_attention(q, q, q, cu, causal=flag)
+    flag.fill_(False)
+    b = varlen_attention(q, q, q, cu, causal=flag)
+    assert torch.equal(a, varlen_attention(q, q, q, cu, causal=True))
+    assert torch.equal(b, varlen_attention(q, q, q, cu, causal=False)) and not torch.equal(a, b)
+
+
+def test_a_negated_or_differentiable_lse_is_refused(gpu):
+    q = torch.randn(1, 1, 64, device=gpu).half()
+    cu = _i32([0, 1], gpu)
+    lse = torch.zeros(1, 1, device=gpu)
+    varlen_attention(q, q, q, cu, lse=lse)
+    for bad in (torch._neg_view(lse), torch.zeros(1, 1, device=gpu, requires_grad=True)):
+        with pytest.raises(ValueError):
+            varlen_attention(q, q, q, cu, lse=bad)
+
+
 def test_a_batch_of_too_many_requests_is_refused(gpu):
     B = 8193
     q = torch.zeros(1, 1, 64, device=gpu, dtype=torch.half)

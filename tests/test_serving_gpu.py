@@ -237,6 +237,21 @@ def test_write_cache_past_32_bit_offsets(gpu):
     torch.cuda.empty_cache()
 
 
+def test_write_cache_of_more_rows_than_a_launch_has_waves(gpu):
+    T, HK, D, blocks, size = 2**26 + 77, 8, 64, 3, 16
+    kc, vc = (torch.zeros(blocks, size, HK, D, dtype=torch.float16, device=gpu) for _ in range(2))
+    k, v = (torch.randn(1, HK, D, device=gpu).half().expand(T, HK, D) for _ in range(2))
+    slots = torch.full((T,), -1, dtype=torch.int64, device=gpu)
+    taken = {0: 5, 2**24 - 1: 6, 2**24: 7, T // 2: 40, T - 1: 47}
+    for t, s in taken.items():
+        slots[t] = s
+    write_cache(k, v, kc, vc, slots)
+    for got, row in ((kc, k[0]), (vc, v[0])):
+        want = torch.zeros_like(got).view(-1, HK, D)
+        want[list(taken.values())] = row
+        assert torch.equal(got.view(-1, HK, D), want)
+
+
 SLOTS = [
     # lengths, counts, size, width, free, start, T - sum(counts)
     ([0], [1], 16, 4, 4, None, 0),
