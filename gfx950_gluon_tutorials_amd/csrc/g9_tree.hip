@@ -99,9 +99,11 @@ G9_DEV void make_uniform(Place& a) {
 }
 
 // The line of tiles: KEYS keys a tile, blocks of BLOCK query rows, WORKERS parts.
-template <int KEYS, int BLOCK, int WORKERS>
+// A block's tiles have LEAD places without work before them, for what its
+// beginning and end cost: else the parts of many short requests take longest.
+template <int KEYS, int BLOCK, int WORKERS, int LEAD>
 struct Line {
-  static constexpr int kKeys = KEYS, kBlock = BLOCK, kWorkers = WORKERS;
+  static constexpr int kKeys = KEYS, kBlock = BLOCK, kWorkers = WORKERS, kLead = LEAD;
 
   static G9_DEV Req request(const Params& p, int b) {
     Req r;
@@ -114,18 +116,18 @@ struct Line {
     return r;
   }
   static G9_DEV unsigned long long tiles_of(const Params& p, const Req& r) {
-    return (unsigned long long)r.blocks * (unsigned)p.HK * (unsigned)r.tiles;
+    return (unsigned long long)r.blocks * (unsigned)p.HK * (unsigned)(kLead + r.tiles);
   }
-  // Worker w of W takes the tiles [w n / W, (w + 1) n / W) of a line of n; W is at
+  // Worker w of W takes the places [w n / W, (w + 1) n / W) of a line of n; W is at
   // most n, so that no part in between is empty.
   static G9_DEV unsigned workers(unsigned long long n) { return n < kWorkers ? (unsigned)n : kWorkers; }
   static G9_DEV unsigned long long part_begin(unsigned w, unsigned long long n) { return quotient(w * n, workers(n)); }
-  static G9_DEV unsigned worker_of(unsigned long long tile, unsigned long long n) {
-    return (unsigned)quotient((tile + 1) * workers(n) - 1, n);
+  static G9_DEV unsigned worker_of(unsigned long long place, unsigned long long n) {
+    return (unsigned)quotient((place + 1) * workers(n) - 1, n);
   }
 
-  // Where this worker's part begins, and its tiles.  The workgroup sums the
-  // requests' tiles into LDS (first[B + 1]).
+  // This worker's first tile, and the places of its part from there on (none or
+  // less: no tile).  The workgroup sums the requests' places into LDS (first[B + 1]).
   template <int THREADS>
   static G9_DEV int locate(const Params& p, char* smem, unsigned worker, Place& at) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -156,10 +158,10 @@ struct Line {
     if (tid == 0) first[p.B] = total;
     __syncthreads();
     total = uniform(total);
-    int count = 0;
+    int left = 0;
     if (worker < workers(total)) {
       const unsigned long long begin = uniform(part_begin(worker, total));
-      count = uniform((int)(part_begin(worker + 1, total) - begin));
+      left = uniform((int)(part_begin(worker + 1, total) - begin));
       // The last request that begins at or before the part (empty ones begin
       // where the next one does).
       int lo = 0, hi = p.B;
@@ -173,17 +175,19 @@ struct Line {
       at.b = uniform(lo);
       at.r = request(p, at.b);
       const unsigned long long in = uniform(begin - first[lo]);
-      const unsigned long long unit = quotient(in, (unsigned)at.r.tiles);
-      at.tile = (int)(in - unit * (unsigned)at.r.tiles);
+      const unsigned long long unit = quotient(in, (unsigned)(kLead + at.r.tiles));
+      const int place = (int)(in - unit * (unsigned)(kLead + at.r.tiles));
+      at.tile = max(place - kLead, 0);
+      left -= uniform(max(kLead - place, 0));
       at.hk = (int)quotient(unit, (unsigned)at.r.blocks);
       at.block = (int)(unit - (unsigned long long)at.hk * at.r.blocks);
       make_uniform(at);
     }
     // Worker 0 says how long the line is, also where it is empty.
-    if ((worker == 0 || count > 0) && (THREADS == 64 * (kWorkers / kWgs) ? lane == 0 : tid == 0))
+    if ((worker == 0 || worker < workers(total)) && (THREADS == 64 * (kWorkers / kWgs) ? lane == 0 : tid == 0))
       p.start[worker] = {at.r.q0, at.r.n, at.hk, at.block, at.tile, at.r.tiles, (u32)total, (u32)(total >> 32)};
     __syncthreads();  // first[] is read: what comes next takes its place
-    return count;
+    return left;
   }
   // The first tile of the block behind `a`'s (there is one).
   static G9_DEV Place next_block(const Params& p, const Place& a) {
@@ -200,12 +204,27 @@ struct Line {
     make_uniform(n);
     return n;
   }
+  // To the part's next tile, if it has one.
+  static G9_DEV bool advance(const Params& p, Place& a, int& left) {
+    const bool end = a.tile + 1 == a.r.tiles;
+    left -= end ? 1 + kLead : 1;
+    if (left <= 0) return false;
+    if (end)
+      a = next_block(p, a);
+    else
+      ++a.tile;
+    return true;
+  }
 };
-// A wave's own tiles of up to 8 KB, or a workgroup's of 16 KB.
+// A wave's own tiles of up to 8 KB, or a workgroup's of 16 KB.  A block costs a
+// wave nothing beside its tiles that shows (1 to 3 places: 0 to 5% slower); a
+// workgroup it costs as much as 384 keys (us, blocks of 256 rows of head dim 128,
+// 64 rows a request, with and without the places: 64 x 100-8192 tokens 243 and
+// 331, 64 x 100-2000 96 and 140, 4 x 8000 with 200 x 100 96 and 148).
 template <int HD, int NQ>
-using Narrow = Line<4096 / HD, 32 * NQ, 4 * kWgs>;
+using Narrow = Line<4096 / HD, 32 * NQ, 4 * kWgs, 0>;
 template <int HD>
-using Wide = Line<8192 / HD, 256, kWgs>;
+using Wide = Line<8192 / HD, 256, kWgs, 384 * HD / 8192>;
 
 // A lane's query row of the block.
 template <class L>
@@ -304,37 +323,28 @@ G9_DEV void narrow(const Params& p, char* smem) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned worker = my_part() * 4 + wave;
   Place cur{};
-  const int count = L::template locate<256>(p, smem, worker, cur);
-  if (count <= 0) return;
+  int left = L::template locate<256>(p, smem, worker, cur);
+  if (left <= 0) return;
 
   W w(p);
   w.init(smem, wave, p.k_t, p.v_t);
-  const auto next = [&](const Place& a) {
-    if (a.tile + 1 == a.r.tiles) return L::next_block(p, a);
-    Place n = a;
-    ++n.tile;
-    return n;
-  };
   int pg[W::kPieces];
   pages_of<W>(p, cur, pg);
   fill(p, w, cur, pg, 0);
   Place nxt = cur;
-  if (count > 1) {
-    nxt = next(cur);
-    pages_of<W>(p, nxt, pg);
-  }
+  bool more = L::advance(p, nxt, left);  // nxt is a tile
+  if (more) pages_of<W>(p, nxt, pg);
   bool fresh = true, from_start = cur.tile == 0;
-  for (int i = 0; i < count; ++i) {
+  for (int i = 0;; ++i) {
     // The stage that tile i + 1 takes was last read for tile i - 1.
     waitcnt<63, 0>();
     __builtin_amdgcn_sched_barrier(0);
     Place aft = nxt;
-    if (i + 1 < count) {
+    bool more_aft = false;
+    if (more) {
       fill(p, w, nxt, pg, (i + 1) & 1);
-      if (i + 2 < count) {
-        aft = next(nxt);
-        pages_of<W>(p, aft, pg);
-      }
+      more_aft = L::advance(p, aft, left);
+      if (more_aft) pages_of<W>(p, aft, pg);
       if (fresh) begin<W, L, NQ>(p, w, cur);
       waitcnt<2 * W::kDmas, 15>();
     } else {
@@ -346,7 +356,7 @@ G9_DEV void narrow(const Params& p, char* smem) {
     w.tile(cur.tile * W::kKeys, i & 1, tail);
     const bool last = cur.tile + 1 == cur.r.tiles;
     fresh = last;
-    if (last || i + 1 == count) {
+    if (last || !more) {
       // Slot 0 of the worker: a block that another worker began; slot 1: one
       // that the next worker goes on with.
 #pragma unroll
@@ -355,8 +365,10 @@ G9_DEV void narrow(const Params& p, char* smem) {
                             w.node[t], w.o[t], w.m[t], w.l[t]);
       from_start = true;
     }
+    if (!more) break;
     cur = nxt;
     nxt = aft;
+    more = more_aft;
   }
 }
 
@@ -375,7 +387,7 @@ G9_DEV void wide(const Params& p, char* smem) {
   static_assert(PipeT::kBN == L::kKeys && kBlockM == L::kBlock);
   const unsigned worker = my_part();
   Place cur{};
-  int count = L::template locate<kThreads>(p, smem, worker, cur);
+  int left = L::template locate<kThreads>(p, smem, worker, cur);
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   PipeT P(p);
   P.wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -393,8 +405,8 @@ G9_DEV void wide(const Params& p, char* smem) {
   }
   const bool lag = P.wave >= 4;
   const int row = P.wave * 32 + (lane & 31);
-  while (count > 0) {
-    const int seg = min(count, cur.r.tiles - cur.tile);
+  while (left > 0) {
+    const int seg = min(left, cur.r.tiles - cur.tile);
     P.keys = min(cur.r.keys, (cur.tile + seg) * PipeT::kBN);
     P.wlim = min(cur.r.context, P.keys);
     P.t0 = cur.tile;
@@ -466,8 +478,8 @@ G9_DEV void wide(const Params& p, char* smem) {
     const bool from_start = cur.tile == 0, last = cur.tile + seg == cur.r.tiles;
     finish<BF16, HD, L>(p, cur, last && from_start ? -1 : (int)(2 * worker + (from_start ? 1 : 0)), row, P.row.node, P.o,
                         P.m, P.l);
-    count -= seg;
-    if (count > 0) cur = L::next_block(p, cur);
+    left -= seg + L::kLead;
+    if (left > 0) cur = L::next_block(p, cur);
     barrier();  // the stages are read: the next block's tiles take them
   }
 }
@@ -616,11 +628,18 @@ G9_TREE_WIDE(f16_d64_q256, false, 64)
 namespace {
 
 // Query rows of a block, by the rows that the requests of a batch bring on
-// average to one K/V head.  Measured (us, without the joins), 8 K/V heads, one
-// MI355X: head dim 128, 16 x 6000 tokens: 40 rows 101 in blocks of 256 against
-// 119 of 64, 128 rows 138 and 203; so 64 is not built.  Head dim 64, whose
-// blocks of 256 spill: 40 rows 58 of 64 and 96 of 256, 128 rows 99 and 99, 256
-// rows 173 and 112.
+// average to one K/V head.  Measured (us a call, blocks of 32, 64 and 256 rows;
+// 8 K/V heads, a cache that no last level holds, one MI355X):
+//   head dim 64     16 x 6000 tokens    64 x 100-8192     256 x 200-600
+//     32 rows        62   69  123       147  164  309      73   80  200
+//     64 rows        99   73  125       262  175  315     116   89  208
+//     128 rows      147  118  121       495  304  298     207  151  238
+//     256 rows      254  182  138       983  577  337     411  283  295
+//   head dim 128 (blocks of 64 do not fit its registers)
+//     32 rows       100    -   96       248    -  230     125    -  139
+//     64 rows       153    -   98       460    -  245     204    -  150
+//     128 rows      239    -  105       875    -  268     360    -  179
+// and 1 x 700 tokens, 32 rows: 16 and 24 (head dim 64), 19 and 22.
 enum { Q32, Q64, Q256 };
 int form_of(int64_t B, int64_t T, int64_t group, int64_t D) {
   const int64_t rows = (T + B - 1) / B * group;
