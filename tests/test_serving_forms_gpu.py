@@ -236,6 +236,20 @@ def test_a_long_request_among_short_ones(gpu, D, nodes):
     _tree(gpu, "bf16", [20000] + [50] * 9, [nodes] * 10, 8, 2, D, 64, "chain", seed=nodes)
 
 
+@pytest.mark.parametrize("D,nodes,B", [(128, 24, 300), (64, 70, 200), (64, 20, 300), (128, 5, 400)])
+def test_many_short_requests_among_long_ones(gpu, D, nodes, B):
+    """Parts of many blocks, of one, and of a piece of one."""
+    ctx = [0, 1, 63, 90, 40] * (B // 5)
+    ctx[B // 3], ctx[-1] = 9000, 4000
+    _tree(gpu, "fp16", ctx, [nodes] * B, 4, 2, D, 16, "chain", seed=B)
+
+
+@pytest.mark.parametrize("ctx", [0, 1, 50, 130, 800])
+@pytest.mark.parametrize("D,HK", [(128, 1), (64, 3)])
+def test_fewer_tiles_than_workers(gpu, ctx, D, HK):
+    _tree(gpu, "bf16", [ctx], [140], HK, HK, D, 16, "tree", seed=ctx)
+
+
 @pytest.mark.parametrize("D,nodes", [(128, 1), (128, 24), (64, 20), (64, 80)])
 def test_long_contexts(gpu, D, nodes):
     """More than 64 tiles for every part: parts that cross heads, pages asked for
