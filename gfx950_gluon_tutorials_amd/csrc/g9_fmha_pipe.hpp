@@ -269,6 +269,30 @@ struct Pipe : Where<Params, KIND> {
   G9_DEV u32 second(u32 a) const {
     return KIND == kPaged ? a + kGroupV : a + 128;
   }
+  // kPaged: the lane's offsets, worked out at each use (held they would be
+  // spilled, and a reload waits for every DMA in flight).  A DMA's lane i fetches
+  // chunk i / 8 of row i % 8 (V: of row i % 8 ^ 4 (chunk / 2 % 2), see Kind).
+  static G9_DEV u32 lane_now() {
+    u32 x;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
+    return x;
+  }
+  G9_DEV u32 voff_k() const {
+    const u32 i = lane_now();
+    return (i & 7) * p.k_t + (i >> 3) * 16;
+  }
+  G9_DEV u32 voff_v() const {
+    const u32 i = lane_now();
+    return ((i & 7) ^ (i >> 2 & 4)) * p.v_t + (i >> 3) * 16;
+  }
+  G9_DEV u32 at_k() const {
+    const u32 i = lane_now();
+    return lds0 + ((i & 31) >> 3) * kGroupK + (i >> 5) * 128 + (i & 7) * 16;
+  }
+  G9_DEV u32 at_v() const {
+    const u32 i = lane_now(), G = i >> 4 & 1, jj = i & 15;
+    return lds0 + kLdsV + (2 * G + ((jj & 3) >> 1)) * 128 + ((4 * (i >> 5) + (jj >> 2)) ^ (4 * G)) * 16 + 8 * (jj & 1);
+  }
   // kPaged: this wave's rows of a tile, 8 by 256 bytes or 16 by 128.
   static constexpr int kMine = kBN / kWaves;
   G9_DEV int my_key(int tile) const { return (this->t0 + tile) * kBN + kMine * wave; }
@@ -292,7 +316,7 @@ struct Pipe : Where<Params, KIND> {
   }
   G9_DEV void dma_k(int tile, int buf) {
     if constexpr (KIND == kPaged) {
-      dma_paged(kp, tile, this->pgk, lds0 + buf * kTileK + kMine / 8 * wave * kGroupK, HD == 128 ? 1024 : kGroupK, voffk,
+      dma_paged(kp, tile, this->pgk, lds0 + buf * kTileK + kMine / 8 * wave * kGroupK, HD == 128 ? 1024 : kGroupK, voff_k(),
                 p.k_b, p.k_t);
     } else if constexpr (KIND == kPacked) {
       const rsrc_t r4 = tile_rows(kp, tile, p.ldk);
@@ -312,7 +336,7 @@ struct Pipe : Where<Params, KIND> {
   }
   G9_DEV void dma_v(int tile, int buf) {
     if constexpr (KIND == kPaged) {
-      dma_paged(vp, tile, this->pgv, lds0 + kLdsV + buf * kTileV + kMine / 8 * wave * kGroupV, 1024, voffv, p.v_b, p.v_t);
+      dma_paged(vp, tile, this->pgv, lds0 + kLdsV + buf * kTileV + kMine / 8 * wave * kGroupV, 1024, voff_v(), p.v_b, p.v_t);
     } else if constexpr (KIND == kPacked) {
       const rsrc_t r4 = tile_rows(vp, tile, p.ldv);
 #pragma unroll
@@ -332,7 +356,8 @@ struct Pipe : Where<Params, KIND> {
   // BUF < 0: buffer `buf` (kPaged).
   template <int BUF>
   G9_DEV void read_k(int buf = 0) {
-    const u32 ak_buf = BUF < 0 ? ak + buf * kTileK : ak;
+    u32 ak_buf = ak;
+    if constexpr (KIND == kPaged) ak_buf = at_k() + buf * kTileK;
 #pragma unroll
     for (int s = 0; s < kNS; ++s)
 #pragma unroll
@@ -342,7 +367,8 @@ struct Pipe : Where<Params, KIND> {
   }
   template <int BUF>
   G9_DEV void read_v(int buf = 0) {
-    const u32 av_buf = BUF < 0 ? av + buf * kTileV : av;
+    u32 av_buf = av;
+    if constexpr (KIND == kPaged) av_buf = at_v() + buf * kTileV;
 #pragma unroll
     for (int t = 0; t < kKS; ++t)
 #pragma unroll

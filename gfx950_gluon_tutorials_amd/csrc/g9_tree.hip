@@ -380,6 +380,27 @@ struct WidePipe {
   static constexpr int kLds = T::kLdsBytes + kWaves * T::kScratchBytes;
 };
 
+// The kernel's argument, read again (scalar loads) where the compiler cannot take
+// it for what it has: what only a block's beginning and end need is not held, and
+// spilled, through the loop.
+G9_DEV Params again() {
+  typedef const u32 __attribute__((address_space(4))) Const;
+  struct Words {
+    u32 w[sizeof(Params) / 4];
+  } x;
+  Const* a = (Const*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(Params) / 4; ++i) x.w[i] = a[i];
+  Params p = __builtin_bit_cast(Params, x);
+  const auto global = [](auto*& t) {
+    typedef std::remove_reference_t<decltype(*t)> T;
+    t = (T*)(__attribute__((address_space(1))) T*)t;
+  };
+  global(p.q), global(p.kc), global(p.vc), global(p.o), global(p.lse), global(p.table), global(p.part);
+  return p;
+}
+
 template <bool BF16, int HD>
 G9_DEV void wide(const Params& p, char* smem) {
   using L = Wide<HD>;
@@ -394,29 +415,21 @@ G9_DEV void wide(const Params& p, char* smem) {
   P.lds0 = (u32)(uintptr_t)to_lds(smem);
   P.pscratch = smem + PipeT::kLdsBytes + P.wave * PipeT::kScratchBytes;
   P.sc = p.scale_log2;
-  // A DMA's lane i fetches chunk i / 8 of row i % 8 (V: of row i % 8 ^ 4 (chunk /
-  // 2 % 2), see Kind).
-  P.voffk = (u32)(lane & 7) * p.k_t + (lane >> 3) * 16;
-  P.voffv = (u32)((lane & 7) ^ (4 * (lane >> 4 & 1))) * p.v_t + (lane >> 3) * 16;
-  P.ak = P.lds0 + ((lane & 31) >> 3) * PipeT::kGroupK + h * 128 + (lane & 7) * 16;
-  {
-    const int G = lane >> 4 & 1, jj = lane & 15;
-    P.av = P.lds0 + PipeT::kLdsV + (2 * G + ((jj & 3) >> 1)) * 128 + ((4 * h + (jj >> 2)) ^ (4 * G)) * 16 + 8 * (jj & 1);
-  }
   const bool lag = P.wave >= 4;
   const int row = P.wave * 32 + (lane & 31);
   while (left > 0) {
     const int seg = min(left, cur.r.tiles - cur.tile);
+    const Params pb = again();
     P.keys = min(cur.r.keys, (cur.tile + seg) * PipeT::kBN);
     P.wlim = min(cur.r.context, P.keys);
     P.t0 = cur.tile;
-    P.table = p.table + cur.b * p.table_stride;
-    P.row = row_of<L>(p, cur, row);
+    P.table = pb.table + cur.b * pb.table_stride;
+    P.row = row_of<L>(pb, cur, row);
     P.nte = max((seg + 1) & ~1, 2);
-    P.kp = p.kc + cur.hk * p.k_h;
-    P.vp = p.vc + cur.hk * p.v_h;
+    P.kp = pb.kc + cur.hk * pb.k_h;
+    P.vp = pb.vc + cur.hk * pb.v_h;
     const int nte = P.nte;
-    const char* const qrow = query_of<L>(p, cur, row, P.row.node);
+    const char* const qrow = query_of<L>(pb, cur, row, P.row.node);
 #pragma unroll
     for (int s = 0; s < PipeT::kNS; ++s) P.qf[s] = *reinterpret_cast<const u32x4*>(qrow + (16 * s + 8 * h) * 2);
     // The prologue of g9_fmha.hip's kernel, with more tiles asked for.
@@ -464,7 +477,7 @@ G9_DEV void wide(const Params& p, char* smem) {
     waitcnt<63, 0>();
     if (lag) barrier();
     // A wave without query rows leaves the tiles to the others.
-    const int own = (cur.block * L::kBlock + P.wave * 32) / p.group < cur.r.n ? nte : 2;
+    const int own = (cur.block * L::kBlock + P.wave * 32) / pb.group < cur.r.n ? nte : 2;
     int j = 0;
     for (; j + 2 < own; j += 2) {
       P.template step<0, true>(j, sa, sb);
@@ -476,10 +489,11 @@ G9_DEV void wide(const Params& p, char* smem) {
     for (j += 2; j < nte; ++j) P.idle(j);
     if (!lag) barrier();
     const bool from_start = cur.tile == 0, last = cur.tile + seg == cur.r.tiles;
-    finish<BF16, HD, L>(p, cur, last && from_start ? -1 : (int)(2 * worker + (from_start ? 1 : 0)), row, P.row.node, P.o,
+    const Params pe = again();
+    finish<BF16, HD, L>(pe, cur, last && from_start ? -1 : (int)(2 * worker + (from_start ? 1 : 0)), row, P.row.node, P.o,
                         P.m, P.l);
     left -= seg + L::kLead;
-    if (left > 0) cur = L::next_block(p, cur);
+    if (left > 0) cur = L::next_block(pe, cur);
     barrier();  // the stages are read: the next block's tiles take them
   }
 }
