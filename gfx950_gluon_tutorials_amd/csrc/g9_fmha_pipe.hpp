@@ -269,30 +269,28 @@ struct Pipe : Where<Params, KIND> {
   G9_DEV u32 second(u32 a) const {
     return KIND == kPaged ? a + kGroupV : a + 128;
   }
-  // kPaged: the lane's offsets, worked out at each use (held they would be
-  // spilled, and a reload waits for every DMA in flight).  A DMA's lane i fetches
-  // chunk i / 8 of row i % 8 (V: of row i % 8 ^ 4 (chunk / 2 % 2), see Kind).
+  // kPaged: lane i's offsets.  A DMA's lane i fetches chunk i / 8 of row i % 8 (V:
+  // of row i % 8 ^ 4 (chunk / 2 % 2), see Kind).
+  G9_DEV u32 voff_k_of(u32 i) const { return (i & 7) * p.k_t + (i >> 3) * 16; }
+  G9_DEV u32 voff_v_of(u32 i) const { return ((i & 7) ^ (i >> 2 & 4)) * p.v_t + (i >> 3) * 16; }
+  G9_DEV u32 ak_of(u32 i) const { return lds0 + ((i & 31) >> 3) * kGroupK + (i >> 5) * 128 + (i & 7) * 16; }
+  G9_DEV u32 av_of(u32 i) const {
+    const u32 G = i >> 4 & 1, jj = i & 15;
+    return lds0 + kLdsV + (2 * G + ((jj & 3) >> 1)) * 128 + ((4 * (i >> 5) + (jj >> 2)) ^ (4 * G)) * 16 + 8 * (jj & 1);
+  }
+  // At head dim 64 they are worked out at each use: held, they and others were
+  // spilled, and a reload waits for every DMA in flight (16 x 6000 tokens by 64
+  // rows 120 us instead of 66).  At 128 there is room, and neither is better (held
+  // and worked out, 64 rows: 4 x 8000 and 200 x 100 tokens 97 and 104, 16 x 6000
+  // 101 and 95).
+  static constexpr bool kHeld = HD == 128;
   static G9_DEV u32 lane_now() {
     u32 x;
     asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
     return x;
   }
-  G9_DEV u32 voff_k() const {
-    const u32 i = lane_now();
-    return (i & 7) * p.k_t + (i >> 3) * 16;
-  }
-  G9_DEV u32 voff_v() const {
-    const u32 i = lane_now();
-    return ((i & 7) ^ (i >> 2 & 4)) * p.v_t + (i >> 3) * 16;
-  }
-  G9_DEV u32 at_k() const {
-    const u32 i = lane_now();
-    return lds0 + ((i & 31) >> 3) * kGroupK + (i >> 5) * 128 + (i & 7) * 16;
-  }
-  G9_DEV u32 at_v() const {
-    const u32 i = lane_now(), G = i >> 4 & 1, jj = i & 15;
-    return lds0 + kLdsV + (2 * G + ((jj & 3) >> 1)) * 128 + ((4 * (i >> 5) + (jj >> 2)) ^ (4 * G)) * 16 + 8 * (jj & 1);
-  }
+  G9_DEV u32 voff_k() const { return kHeld ? voffk : voff_k_of(lane_now()); }
+  G9_DEV u32 voff_v() const { return kHeld ? voffv : voff_v_of(lane_now()); }
   // kPaged: this wave's rows of a tile, 8 by 256 bytes or 16 by 128.
   static constexpr int kMine = kBN / kWaves;
   G9_DEV int my_key(int tile) const { return (this->t0 + tile) * kBN + kMine * wave; }
@@ -357,7 +355,7 @@ struct Pipe : Where<Params, KIND> {
   template <int BUF>
   G9_DEV void read_k(int buf = 0) {
     u32 ak_buf = ak;
-    if constexpr (KIND == kPaged) ak_buf = at_k() + buf * kTileK;
+    if constexpr (KIND == kPaged) ak_buf = (kHeld ? ak : ak_of(lane_now())) + buf * kTileK;
 #pragma unroll
     for (int s = 0; s < kNS; ++s)
 #pragma unroll
@@ -368,7 +366,7 @@ struct Pipe : Where<Params, KIND> {
   template <int BUF>
   G9_DEV void read_v(int buf = 0) {
     u32 av_buf = av;
-    if constexpr (KIND == kPaged) av_buf = at_v() + buf * kTileV;
+    if constexpr (KIND == kPaged) av_buf = (kHeld ? av : av_of(lane_now())) + buf * kTileV;
 #pragma unroll
     for (int t = 0; t < kKS; ++t)
 #pragma unroll

@@ -415,6 +415,8 @@ G9_DEV void wide(const Params& p, char* smem) {
   P.lds0 = (u32)(uintptr_t)to_lds(smem);
   P.pscratch = smem + PipeT::kLdsBytes + P.wave * PipeT::kScratchBytes;
   P.sc = p.scale_log2;
+  P.voffk = P.voff_k_of(lane), P.voffv = P.voff_v_of(lane);
+  P.ak = P.ak_of(lane), P.av = P.av_of(lane);
   const bool lag = P.wave >= 4;
   const int row = P.wave * 32 + (lane & 31);
   while (left > 0) {
@@ -645,19 +647,19 @@ namespace {
 // average to one K/V head.  Measured (us a call, blocks of 32, 64 and 256 rows;
 // 8 K/V heads, a cache that no last level holds, one MI355X):
 //   head dim 64     16 x 6000 tokens    64 x 100-8192     256 x 200-600
-//     32 rows        62   69  123       147  164  309      73   80  200
-//     64 rows        99   73  125       262  175  315     116   89  208
-//     128 rows      147  118  121       495  304  298     207  151  238
-//     256 rows      254  182  138       983  577  337     411  283  295
+//     32 rows        62   69   62       149  166  173      73   80  136
+//     64 rows        99   72   66       262  175  177     116   88  141
+//     96 rows       133  117   70       375  301  183     160  143  155
+//     128 rows      147  118   73       497  304  196     206  152  162
 //   head dim 128 (blocks of 64 do not fit its registers)
 //     32 rows       100    -   96       248    -  230     125    -  139
-//     64 rows       153    -   98       460    -  245     204    -  150
-//     128 rows      239    -  105       875    -  268     360    -  179
-// and 1 x 700 tokens, 32 rows: 16 and 24 (head dim 64), 19 and 22.
+//     64 rows       155    -   97       460    -  240     204    -  151
+//     128 rows      239    -  105       876    -  268     361    -  179
+// and 1 x 700 tokens, 32 rows: 15 and 21 (head dim 64), 19 and 22.
 enum { Q32, Q64, Q256 };
 int form_of(int64_t B, int64_t T, int64_t group, int64_t D) {
   const int64_t rows = (T + B - 1) / B * group;
-  return rows <= 32 ? Q32 : D == 64 && rows <= 128 ? Q64 : Q256;
+  return rows <= 32 ? Q32 : D == 64 && rows <= 64 ? Q64 : Q256;
 }
 // The sums of 2 x 1024 blocks of 32 or 64 rows, or of 2 x 256 of 256.
 size_t part_floats(int form, int64_t D) { return (size_t)2 * (form == Q32 ? 1024 * 32 : 1024 * 64) * (D + 2); }
