@@ -18,7 +18,8 @@ def varlen_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
 
     q is (T, HQ, D), k and v are (TK, HK, D) with HQ a multiple of HK, fp16 or
     bf16, head dim 64 or 128; any strides with a unit head-dim stride and steps
-    of 16 bytes, so slices of one fused q/k/v projection are read in place.
+    of 16 bytes, below 8 MiB a token, so slices of one fused q/k/v projection, and
+    expanded or overlapping q, k and v, are read in place.
     ``cu_seqlens`` (B + 1, int32, on the GPU) holds the sequences' row offsets in
     q, and in k and v unless ``cu_seqlens_k`` gives theirs.  With ``causal`` query
     i of Lq reads the keys j <= i + Lk - Lq: where a prompt's first part is

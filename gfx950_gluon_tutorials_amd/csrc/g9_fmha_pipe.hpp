@@ -62,6 +62,11 @@ G9_DEV float xhalf(float x, F op) {
   return op(__int_as_float(r[0]), __int_as_float(r[1]));
 }
 
+// Bytes from the first of `rows` rows to the end of the last one, `ld` apart and
+// `row` long: a descriptor's range.  Not rows * ld, which leaves out values where
+// rows are closer than they are long (expanded or overlapping tensors).
+G9_DEV u32 extent(int rows, u32 ld, u32 row) { return rows > 0 ? (u32)(rows - 1) * ld + row : 0; }
+
 // LDS-DMA of 16 bytes per lane (lane i writes lds + 16 i, reading global
 // voff + soff) issued as inline assembly, so the compiler does not track it:
 // it adds no wait for these DMAs before LDS reads (it cannot tell the read
@@ -252,14 +257,15 @@ struct Pipe : Where<Params, KIND> {
 
   // DMA q = kDW w + i of wave w covers chunk column q / kRH, rows 64 (q % kRH)
   // .. +63 of a tile: lane i fetches row 64 (q % kRH) + i.
-  // kPacked: the rows of a tile that the sequence has.
+  // kPacked: the rows of a tile that the sequence has.  Rows behind them read as
+  // zeros, or as values of the last row where rows overlap: masked either way.
   G9_DEV rsrc_t tile_rows(const char* base, int tile, u32 ld) const {
     const int left = min(max(keys - tile * kBN, 0), kBN);
     const unsigned long long at = (unsigned long long)base + (unsigned long long)(u32)(tile * kBN) * ld;
     // Uniform, but the 64-bit product may be formed on the vector unit.
     const u32 lo = (u32)__builtin_amdgcn_readfirstlane((int)at), hi = (u32)__builtin_amdgcn_readfirstlane((int)(at >> 32));
     return make_rsrc(reinterpret_cast<const void*>((unsigned long long)hi << 32 | lo),
-                     (u32)__builtin_amdgcn_readfirstlane((int)((u32)left * ld)));
+                     (u32)__builtin_amdgcn_readfirstlane((int)extent(left, ld, HD * 2)));
   }
   G9_DEV int first_tile() const {
     if constexpr (KIND == kPaged) return this->t0;

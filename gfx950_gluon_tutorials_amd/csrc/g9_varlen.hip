@@ -210,7 +210,7 @@ G9_DEV void varlen_fwd(const VarParams& p, char* smem) {
   P.pscratch = smem + PipeT::kLdsBytes + wave * PipeT::kScratchBytes;
   const int nte = P.nte;
   const char* qb = p.q + hq * p.q_h + (size_t)(t.q0 + t.mb * kBlockM) * p.ldq;
-  const rsrc_t rq = make_rsrc(qb, (u32)min(t.lq - t.mb * kBlockM, kBlockM) * p.ldq);
+  const rsrc_t rq = make_rsrc(qb, extent(min(t.lq - t.mb * kBlockM, kBlockM), p.ldq, HD * 2));
   P.kp = p.k + hk * p.k_h + (size_t)t.k0 * p.ldk;
   P.vp = p.v + hk * p.v_h + (size_t)t.k0 * p.ldv;
 #pragma unroll
@@ -432,15 +432,17 @@ extern "C" int g9_varlen_fwd(const void* q, const void* k, const void* v, void* 
       HQ % HK || (D != 64 && D != 128) || !scale_ok(sm_scale))
     return G9_ERR_SHAPE;
   if (!q_strides || !k_strides || !v_strides || !o_strides) return G9_ERR_LAYOUT;
-  if (!steps(q_strides, 2) || !steps(k_strides, 2) || !steps(v_strides, 2) || !steps(o_strides, 2))
-    return G9_ERR_LAYOUT;
+  // The step of a single row is never taken.
+  const int64_t qs[2] = {T > 1 ? q_strides[0] : D, q_strides[1]}, os[2] = {T > 1 ? o_strides[0] : D, o_strides[1]};
+  const int64_t ks[2] = {TK > 1 ? k_strides[0] : D, k_strides[1]}, vs[2] = {TK > 1 ? v_strides[0] : D, v_strides[1]};
+  if (!steps(qs, 2) || !steps(ks, 2) || !steps(vs, 2) || !steps(os, 2)) return G9_ERR_LAYOUT;
   const int64_t size[2] = {T, HQ};
-  if (!apart(size, o_strides, 2, D)) return G9_ERR_LAYOUT;
+  if (!apart(size, os, 2, D)) return G9_ERR_LAYOUT;
   if (B == 0 || T == 0) return G9_OK;
   if (!q || !o || (TK && (!k || !v)) || !cu_q || !cu_k) return G9_ERR_LAYOUT;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || ((uintptr_t)lse & 3)) return G9_ERR_LAYOUT;
   // Token strides within 32 bits, a tile's rows within a descriptor's range.
-  for (const int64_t* st : {q_strides, k_strides, v_strides, o_strides})
+  for (const int64_t* st : {qs, ks, vs, os})
     if (st[0] * 2 * fa::kBlockM >= (int64_t(1) << 31)) return G9_ERR_LAYOUT;
   fa::VarParams p{};
   p.q = static_cast<const char*>(q);
@@ -450,9 +452,8 @@ extern "C" int g9_varlen_fwd(const void* q, const void* k, const void* v, void* 
   p.lse = lse;
   p.cu_q = cu_q;
   p.cu_k = cu_k;
-  p.q_h = q_strides[1] * 2, p.k_h = k_strides[1] * 2, p.v_h = v_strides[1] * 2, p.o_h = o_strides[1] * 2;
-  p.ldq = (u32)(q_strides[0] * 2), p.ldk = (u32)(k_strides[0] * 2);
-  p.ldv = (u32)(v_strides[0] * 2), p.ldo = (u32)(o_strides[0] * 2);
+  p.q_h = qs[1] * 2, p.k_h = ks[1] * 2, p.v_h = vs[1] * 2, p.o_h = os[1] * 2;
+  p.ldq = (u32)(qs[0] * 2), p.ldk = (u32)(ks[0] * 2), p.ldv = (u32)(vs[0] * 2), p.ldo = (u32)(os[0] * 2);
   p.B = (int)B, p.T = (int)T, p.TK = (int)TK, p.HQ = (int)HQ, p.HK = (int)HK;
   p.causal = causal != 0;
   p.scale_log2 = sm_scale * fa::kLog2e;

@@ -81,10 +81,11 @@ struct Wave {
   }
 
   // Rows 16 i .. 16 i + 15 of a tile, `rows` of them there (the others read as
-  // zeros), K's at k, V's at v, k_t and v_t bytes apart.
+  // zeros, or as values of the last one where rows overlap), K's at k, V's at v, k_t
+  // and v_t bytes apart.
   G9_DEV void fill_piece(int i, int stage, const char* k, const char* v, int rows, u32 k_t, u32 v_t) const {
-    const rsrc_t rk = make_rsrc(uniform(k), uniform((u32)rows * k_t));
-    const rsrc_t rv = make_rsrc(uniform(v), uniform((u32)rows * v_t));
+    const rsrc_t rk = make_rsrc(uniform(k), uniform(extent(rows, k_t, kRow)));
+    const rsrc_t rv = make_rsrc(uniform(v), uniform(extent(rows, v_t, kRow)));
 #pragma unroll
     for (int jj = 0; jj < 16 / kRows; ++jj) {
       const int j = i * (16 / kRows) + jj;

@@ -67,7 +67,8 @@ int g9_fmha_fwd(const void* q, const void* k, const void* v, void* o, float* lse
  * - Strides are in ELEMENTS with a unit head-dim stride left out: (token, head)
  *   for packed tensors, (block, token, head) for caches.  They are multiples of
  *   8 and not negative; base pointers are 16-byte aligned.  What is written (o,
- *   the caches) must not overlap itself.  Offsets are 64-bit throughout.
+ *   the caches) must not overlap itself; what is only read may (expanded tensors),
+ *   but for g9_tree_fwd's caches.  Offsets are 64-bit throughout.
  * - Lengths, tables and offsets are device data, read when the kernel runs.
  *   Whatever they hold, nothing outside the tensors is touched: negative lengths
  *   count as 0, cu_seqlens are held inside the packed tensor, a table entry
@@ -122,7 +123,8 @@ int g9_write_cache(const void* k, const void* v, void* k_cache, void* v_cache, c
  * causal != 0 lets query i of Lq read the keys j <= i + Lk - Lq, so that a prompt
  * whose first part is cached passes its new queries only.  lse: optional fp32
  * HQ x T, contiguous: the natural-log log-sum-exp of each query's scaled scores.
- * (T / 256 + min(B, T)) x HQ below 2^23.
+ * (T / 256 + min(B, T)) x HQ below 2^23; token strides below 2^22 elements (of one
+ * row, any).
  */
 int g9_varlen_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* cu_q,
                   const int32_t* cu_k, int64_t B, int64_t T, int64_t TK, int64_t HQ, int64_t HK, int64_t D,
