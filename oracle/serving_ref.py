@@ -74,13 +74,16 @@ def tolerances(o, lse, mag, spread, dtype_eps, longest, D, vmax, subnormal):
       and 2^-22 more for the scale, the exponent's argument and the exponential;
     * sums over the keys are fp32: longest 2^-24 relative;
     * each weight is rounded to the 16-bit type before its product with v: half a
-      step of the average of |v| (and `subnormal` per key below the type's normal
-      range, against a largest weight of at least 1/256);
+      step of the average of |v|, and `subnormal` per key below the type's normal
+      range.  Weights are 2^(score - m), m the row's largest score or (the lazy
+      maximum) at most 8 below it: the largest weight is at least 1, but for the
+      rounding of its exponent, and so is the sum that divides.  Parts of a row are
+      scaled to the largest of their m, by factors of at most 1;
     * the output is rounded once more: half a step of its value.
     """
     h = dtype_eps / 2
     e = D * 2.0**-24 * spread + 2.0**-22 * (1 + spread) + longest * 2.0**-24
-    to = h * np.abs(o) * (1 + h) + (h + 3 * e) * mag + 256 * longest * subnormal * vmax + 1e-7
+    to = h * np.abs(o) * (1 + h) + (h + 3 * e) * mag + (1 + 2 * e) * longest * subnormal * vmax + 1e-7
     tl = 2 * e + 2.0**-23 * np.abs(lse) + 1e-7
     return to, tl
 

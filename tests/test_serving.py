@@ -306,6 +306,27 @@ def test_oracle_attention_against_torch(lq, lk, causal):
     assert np.allclose(lse, torch.logsumexp(x, 1).numpy(), atol=1e-12)
 
 
+@pytest.mark.parametrize("n", [1100, 3000, 9000])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_the_bound_tells_a_wrong_output_at_the_longest_lengths(n, D, dtype):
+    """Outputs of zeros, and those of the first half of the keys, leave it nearly
+    everywhere; the weights and the output rounded to 16 bits do not."""
+    gen = torch.Generator().manual_seed(n + D)
+    q, k, v = (torch.randn(m, D, generator=gen).to(dtype).double().numpy() for m in (8, n, n))
+    reads = np.ones((8, n), bool)
+    o, lse, mag, spread = R.masked_attention(q, k, v, reads, D**-0.5)
+    subnormal = 2.0**-25 if dtype == torch.float16 else 0.0
+    to, _ = R.tolerances(o, lse, mag, spread, torch.finfo(dtype).eps, n, D, float(np.abs(v).max()), subnormal)
+    half = R.masked_attention(q, k[:n // 2], v[:n // 2], reads[:, :n // 2], D**-0.5)[0]
+    assert (np.abs(o) > to).mean() > 0.5 and (np.abs(half - o) > to).mean() > 0.5
+    for lag in (0.0, 8.0):  # of the running maximum, in powers of two
+        s = torch.from_numpy(q @ k.T * D**-0.5 / np.log(2.0))
+        w = torch.exp2(s - (s.amax(1, keepdim=True) - lag))
+        got = (w.to(dtype).double() @ torch.from_numpy(v) / w.sum(1, keepdim=True)).to(dtype).double().numpy()
+        assert (np.abs(got - o) <= to).all()
+
+
 def test_oracle_slots_by_hand():
     cu, slots, pos, taken, table = R.slots([3, 4], [2, 5], np.array([[9, 0, 0], [7, 0, 0]], np.int32), [5, 6], 0, 4, 8)
     assert cu.tolist() == [0, 2, 7] and taken == 3
