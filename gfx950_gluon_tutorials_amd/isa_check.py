@@ -250,6 +250,10 @@ def _lds_step(state: dict, ins: Instr, violations: list, func: str):
 
 
 _SCALAR = re.compile(r"\b(vcc|m0)(?:_lo|_hi)?\b")
+# Scalar instructions whose first operand is not a result, or one that they may
+# leave as it was (s_cmov); vector ones with a scalar result behind the first.
+_SCALAR_KEEPS = ("s_cmp", "s_bitcmp", "s_cmov", "s_set", "s_cbranch")
+_SCALAR_SECOND = re.compile(r"v_(?:(?:add|sub|subrev|addc|subb|subbrev)_co_|div_scale_|mad_[ui]64_)")
 
 
 def _sregs(ops: str) -> set[tuple[str, int]]:
@@ -278,10 +282,11 @@ def _sgpr_step(state: dict, ins: Instr, violations: list, func: str):
         else:
             state[r] = (rem, state[r][1])
     if ins.mnemonic.startswith("s_"):
-        for r in _sregs(operands[0]) if operands else ():
-            state.pop(r, None)  # written again, by the scalar unit
+        if operands and not ins.mnemonic.startswith(_SCALAR_KEEPS):
+            for r in _sregs(operands[0]):
+                state.pop(r, None)  # written again, by the scalar unit
     elif ins.mnemonic.startswith("v_") and operands:
-        for r in _sregs(operands[0]):
+        for r in _sregs(",".join(operands[:2]) if _SCALAR_SECOND.match(ins.mnemonic) else operands[0]):
             state[r] = (VMEM_AFTER_VALU_SGPR, ins.line)
 
 
