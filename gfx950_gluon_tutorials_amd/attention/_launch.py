@@ -6,6 +6,7 @@ call raises."""
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from .common import get_shape_from_layout, get_strides_from_layout
@@ -128,12 +129,15 @@ def lse_fits(lse, HQ, T) -> None:
 
 
 def plain(*tensors) -> None:
-    """Refuses what the kernels would silently lose: a gradient, a pending negation."""
+    """Refuses what the kernels would silently lose: a gradient, a tangent, a pending negation."""
+    dual = forward_ad._current_level >= 0
     for t in tensors:
         if t is None:
             continue
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError("forward only: call it under torch.no_grad(), or detach the tensors that require a gradient")
+        if dual and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError("forward only: a tensor has a forward-mode tangent; pass its primal")
         if t.is_neg():
             raise ValueError("a lazily negated view: call resolve_neg() first")
 

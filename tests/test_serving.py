@@ -172,6 +172,28 @@ def test_requires_grad_is_fine_without_a_graph(calls):
     assert len(calls) == 1
 
 
+def test_forward_mode_tangents_are_refused(calls):
+    """Of anything read or written, with grad mode off too; not of plain tensors
+    inside the level, nor outside of one."""
+    def dual(t):
+        return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+
+    with torch.autograd.forward_ad.dual_level():
+        _prompt(), _tree(), _write()
+        assert len(calls) == 3
+        calls.clear()
+        bad = [(_prompt, dict(q=dual(torch.zeros(6, 4, 64).bfloat16()))), (_prompt, dict(v=dual(torch.zeros(6, 2, 64).bfloat16()))),
+               (_prompt, dict(o=dual(torch.zeros(6, 4, 64).bfloat16()))), (_prompt, dict(lse=dual(torch.zeros(4, 6)))),
+               (_tree, dict(q=dual(torch.zeros(6, 4, 64).bfloat16()))), (_tree, dict(k_cache=dual(torch.zeros(3, 16, 2, 64).bfloat16()))),
+               (_write, dict(k=dual(torch.zeros(6, 2, 64).half()))), (_write, dict(v_cache=dual(torch.zeros(3, 16, 2, 64).half())))]
+        for f, kw in bad:
+            with pytest.raises(ValueError, match="forward only"):
+                f(**kw)
+            with pytest.raises(ValueError, match="forward only"), torch.no_grad():
+                f(**kw)
+    assert not calls
+
+
 # --- the C entries -------------------------------------------------------------
 
 def _arr(*v):
