@@ -526,9 +526,8 @@ G9_DEV void join(const Params& p, float* lds) {
   if (w >= L::workers(total) || st.tile == 0) return;
   const unsigned long long u0 = L::part_begin(w, total) - (unsigned)st.tile;
   const unsigned w0 = L::worker_of(u0, total), n = L::worker_of(u0 + st.tiles - 1, total) - w0 + 1;
-  // Worker w0 has the block in slot 1 unless it began it before its part; the
-  // others in slot 0.
-  const size_t head = (size_t)2 * w0 + (L::part_begin(w0, total) <= u0 ? 1 : 0);
+  // Worker w0, in whose part the block begins, has it in slot 1, the others in slot 0.
+  const size_t head = (size_t)2 * w0 + 1;
   const float* const ml = p.part + (size_t)2 * L::kWorkers * L::kBlock * HD;
   const int row0 = st.block * L::kBlock;
   const u32 rows = (u32)min((long long)st.n * p.group - row0, (long long)L::kBlock);

@@ -109,7 +109,7 @@ G9_DEV bool find_tile(const VarParams& p, int rank, int per, int* lds, Tile& t) 
     for (int i = 0; i < nth; ++i) who &= who - 1;
     seq = __builtin_ctzll(who);
   } else {
-    // Thread i holds the sequences i, i + 512, ... (again from memory each time:
+    // Thread i holds the sequences i, i + THREADS, ... (again from memory each time:
     // they are in L1).
     const auto total = [&](auto f) {
       int x = 0;
