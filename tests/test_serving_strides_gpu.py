@@ -71,7 +71,7 @@ def test_expanded_tensors_against_the_oracle(gpu, D, dtype, HQ):
 
 
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("step", [0, 8, 4096])
+@pytest.mark.parametrize("step", [0, 3, 8, 4096])
 def test_a_single_row_of_any_stride(gpu, D, step):
     gen = torch.Generator().manual_seed(D)
     q, k, v = (torch.randn(1, 2, D, generator=gen).half().to(gpu) for _ in range(3))
