@@ -144,7 +144,8 @@ def plain(*tensors) -> None:
 
 # What a call's arguments are but for their addresses and contents, to the
 # arguments of the C call that follow from it: a call of the same kind as an
-# earlier one is not checked again (decoding's host time is 6.9 us instead of 10.6).
+# earlier one is not checked again (a call's host time: write_cache 8.5 us instead of
+# 13.8, varlen_attention 10.8 instead of 16.7, decoding 16.8 instead of 24.5).
 _plans: dict = {}
 
 

@@ -138,8 +138,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     fp16 or bf16, head dim 64 or 128, grouped heads; block_size a power of two
     from 16 to 1024.  Returns ``o`` (T, HQ, D), allocated when not given; rows
     behind the last request are left as they were, a row that reads nothing gives
-    zeros.  ``lse`` as in ``varlen_attention``.  Asynchronous on the current
-    stream; forward only."""
+    zeros.  ``lse`` and the arithmetic as in ``varlen_attention``.  Asynchronous on
+    the current stream; forward only."""
     sm_scale = None if sm_scale is None else float(sm_scale)
     key = ("tree", sm_scale, sig(q), sig(k_cache), sig(v_cache), sig(block_table), sig(lengths), sig(cu_seqlens),
            tree_mask is not None and sig(tree_mask), o is not None and sig(o), lse is not None and sig(lse))

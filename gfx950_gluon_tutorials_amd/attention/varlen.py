@@ -23,13 +23,16 @@ def varlen_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     ``cu_seqlens`` (B + 1, int32, on the GPU) holds the sequences' row offsets in
     q, and in k and v unless ``cu_seqlens_k`` gives theirs.  With ``causal`` query
     i of Lq reads the keys j <= i + Lk - Lq: where a prompt's first part is
-    cached already, its new queries read all of it.  A query without a key gives
-    zeros (lse -inf).
+    cached already, its new queries read all of it (a sequence's keys are not divided
+    among workgroups here: few queries behind thousands of keys are faster through
+    ``tree_attention``, which does that).  A query without a key gives zeros (lse
+    -inf).
 
     Returns ``o`` (T, HQ, D), allocated when not given; rows behind the last
     sequence are left as they were.  ``lse``, if given, is a contiguous fp32
     (HQ, T) tensor that receives each query's natural-log log-sum-exp.
-    Asynchronous on the current stream; forward only."""
+    Scores, softmax and sums are fp32, each weight is rounded to the input type for
+    its product with v.  Asynchronous on the current stream; forward only."""
     causal, sm_scale = bool(causal), None if sm_scale is None else float(sm_scale)
     key = ("varlen", causal, sm_scale, sig(q), sig(k), sig(v), sig(cu_seqlens), cu_seqlens_k is not None and sig(cu_seqlens_k),
            o is not None and sig(o), lse is not None and sig(lse))

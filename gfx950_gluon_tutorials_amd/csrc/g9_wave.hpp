@@ -4,7 +4,9 @@
 //
 // Per tile a wave computes S^T = K Q^T and O^T += V^T P^T with 32x32x16 MFMAs in
 // the register layouts that g9_fmha.hip describes: the scores are the second
-// product's operand as they stand, V is read by transposing LDS reads.
+// product's operand as they stand, V is read by transposing LDS reads.  The weights
+// P are rounded to the 16-bit type for that product, whose operands are of one type
+// (fp32 products have a sixteenth of the rate); their sum l is taken before.
 #pragma once
 
 #include "g9_fmha_pipe.hpp"

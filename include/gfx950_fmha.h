@@ -62,8 +62,11 @@ int g9_fmha_fwd(const void* q, const void* k, const void* v, void* o, float* lse
  * non-causal over equal lengths).  Common to the entries below:
  *
  * - 16-bit elements (`dtype` G9_F16 or G9_BF16; g9_write_cache moves either),
- *   head dim D 64 or 128, fp32 softmax and accumulation; query head h reads K/V
- *   head h * HK / HQ.
+ *   head dim D 64 or 128; query head h reads K/V head h * HK / HQ.  Scores, the
+ *   softmax's maxima and sums, and the accumulation are fp32; each weight is rounded
+ *   to the input type before its product with V, as in g9_fmha_fwd (the matrix unit
+ *   takes both alike): up to half a step, 2^-8 (bf16) or 2^-11 (fp16), of the average
+ *   of |V|.
  * - Strides are in ELEMENTS with a unit head-dim stride left out: (token, head)
  *   for packed tensors, (block, token, head) for caches.  They are multiples of
  *   8 and not negative; base pointers are 16-byte aligned.  What is written (o,
