@@ -82,6 +82,14 @@ SIGNATURES = {
     "g9_tree_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64,
                            _i64, _i64, _vp, _vp, _vp, _vp, ctypes.c_float, _int, _vp, _sz, _vp]),
     "g9_tree_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "g9_rotary": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, ctypes.c_float, _int, _int, _int, _vp]),
+    "g9_write_latent": (_int, [_vp, _vp, _vp, _vp, _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
+                               _vp, _i64, _i64, ctypes.c_float, _int, _int, _vp]),
+    "g9_latent_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp,
+                             _vp, _vp, ctypes.c_float, _int, _vp, _sz, _vp]),
+    "g9_latent_workspace_size": (_sz, [_i64, _i64, _i64]),
+    "g9_latent_varlen_fwd": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp,
+                                    _i64, _vp, ctypes.c_float, _int, _int, _vp]),
     "g9_workspace_size": (_sz, [_int, _i64, _i64, _i64, _int, _int]),
     "g9_workspace_init": (_int, [_vp, _sz, _vp]),
     "g9_workspace_error": (_int, [_vp, _sz, _vp, ctypes.POINTER(_int)]),

@@ -128,6 +128,18 @@ def lse_fits(lse, HQ, T) -> None:
         raise ValueError("lse must be a contiguous fp32 (query heads, rows) tensor")
 
 
+def mask_words(tree_mask, T) -> int:
+    """64-bit words of a node's row of a tree mask, 0 without one."""
+    if tree_mask is None:
+        return 0
+    if tree_mask.dtype != torch.int64 or tree_mask.dim() not in (1, 2) or not tree_mask.is_contiguous():
+        raise ValueError("tree_mask must be a contiguous int64 (T, words) or (T,) tensor")
+    words = 1 if tree_mask.dim() == 1 else tree_mask.shape[1]
+    if tree_mask.shape[0] != T or words == 0:
+        raise ValueError(f"tree_mask {tuple(tree_mask.shape)} does not fit {T} rows")
+    return words
+
+
 def plain(*tensors) -> None:
     """Refuses what the kernels would silently lose: a gradient, a tangent, a pending negation."""
     dual = forward_ad._current_level >= 0

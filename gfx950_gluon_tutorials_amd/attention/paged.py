@@ -166,13 +166,7 @@ def _plan_tree(key, q, k_cache, v_cache, block_table, lengths, cu_seqlens, tree_
     _launch.int32_of("block_table", block_table, 2)
     if lengths.shape[0] != B or block_table.shape[0] != B:
         raise ValueError(f"cu_seqlens, lengths and block_table hold {B}, {lengths.shape[0]} and {block_table.shape[0]} requests")
-    words = 0
-    if tree_mask is not None:
-        if tree_mask.dtype != torch.int64 or tree_mask.dim() not in (1, 2) or not tree_mask.is_contiguous():
-            raise ValueError("tree_mask must be a contiguous int64 (T, words) or (T,) tensor")
-        words = 1 if tree_mask.dim() == 1 else tree_mask.shape[1]
-        if tree_mask.shape[0] != T or words == 0:
-            raise ValueError(f"tree_mask {tuple(tree_mask.shape)} does not fit {T} rows")
+    words = _launch.mask_words(tree_mask, T)
     _launch.heads_fit(HQ, HK, D)
     if o is not None:
         _launch.rows_of("o", o)

@@ -25,16 +25,18 @@ LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 # profiling.py; never loaded by the wrappers unless G9_LIBRARY points at it.
 LIB_TIMING_PATH = os.path.join(PKG_DIR, "libg9gemm_timing.so")
 # GEMM + MoE + C ABI; small tiles; operand quantizers; flash-attention forward;
-# attention over packed prompts, over a paged cache; the cache's bookkeeping
+# attention over packed prompts, over a paged cache; the cache's bookkeeping;
+# rotary positions; latent attention over a paged cache, over packed prompts
 SOURCES = ["g9_capi.hip", "g9_tile.hip", "g9_quant.hip", "g9_fmha.hip", "g9_varlen.hip",
-           "g9_tree.hip", "g9_paged.hip"]
+           "g9_tree.hip", "g9_paged.hip", "g9_rotary.hip", "g9_latent.hip", "g9_latent_varlen.hip"]
 # Per-source flags.  The flash-attention pipeline: without NaN-preserving semantics for fmax
 # the row-max reduction is one v_max3 per two scores instead of also
 # canonicalizing every MFMA result first (NaN inputs still give NaN rows:
 # their exponentials are NaN).
-SOURCE_FLAGS = {s: ["-fno-honor-nans"] for s in ("g9_fmha.hip", "g9_varlen.hip", "g9_tree.hip")}
+SOURCE_FLAGS = {s: ["-fno-honor-nans"] for s in ("g9_fmha.hip", "g9_varlen.hip", "g9_tree.hip", "g9_latent.hip",
+                                               "g9_latent_varlen.hip")}
 HEADERS = ["g9_common.hpp", "g9_gemm.hpp", "g9_tile.hpp", "g9_tile_pick.hpp",
-           "g9_fmha_pipe.hpp", "g9_wave.hpp", "g9_attn_host.hpp"]
+           "g9_fmha_pipe.hpp", "g9_wave.hpp", "g9_line.hpp", "g9_attn_host.hpp"]
 
 # -packed-fp32-ops: keep the compiler from forming v_pk_*_f32, whose results
 # have been unreliable on the target machines.

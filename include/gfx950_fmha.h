@@ -2,7 +2,8 @@
  * gfx950_fmha.h -- C ABI of the MI355X (gfx950) attention forward passes, built
  * into the same library as gfx950_gemm.h (whose status codes and element types
  * it uses): g9_fmha_fwd (below) over equal lengths, g9_varlen_fwd over packed
- * prompts, g9_tree_fwd over a paged cache, and the cache's bookkeeping.
+ * prompts, g9_tree_fwd over a paged cache, and the cache's bookkeeping; rotary
+ * positions; and latent attention over a paged cache and over packed prompts.
  *
  * g9_fmha_fwd:
  * O = softmax(Q K^T * sm_scale) V for every (batch, query head), non-causal,
@@ -157,6 +158,71 @@ int g9_tree_fwd(const void* q, const void* k_cache, const void* v_cache, void* o
                 const int64_t* kc_strides, const int64_t* vc_strides, const int64_t* o_strides, float sm_scale,
                 int dtype, void* workspace, size_t workspace_bytes, void* stream);
 size_t g9_tree_workspace_size(int64_t B, int64_t T, int64_t HQ, int64_t HK, int64_t D);
+
+/*
+ * Rotary positions (no reference counterpart).  Row t, head h of x (T x H x D, 16
+ * bit) to the same place of o: of its values first .. first + dim - 1 the pairs i of
+ * dim / 2 are turned by the angle positions[t] * freqs[i] (radians, 64 bit) and
+ * multiplied by scale,
+ *   (a, b) -> scale * (a cos - b sin, a sin + b cos),
+ * in fp32, rounded once; the others are copied.  A pair is (first + i, first + dim /
+ * 2 + i), or with interleaved != 0 (first + 2 i, first + 2 i + 1).  inverse != 0 turns
+ * back (the angle's negative): with the same scale that is the gradient of x from
+ * the gradient of o.
+ *
+ * D and first multiples of 8, dim of 16; strides (token, head) in elements,
+ * multiples of 8.  o may be x itself, with the same strides, and must not overlap it
+ * otherwise.
+ */
+int g9_rotary(const void* x, void* o, const int64_t* positions, const double* freqs, int64_t T, int64_t H, int64_t D,
+              int64_t first, int64_t dim, const int64_t* x_strides, const int64_t* o_strides, float scale,
+              int interleaved, int inverse, int dtype, void* stream);
+
+/*
+ * Latent attention (no reference counterpart): every head's keys and values come
+ * from one latent c of 512 values a token, beside which a rotated key of 64 values
+ * serves all heads.  A cache holds a row of 576 values a token, the latent first:
+ * num_blocks x block_size x 576, strides (block, token).  What is common to the packed
+ * and the paged attention above holds here too.
+ *
+ * g9_write_latent: row t of c (T x 512) and of k_rope (T x 64) to slot slots[t] of the
+ * cache; rows whose slot lies outside it are skipped, slots must be distinct.
+ * weight (512 values; NULL: no norm) replaces c by c / sqrt(mean(c^2) + eps) * weight;
+ * freqs (32 values; NULL: no rotation) turns k_rope as g9_rotary does.  c_out (T x
+ * 512) and k_out (T x 64), optional, receive every row as the cache would; they may be
+ * c and k_rope.
+ */
+int g9_write_latent(const void* c, const void* k_rope, void* cache, const int64_t* slots, const void* weight, float eps,
+                    const int64_t* positions, const double* freqs, void* c_out, void* k_out, int64_t T,
+                    int64_t num_blocks, int64_t block_size, int64_t c_stride, int64_t k_stride,
+                    const int64_t* cache_strides, int64_t c_out_stride, int64_t k_out_stride, float scale,
+                    int interleaved, int dtype, void* stream);
+
+/*
+ * The absorbed form: q (T x H x 576) is each head's query times its key projection,
+ * then its rotated part, o (T x H x 512) the weighted latents, which the caller
+ * multiplies by the heads' value projections.  score = sm_scale * q . row; requests,
+ * nodes, masks and workspace (g9_latent_workspace_size bytes) as in g9_tree_fwd.
+ * The cache's tokens at least 576 elements apart.
+ */
+int g9_latent_fwd(const void* q, const void* cache, void* o, float* lse, const int32_t* block_table,
+                  int64_t table_stride, int64_t width, const int32_t* lengths, const int32_t* cu_q,
+                  const int64_t* tree_mask, int64_t words, int64_t B, int64_t T, int64_t H, int64_t num_blocks,
+                  int64_t block_size, const int64_t* q_strides, const int64_t* cache_strides, const int64_t* o_strides,
+                  float sm_scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+size_t g9_latent_workspace_size(int64_t B, int64_t T, int64_t H);
+
+/*
+ * The expanded form over packed sequences: q T x HQ x 192, k and v TK x HK x 128 (the
+ * latents times the heads' projections), k_rope TK x 64, o T x HQ x 128; score =
+ * sm_scale * (q[:128] . k + q[128:] . k_rope).  Sequences, causal and lse as in
+ * g9_varlen_fwd.
+ */
+int g9_latent_varlen_fwd(const void* q, const void* k, const void* v, const void* k_rope, void* o, float* lse,
+                         const int32_t* cu_q, const int32_t* cu_k, int64_t B, int64_t T, int64_t TK, int64_t HQ,
+                         int64_t HK, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                         int64_t k_rope_stride, const int64_t* o_strides, float sm_scale, int dtype, int causal,
+                         void* stream);
 
 #ifdef __cplusplus
 }
