@@ -35,8 +35,8 @@ constexpr int kKeys = 32;               // of a tile
 constexpr int kTile = kKeys * kRowBytes;
 constexpr int kQk = kRow / 16, kPv = kRank / 32;  // products' steps of 16, blocks of 32 values
 constexpr int kDepth = 6;                          // fragments read ahead
-constexpr int kScratch = 32 * kKeys * 2;          // P of a wave's tile, 16 bit
-constexpr int kLds = 4 * kTile + 4 * kScratch;
+constexpr int kLds = 4 * kTile;
+constexpr float kNone = -3.0e38f;                // the maximum of a row that has read nothing: finite, weights 0
 
 struct Params {
   const char* q;
@@ -91,6 +91,21 @@ G9_DEV void settle(f32x16 (&c)[kPv]) {
 // Operands that the vector unit wrote, before the products that take them.
 G9_DEV void ready(u32x4 (&x)[2]) { asm volatile("s_nop 1" : "+v"(x[0]), "+v"(x[1])); }
 
+// One sum out of the accumulation registers (as assembly: the compiler would move all 16 of
+// a block at once, and keep what it had in their place in scratch memory).
+G9_DEV float sum_of(const f32x16& c, int i) {
+  float x;
+  asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(x) : "a"(c[i]));
+  return x;
+}
+
+// The lane, worked out where it is used: what follows from it is not held through the loop.
+G9_DEV int lane_here() {
+  int x;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
+  return x;
+}
+
 // RB blocks of 32 rows share a tile; a step of the workgroup is 4 / RB tiles.
 template <int RB>
 using Steps = Line<Params, kKeys * (4 / RB), 32 * RB, kWgs, 0>;
@@ -101,13 +116,10 @@ struct Rows {
   static constexpr int kGroups = 4 / RB;       // waves that take tiles in turn
   static constexpr int kPieces = 2;            // 16-row pieces of a tile: never across a page
   static constexpr int kDmas = 36 / RB;        // of a wave, for its group's tile
-  static constexpr int kOffs = RB == 4 ? 9 : 18;  // different lane offsets of them
 
   const Params& p;
-  int lane, h, col;
   u32 lds;             // of the workgroup
-  char* scratch;
-  u32 voff[kOffs];
+  u32 voff[9], flip;
   u32 ak, av;          // LDS read bases in a tile (K, V)
   u32x4 qf[kQk];
   f32x16 o[kPv];
@@ -124,14 +136,16 @@ struct Rows {
   static G9_DEV int swz(int r) { return (r >> 1 & 1) << 2 | (r >> 2 & 3); }
 
   G9_DEV void init(char* smem, int wave) {
-    lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
+    const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
     lds = (u32)(uintptr_t)to_lds(smem);
-    scratch = smem + 4 * kTile + wave * kScratch;
-    // DMA j of a 16-row piece writes its bytes 1024 j + 16 lane.
+    // Nine DMAs fill 8 rows: DMA j writes the bytes 1024 j + 16 lane of them.  The 8
+    // rows behind them have bit 1 of their places the other way round: 32 bytes up or down.
+    flip = 0;
 #pragma unroll
-    for (int j = 0; j < kOffs; ++j) {
-      const int n = 64 * (j + (RB == 4 ? 9 * (wave & 1) : 0)) + lane, r = n / 72, place = n - 72 * r;
-      voff[j] = (u32)r * p.c_t + 16 * (place ^ swz(r));
+    for (int j = 0; j < 9; ++j) {
+      const int n = 64 * j + lane, r = n / 72, c = (n - 72 * r) ^ swz(r + (RB == 4 ? 8 * (wave & 1) : 0));
+      voff[j] = (u32)r * p.c_t + 16 * c;
+      flip |= (u32)(c >> 1 & 1) << j;
     }
     ak = col * kRowBytes + 16 * (h ^ swz(col));
     // 16 lanes cover 4 rows and 16 values: lane jj of them row jj / 4, values 4 (jj % 4)
@@ -140,8 +154,8 @@ struct Rows {
     av = r4 * kRowBytes + 16 * ((2 * (lane >> 4 & 1) + ((jj & 3) >> 1)) ^ swz(r4)) + 8 * (jj & 1);
   }
 
-  // This wave's share of the tile that begins with key k0 of request b, into stage
-  // `stage`: pieces by = the pages of its two 16-row pieces.
+  // This wave's share of the tile that begins with key k0, of `all` keys, into stage
+  // `stage`; pg: the pages of the tile's two 16-row pieces.
   G9_DEV void fill(int stage, int k0, int all, const int (&pg)[kPieces], int wave) const {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
@@ -152,25 +166,32 @@ struct Rows {
       const int rows = in ? min(max(all - k, 0), 16) : 0;
       const char* const base = p.cache + (long long)(in ? pg[i] : 0) * p.c_b + (unsigned long long)(u32)off * p.c_t;
       const rsrc_t r = make_rsrc(uniform(base), uniform(extent(rows, p.c_t, kRowBytes)));
-      const u32 to = lds + stage * kTile + i * 16 * kRowBytes + (RB == 4 ? 9 * 1024 * (wave & 1) : 0);
+      const u32 to = lds + stage * kTile + i * 16 * kRowBytes;
 #pragma unroll
-      for (int j = 0; j < kOffs; ++j) dma16_fresh(r, to + 1024 * j, voff[j], 0);
+      for (int half = 0; half < 2; ++half) {
+        if (RB == 4 && half != (wave & 1)) continue;
+#pragma unroll
+        for (int j = 0; j < 9; ++j) {
+          const u32 at = RB == 4 || !half ? voff[j] : voff[j] + 32 - ((flip >> j & 1) << 6);
+          dma16_fresh(r, to + 9216 * half + 1024 * j, at, half * 8 * p.c_t);
+        }
+      }
     }
   }
 
   G9_DEV void begin(const char* qrow) {
+    const int h = lane_here() >> 5;
 #pragma unroll
     for (int s = 0; s < kQk; ++s) qf[s] = *reinterpret_cast<const u32x4*>(qrow + (16 * s + 8 * h) * 2);
-    m = -3.0e38f, l = 0.f;  // finite: a row that has read nothing has weights of 0
+    m = kNone, l = 0.f;
 #pragma unroll
-    for (int d = 0; d < kPv; ++d) o[d] = f32x16{};
-  }
-
-  G9_DEV u32x4 v_at(u32 base, int k, int d) const {
-    const u32 a = (base ^ (64 * (d & 1))) + 128 * (d >> 1) + 16 * kRowBytes * k;
-    const u32 b = (base ^ (64 * (d & 1) + 32)) + 128 * (d >> 1) + 16 * kRowBytes * k + 8 * kRowBytes;
-    const u32x2 lo = tr_read(a), hi = tr_read(b);
-    return u32x4{lo.x, lo.y, hi.x, hi.y};
+    for (int d = 0; d < kPv; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float x;
+        asm volatile("v_accvgpr_write_b32 %0, 0" : "=a"(x));
+        o[d][i] = x;
+      }
   }
 
   // Adds the tile in `stage`, whose first key is k0; TAIL: not every row may read all of it.
@@ -200,28 +221,50 @@ struct Rows {
       f[s % kDepth] = s + kDepth < kQk ? k_at(s + kDepth) : v_at(s + kDepth - kQk);
     }
     settle(sc);
+    u32x4 keep[2];  // TAIL: the keys whose values enter the product
     if constexpr (TAIL) {
-      const u32 bits = (u32)node_reads(p, row, k0, keys) >> (4 * h);
+      const int h = lane_here() >> 5;
+      const u32 reads = (u32)node_reads(p, row, k0, keys), bad = special(stage);
+      u32 quiet;  // a NaN that the compiler, told not to mind them, does not see
+      asm("v_mov_b32 %0, 0x7fc00000" : "=v"(quiet));
+      const u32 bits = reads >> (4 * h), nan = (reads & bad) >> (4 * h);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float x = sc[i];
-        sc[i] = bits >> (8 * (i / 4) + i % 4) & 1 ? x : -__builtin_inff();
+        const int key = 8 * (i / 4) + i % 4;
+        const float x = __uint_as_float(nan >> key & 1 ? quiet : __float_as_uint(sc[i]));
+        sc[i] = bits >> key & 1 ? x : -__builtin_inff();
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const u32 two = bad >> (4 * h + 16 * (i / 4) + 8 * (i / 2 % 2) + 2 * (i % 2));
+        keep[i / 4][i % 4] = (two & 1 ? 0 : 0xffffu) | (two & 2 ? 0 : 0xffff0000u);
       }
     }
     float top = sc[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) top = __builtin_fmaxf(top, sc[i]);
     top = xhalf(top, [](float x, float y) { return __builtin_fmaxf(x, y); }) * p.scale_log2;
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(top - m > kLazyThreshold) != 0, 0)) {
-      const float m_new = top - m > kLazyThreshold ? top : m;
+    const bool moves = top - m > kLazyThreshold;
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(moves) != 0, 0)) {
+      const float m_new = moves ? top : m;
       const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+      const bool first = m < kNone * 0.5f;
       m = m_new;
       l *= alpha;
-      settle(o);
+      // A row's first tile moves its maximum, but not its sums, which are zeros.
+      if (__builtin_amdgcn_ballot_w64(moves && !first)) {
+        settle(o);
 #pragma unroll
-      for (int d = 0; d < kPv; ++d) {
-        o[d] *= alpha;
-        __builtin_amdgcn_sched_barrier(0);
+        for (int d = 0; d < kPv; ++d) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float x = o[d][i], y;
+            asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %1, %2\n\tv_accvgpr_write_b32 %0, %1"
+                         : "+a"(x), "=&v"(y)
+                         : "v"(alpha));
+            o[d][i] = x;
+          }
+        }
       }
     }
     u32x4 pf[2];
@@ -235,84 +278,89 @@ struct Rows {
     }
     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     ready(pf);
-    if constexpr (TAIL)
-      if (has_special(stage)) {
-        special(k0, stage, pf);
-        return;
-      }
 #pragma unroll
     for (int i = 0; i < 2 * kPv; ++i) {
       // Block d of the sums, 16 of the keys at a time: fragment kQk + i.
+      if constexpr (TAIL) {
+        f[(kQk + i) % kDepth] &= keep[i / kPv];
+        asm volatile("s_nop 1" : "+v"(f[(kQk + i) % kDepth]));
+      }
       product<BF16>(o[i % kPv], f[(kQk + i) % kDepth], pf[i / kPv]);
       __builtin_amdgcn_sched_barrier(0);
       if (i + kDepth < 2 * kPv) f[(kQk + i) % kDepth] = v_at(i + kDepth);
     }
   }
 
-  static constexpr u32 kExp = BF16 ? 0x7f80u : 0x7c00u;
-  // Whether a latent of the tile is infinite or NaN.
-  G9_DEV bool has_special(int stage) const {
+  // The keys of the tile that hold an infinite or NaN latent.  A weight of 0 would not
+  // keep such a value out of a row that does not read its key: where not every row
+  // reads every key, these keys' values are left out of the product, and the rows that do
+  // read one get a score of NaN (the latent is the key too: its product with the
+  // query would be infinite or NaN).
+  G9_DEV u32 special(int stage) const {
     typedef unsigned short h2 __attribute__((ext_vector_type(2)));
+    constexpr u32 kExp = BF16 ? 0x7f80u : 0x7c00u;
     h2 top = {0, 0};
-    // Every piece, the rotated keys' too.
-#pragma unroll 4
-    for (int j = 0; j < kTile / 1024; ++j) {
-      const u32x4 x = *(const G9_LDS u32x4*)(uintptr_t)(lds + stage * kTile + 1024 * j + 16 * lane);
+    const int lane = lane_here(), h = lane >> 5, col = lane & 31;
+    // Half a latent a lane; the order of its pieces so that 16 rows touch every bank once.
+    const u32 at = lds + stage * kTile + col * kRowBytes + 512 * h + 16 * (col >> 1 & 7);
+#pragma unroll 8
+    for (int j = 0; j < 32; ++j) {
+      const u32x4 x = *(const G9_LDS u32x4*)(uintptr_t)((at ^ (16 * (j & 7))) + 128 * (j >> 3));
 #pragma unroll
       for (int e = 0; e < 4; ++e) top = __builtin_elementwise_max(top, __builtin_bit_cast(h2, x[e] & 0x7fff7fffu));
     }
-    return __builtin_expect(__builtin_amdgcn_ballot_w64(top.x >= kExp || top.y >= kExp) != 0, 0);
-  }
-  // Such a tile, where not every row reads every key: a weight of 0 does not keep an
-  // infinite or NaN value out of the product.  It is taken out there, and added on the
-  // vector unit to the rows that read its key; all other sums keep their bits.
-  G9_DEV void special(int k0, int stage, const u32x4 (&pf)[2]) {
-    const u32 vs = lds + stage * kTile + av;
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int d = 0; d < kPv; ++d) {
-        u32x4 v = v_at(vs, k, d);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if ((v[e] & kExp) == kExp) v[e] &= 0xffff0000u;
-          if (((v[e] >> 16) & kExp) == kExp) v[e] &= 0xffffu;
-        }
-        asm volatile("s_nop 1" : "+v"(v));
-        product<BF16>(o[d], v, pf[k]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    settle(o);
-    // P in LDS: row of the query, column of the key.
-    uint16_t* const prow = reinterpret_cast<uint16_t*>(scratch) + col * kKeys;
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) *reinterpret_cast<u32*>(prow + 16 * k + 8 * (e >> 1) + 4 * h + 2 * (e & 1)) = pf[k][e];
-    const u32 reads = (u32)node_reads(p, row, k0, keys);
-    waitcnt<63, 0>();
-#pragma unroll 1
-    for (int key = 0; key < kKeys; ++key) {
-      if (!(reads >> key & 1)) continue;
-      const float w = unpack2<BF16>(prow[key]).x;
-      const u32 vr = lds + stage * kTile + key * kRowBytes + 8 * h;
-      const u32 sw = swz(key);
-#pragma unroll
-      for (int d = 0; d < kPv; ++d)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const u32x2 x = *(const G9_LDS u32x2*)(uintptr_t)(vr + 16 * ((4 * d + r) ^ sw));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            u32 y = (e & 1 ? x[e / 2] >> 16 : x[e / 2]) & 0xffffu;
-            if ((y & kExp) != kExp) y = 0;
-            o[d][4 * r + e] += w * unpack2<BF16>(y).x;
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-    }
+    const unsigned long long who = __builtin_amdgcn_ballot_w64(top.x >= kExp || top.y >= kExp);
+    return (u32)who | (u32)(who >> 32);
   }
 };
+
+// A wave's results, or its sums to slot `slot` of the workspace, where no other wave
+// has summed the same rows.  Branches of lanes are not nested: nothing may come between the
+// ends of two of them.
+template <bool BF16, int RB, class L>
+G9_DEV void finish_rows(const Params& p, const Place& at, int slot, int in_block, const Rows<BF16, RB>& w) {
+  const int h = lane_here() >> 5;
+  const float l = xhalf(w.l, [](float x, float y) { return x + y; });
+  const int node = w.row.node;
+  if (slot >= 0) {
+    const size_t to = (size_t)slot * L::kBlock + in_block;
+    float* const sum = p.part + to * kRank + 4 * h;
+    if (node >= 0) {
+#pragma unroll
+      for (int d = 0; d < kPv; ++d) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          *reinterpret_cast<f32x4*>(sum + 32 * d + 8 * r) =
+              f32x4{w.o[d][4 * r], w.o[d][4 * r + 1], w.o[d][4 * r + 2], w.o[d][4 * r + 3]};
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (node >= 0 && h == 0) {
+      float* const ml = p.part + (size_t)2 * L::kWorkers * L::kBlock * kRank + to * 2;
+      ml[0] = w.m, ml[1] = l;
+    }
+    return;
+  }
+  const int hq = at.block * L::kBlock + in_block - node * p.group;
+  const long long tok = at.r.q0 + node;
+  // By its bits: comparisons here may take NaN for a number.
+  const bool none = (__float_as_uint(l) << 1) == 0;
+  const float inv = none ? 0.f : 1.f / l;
+  char* const orow = p.o + tok * p.o_t + hq * p.o_h + 8 * h;
+  if (node >= 0) {
+#pragma unroll
+    for (int d = 0; d < kPv; ++d) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *reinterpret_cast<u32x2*>(orow + (32 * d + 8 * r) * 2) =
+            u32x2{pack2<BF16>(sum_of(w.o[d], 4 * r) * inv, sum_of(w.o[d], 4 * r + 1) * inv),
+                  pack2<BF16>(sum_of(w.o[d], 4 * r + 2) * inv, sum_of(w.o[d], 4 * r + 3) * inv)};
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  if (node >= 0 && h == 0 && p.lse)
+    p.lse[(long long)hq * p.T + tok] = none ? -__builtin_inff() : (w.m + __builtin_log2f(l)) * kLn2;
+}
 
 // The waves of a block's groups have summed different keys of the same rows: joined in
 // LDS, 256 of the 512 values at a time, and written as `finish` does.
@@ -322,9 +370,10 @@ G9_DEV void finish_groups(const Params& p, const Place& at, int slot, char* smem
   static_assert((4 * kSums + 4 * 64) * 4 <= kLds);
   float* const sums = reinterpret_cast<float*>(smem);
   float* const ml = sums + 4 * kSums;  // maximum and weight of wave w's row r: [w][2][32]
+  const int lane = lane_here(), h = lane >> 5, col = lane & 31;
   const float lw = xhalf(w.l, [](float x, float y) { return x + y; });
   barrier();  // every wave has read its tiles
-  if (w.h == 0) ml[wave * 64 + w.col] = w.m, ml[wave * 64 + 32 + w.col] = lw;
+  if (h == 0) ml[wave * 64 + col] = w.m, ml[wave * 64 + 32 + col] = lw;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     if (half) __syncthreads();
@@ -333,8 +382,9 @@ G9_DEV void finish_groups(const Params& p, const Place& at, int slot, char* smem
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const f32x16& x = w.o[8 * half + d];
-        *reinterpret_cast<f32x4*>(sums + wave * kSums + w.col * kPitch + 32 * d + 8 * r + 4 * w.h) =
-            f32x4{x[4 * r], x[4 * r + 1], x[4 * r + 2], x[4 * r + 3]};
+        *reinterpret_cast<f32x4*>(sums + wave * kSums + col * kPitch + 32 * d + 8 * r + 4 * h) =
+            f32x4{sum_of(x, 4 * r), sum_of(x, 4 * r + 1), sum_of(x, 4 * r + 2), sum_of(x, 4 * r + 3)};
+        __builtin_amdgcn_sched_barrier(0);
       }
     __syncthreads();
     // A wave per row, 4 values a lane.
@@ -342,7 +392,7 @@ G9_DEV void finish_groups(const Params& p, const Place& at, int slot, char* smem
       const int node = row_of<L>(p, at, row).node;
       if (node < 0) break;  // rows behind it neither
       const int rb = row >> 5, in = row & 31;
-      float m = -3.0e38f, f[kGroups], l = 0.f;
+      float m = kNone, f[kGroups], l = 0.f;
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) m = __builtin_fmaxf(m, ml[(g * RB + rb) * 64 + in]);
       f32x4 x = {};
@@ -350,12 +400,12 @@ G9_DEV void finish_groups(const Params& p, const Place& at, int slot, char* smem
       for (int g = 0; g < kGroups; ++g) {
         f[g] = __builtin_amdgcn_exp2f(ml[(g * RB + rb) * 64 + in] - m);
         l += f[g] * ml[(g * RB + rb) * 64 + 32 + in];
-        x += f[g] * *reinterpret_cast<const f32x4*>(sums + (g * RB + rb) * kSums + in * kPitch + 4 * w.lane);
+        x += f[g] * *reinterpret_cast<const f32x4*>(sums + (g * RB + rb) * kSums + in * kPitch + 4 * lane);
       }
-      const int col = 256 * half + 4 * w.lane;
+      const int col = 256 * half + 4 * lane;
       if (slot >= 0) {
         *reinterpret_cast<f32x4*>(p.part + ((size_t)slot * L::kBlock + row) * kRank + col) = x;
-        if (half == 0 && w.lane == 0) {
+        if (half == 0 && lane == 0) {
           float* const to = p.part + (size_t)2 * L::kWorkers * L::kBlock * kRank + ((size_t)slot * L::kBlock + row) * 2;
           to[0] = m, to[1] = l;
         }
@@ -384,7 +434,7 @@ G9_DEV void fwd(const Params& p, char* smem) {
     const int seg = min(left, cur.r.tiles - cur.tile);
     const bool last = cur.tile + seg == cur.r.tiles, from_start = cur.tile == 0;
     const int first = cur.tile * L::kKeys + group * kKeys;  // this wave's first key
-    const int in_block = 32 * (wave % RB) + w.col;
+    const int in_block = 32 * (wave % RB) + (lane_here() & 31);
     w.row = row_of<L>(p, cur, in_block);
     w.keys = cur.r.keys;
     const int* const table = p.table + cur.b * p.table_stride;
@@ -451,7 +501,7 @@ G9_DEV void fwd(const Params& p, char* smem) {
     settle(w.o);
     const int slot = last && from_start ? -1 : (int)(2 * worker + (from_start ? 1 : 0));
     if constexpr (kGroups == 1) {
-      finish<BF16, kRank, L>(p, cur, slot, in_block, w.row.node, w.o, w.m, w.l);
+      finish_rows<BF16, RB, L>(p, cur, slot, in_block, w);
       barrier();  // the stages are read: the next block's tiles take them
     } else {
       finish_groups<BF16, RB, L>(p, cur, slot, smem, wave, w);
