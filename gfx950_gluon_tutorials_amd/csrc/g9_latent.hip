@@ -47,7 +47,7 @@ struct Params {
   const int* lengths;
   const int* cu;
   const unsigned long long* mask;                  // or null: a chain
-  float* part;                                     // sums [2 kWgs][rows][512], then (m, l) pairs
+  float* part;                                     // sums of 2 kWgs blocks (part_at), then (m, l) pairs
   Start* start;                                    // [kWgs]: where each part begins
   long long q_t, q_h, o_t, o_h;                    // token / head strides, bytes
   long long c_b;                                   // block stride, bytes
@@ -108,14 +108,12 @@ G9_DEV int lane_here() {
 
 // RB blocks of 32 rows share a tile; a step of the workgroup is 4 / RB tiles.
 template <int RB>
-using Steps = Line<Params, kKeys * (4 / RB), 32 * RB, kWgs, 0>;
+using Steps = Line<Params, kKeys * (4 / RB), 32 * RB, kWgs, RB == 4 ? 5 : 2>;
 
 // One wave's rows and their sums.
 template <bool BF16, int RB>
 struct Rows {
   static constexpr int kGroups = 4 / RB;       // waves that take tiles in turn
-  static constexpr int kPieces = 2;            // 16-row pieces of a tile: never across a page
-  static constexpr int kDmas = 36 / RB;        // of a wave, for its group's tile
 
   const Params& p;
   u32 lds;             // of the workgroup
@@ -154,35 +152,46 @@ struct Rows {
     av = r4 * kRowBytes + 16 * ((2 * (lane >> 4 & 1) + ((jj & 3) >> 1)) ^ swz(r4)) + 8 * (jj & 1);
   }
 
-  // This wave's share of the tile that begins with key k0, of `all` keys, into stage
-  // `stage`; pg: the pages of the tile's two 16-row pieces.
-  G9_DEV void fill(int stage, int k0, int all, const int (&pg)[kPieces], int wave) const {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      if (RB == 4 && i != wave >> 1) continue;
-      if (RB == 2 && i != (wave & 1)) continue;
-      const int k = k0 + 16 * i, off = k & ((1 << p.shift) - 1);
-      const bool in = (u32)pg[i] < (u32)p.num_blocks;
-      const int rows = in ? min(max(all - k, 0), 16) : 0;
-      const char* const base = p.cache + (long long)(in ? pg[i] : 0) * p.c_b + (unsigned long long)(u32)off * p.c_t;
-      const rsrc_t r = make_rsrc(uniform(base), uniform(extent(rows, p.c_t, kRowBytes)));
-      const u32 to = lds + stage * kTile + i * 16 * kRowBytes;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        if (RB == 4 && half != (wave & 1)) continue;
-#pragma unroll
-        for (int j = 0; j < 9; ++j) {
-          const u32 at = RB == 4 || !half ? voff[j] : voff[j] + 32 - ((flip >> j & 1) << 6);
-          dma16_fresh(r, to + 9216 * half + 1024 * j, at, half * 8 * p.c_t);
-        }
-      }
+  // A 16-row piece of a tile to come: its rows' descriptor, its place in LDS.
+  struct Piece {
+    rsrc_t r;
+    u32 to;
+  };
+  // Piece i of the tile that begins with key k0, of `all` keys (rows behind them read as
+  // zeros), on page pg, into stage `stage`.
+  G9_DEV Piece aim(int i, int stage, int k0, int all, int pg) const {
+    const int k = k0 + 16 * i, off = k & ((1 << p.shift) - 1);
+    const bool in = (u32)pg < (u32)p.num_blocks;
+    const int rows = in ? min(max(all - k, 0), 16) : 0;
+    const char* const base = p.cache + (long long)(in ? pg : 0) * p.c_b + (unsigned long long)(u32)off * p.c_t;
+    return {make_rsrc(uniform(base), uniform(extent(rows, p.c_t, kRowBytes))),
+            (u32)uniform((int)(lds + stage * kTile + i * 16 * kRowBytes))};
+  }
+  // DMA j of a piece's 18.
+  template <int J>
+  G9_DEV void fetch(const Piece& x, int wave) const {
+    if constexpr (RB == 4) {  // a wave has one half of a piece
+      dma16_fresh(x.r, x.to + 9216 * (wave & 1) + 1024 * J, voff[J], (wave & 1) * 8 * p.c_t);
+    } else {
+      const u32 at = J < 9 ? voff[J % 9] : voff[J % 9] + 32 - ((flip >> (J % 9) & 1) << 6);
+      dma16_fresh(x.r, x.to + 1024 * J, at, J < 9 ? 0 : 8 * p.c_t);
+    }
+  }
+  static constexpr int kOwn = RB == 4 ? 9 : 18;  // a wave's DMAs of a piece
+  template <int J = 0>
+  G9_DEV void fetch_all(const Piece& x, int wave) const {
+    if constexpr (J < kOwn) {
+      fetch<J>(x, wave);
+      fetch_all<J + 1>(x, wave);
     }
   }
 
-  G9_DEV void begin(const char* qrow) {
+  G9_DEV void load_q(const char* qrow) {
     const int h = lane_here() >> 5;
 #pragma unroll
     for (int s = 0; s < kQk; ++s) qf[s] = *reinterpret_cast<const u32x4*>(qrow + (16 * s + 8 * h) * 2);
+  }
+  G9_DEV void clear() {
     m = kNone, l = 0.f;
 #pragma unroll
     for (int d = 0; d < kPv; ++d)
@@ -195,8 +204,10 @@ struct Rows {
   }
 
   // Adds the tile in `stage`, whose first key is k0; TAIL: not every row may read all of it.
+  // The DMAs of piece `next` (RB > 1) are issued between the products: all at once, they
+  // would hold the wave until memory has taken them.
   template <bool TAIL>
-  G9_DEV void tile(int k0, int stage) {
+  G9_DEV void tile(int k0, int stage, const Piece& next, int wave) {
     const u32 ks = lds + stage * kTile + ak, vs = lds + stage * kTile + av;
     // Fragments are read kDepth ahead of the product that takes them (the compiler takes
     // assembly for instructions without a latency, and would read each just before).
@@ -208,18 +219,27 @@ struct Rows {
       return u32x4{lo.x, lo.y, hi.x, hi.y};
     };
     u32x4 f[kDepth];
+    // DMA J behind product (2 J + 1) / 2 / kOwn of all.
+    const auto slot = [&]<int S>() {
+      constexpr int kAll = kQk + 2 * kPv, J = (2 * S + 1) * kOwn / (2 * kAll), K = (2 * S + 3) * kOwn / (2 * kAll);
+      if constexpr (RB > 1 && J != K && J < kOwn) fetch<J>(next, wave);
+    };
     f32x16 sc;
 #pragma unroll
     for (int s = 0; s < kDepth; ++s) f[s] = k_at(s);
-#pragma unroll
-    for (int s = 0; s < kQk; ++s) {
-      if (s == 0)
-        first_score<BF16>(sc, f[0], qf[0]);
-      else
-        score<BF16>(sc, f[s % kDepth], qf[s]);
-      __builtin_amdgcn_sched_barrier(0);
-      f[s % kDepth] = s + kDepth < kQk ? k_at(s + kDepth) : v_at(s + kDepth - kQk);
-    }
+    const auto qk_step = [&]<int S>(auto self) {
+      if constexpr (S < kQk) {
+        if constexpr (S == 0)
+          first_score<BF16>(sc, f[0], qf[0]);
+        else
+          score<BF16>(sc, f[S % kDepth], qf[S]);
+        __builtin_amdgcn_sched_barrier(0);
+        f[S % kDepth] = S + kDepth < kQk ? k_at(S + kDepth) : v_at(S + kDepth - kQk);
+        slot.template operator()<S>();
+        self.template operator()<S + 1>(self);
+      }
+    };
+    qk_step.template operator()<0>(qk_step);
     settle(sc);
     u32x4 keep[2];  // TAIL: the keys whose values enter the product
     if constexpr (TAIL) {
@@ -278,17 +298,22 @@ struct Rows {
     }
     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     ready(pf);
-#pragma unroll
-    for (int i = 0; i < 2 * kPv; ++i) {
-      // Block d of the sums, 16 of the keys at a time: fragment kQk + i.
-      if constexpr (TAIL) {
-        f[(kQk + i) % kDepth] &= keep[i / kPv];
-        asm volatile("s_nop 1" : "+v"(f[(kQk + i) % kDepth]));
+    const auto pv_step = [&]<int I>(auto self) {
+      if constexpr (I < 2 * kPv) {
+        // Block d of the sums, 16 of the keys at a time: fragment kQk + I.
+        u32x4& v = f[(kQk + I) % kDepth];
+        if constexpr (TAIL) {
+          v &= keep[I / kPv];
+          asm volatile("s_nop 1" : "+v"(v));
+        }
+        product<BF16>(o[I % kPv], v, pf[I / kPv]);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (I + kDepth < 2 * kPv) v = v_at(I + kDepth);
+        slot.template operator()<kQk + I>();
+        self.template operator()<I + 1>(self);
       }
-      product<BF16>(o[i % kPv], f[(kQk + i) % kDepth], pf[i / kPv]);
-      __builtin_amdgcn_sched_barrier(0);
-      if (i + kDepth < 2 * kPv) f[(kQk + i) % kDepth] = v_at(i + kDepth);
-    }
+    };
+    pv_step.template operator()<0>(pv_step);
   }
 
   // The keys of the tile that hold an infinite or NaN latent.  A weight of 0 would not
@@ -314,115 +339,248 @@ struct Rows {
   }
 };
 
-// A wave's results, or its sums to slot `slot` of the workspace, where no other wave
-// has summed the same rows.  Branches of lanes are not nested: nothing may come between the
-// ends of two of them.
-template <bool BF16, int RB, class L>
-G9_DEV void finish_rows(const Params& p, const Place& at, int slot, int in_block, const Rows<BF16, RB>& w) {
-  const int h = lane_here() >> 5;
-  const float l = xhalf(w.l, [](float x, float y) { return x + y; });
-  const int node = w.row.node;
-  if (slot >= 0) {
-    const size_t to = (size_t)slot * L::kBlock + in_block;
-    float* const sum = p.part + to * kRank + 4 * h;
-    if (node >= 0) {
-#pragma unroll
-      for (int d = 0; d < kPv; ++d) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          *reinterpret_cast<f32x4*>(sum + 32 * d + 8 * r) =
-              f32x4{w.o[d][4 * r], w.o[d][4 * r + 1], w.o[d][4 * r + 2], w.o[d][4 * r + 3]};
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    if (node >= 0 && h == 0) {
-      float* const ml = p.part + (size_t)2 * L::kWorkers * L::kBlock * kRank + to * 2;
-      ml[0] = w.m, ml[1] = l;
-    }
-    return;
-  }
-  const int hq = at.block * L::kBlock + in_block - node * p.group;
-  const long long tok = at.r.q0 + node;
-  // By its bits: comparisons here may take NaN for a number.
-  const bool none = (__float_as_uint(l) << 1) == 0;
-  const float inv = none ? 0.f : 1.f / l;
-  char* const orow = p.o + tok * p.o_t + hq * p.o_h + 8 * h;
-  if (node >= 0) {
-#pragma unroll
-    for (int d = 0; d < kPv; ++d) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        *reinterpret_cast<u32x2*>(orow + (32 * d + 8 * r) * 2) =
-            u32x2{pack2<BF16>(sum_of(w.o[d], 4 * r) * inv, sum_of(w.o[d], 4 * r + 1) * inv),
-                  pack2<BF16>(sum_of(w.o[d], 4 * r + 2) * inv, sum_of(w.o[d], 4 * r + 3) * inv)};
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  }
-  if (node >= 0 && h == 0 && p.lse)
-    p.lse[(long long)hq * p.T + tok] = none ? -__builtin_inff() : (w.m + __builtin_log2f(l)) * kLn2;
+// Sums in the workspace: [slot][32 rows][64 groups of 8 values][lane][4], as the products
+// leave them, a lane being a row and half of the 8 values: whole lines, written and read.
+template <int RB>
+G9_DEV size_t part_at(size_t slot, int rb, int q) {
+  return (((slot * RB + rb) * 64 + q) * 64) * 4;
 }
+template <int RB>
+G9_DEV size_t ml_at(size_t slot, int row) {
+  return (size_t)2 * kWgs * 32 * RB * kRank + (slot * 32 * RB + row) * 2;
+}
+// Where a lane's row goes: row `in` of the block.
+struct Out {
+  char* o;
+  float* lse;
+};
+template <class P>
+G9_DEV Out out_of(const P& p, int q0, int row, int node) {
+  const int hq = row - node * p.group;
+  const long long tok = q0 + node;
+  return {p.o + tok * p.o_t + hq * p.o_h, p.lse ? p.lse + (long long)hq * p.T + tok : nullptr};
+}
+template <bool BF16>
+G9_DEV u32x2 scaled(f32x4 x, float inv) {
+  return u32x2{pack2<BF16>(x[0] * inv, x[1] * inv), pack2<BF16>(x[2] * inv, x[3] * inv)};
+}
+// By its bits: comparisons here may take NaN for a number.
+G9_DEV bool nothing(float l) { return (__float_as_uint(l) << 1) == 0; }
+G9_DEV float lse_of(float m, float l) { return nothing(l) ? -__builtin_inff() : (m + __builtin_log2f(l)) * kLn2; }
 
-// The waves of a block's groups have summed different keys of the same rows: joined in
-// LDS, 256 of the 512 values at a time, and written as `finish` does.
+// A block's results, or its sums to slot `slot` of the workspace.  The groups' sums of the
+// same rows (over different keys) are joined in LDS, 256 of the 512 values at a time; every
+// wave takes a share of the values.  Branches of lanes are not nested: nothing may come
+// between the ends of two of them.
 template <bool BF16, int RB, class L>
-G9_DEV void finish_groups(const Params& p, const Place& at, int slot, char* smem, int wave, const Rows<BF16, RB>& w) {
+G9_DEV void finish_block(const Params& p, const Place& at, int slot, char* smem, int wave, const Rows<BF16, RB>& w) {
   constexpr int kGroups = 4 / RB, kPitch = 256 + 4, kSums = 32 * kPitch;  // 16 bytes more a row: banks
   static_assert((4 * kSums + 4 * 64) * 4 <= kLds);
+  const int lane = lane_here(), h = lane >> 5, col = lane & 31;
   float* const sums = reinterpret_cast<float*>(smem);
   float* const ml = sums + 4 * kSums;  // maximum and weight of wave w's row r: [w][2][32]
-  const int lane = lane_here(), h = lane >> 5, col = lane & 31;
-  const float lw = xhalf(w.l, [](float x, float y) { return x + y; });
-  barrier();  // every wave has read its tiles
-  if (h == 0) ml[wave * 64 + col] = w.m, ml[wave * 64 + 32 + col] = lw;
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    if (half) __syncthreads();
-#pragma unroll
-    for (int d = 0; d < 8; ++d)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const f32x16& x = w.o[8 * half + d];
-        *reinterpret_cast<f32x4*>(sums + wave * kSums + col * kPitch + 32 * d + 8 * r + 4 * h) =
-            f32x4{sum_of(x, 4 * r), sum_of(x, 4 * r + 1), sum_of(x, 4 * r + 2), sum_of(x, 4 * r + 3)};
-        __builtin_amdgcn_sched_barrier(0);
-      }
+  const int rb = wave % RB, row = at.block * L::kBlock + 32 * rb + col, node = w.row.node;
+  float m = w.m, l = xhalf(w.l, [](float x, float y) { return x + y; }), f[kGroups];
+  waitcnt<0, 15>();  // the DMAs behind the last step
+  barrier();         // every wave has read its tiles
+  if constexpr (kGroups > 1) {
+    if (h == 0) ml[wave * 64 + col] = m, ml[wave * 64 + 32 + col] = l;
     __syncthreads();
-    // A wave per row, 4 values a lane.
-    for (int row = wave; row < 32 * RB; row += 4) {
-      const int node = row_of<L>(p, at, row).node;
-      if (node < 0) break;  // rows behind it neither
-      const int rb = row >> 5, in = row & 31;
-      float m = kNone, f[kGroups], l = 0.f;
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) m = __builtin_fmaxf(m, ml[(g * RB + rb) * 64 + in]);
-      f32x4 x = {};
+    for (int g = 0; g < kGroups; ++g) m = __builtin_fmaxf(m, ml[(g * RB + rb) * 64 + col]);
+    l = 0.f;
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        f[g] = __builtin_amdgcn_exp2f(ml[(g * RB + rb) * 64 + in] - m);
-        l += f[g] * ml[(g * RB + rb) * 64 + 32 + in];
-        x += f[g] * *reinterpret_cast<const f32x4*>(sums + (g * RB + rb) * kSums + in * kPitch + 4 * lane);
-      }
-      const int col = 256 * half + 4 * lane;
-      if (slot >= 0) {
-        *reinterpret_cast<f32x4*>(p.part + ((size_t)slot * L::kBlock + row) * kRank + col) = x;
-        if (half == 0 && lane == 0) {
-          float* const to = p.part + (size_t)2 * L::kWorkers * L::kBlock * kRank + ((size_t)slot * L::kBlock + row) * 2;
-          to[0] = m, to[1] = l;
-        }
-      } else {
-        const int hq = at.block * L::kBlock + row - node * p.group;
-        store4<BF16>(p, at.r.q0 + node, hq, col / 4, x, m, l);
-      }
+    for (int g = 0; g < kGroups; ++g) {
+      f[g] = __builtin_amdgcn_exp2f(ml[(g * RB + rb) * 64 + col] - m);
+      l += f[g] * ml[(g * RB + rb) * 64 + 32 + col];
     }
   }
-  __syncthreads();  // the next block's tiles take the sums' place
+  const float inv = nothing(l) ? 0.f : 1.f / l;
+  const Out out = out_of(p, at.r.q0, row, max(node, 0));
+  const auto put = [&](int q, f32x4 x) {
+    if (slot >= 0)
+      *reinterpret_cast<f32x4*>(p.part + part_at<RB>(slot, rb, q) + 4 * lane) = x;
+    else if (node >= 0)
+      *reinterpret_cast<u32x2*>(out.o + 16 * q + 8 * h) = scaled<BF16>(x, inv);
+  };
+  const auto quad = [&](int q) {
+    const f32x16& x = w.o[q / 4];
+    const int r = 4 * (q % 4);
+    return f32x4{sum_of(x, r), sum_of(x, r + 1), sum_of(x, r + 2), sum_of(x, r + 3)};
+  };
+  if constexpr (kGroups == 1) {
+    if (slot >= 0) {
+#pragma unroll
+      for (int q = 0; q < 64; ++q) {
+        put(q, quad(q));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 64; ++q) {
+        put(q, quad(q));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (half) __syncthreads();
+#pragma unroll
+      for (int q = 0; q < 32; ++q) {
+        *reinterpret_cast<f32x4*>(sums + wave * kSums + col * kPitch + 8 * q + 4 * h) = quad(32 * half + q);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      __syncthreads();
+#pragma unroll 4
+      for (int i = 0; i < 32 / kGroups; ++i) {
+        const int q = wave / RB * (32 / kGroups) + i;
+        f32x4 x = {};
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g)
+          x += f[g] * *reinterpret_cast<const f32x4*>(sums + (g * RB + rb) * kSums + col * kPitch + 8 * q + 4 * h);
+        put(32 * half + q, x);
+      }
+    }
+    __syncthreads();  // the next block's tiles take the sums' place
+  }
+  if (wave / RB == 0) {
+    if (slot >= 0) {
+      if (h == 0) *reinterpret_cast<f32x2*>(p.part + ml_at<RB>(slot, 32 * rb + col)) = f32x2{m, l};
+    } else {
+      if (h == 0 && node >= 0 && out.lse) *out.lse = lse_of(m, l);
+    }
+  }
+}
+
+// Joins the blocks that are cut.  A block of n parts has the n - 1 workers whose parts
+// begin within it, and with each of them gridDim.y workgroups here, which share its groups
+// of 32 rows by 8 values: a wave each where the parts are few, else a workgroup, whose
+// waves share the parts.  In the order of the keys: with m the largest of the parts'
+// maxima, the sum of 2^(m_i - m) O_i over the sum of 2^(m_i - m) l_i.
+constexpr int kJoinWaves = 8, kFewParts = 8, kJoinUnits = 4;
+constexpr int kJoinLds = kJoinWaves * 64 * (4 * kJoinUnits + 2);
+template <bool BF16, int RB>
+G9_DEV void join_parts(const Params& p, float* lds) {
+  using L = Steps<RB>;
+  const unsigned w = blockIdx.x + 1;
+  const Start zero = p.start[0];
+  const unsigned long long total = (unsigned long long)zero.total_hi << 32 | zero.total_lo;
+  const Start st = p.start[w];  // asked for together with worker 0's
+  if (w >= L::workers(total) || st.tile == 0) return;
+  const unsigned long long u0 = L::part_begin(w, total) - (unsigned)st.tile;  // the block's first tile
+  const unsigned w0 = L::worker_of(u0, total), n = L::worker_of(u0 + st.tiles - 1, total) - w0 + 1;
+  const int row0 = st.block * L::kBlock;
+  const int rows = (int)min((long long)st.n * p.group - row0, (long long)L::kBlock);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int share = (int)((w - w0 - 1) * gridDim.y + blockIdx.y), shares = (int)((n - 1) * gridDim.y);
+  const int units = (rows + 31) / 32 * 64;
+  // The worker in whose part the block begins has it in slot 1, the others in slot 0.
+  const auto slot_of = [&](unsigned i) { return i ? (size_t)2 * (w0 + i) : (size_t)2 * w0 + 1; };
+  const auto store = [&](int u, f32x4 x, float m, float l) {
+    const int q = u & 63, row = row0 + 32 * (u >> 6) + (lane & 31), node = row / p.group;
+    const Out out = out_of(p, st.q0, row, node);
+    *reinterpret_cast<u32x2*>(out.o + 16 * q + 8 * h) = scaled<BF16>(x, nothing(l) ? 0.f : 1.f / l);
+    if (q == 0 && h == 0 && out.lse) *out.lse = lse_of(m, l);
+  };
+  // The sums of U units from u on over the parts k0, k0 + step, ..: first their largest
+  // maximum, then the sums, 16 loads asked for together.
+  const auto sum_parts = [&]<int U>(int u, unsigned k0, unsigned step, f32x4 (&sum)[U], float& m, float& l) {
+    constexpr unsigned kAtOnce = 16 / U;
+    const int rb = u >> 6, q = u & 63, in = 32 * rb + (lane & 31);
+    const auto ml = [&](unsigned k) {
+      return *reinterpret_cast<const f32x2*>(p.part + ml_at<RB>(slot_of(min(k, n - 1)), in));
+    };
+    m = kNone, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < U; ++i) sum[i] = f32x4{};
+    for (unsigned k = k0; k < n; k += 8 * step) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = ml(k + e * step).x;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (k + e * step < n) m = __builtin_fmaxf(m, x[e]);
+    }
+    for (unsigned k = k0; k < n; k += kAtOnce * step) {
+      f32x4 x[kAtOnce][U];
+      f32x2 v[kAtOnce];
+#pragma unroll
+      for (unsigned e = 0; e < kAtOnce; ++e) {
+        const unsigned i = min(k + e * step, n - 1);
+        v[e] = ml(i);
+        const f32x4* const at = reinterpret_cast<const f32x4*>(p.part + part_at<RB>(slot_of(i), rb, q) + 4 * lane);
+#pragma unroll
+        for (int j = 0; j < U; ++j) x[e][j] = at[64 * j];
+      }
+#pragma unroll
+      for (unsigned e = 0; e < kAtOnce; ++e) {
+        if (k + e * step >= n) break;
+        const float f = __builtin_amdgcn_exp2f(v[e].x - m);
+        l += f * v[e].y;
+#pragma unroll
+        for (int j = 0; j < U; ++j) sum[j] += f * x[e][j];
+      }
+    }
+  };
+  if (n <= kFewParts) {
+    const auto run = [&]<int U>() {
+      for (int u = (share * kJoinWaves + wave) * U; u < units; u += shares * kJoinWaves * U) {
+        f32x4 sum[U];
+        float m, l;
+        sum_parts.template operator()<U>(u, 0, 1, sum, m, l);
+        if (32 * (u >> 6) + (lane & 31) < rows)
+#pragma unroll
+          for (int i = 0; i < U; ++i) store(u + i, sum[i], m, l);
+      }
+    };
+    if (n <= 4)
+      run.template operator()<8>();
+    else
+      run.template operator()<4>();
+    return;
+  }
+  const auto run = [&]<int U>() {
+    constexpr int kWords = 4 * U + 2;
+    for (int u = share * U; u < units; u += shares * U) {
+      f32x4 sum[U];
+      float m, l;
+      sum_parts.template operator()<U>(u, wave, kJoinWaves, sum, m, l);
+      float* const mine = lds + wave * 64 * kWords + lane;  // words 64 apart: a bank a lane
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mine[64 * (4 * i + e)] = sum[i][e];
+      mine[64 * 4 * U] = m, mine[64 * (4 * U + 1)] = l;
+      __syncthreads();
+      if (wave < U && 32 * (u >> 6) + (lane & 31) < rows) {
+        const auto of = [&](int i, int word) { return lds[(i * kWords + word) * 64 + lane]; };
+        float m_all = kNone, l_all = 0.f;
+#pragma unroll
+        for (int i = 0; i < kJoinWaves; ++i) m_all = __builtin_fmaxf(m_all, of(i, 4 * U));
+        f32x4 x = {};
+#pragma unroll
+        for (int i = 0; i < kJoinWaves; ++i) {
+          const float f = __builtin_amdgcn_exp2f(of(i, 4 * U) - m_all);
+          l_all += f * of(i, 4 * U + 1);
+          x += f * f32x4{of(i, 4 * wave), of(i, 4 * wave + 1), of(i, 4 * wave + 2), of(i, 4 * wave + 3)};
+        }
+        store(u + wave, x, m_all, l_all);
+      }
+      __syncthreads();
+    }
+  };
+  if (units <= shares)
+    run.template operator()<1>();
+  else
+    run.template operator()<kJoinUnits>();
 }
 
 template <bool BF16, int RB>
 G9_DEV void fwd(const Params& p, char* smem) {
   using L = Steps<RB>;
   using R = Rows<BF16, RB>;
-  constexpr int kGroups = R::kGroups, kAhead = RB - 1;  // steps asked for ahead: the stages of a group but one
+  constexpr int kAhead = RB - 1;  // steps asked for ahead: the stages of a group but one
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int group = wave / RB;
   const unsigned worker = my_part();
@@ -437,61 +595,63 @@ G9_DEV void fwd(const Params& p, char* smem) {
     const int in_block = 32 * (wave % RB) + (lane_here() & 31);
     w.row = row_of<L>(p, cur, in_block);
     w.keys = cur.r.keys;
+    // The pages of 32 steps' tiles, two 16-row pieces each, are held in the lanes: a load in
+    // every step would be waited for in it, as scalar loads are behind the next LDS read.
     const int* const table = p.table + cur.b * p.table_stride;
-    const auto pages = [&](int step, int (&pg)[2]) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int k = first + step * L::kKeys + 16 * i;
-        pg[i] = k < cur.r.keys ? table[k >> p.shift] : -1;
+    int held;
+    const auto hold = [&](int step) {
+      const int lane = lane_here(), k = first + (step + (lane >> 1)) * L::kKeys + 16 * (lane & 1);
+      held = k < cur.r.keys ? table[k >> p.shift] : -1;
+      waitcnt<0, 15>();
+    };
+    // Piece i of a step's tile of this wave's group.
+    const auto piece = [&](int i, int step) {
+      return w.aim(i, group * RB + step % RB, first + step * L::kKeys, step < seg ? cur.r.keys : 0,
+                   __builtin_amdgcn_readlane(held, 2 * (step & 31) + i));
+    };
+    const int mine = RB == 4 ? wave >> 1 : wave & 1;
+    const auto ask = [&](int step) {
+      if constexpr (RB == 1) {
+        w.fetch_all(piece(0, step), wave);
+        w.fetch_all(piece(1, step), wave);
+      } else {
+        w.fetch_all(piece(mine, step), wave);
       }
     };
-    const auto ask = [&](int step, const int (&pg)[2]) {
-      w.fill(group * RB + step % RB, first + step * L::kKeys, cur.r.keys, pg, wave);
-    };
-    int pg[2];
+    hold(0);
+    ask(0);
+    w.load_q(query_of<L>(p, cur, in_block, w.row.node));
+    waitcnt<0, 0>();  // here: a wait of the compiler's for the queries would be one in every step
 #pragma unroll
-    for (int i = 0; i < (kAhead ? kAhead : 1); ++i)
-      if (i < seg) {
-        pages(i, pg);
-        ask(i, pg);
-      }
-    const int next = kAhead ? kAhead : 1;
-    if (next < seg) pages(next, pg);
-    w.begin(query_of<L>(p, cur, in_block, w.row.node));
-    waitcnt<0, 0>();
+    for (int i = 1; i < kAhead; ++i) ask(i);
+    w.clear();
     // Rows of this wave, tiles that none of them reads.
     const bool some = cur.block * L::kBlock + 32 * (wave % RB) < cur.r.n * p.group;
     const int whole = min(cur.r.context, cur.r.keys);  // keys that every row reads
     const auto steps = [&]<bool TAIL>(int from, int to) {
 #pragma unroll 1
       for (int j = from; j < to; ++j) {
-          if constexpr (RB > 1) {
-            // Step j has landed (steps up to j + kAhead - 1 are asked for), for every wave of the group.
-            if (kAhead > 2 && j + 2 < seg)
-              waitcnt<2 * R::kDmas, 15>();
-            else if (kAhead > 1 && j + 1 < seg)
-              waitcnt<R::kDmas, 15>();
-            else
-              waitcnt<0, 15>();
-            barrier();
-            if (j + kAhead < seg) {
-              ask(j + kAhead, pg);
-              if (j + kAhead + 1 < seg) pages(j + kAhead + 1, pg);
-            }
-          } else {
-            waitcnt<0, 15>();
-            __builtin_amdgcn_sched_barrier(0);
-          }
-          const int k0 = first + j * L::kKeys;
-          if (some) w.template tile<TAIL>(k0, group * RB + j % RB);
-          if constexpr (RB == 1) {
-            waitcnt<63, 0>();
-            __builtin_amdgcn_sched_barrier(0);
-            if (j + 1 < seg) {
-              ask(j + 1, pg);
-              if (j + 2 < seg) pages(j + 2, pg);
-            }
-          }
+        // The step's tile has landed, for every wave that shares it (a wave of RB 1 has its own).
+        waitcnt<(RB == 4 ? 2 * R::kOwn : 0), 15>();
+        typename R::Piece next;
+        if constexpr (RB > 1) {
+          barrier();
+          if (((j + kAhead) & 31) == 0) hold(j + kAhead);
+          next = piece(mine, j + kAhead);
+        } else {
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        const int k0 = first + j * L::kKeys;
+        if (some)
+          w.template tile<TAIL>(k0, group * RB + j % RB, next, wave);
+        else if constexpr (RB > 1)
+          w.fetch_all(next, wave);
+        if constexpr (RB == 1) {
+          waitcnt<63, 0>();
+          __builtin_amdgcn_sched_barrier(0);
+          if (((j + 1) & 31) == 0) hold(j + 1);
+          if (j + 1 < seg) ask(j + 1);
+        }
       }
     };
     // The steps whose tiles every row reads whole, then the others.
@@ -500,12 +660,7 @@ G9_DEV void fwd(const Params& p, char* smem) {
     steps.template operator()<true>(mid, seg);
     settle(w.o);
     const int slot = last && from_start ? -1 : (int)(2 * worker + (from_start ? 1 : 0));
-    if constexpr (kGroups == 1) {
-      finish_rows<BF16, RB, L>(p, cur, slot, in_block, w);
-      barrier();  // the stages are read: the next block's tiles take them
-    } else {
-      finish_groups<BF16, RB, L>(p, cur, slot, smem, wave, w);
-    }
+    finish_block<BF16, RB, L>(p, cur, slot, smem, wave, w);
     left -= seg + L::kLead;
     if (left > 0) cur = L::next_block(p, cur);
   }
@@ -523,9 +678,9 @@ using namespace g9::host;
     __shared__ __attribute__((aligned(1024))) char smem[latent::kLds];                                            \
     latent::fwd<BF16, RB>(p, smem);                                                                               \
   }                                                                                                               \
-  extern "C" __global__ __launch_bounds__(fa::kJoinThreads<512>) void g9_latent_join_##NAME(latent::Params p) {   \
-    __shared__ float lds[fa::kJoinThreads<512> * 7];                                                              \
-    fa::join<BF16, 512, latent::Steps<RB>>(p, lds);                                                               \
+  extern "C" __global__ __launch_bounds__(64 * latent::kJoinWaves) void g9_latent_join_##NAME(latent::Params p) { \
+    __shared__ float lds[latent::kJoinLds];                                                            \
+    latent::join_parts<BF16, RB>(p, lds);                                                                         \
   }
 G9_LATENT_KERNEL(bf16_q32, true, 1)
 G9_LATENT_KERNEL(f16_q32, false, 1)
@@ -609,6 +764,6 @@ extern "C" int g9_latent_fwd(const void* q, const void* cache, void* o, float* l
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int bf16 = dtype == G9_BF16;
   if (hipLaunchKernel(kRun[form][bf16], dim3(fa::kWgs), dim3(256), args, 0, st) != hipSuccess) return G9_ERR_HIP;
-  return launched(hipLaunchKernel(kJoin[form][bf16], dim3(fa::kWgs - 1, form == Q128 ? 4 : 1),
-                                  dim3(fa::kJoinThreads<512>), args, 0, st));
+  return launched(hipLaunchKernel(kJoin[form][bf16], dim3(fa::kWgs - 1, 2),
+                                  dim3(64 * latent::kJoinWaves), args, 0, st));
 }
