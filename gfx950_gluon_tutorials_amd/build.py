@@ -43,7 +43,7 @@ NO_SPILLS = {"g9_latent.hip"}
 for _s in NO_SPILLS:
     SOURCE_FLAGS[_s] = SOURCE_FLAGS[_s] + ["-mllvm", "-amdgpu-remove-redundant-endcf=0"]
 HEADERS = ["g9_common.hpp", "g9_gemm.hpp", "g9_tile.hpp", "g9_tile_pick.hpp",
-           "g9_fmha_pipe.hpp", "g9_wave.hpp", "g9_line.hpp", "g9_attn_host.hpp"]
+           "g9_fmha_pipe.hpp", "g9_wave.hpp", "g9_line.hpp", "g9_packed.hpp", "g9_attn_host.hpp"]
 
 # -packed-fp32-ops: keep the compiler from forming v_pk_*_f32, whose results
 # have been unreliable on the target machines.

@@ -152,6 +152,13 @@ G9_DEV u32x2 tr_read(u32 addr) {
 #define G9_FMHA_VEC1_EXPS 22  // exponentials of a tile done in D2 (of 32 per lane); the rest in D1
 #endif
 
+#ifndef G9_FMHA_VN1_SHARED
+#define G9_FMHA_VN1_SHARED 3  // VALU instructions after each of D1's 24 QK MFMAs with shared keys
+#endif
+#ifndef G9_FMHA_RD1
+#define G9_FMHA_RD1 4  // the MFMA of D1 beside which the shared keys' reads begin
+#endif
+
 #ifndef G9_FMHA_VN1_64
 #define G9_FMHA_VN1_64 8  // head dim 64 (128-key tiles): VALU after each QK MFMA of D1
 #endif
@@ -208,9 +215,21 @@ struct Where<Params, kPaged> {
   int t0, held, pgk, pgv;
   typename Params::Row row;
 };
-template <class Params, bool BF16, bool LAZY, bool SOQ, int HD, Kind KIND = kEqual>
-struct Pipe : Where<Params, KIND> {
+// ROPE: 64 more values of every key, which all heads share: rows of their own,
+// behind the key's chunk columns in LDS.  Their fragments are not held: a dot
+// cluster D1 reads them beside its first MFMAs, so their buffer is free one cluster
+// later than the other columns', and their DMA goes out in M2.
+template <int ROPE>
+struct SharedKeys {};
+template <>
+struct SharedKeys<64> {
+  const char* rp;  // the sequence's first row
+  u32 voffr;       // lane's row offset
+};
+template <class Params, bool BF16, bool LAZY, bool SOQ, int HD, Kind KIND = kEqual, int ROPE = 0>
+struct Pipe : Where<Params, KIND>, SharedKeys<ROPE> {
   static_assert(HD == 64 || HD == 128, "head dim 64 or 128");
+  static_assert(ROPE == 0 || (HD == 128 && KIND == kPacked), "shared keys of packed sequences");
   static constexpr int kBN = 8192 / HD;        // keys per tile
   static constexpr int kNB = kBN / 32;         // 32-key score blocks per tile
   static constexpr int kKS = kBN / 16;         // PV steps of 16 keys
@@ -224,7 +243,8 @@ struct Pipe : Where<Params, KIND> {
   // Bytes between V chunk columns (pad: distinct banks).
   static constexpr int kPitchV = kBN * 16 + (KIND == kPaged ? 0 : 64);
   static constexpr int kGroupV = kNC * 128, kGroupK = kGroupV + 128;  // kPaged: 8 rows
-  static constexpr int kTileK = KIND == kPaged ? kBN / 8 * kGroupK : kNC * kPitchK;  // one K tile in LDS
+  static constexpr int kNR = ROPE / 16, kRC = ROPE / 8;  // QK steps and chunk columns of the shared keys
+  static constexpr int kTileK = KIND == kPaged ? kBN / 8 * kGroupK : (kNC + kRC) * kPitchK;  // one K tile in LDS
   static constexpr int kTileV = kNC * kPitchV;  // one V tile in LDS
   static constexpr int kBufs = KIND == kPaged ? 4 : 2;  // tiles of K and of V in LDS
   static constexpr int kLdsV = kBufs * kTileK;  // V buffers after the K buffers
@@ -243,7 +263,7 @@ struct Pipe : Where<Params, KIND> {
   u32 voffk, voffv;  // lane's row offset in global K / V
   u32 ak, av;        // lane's LDS read base for K / V
   float sc;
-  u32x4 qf[kNS];
+  u32x4 qf[kNS + kNR];
   u32x4 kv[kNF];  // K_t (kv[kNB s + blk]: step s of 16 head-dim values, key block blk) or V_t (kv[kND t + d])
   f32x16 o[kND];  // O^T, head-dim block d
   float m, l, alpha;
@@ -259,13 +279,13 @@ struct Pipe : Where<Params, KIND> {
   // .. +63 of a tile: lane i fetches row 64 (q % kRH) + i.
   // kPacked: the rows of a tile that the sequence has.  Rows behind them read as
   // zeros, or as values of the last row where rows overlap: masked either way.
-  G9_DEV rsrc_t tile_rows(const char* base, int tile, u32 ld) const {
+  G9_DEV rsrc_t tile_rows(const char* base, int tile, u32 ld, u32 row = HD * 2) const {
     const int left = min(max(keys - tile * kBN, 0), kBN);
     const unsigned long long at = (unsigned long long)base + (unsigned long long)(u32)(tile * kBN) * ld;
     // Uniform, but the 64-bit product may be formed on the vector unit.
     const u32 lo = (u32)__builtin_amdgcn_readfirstlane((int)at), hi = (u32)__builtin_amdgcn_readfirstlane((int)(at >> 32));
     return make_rsrc(reinterpret_cast<const void*>((unsigned long long)hi << 32 | lo),
-                     (u32)__builtin_amdgcn_readfirstlane((int)extent(left, ld, HD * 2)));
+                     (u32)__builtin_amdgcn_readfirstlane((int)extent(left, ld, row)));
   }
   G9_DEV int first_tile() const {
     if constexpr (KIND == kPaged) return this->t0;
@@ -338,6 +358,14 @@ struct Pipe : Where<Params, KIND> {
       }
     }
   }
+  // The shared keys' chunk column that this wave fetches.
+  G9_DEV void dma_r(int tile, int buf) {
+    if constexpr (ROPE != 0) {
+      static_assert(kRC == kWaves && kRH == 1);
+      dma16_fresh(tile_rows(this->rp, tile, p.ldr, ROPE * 2), lds0 + buf * kTileK + (kNC + wave) * kPitchK, this->voffr,
+                  wave * 16);
+    }
+  }
   G9_DEV void dma_v(int tile, int buf) {
     if constexpr (KIND == kPaged) {
       dma_paged(vp, tile, this->pgv, lds0 + kLdsV + buf * kTileV + kMine / 8 * wave * kGroupV, 1024, voff_v(), p.v_b, p.v_t);
@@ -383,7 +411,8 @@ struct Pipe : Where<Params, KIND> {
         kv[kND * t + d] = u32x4{lo.x, lo.y, hi.x, hi.y};
       }
   }
-  // S^T of the tile in kv: kNB 32-key blocks.
+  // S^T of the tile in kv: kNB 32-key blocks; BUF: where its shared keys are.
+  template <int BUF = 0>
   G9_DEV void qk(Sc& S) {
 #pragma unroll
     for (int blk = 0; blk < kNB; ++blk) S.b[blk] = mfma<BF16>(kv[blk], qf[0], f32x16{});
@@ -391,6 +420,13 @@ struct Pipe : Where<Params, KIND> {
     for (int s = 1; s < kNS; ++s)
 #pragma unroll
       for (int blk = 0; blk < kNB; ++blk) S.b[blk] = mfma<BF16>(kv[kNB * s + blk], qf[s], S.b[blk]);
+#pragma unroll
+    for (int s = kNS; s < kNS + kNR; ++s)
+#pragma unroll
+      for (int blk = 0; blk < kNB; ++blk) {
+        const u32x4 kr = *(const G9_LDS u32x4*)(uintptr_t)(ak + BUF * kTileK + 2 * s * kPitchK + blk * 512);
+        S.b[blk] = mfma<BF16>(kr, qf[s], S.b[blk]);
+      }
   }
   // O^T += V^T P^T; P in 16 bit as vec2 left it in S.
   G9_DEV void pv(const Sc& S) {
@@ -668,6 +704,19 @@ struct Pipe : Where<Params, KIND> {
     }
   }
 
+  // D1 with the shared keys: 24 MFMAs; eight LDS reads go beside the 5th to the 12th, whose
+  // registers they take.
+  template <int VN, int I = 0>
+  G9_DEV static void interleave_shared() {
+    if constexpr (I < kNF + kNR * kNB) {
+      __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 0);
+      if constexpr (I >= G9_FMHA_RD1 && I < G9_FMHA_RD1 + kNR * kNB) __builtin_amdgcn_sched_group_barrier(SG_DS_RD, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(SG_VALU, VN, 0);
+      if constexpr (I < 16 && kEp1[I % 16] > 0) __builtin_amdgcn_sched_group_barrier(SG_TRANS, kEp1[I % 16], 0);
+      interleave_shared<VN, I + 1>();
+    }
+  }
+
   // Not kEqual: V_{j+1} landed, for a wave that has no more use for it.
   G9_DEV void wait_v(int j) const {
     if (j + 1 >= nte) return;
@@ -703,6 +752,8 @@ struct Pipe : Where<Params, KIND> {
     if constexpr (KIND == kPaged) {
       ask_v(j);
     } else {
+      if constexpr (ROPE != 0)
+        if (j + 3 < nte) dma_r(j + 3, (j & 1) ^ 1);
       if (j + 2 < nte) dma_v(j + 2, j & 1);
     }
     barrier();
@@ -720,10 +771,16 @@ struct Pipe : Where<Params, KIND> {
     // D1(j)
     __builtin_amdgcn_s_setprio(0);
     if constexpr (NEXT) {
-      qk(n);
+      if constexpr (ROPE != 0)
+        qk<PAR ^ 1>(n);
+      else
+        qk(n);
       vec2(c);
       rescale_early();
-      interleave<(kSplit ? G9_FMHA_VN1_EAGER : kVN1), 1>();
+      if constexpr (ROPE != 0)
+        interleave_shared<G9_FMHA_VN1_SHARED>();
+      else
+        interleave<(kSplit ? G9_FMHA_VN1_EAGER : kVN1), 1>();
       pin_sc(n);
     } else {
       vec2(c);
@@ -801,6 +858,8 @@ struct Pipe : Where<Params, KIND> {
     if constexpr (KIND == kPaged) {
       ask_v(j);
     } else {
+      if constexpr (ROPE != 0)
+        if (j + 3 < nte) dma_r(j + 3, PAR ^ 1);
       if (j + 2 < nte) dma_v(j + 2, PAR);
     }
     waitcnt<63, 0>();

@@ -1,71 +1,21 @@
 // Attention over packed sequences whose keys and values were expanded from
 // latents (g9_latent_varlen_fwd, include/gfx950_fmha.h): a head's key is 128 values
 // of its own and 64 rotated ones that all heads share, its value 128.
+//
+// g9_varlen.hip's kernel with 192 values of QK: the pipeline reads the shared keys as
+// chunk columns of their own behind the head's, so that nothing is copied together.
+// Bound by the matrix unit (640 flops a query and key of a head).
 #include "../../include/gfx950_fmha.h"
 #include "g9_attn_host.hpp"
-#include "g9_wave.hpp"
+#include "g9_packed.hpp"
 
 namespace g9 {
 namespace fa {
 
-struct LatentVarParams {
-  const char* q;
-  const char* k;
-  const char* v;
-  const char* r;                               // the shared keys
-  char* o;
-  float* lse;                                  // [HQ][T] fp32, or null
-  const int* cu_q;
-  const int* cu_k;
-  long long q_h, k_h, v_h, o_h;                // head strides, bytes
-  u32 ldq, ldk, ldv, ldr, ldo;                 // token strides, bytes
-  int B, T, TK, HQ, HK, causal;
-  float scale_log2;
+struct LatentVarParams : VarParams {
+  const char* r;  // the shared keys, ldr bytes a token
+  u32 ldr;
 };
-
-// A wave per query and head, a key at a time: lane i has the values 2 i and 2 i + 1
-// of a head's own key and value, and 128 + i of the shared one.
-template <bool BF16>
-G9_DEV void latent_varlen_plain(const LatentVarParams& p) {
-  const int lane = threadIdx.x & 63;
-  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int t = (int)(w / p.HQ), h = (int)(w - (long long)t * p.HQ), hk = h / (p.HQ / p.HK);
-  if (t >= p.T) return;
-  int b = -1, q0 = 0, lq = 0;
-  for (int i = 0; i < p.B; ++i) {
-    q0 = min(max(p.cu_q[i], 0), p.T);
-    lq = min(max(p.cu_q[i + 1], q0), p.T) - q0;
-    if (t >= q0 && t < q0 + lq) {
-      b = i;
-      break;
-    }
-  }
-  if (b < 0) return;
-  const int k0 = min(max(p.cu_k[b], 0), p.TK), lk = min(max(p.cu_k[b + 1], k0), p.TK) - k0;
-  const int end = p.causal ? min(t - q0 + 1 + lk - lq, lk) : lk;
-  const auto two = [&](const char* at) { return unpack2<BF16>(*reinterpret_cast<const u32*>(at + lane * 4)); };
-  const auto one = [&](const char* at) { return unpack2<BF16>(*reinterpret_cast<const uint16_t*>(at + lane * 2)).x; };
-  const char* const q = p.q + (long long)t * p.ldq + h * p.q_h;
-  const f32x2 qn = two(q);
-  const float qr = one(q + 256);
-  f32x2 o = {0.f, 0.f};
-  float m = -3.0e38f, l = 0.f;
-  for (int j = k0; j < k0 + end; ++j) {
-    const f32x2 kn = two(p.k + (long long)j * p.ldk + hk * p.k_h), x = two(p.v + (long long)j * p.ldv + hk * p.v_h);
-    float s = qn.x * kn.x + qn.y * kn.y + qr * one(p.r + (long long)j * p.ldr);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d, 64);
-    s *= p.scale_log2;
-    const float m_new = __builtin_fmaxf(m, s), f = __builtin_amdgcn_exp2f(m - m_new), g = __builtin_amdgcn_exp2f(s - m_new);
-    l = l * f + g;
-    o.x = o.x * f + g * x.x, o.y = o.y * f + g * x.y;
-    m = m_new;
-  }
-  const bool none = l == 0.f;
-  const float inv = none ? 0.f : 1.f / l;
-  *reinterpret_cast<u32*>(p.o + (long long)t * p.ldo + h * p.o_h + lane * 4) = pack2<BF16>(o.x * inv, o.y * inv);
-  if (p.lse && lane == 0) p.lse[(long long)h * p.T + t] = none ? -__builtin_inff() : (m + __builtin_log2f(l)) * kLn2;
-}
 
 }  // namespace fa
 }  // namespace g9
@@ -73,12 +23,14 @@ G9_DEV void latent_varlen_plain(const LatentVarParams& p) {
 using namespace g9;
 using namespace g9::host;
 
-extern "C" __global__ __launch_bounds__(256) void g9_latent_varlen_bf16(fa::LatentVarParams p) {
-  fa::latent_varlen_plain<true>(p);
-}
-extern "C" __global__ __launch_bounds__(256) void g9_latent_varlen_f16(fa::LatentVarParams p) {
-  fa::latent_varlen_plain<false>(p);
-}
+#define G9_LATENT_VARLEN_KERNEL(NAME, BF16)                                                                   \
+  extern "C" __global__ __launch_bounds__(fa::kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void      \
+  NAME(fa::LatentVarParams p) {                                                                              \
+    __shared__ __attribute__((aligned(1024))) char smem[fa::VarPipe<fa::LatentVarParams, BF16, 128, 64>::kLds]; \
+    fa::varlen_fwd<BF16, 128, 64>(p, smem);                                                                  \
+  }
+G9_LATENT_VARLEN_KERNEL(g9_latent_varlen_bf16, true)
+G9_LATENT_VARLEN_KERNEL(g9_latent_varlen_f16, false)
 
 extern "C" int g9_latent_varlen_fwd(const void* q, const void* k, const void* v, const void* k_rope, void* o, float* lse,
                                     const int32_t* cu_q, const int32_t* cu_k, int64_t B, int64_t T, int64_t TK,
@@ -121,11 +73,12 @@ extern "C" int g9_latent_varlen_fwd(const void* q, const void* k, const void* v,
   p.B = (int)B, p.T = (int)T, p.TK = (int)TK, p.HQ = (int)HQ, p.HK = (int)HK;
   p.causal = causal != 0;
   p.scale_log2 = sm_scale * fa::kLog2e;
-  const int64_t waves = T * HQ;
-  if ((waves + 3) / 4 * 256 > UINT32_MAX) return G9_ERR_SHAPE;  // the threads of a launch
+  // At most T / 256 whole tiles and a partial one per sequence.
+  const int64_t group = HQ / HK, tiles = T / fa::kBlockM + (B < T ? B : T);
+  const int64_t grid = 8 * group * ((tiles * HK + 7) / 8);
+  if (grid * fa::kThreads > UINT32_MAX) return G9_ERR_SHAPE;  // the threads of a launch
   void* args[] = {&p};
   return launched(hipLaunchKernel(dtype == G9_BF16 ? reinterpret_cast<const void*>(g9_latent_varlen_bf16)
                                                    : reinterpret_cast<const void*>(g9_latent_varlen_f16),
-                                  dim3((unsigned)((waves + 3) / 4)), dim3(256), args, 0,
-                                  reinterpret_cast<hipStream_t>(stream)));
+                                  dim3((unsigned)grid), dim3(fa::kThreads), args, 0, reinterpret_cast<hipStream_t>(stream)));
 }
