@@ -37,11 +37,12 @@ SOURCE_FLAGS = {s: ["-fno-honor-nans"] for s in ("g9_fmha.hip", "g9_varlen.hip",
                                                "g9_latent_varlen.hip")}
 # Sources whose kernels hold almost every register through branches of lanes.  Where two
 # such branches end at once the compiler turns the lanes on again at the outer end only, and
-# has reloaded spilled registers between the two, in some of the lanes: each
-# branch turns its lanes on again, and nothing may spill.
-NO_SPILLS = {"g9_latent.hip"}
-for _s in NO_SPILLS:
+# has reloaded spilled registers between the two, in some of the lanes: here each
+# branch turns its lanes on again.  The kernels of NO_SPILLS must not spill at all (the build
+# fails if they do).
+for _s in ("g9_latent.hip", "g9_latent_varlen.hip"):
     SOURCE_FLAGS[_s] = SOURCE_FLAGS[_s] + ["-mllvm", "-amdgpu-remove-redundant-endcf=0"]
+NO_SPILLS = {"g9_latent.hip"}
 HEADERS = ["g9_common.hpp", "g9_gemm.hpp", "g9_tile.hpp", "g9_tile_pick.hpp",
            "g9_fmha_pipe.hpp", "g9_wave.hpp", "g9_line.hpp", "g9_packed.hpp", "g9_attn_host.hpp"]
 

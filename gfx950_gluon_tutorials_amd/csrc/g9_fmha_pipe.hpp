@@ -155,8 +155,11 @@ G9_DEV u32x2 tr_read(u32 addr) {
 #ifndef G9_FMHA_VN1_SHARED
 #define G9_FMHA_VN1_SHARED 3  // VALU instructions after each of D1's 24 QK MFMAs with shared keys
 #endif
+#ifndef G9_FMHA_VEC1_EXPS_SHARED
+#define G9_FMHA_VEC1_EXPS_SHARED 20  // with shared keys: exponentials of a tile (of 32 per lane) done in D2
+#endif
 #ifndef G9_FMHA_RD1
-#define G9_FMHA_RD1 4  // the MFMA of D1 beside which the shared keys' reads begin
+#define G9_FMHA_RD1 8  // the MFMA of D1 beside which the shared keys' reads begin
 #endif
 
 #ifndef G9_FMHA_VN1_64
@@ -249,7 +252,7 @@ struct Pipe : Where<Params, KIND>, SharedKeys<ROPE> {
   static constexpr int kBufs = KIND == kPaged ? 4 : 2;  // tiles of K and of V in LDS
   static constexpr int kLdsV = kBufs * kTileK;  // V buffers after the K buffers
   static constexpr int kLdsBytes = kBufs * (kTileK + kTileV);
-  static constexpr int kE1 = HD == 128 ? G9_FMHA_VEC1_EXPS : G9_FMHA_VEC1_EXPS_64;
+  static constexpr int kE1 = ROPE ? G9_FMHA_VEC1_EXPS_SHARED : HD == 128 ? G9_FMHA_VEC1_EXPS : G9_FMHA_VEC1_EXPS_64;
   static constexpr int kVN1 = HD == 128 ? G9_FMHA_VN1 : G9_FMHA_VN1_64;
   static constexpr int kVN2 = HD == 128 ? G9_FMHA_VN2 : G9_FMHA_VN2_64;
   static_assert(kNF == 16 && kKS * kND == 16, "16 MFMAs per dot cluster");
@@ -681,16 +684,22 @@ struct Pipe : Where<Params, KIND>, SharedKeys<ROPE> {
   static constexpr int kEp2[16] = {1, 1, 2, 2, 2, 2, 2, 2, 2, 2, 2, 2};
   static constexpr int kEp1_64[16] = {1, 1, 1, 1, 2, 2, 2, 2, 2, 2, 2, 2};
   static constexpr int kEp2_64[16] = {2, 3, 3, 3, 3, 3, 3, 3, 3, 3, 3, 3, 3, 3, 3};
+  // With shared keys: `all` exponentials over the first `slots` slots.
+  static constexpr int shared_exps(int i, int all, int slots) {
+    return i < slots ? (i + 1) * all / slots - i * all / slots : 0;
+  }
   template <int W, int I>
   G9_DEV static constexpr int exps_in_slot() {
-    if constexpr (HD == 128)
+    if constexpr (ROPE != 0)
+      return W == 1 ? shared_exps(I, 32 - kE1, kNF) : shared_exps(I, kE1, kNF - 2);
+    else if constexpr (HD == 128)
       return W == 1 ? (LAZY ? kEp1[I] : kEp1e[I]) : kEp2[I];
     else
       return W == 1 ? kEp1_64[I] : kEp2_64[I];
   }
-  static_assert(HD != 128 || sum16(kEp1) == 32 - kE1, "D1 exponentials per slot: re-chosen with the D1/D2 split");
-  static_assert(HD != 128 || sum16(kEp1e) == 32 - kE1, "D1 exponentials per slot: re-chosen with the D1/D2 split");
-  static_assert(HD != 128 || sum16(kEp2) == kE1, "D2 exponentials per slot: re-chosen with the D1/D2 split");
+  static_assert(HD != 128 || ROPE || sum16(kEp1) == 32 - kE1, "D1 exponentials per slot: re-chosen with the D1/D2 split");
+  static_assert(HD != 128 || ROPE || sum16(kEp1e) == 32 - kE1, "D1 exponentials per slot: re-chosen with the D1/D2 split");
+  static_assert(HD != 128 || ROPE || sum16(kEp2) == kE1, "D2 exponentials per slot: re-chosen with the D1/D2 split");
   static_assert(HD == 128 || sum16(kEp1_64) == 64 - kE1, "D1 exponentials per slot: re-chosen with the D1/D2 split");
   static_assert(HD == 128 || sum16(kEp2_64) == kE1, "D2 exponentials per slot: re-chosen with the D1/D2 split");
   template <int VN, int W, int I = 0>
@@ -712,7 +721,8 @@ struct Pipe : Where<Params, KIND>, SharedKeys<ROPE> {
       __builtin_amdgcn_sched_group_barrier(SG_MFMA, 1, 0);
       if constexpr (I >= G9_FMHA_RD1 && I < G9_FMHA_RD1 + kNR * kNB) __builtin_amdgcn_sched_group_barrier(SG_DS_RD, 1, 0);
       __builtin_amdgcn_sched_group_barrier(SG_VALU, VN, 0);
-      if constexpr (I < 16 && kEp1[I % 16] > 0) __builtin_amdgcn_sched_group_barrier(SG_TRANS, kEp1[I % 16], 0);
+      constexpr int e = exps_in_slot<1, I>();
+      if constexpr (e > 0) __builtin_amdgcn_sched_group_barrier(SG_TRANS, e, 0);
       interleave_shared<VN, I + 1>();
     }
   }

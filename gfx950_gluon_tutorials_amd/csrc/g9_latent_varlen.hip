@@ -29,8 +29,26 @@ using namespace g9::host;
     __shared__ __attribute__((aligned(1024))) char smem[fa::VarPipe<fa::LatentVarParams, BF16, 128, 64>::kLds]; \
     fa::varlen_fwd<BF16, 128, 64>(p, smem);                                                                  \
   }
+#define G9_LATENT_SHORT_KERNEL(NAME, BF16)                                                                    \
+  extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void               \
+  NAME(fa::LatentVarParams p) {                                                                              \
+    __shared__ __attribute__((aligned(1024))) char smem[fa::ShortWave<fa::LatentVarParams, BF16, 128, 64>::kLds]; \
+    fa::varlen_short<BF16, 128, 64>(p, smem);                                                                \
+  }
+G9_LATENT_SHORT_KERNEL(g9_latent_varlen_short_bf16, true)
+G9_LATENT_SHORT_KERNEL(g9_latent_varlen_short_f16, false)
 G9_LATENT_VARLEN_KERNEL(g9_latent_varlen_bf16, true)
 G9_LATENT_VARLEN_KERNEL(g9_latent_varlen_f16, false)
+
+// The short form runs up to this many rows (queries by query heads), and where the sequences
+// have fewer than kShortQueries queries on average: a pipeline's workgroup of 256 rows is
+// mostly empty there.  Measured (us, short form against the pipeline), one MI355X: 197
+// queries by 16 heads 11.4 and 17.7, 1024 19.8 and 37.6, 2048 47 and 63, 8 x 200 16.8 and
+// 18.8, 256 x 1 51 and 154, 512 by 64 heads 23.4 and 26.5, 16 behind 4096 keys 53 and 82; 1350
+// by 32 47.7 and 44.8, 2048 by 24 65 and 64, 1024 by 64 53 and 41, 4096 by 16 146 and 118.
+// Beyond that many rows: 64 x 30 by 32 27 and 82, 500 x 20 behind 500 keys 919 and 1574, 256 x
+// 64 by 16 144 and 203, but 128 x 64 behind 1000 403 and 338, 32 x 200 62 and 43.
+static constexpr int64_t kShortRows = 40 * 1024, kShortQueries = 48;
 
 extern "C" int g9_latent_varlen_fwd(const void* q, const void* k, const void* v, const void* k_rope, void* o, float* lse,
                                     const int32_t* cu_q, const int32_t* cu_k, int64_t B, int64_t T, int64_t TK,
@@ -73,12 +91,22 @@ extern "C" int g9_latent_varlen_fwd(const void* q, const void* k, const void* v,
   p.B = (int)B, p.T = (int)T, p.TK = (int)TK, p.HQ = (int)HQ, p.HK = (int)HK;
   p.causal = causal != 0;
   p.scale_log2 = sm_scale * fa::kLog2e;
+  void* args[] = {&p};
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const int64_t group = HQ / HK;
+  const bool few = T * HQ <= kShortRows || T < kShortQueries * B;
+  if (few) {
+    const int64_t blocks = T * group / 32 + (B < T ? B : T);
+    if (blocks * HK * 256 > UINT32_MAX) return G9_ERR_SHAPE;  // the threads of a launch
+    return launched(hipLaunchKernel(dtype == G9_BF16 ? reinterpret_cast<const void*>(g9_latent_varlen_short_bf16)
+                                                     : reinterpret_cast<const void*>(g9_latent_varlen_short_f16),
+                                    dim3((unsigned)(blocks * HK)), dim3(256), args, 0, st));
+  }
   // At most T / 256 whole tiles and a partial one per sequence.
-  const int64_t group = HQ / HK, tiles = T / fa::kBlockM + (B < T ? B : T);
+  const int64_t tiles = T / fa::kBlockM + (B < T ? B : T);
   const int64_t grid = 8 * group * ((tiles * HK + 7) / 8);
   if (grid * fa::kThreads > UINT32_MAX) return G9_ERR_SHAPE;  // the threads of a launch
-  void* args[] = {&p};
   return launched(hipLaunchKernel(dtype == G9_BF16 ? reinterpret_cast<const void*>(g9_latent_varlen_bf16)
                                                    : reinterpret_cast<const void*>(g9_latent_varlen_f16),
-                                  dim3((unsigned)grid), dim3(fa::kThreads), args, 0, reinterpret_cast<hipStream_t>(stream)));
+                                  dim3((unsigned)grid), dim3(fa::kThreads), args, 0, st));
 }

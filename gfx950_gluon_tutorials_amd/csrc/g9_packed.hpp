@@ -292,5 +292,104 @@ G9_DEV void varlen_fwd(const Params& p, char* smem) {
   }
 }
 
+// Few queries: a workgroup per 32 rows (queries by the query heads of a K/V head),
+// its 4 waves taking the key tiles in turn and joining their sums in LDS; two
+// workgroups a CU, so that one computes while the other waits for its tile (one,
+// with two stages a wave: 66 us for 2048 queries instead of 38).  The pipeline's
+// workgroups of 256 queries leave most of the chip idle there, and its 60 KB of code
+// are fetched for a few tiles.
+template <class P, bool BF16, int HD, int ROPE = 0>
+struct ShortWave {
+  using T = Wave<P, BF16, HD, 1, 1, ROPE>;
+  static constexpr int kLds = 4 * T::kWaveLds;
+};
+template <bool BF16, int HD, int ROPE = 0, class Params>
+G9_DEV void varlen_short(const Params& p, char* smem) {
+  using W = typename ShortWave<Params, BF16, HD, ROPE>::T;
+  const int group = p.HQ / p.HK;
+  const int rank = blockIdx.x / p.HK, hk = blockIdx.x - rank * p.HK;
+  Tile t;
+  if (!find_tile<32, 256>(p, rank, group, reinterpret_cast<int*>(smem), t)) return;
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  W w(p);
+  w.init(smem, wave, p.ldk, p.ldv);
+  if constexpr (ROPE != 0) w.init_shared(p.ldr);
+  const int row = t.mb * 32 + w.col, nd = row / group, hq = hk * group + row - nd * group;
+  const bool in = nd < t.lq;
+  w.node[0] = in ? nd : -1;
+  w.context = p.causal ? t.lk - t.lq : t.lk;
+  w.q0 = t.q0, w.keys = t.lk;
+  // The first row of the block reads the keys below `all`, the last one those
+  // below `need`.
+  const int last = min((t.mb * 32 + 31) / group, t.lq - 1);
+  const int need = uniform(min(max(last + 1 + w.context, 0), t.lk));
+  const int all = uniform(min(max(t.mb * 32 / group + 1 + w.context, 0), t.lk));
+  const char* const kp = p.k + hk * p.k_h + (size_t)t.k0 * p.ldk;
+  const char* const vp = p.v + hk * p.v_h + (size_t)t.k0 * p.ldv;
+  const auto fill = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < W::kPieces; ++i) {
+      const int k = tile * W::kKeys + 16 * i;
+      w.fill_piece(i, 0, kp + (size_t)(u32)k * p.ldk, vp + (size_t)(u32)k * p.ldv, min(max(t.lk - k, 0), 16), p.ldk,
+                   p.ldv);
+      if constexpr (ROPE != 0)
+        w.fill_shared(i, p.r + (size_t)(u32)(t.k0 + k) * p.ldr, min(max(t.lk - k, 0), 16), p.ldr);
+    }
+  };
+  const int tiles = (need + W::kKeys - 1) / W::kKeys;
+  if (wave < tiles) fill(wave);
+  w.load_q(0, p.q + (size_t)(t.q0 + (in ? nd : 0)) * p.ldq + (in ? hq : hk * group) * p.q_h);
+  w.clear();
+  for (int i = wave; i < tiles; i += 4) {
+    waitcnt<0, 0>();
+    __builtin_amdgcn_sched_barrier(0);
+    w.tile(i * W::kKeys, 0, (i + 1) * W::kKeys > all);
+    waitcnt<63, 0>();
+    __builtin_amdgcn_sched_barrier(0);
+    if (i + 4 < tiles) fill(i + 4);
+  }
+  // The waves' sums, each in its own stage: rows 16 bytes more than HD floats
+  // apart (banks), behind them maximum and weight.
+  constexpr int kPitch = HD + 4, kSums = 32 * kPitch;
+  static_assert((kSums + 64) * 4 <= W::kWaveLds);
+  const float lw = xhalf(w.l[0], [](float x, float y) { return x + y; });
+  waitcnt<63, 0>();
+  const auto sums = [&](int i) { return reinterpret_cast<float*>(smem + i * W::kWaveLds); };
+#pragma unroll
+  for (int d = 0; d < W::kND; ++d)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      *reinterpret_cast<f32x4*>(sums(wave) + w.col * kPitch + 32 * d + 8 * r + 4 * w.h) =
+          f32x4{w.o[0][d][4 * r], w.o[0][d][4 * r + 1], w.o[0][d][4 * r + 2], w.o[0][d][4 * r + 3]};
+  if (w.h == 0) sums(wave)[kSums + w.col] = w.m[0], sums(wave)[kSums + 32 + w.col] = lw;
+  __syncthreads();
+  // Eight threads a row.
+  const int r = tid >> 3, c = tid & 7, mine = t.mb * 32 + r, n = mine / group;
+  if (n >= t.lq) return;
+  float m = sums(0)[kSums + r];
+#pragma unroll
+  for (int i = 1; i < 4; ++i) m = __builtin_fmaxf(m, sums(i)[kSums + r]);
+  float f[4], l = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[i] = __builtin_amdgcn_exp2f(sums(i)[kSums + r] - m);
+    l += f[i] * sums(i)[kSums + 32 + r];
+  }
+  const bool none = (__float_as_uint(l) << 1) == 0;
+  const float inv = none ? 0.f : 1.f / l;
+  const int head = hk * group + mine - n * group;
+  char* const orow = p.o + head * p.o_h + (size_t)(t.q0 + n) * p.ldo;
+#pragma unroll
+  for (int j = 0; j < HD / 32; ++j) {
+    const int col = 32 * j + 4 * c;
+    f32x4 x = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x += f[i] * *reinterpret_cast<const f32x4*>(sums(i) + r * kPitch + col);
+    *reinterpret_cast<u32x2*>(orow + col * 2) = u32x2{pack2<BF16>(x[0] * inv, x[1] * inv), pack2<BF16>(x[2] * inv, x[3] * inv)};
+  }
+  if (p.lse && c == 0) p.lse[(size_t)head * p.T + t.q0 + n] = none ? -__builtin_inff() : (m + __builtin_log2f(l)) * kLn2;
+}
+
 }  // namespace fa
 }  // namespace g9

@@ -27,8 +27,17 @@ G9_DEV V uniform(V x) {
 
 // p.reads says which keys a row reads, p.scale_log2 the scale.
 // NQ groups of 32 query rows, which share every K and V register read from LDS.
-template <class Params, bool BF16, int HD, int NQ, int STAGES = 2>
-struct Wave {
+// ROPE: 64 more values of every key, from rows of their own, which all heads share; a
+// stage has 4 KB more for them, which P's scratch takes over (the scores are formed then).
+template <int ROPE>
+struct SharedLanes {};
+template <>
+struct SharedLanes<64> {
+  u32 voffr[2], ar;  // lane's row offsets of the shared keys, LDS read base
+};
+template <class Params, bool BF16, int HD, int NQ, int STAGES = 2, int ROPE = 0>
+struct Wave : SharedLanes<ROPE> {
+  static_assert(ROPE == 0 || (ROPE == 64 && HD == 128 && STAGES == 1));
   static constexpr int kKeys = 4096 / HD;          // keys per tile
   static constexpr int kNB = kKeys / 32;           // 32-key score blocks
   static constexpr int kNS = HD / 16;              // QK steps of 16 head-dim values
@@ -38,9 +47,11 @@ struct Wave {
   static constexpr int kRows = 1024 / kRow;        // rows of one DMA
   static constexpr int kPieces = kKeys / 16;       // 16-row pieces: never across a page
   static constexpr int kDmas = 8;                  // per tile and operand
-  static constexpr int kStage = 16384, kV = 8192;  // a stage; V behind K
+  static constexpr int kNR = ROPE / 16;            // QK steps of the shared keys
+  static constexpr int kV = 8192, kR = 16384;      // V behind K; the shared keys behind both
+  static constexpr int kStage = kR + kKeys * ROPE * 2;
   static constexpr int kScratch = 32 * kKeys * 2;  // P of one tile and 32 rows, 16 bit
-  static constexpr int kWaveLds = STAGES * kStage + kScratch;
+  static constexpr int kWaveLds = STAGES * kStage + (ROPE ? 0 : kScratch);
 
   const Params& p;
   int lane, h, col;  // lane, lane / 32, lane % 32
@@ -48,7 +59,7 @@ struct Wave {
   char* scratch;
   u32 voffk[4], voffv[1];
   u32 ak, av;        // LDS read bases in a stage (K, V)
-  u32x4 qf[NQ][kNS];
+  u32x4 qf[NQ][kNS + kNR];
   f32x16 o[NQ][kND];
   float m[NQ], l[NQ];
   int node[NQ];      // of this lane's queries, -1 where there is none
@@ -67,7 +78,7 @@ struct Wave {
   G9_DEV void init(char* smem, int wave, u32 k_t, u32 v_t) {
     lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
     lds = (u32)(uintptr_t)to_lds(smem) + wave * kWaveLds;
-    scratch = smem + wave * kWaveLds + STAGES * kStage;
+    scratch = smem + wave * kWaveLds + (ROPE ? kR : STAGES * kStage);
     constexpr int kPer = kRow / 16;  // chunks of a row
     const int r = lane / kPer, slot = lane % kPer;
 #pragma unroll
@@ -95,9 +106,25 @@ struct Wave {
       dma16_fresh(rv, lds + stage * kStage + kV + j * 1024, voffv[0], jj * kRows * v_t);
     }
   }
+  // The shared keys' rows of 128 bytes, permuted like K's of head dim 64.
+  static G9_DEV int swz_r(int r) { return (r >> 1) & 7; }
+  G9_DEV void init_shared(u32 r_t) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = 8 * j + lane / 8;
+      this->voffr[j] = r * r_t + 16 * ((lane & 7) ^ swz_r(r));
+    }
+    this->ar = lds + kR + col * 128 + 16 * (h ^ swz_r(col));
+  }
+  // Rows 16 i .. 16 i + 15 of them.
+  G9_DEV void fill_shared(int i, const char* r, int rows, u32 r_t) const {
+    const rsrc_t rr = make_rsrc(uniform(r), uniform(extent(rows, r_t, 128)));
+#pragma unroll
+    for (int j = 0; j < 2; ++j) dma16_fresh(rr, lds + kR + i * 2048 + j * 1024, this->voffr[j], 0);
+  }
   G9_DEV void load_q(int t, const char* qrow) {
 #pragma unroll
-    for (int s = 0; s < kNS; ++s) qf[t][s] = *reinterpret_cast<const u32x4*>(qrow + (16 * s + 8 * h) * 2);
+    for (int s = 0; s < kNS + kNR; ++s) qf[t][s] = *reinterpret_cast<const u32x4*>(qrow + (16 * s + 8 * h) * 2);
   }
   G9_DEV void clear() {
 #pragma unroll
@@ -122,6 +149,16 @@ struct Wave {
 #pragma unroll
         for (int t = 0; t < NQ; ++t) sc[t][b] = mfma<BF16>(kf, qf[t][s], s ? sc[t][b] : f32x16{});
       }
+    if constexpr (ROPE != 0) {
+#pragma unroll
+      for (int s = 0; s < kNR; ++s)
+#pragma unroll
+        for (int b = 0; b < kNB; ++b) {
+          const u32x4 kf = *(const G9_LDS u32x4*)(uintptr_t)((this->ar ^ (32 * s)) + 32 * b * 128);
+#pragma unroll
+          for (int t = 0; t < NQ; ++t) sc[t][b] = mfma<BF16>(kf, qf[t][kNS + s], sc[t][b]);
+        }
+    }
     u32x4 pf[NQ][kKS];
 #pragma unroll
     for (int t = 0; t < NQ; ++t) {
