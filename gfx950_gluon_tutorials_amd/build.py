@@ -39,7 +39,8 @@ SOURCE_FLAGS = {s: ["-fno-honor-nans"] for s in ("g9_fmha.hip", "g9_varlen.hip",
 # such branches end at once the compiler turns the lanes on again at the outer end only, and
 # has reloaded spilled registers between the two, in some of the lanes: here each
 # branch turns its lanes on again.  The kernels of NO_SPILLS must not spill at all (the build
-# fails if they do).
+# fails if they do), and keep their sums in accumulation registers that the compiler must
+# leave alone (the same).
 for _s in ("g9_latent.hip", "g9_latent_varlen.hip"):
     SOURCE_FLAGS[_s] = SOURCE_FLAGS[_s] + ["-mllvm", "-amdgpu-remove-redundant-endcf=0"]
 NO_SPILLS = {"g9_latent.hip"}
@@ -116,6 +117,7 @@ def build(verbose: bool = False, timing: bool = False) -> str:
             table = isa_check.resource_table(text)
             if src in NO_SPILLS:
                 bad += [f"{r['kernel']}: {r['vgpr_spill']} vector registers spilled" for r in table if r["vgpr_spill"]]
+                bad += isa_check.check_accumulators(text)
             resources += table
         if bad:
             os.unlink(tmp)

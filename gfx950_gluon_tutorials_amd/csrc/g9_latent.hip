@@ -7,20 +7,33 @@
 // do by a little, if the products come near the matrix unit's rate.  So a row of the cache
 // should reach a CU once for all its heads.
 //
-// The work is the line of g9_line.hpp, cut into one part per CU.  A workgroup is four
-// waves, one per SIMD with the whole register file: a wave has 32 query rows, their
-// sums of 512 values (256 accumulation registers a lane) and their queries (144
-// registers).  RB = 1, 2 or 4 waves with different rows share each tile of 32 keys in
-// LDS, and the 4 / RB groups take tiles in turn, whose sums are joined in LDS at the
-// block's end.  Four tiles (147 KB) are in LDS, filled by LDS-DMA.
+// The work is the line of g9_line.hpp, cut into one part per CU.  A workgroup has a block
+// of RB = 1, 2 or 4 times 32 query rows and is four waves, one per SIMD with the whole
+// register file.  Tiles of 32 keys go through four stages of LDS (147 KB), filled by
+// LDS-DMA.  Per tile
+//   S^T = K Q^T    by rows: wave w has the rows 32 w .. (their queries are 144 registers a
+//                  lane), 36 MFMAs 32x32x16;
+//   softmax        of its rows; the weights P go to LDS (16 bit, as the product takes them;
+//                  fp32 products have a sixteenth of the rate);
+//   O^T += V^T P^T by values: wave w has the values 128 w .. of all rows (64 RB accumulation
+//                  registers a lane), 8 RB MFMAs.  V is the row's first 512 values, read
+//                  by transposing LDS reads, each once for the workgroup.
+// in the register layouts that g9_fmha.hip describes.  (All 512 values of a wave's own
+// rows take no exchange, but every wave then reads all of V from LDS.)  A step has the scores
+// of tile j + 1 and the values of tile j: the scores' products, which wait for LDS when alone,
+// go in turn with some of the values', the softmax and the DMAs of tile j + 3 between the rest.
+// A row's maximum moves only where a tile passes it by more than 8 (log2 units); then its
+// factor goes through LDS, too.
 //
-// Per tile a wave computes S^T = K Q^T and O^T += V^T P^T with 32x32x16 MFMAs, 36
-// and 32 of them, in the register layouts that g9_fmha.hip describes: the weights
-// P are rounded to the 16-bit type for that product (fp32 products have a sixteenth of the
-// rate), their sum is taken before.  V is the row's first 512 values, read by
-// transposing LDS reads.  A row's maximum moves only where a tile passes it by more
-// than 8 (log2 units), so that the sums are rarely rescaled.
+// Measured (us, kernel and join, inputs partly in the last-level cache): 64 requests of 100 to
+// 8192 tokens by 16 heads 32 + 8: 1.5 a tile, 6.1 TB/s over the loop, but 14 of the 32 go to
+// finding the part, the first loads and the sums' way out; by 128 heads 48 + 18, 2.1 a tile
+// (68 MFMAs of 32 cycles are 1.2 at the clock that they leave), 25 outside the loop, much of
+// them and of the join for the 256 KB of sums of a part; 16 trees of 12 nodes by 32 heads
+// 79 + 19; one request of 700 tokens by 16 heads 10 + 6.
 #include "../../include/gfx950_fmha.h"
+#include <utility>
+
 #include "g9_attn_host.hpp"
 #include "g9_line.hpp"
 
@@ -33,10 +46,13 @@ constexpr int kRank = 512, kRow = 576;  // values of a latent, of a row
 constexpr int kRowBytes = kRow * 2;
 constexpr int kKeys = 32;               // of a tile
 constexpr int kTile = kKeys * kRowBytes;
-constexpr int kQk = kRow / 16, kPv = kRank / 32;  // products' steps of 16, blocks of 32 values
-constexpr int kDepth = 6;                          // fragments read ahead
-constexpr int kLds = 4 * kTile;
-constexpr float kNone = -3.0e38f;                // the maximum of a row that has read nothing: finite, weights 0
+constexpr int kQk = kRow / 16;          // steps of 16 of the scores' product
+constexpr int kPv = 4;                  // blocks of 32 values of a wave
+constexpr int kAhead = 3;               // steps asked for ahead
+// LDS: the stages, P of up to 128 rows, factors of the rows, a word a wave that says
+// whether there are any, then the rows' maxima and weights at the end.
+constexpr int kP = 4 * kTile, kFactors = kP + 8192, kMoved = kFactors + 512, kMl = kMoved + 64, kLds = kMl + 1024;
+constexpr float kNone = -3.0e38f;       // the maximum of a row that has read nothing: finite, weights 0
 
 struct Params {
   const char* q;
@@ -58,46 +74,86 @@ struct Params {
   float scale_log2;
 };
 
-// The products as assembly, which keeps the sums in accumulation registers and the
-// scores out of them.  The compiler does not look into it: the wait states between
-// a product and the vector unit's use of its result, or of an operand that the vector unit
-// has just written, are `settle` below (isa_check verifies them).
-template <bool BF16>
-G9_DEV void product(f32x16& c, u32x4 a, u32x4 b) {
-  if constexpr (BF16)
-    asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
-  else
-    asm("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+// The sums: 16 blocks of 32 x 32 in all 256 accumulation registers, block N in a[16 N] to
+// a[16 N + 15].  They are no variables: the compiler knows the registers as overwritten by each
+// statement here and keeps nothing in them (as variables, the sums changed places from loop
+// to loop by way of scratch memory; the build checks that no instruction outside assembly names
+// one).  The compiler does not look into assembly: the wait states between a product and the
+// vector unit's use of its result, or of an operand that the vector unit has just written, are
+// `settle` and the s_nop of the statements below (isa_check verifies them).
+template <int N>
+struct Block;
+#define G9_BLOCK(N, LO, HI, ...)                                                                               \
+  template <>                                                                                                 \
+  struct Block<N> {                                                                                            \
+    template <bool BF16>                                                                                       \
+    static G9_DEV void product(u32x4 a, u32x4 b) {                                                             \
+      if constexpr (BF16)                                                                                      \
+        asm volatile("v_mfma_f32_32x32x16_bf16 a[" #LO ":" #HI "], %0, %1, a[" #LO ":" #HI "]"               \
+                     : : "v"(a), "v"(b) : __VA_ARGS__);                                                        \
+      else                                                                                                     \
+        asm volatile("v_mfma_f32_32x32x16_f16 a[" #LO ":" #HI "], %0, %1, a[" #LO ":" #HI "]"                \
+                     : : "v"(a), "v"(b) : __VA_ARGS__);                                                        \
+    }                                                                                                          \
+    template <int E>                                                                                           \
+    static G9_DEV void clear() {                                                                               \
+      asm volatile("v_accvgpr_write_b32 a%c0, 0" : : "i"(LO + E) : __VA_ARGS__);                              \
+    }                                                                                                          \
+    template <int E>                                                                                           \
+    static G9_DEV void multiply(float f) {                                                                     \
+      float x;                                                                                                 \
+      asm volatile("v_accvgpr_read_b32 %0, a%c2\n\tv_mul_f32 %0, %0, %1\n\tv_accvgpr_write_b32 a%c2, %0"    \
+                   : "=&v"(x) : "v"(f), "i"(LO + E) : __VA_ARGS__);                                           \
+    }                                                                                                          \
+    template <int E>                                                                                           \
+    static G9_DEV float value() {                                                                              \
+      float x;                                                                                                 \
+      asm volatile("v_accvgpr_read_b32 %0, a%c1" : "=v"(x) : "i"(LO + E) : __VA_ARGS__);                      \
+      return x;                                                                                                \
+    }                                                                                                          \
+  };
+G9_BLOCK(0, 0, 15, "a0", "a1", "a2", "a3", "a4", "a5", "a6", "a7", "a8", "a9", "a10", "a11", "a12", "a13", "a14", "a15")
+G9_BLOCK(1, 16, 31, "a16", "a17", "a18", "a19", "a20", "a21", "a22", "a23", "a24", "a25", "a26", "a27", "a28", "a29", "a30", "a31")
+G9_BLOCK(2, 32, 47, "a32", "a33", "a34", "a35", "a36", "a37", "a38", "a39", "a40", "a41", "a42", "a43", "a44", "a45", "a46", "a47")
+G9_BLOCK(3, 48, 63, "a48", "a49", "a50", "a51", "a52", "a53", "a54", "a55", "a56", "a57", "a58", "a59", "a60", "a61", "a62", "a63")
+G9_BLOCK(4, 64, 79, "a64", "a65", "a66", "a67", "a68", "a69", "a70", "a71", "a72", "a73", "a74", "a75", "a76", "a77", "a78", "a79")
+G9_BLOCK(5, 80, 95, "a80", "a81", "a82", "a83", "a84", "a85", "a86", "a87", "a88", "a89", "a90", "a91", "a92", "a93", "a94", "a95")
+G9_BLOCK(6, 96, 111, "a96", "a97", "a98", "a99", "a100", "a101", "a102", "a103", "a104", "a105", "a106", "a107", "a108", "a109", "a110", "a111")
+G9_BLOCK(7, 112, 127, "a112", "a113", "a114", "a115", "a116", "a117", "a118", "a119", "a120", "a121", "a122", "a123", "a124", "a125", "a126", "a127")
+G9_BLOCK(8, 128, 143, "a128", "a129", "a130", "a131", "a132", "a133", "a134", "a135", "a136", "a137", "a138", "a139", "a140", "a141", "a142", "a143")
+G9_BLOCK(9, 144, 159, "a144", "a145", "a146", "a147", "a148", "a149", "a150", "a151", "a152", "a153", "a154", "a155", "a156", "a157", "a158", "a159")
+G9_BLOCK(10, 160, 175, "a160", "a161", "a162", "a163", "a164", "a165", "a166", "a167", "a168", "a169", "a170", "a171", "a172", "a173", "a174", "a175")
+G9_BLOCK(11, 176, 191, "a176", "a177", "a178", "a179", "a180", "a181", "a182", "a183", "a184", "a185", "a186", "a187", "a188", "a189", "a190", "a191")
+G9_BLOCK(12, 192, 207, "a192", "a193", "a194", "a195", "a196", "a197", "a198", "a199", "a200", "a201", "a202", "a203", "a204", "a205", "a206", "a207")
+G9_BLOCK(13, 208, 223, "a208", "a209", "a210", "a211", "a212", "a213", "a214", "a215", "a216", "a217", "a218", "a219", "a220", "a221", "a222", "a223")
+G9_BLOCK(14, 224, 239, "a224", "a225", "a226", "a227", "a228", "a229", "a230", "a231", "a232", "a233", "a234", "a235", "a236", "a237", "a238", "a239")
+G9_BLOCK(15, 240, 255, "a240", "a241", "a242", "a243", "a244", "a245", "a246", "a247", "a248", "a249", "a250", "a251", "a252", "a253", "a254", "a255")
+#undef G9_BLOCK
+
+// f<0>(), f<1>(), ..
+template <int N, class F>
+G9_DEV void each(F f) {
+  [&]<int... I>(std::integer_sequence<int, I...>) { (f.template operator()<I>(), ...); }
+  (std::make_integer_sequence<int, N>{});
 }
+
 template <bool BF16>
 G9_DEV void score(f32x16& c, u32x4 a, u32x4 b) {
   if constexpr (BF16)
-    asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
   else
-    asm("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
 }
 template <bool BF16>
 G9_DEV void first_score(f32x16& c, u32x4 a, u32x4 b) {
   if constexpr (BF16)
-    asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b));
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b));
   else
-    asm("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b));
+    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b));
 }
 G9_DEV void settle(f32x16& c) { asm volatile("s_nop 7\n\ts_nop 7" : "+v"(c)); }
-G9_DEV void settle(f32x16 (&c)[kPv]) {
-  asm volatile("s_nop 7\n\ts_nop 7" : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]), "+a"(c[4]), "+a"(c[5]), "+a"(c[6]), "+a"(c[7]));
-  asm volatile("" : "+a"(c[8]), "+a"(c[9]), "+a"(c[10]), "+a"(c[11]), "+a"(c[12]), "+a"(c[13]), "+a"(c[14]), "+a"(c[15]));
-}
-// Operands that the vector unit wrote, before the products that take them.
-G9_DEV void ready(u32x4 (&x)[2]) { asm volatile("s_nop 1" : "+v"(x[0]), "+v"(x[1])); }
-
-// One sum out of the accumulation registers (as assembly: the compiler would move all 16 of
-// a block at once, and keep what it had in their place in scratch memory).
-G9_DEV float sum_of(const f32x16& c, int i) {
-  float x;
-  asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(x) : "a"(c[i]));
-  return x;
-}
+// The sums' products are done.
+G9_DEV void settle() { asm volatile("s_nop 7\n\ts_nop 7"); }
 
 // The lane, worked out where it is used: what follows from it is not held through the loop.
 G9_DEV int lane_here() {
@@ -106,26 +162,31 @@ G9_DEV int lane_here() {
   return x;
 }
 
-// RB blocks of 32 rows share a tile; a step of the workgroup is 4 / RB tiles.
+// RB blocks of 32 rows; a step of the workgroup is a tile.  What a block's beginning and end
+// cost, in tiles, is the line's LEAD (us, the cases above with
+// 5, 9, 12 places: 128 heads 70, 68.5, 66, trees 99, 97, 98; 16 heads with 5 and 7: 40.5, 41.5).
 template <int RB>
-using Steps = Line<Params, kKeys * (4 / RB), 32 * RB, kWgs, RB == 4 ? 5 : 2>;
+using Steps = Line<Params, kKeys, 32 * RB, kWgs, RB == 4 ? 12 : RB == 2 ? 8 : 5>;
 
-// One wave's rows and their sums.
+// One wave: rows 32 wave .. of the block for the scores, values 128 wave .. for the sums.
 template <bool BF16, int RB>
-struct Rows {
-  static constexpr int kGroups = 4 / RB;       // waves that take tiles in turn
-
+struct Wave4 {
   const Params& p;
+  int wave;
   u32 lds;             // of the workgroup
-  u32 voff[9], flip;
+  char* smem;
+  u32 voff[9];
   u32 ak, av;          // LDS read bases in a tile (K, V)
   u32x4 qf[kQk];
-  f32x16 o[kPv];
-  float m, l;
+  float m, l;          // of this lane's row
   NodeRow row;
-  int keys;
+  int keys, whole;     // of the request; keys that every row reads
+  u32 bad;             // keys of the tile whose values come next that hold special values
+  u32x4 weight[2];     // of the last scores' tile, its softmax's factor and whether that matters
+  float factor;
+  bool moves;
 
-  G9_DEV explicit Rows(const Params& pp) : p(pp) {}
+  G9_DEV explicit Wave4(const Params& pp) : p(pp) {}
 
   // A tile in LDS: rows of 1152 bytes (72 pieces of 16 bytes, an odd number of 128-byte
   // lines), piece c of row r at place c ^ swz(r).  A K read takes one piece of 16 rows:
@@ -133,56 +194,47 @@ struct Rows {
   // transposing V read takes 4 pieces of 4 rows: bit 2 of swz is bit 1 of r.
   static G9_DEV int swz(int r) { return (r >> 1 & 1) << 2 | (r >> 2 & 3); }
 
-  G9_DEV void init(char* smem, int wave) {
+  G9_DEV void init(char* sm) {
     const int lane = threadIdx.x & 63, h = lane >> 5, col = lane & 31;
-    lds = (u32)(uintptr_t)to_lds(smem);
-    // Nine DMAs fill 8 rows: DMA j writes the bytes 1024 j + 16 lane of them.  The 8
-    // rows behind them have bit 1 of their places the other way round: 32 bytes up or down.
-    flip = 0;
+    smem = sm;
+    lds = (u32)(uintptr_t)to_lds(sm);
+    // A wave fetches 8 rows of a tile with nine DMAs: DMA j writes the bytes 1024 j + 16 lane.
 #pragma unroll
     for (int j = 0; j < 9; ++j) {
-      const int n = 64 * j + lane, r = n / 72, c = (n - 72 * r) ^ swz(r + (RB == 4 ? 8 * (wave & 1) : 0));
-      voff[j] = (u32)r * p.c_t + 16 * c;
-      flip |= (u32)(c >> 1 & 1) << j;
+      const int n = 64 * j + lane, r = n / 72;
+      voff[j] = (u32)r * p.c_t + 16 * ((n - 72 * r) ^ swz(r + 8 * (wave & 1)));
     }
-    ak = col * kRowBytes + 16 * (h ^ swz(col));
+    ak = lds + col * kRowBytes + 16 * (h ^ swz(col));
     // 16 lanes cover 4 rows and 16 values: lane jj of them row jj / 4, values 4 (jj % 4)
     // of two pieces.
     const int jj = lane & 15, r4 = 4 * h + (jj >> 2);
-    av = r4 * kRowBytes + 16 * ((2 * (lane >> 4 & 1) + ((jj & 3) >> 1)) ^ swz(r4)) + 8 * (jj & 1);
+    av = lds + r4 * kRowBytes + 16 * ((2 * (lane >> 4 & 1) + ((jj & 3) >> 1)) ^ swz(r4)) + 8 * (jj & 1) + 256 * wave;
   }
 
-  // A 16-row piece of a tile to come: its rows' descriptor, its place in LDS.
-  struct Piece {
+  // This wave's 8 rows of a tile to come: their descriptor, their place in LDS.
+  struct Rows8 {
     rsrc_t r;
     u32 to;
   };
-  // Piece i of the tile that begins with key k0, of `all` keys (rows behind them read as
-  // zeros), on page pg, into stage `stage`.
-  G9_DEV Piece aim(int i, int stage, int k0, int all, int pg) const {
-    const int k = k0 + 16 * i, off = k & ((1 << p.shift) - 1);
+  // Of the tile that begins with key k0, of `all` keys (rows behind them read as zeros), on
+  // page pg, into stage `stage`.  A 16-row piece never crosses a page.
+  G9_DEV Rows8 aim(int stage, int k0, int all, int pg) const {
+    const int k = k0 + 8 * wave, off = k & ((1 << p.shift) - 1);
     const bool in = (u32)pg < (u32)p.num_blocks;
-    const int rows = in ? min(max(all - k, 0), 16) : 0;
+    const int rows = in ? min(max(all - k, 0), 8) : 0;
     const char* const base = p.cache + (long long)(in ? pg : 0) * p.c_b + (unsigned long long)(u32)off * p.c_t;
     return {make_rsrc(uniform(base), uniform(extent(rows, p.c_t, kRowBytes))),
-            (u32)uniform((int)(lds + stage * kTile + i * 16 * kRowBytes))};
+            (u32)uniform((int)(lds + stage * kTile + wave * 8 * kRowBytes))};
   }
-  // DMA j of a piece's 18.
   template <int J>
-  G9_DEV void fetch(const Piece& x, int wave) const {
-    if constexpr (RB == 4) {  // a wave has one half of a piece
-      dma16_fresh(x.r, x.to + 9216 * (wave & 1) + 1024 * J, voff[J], (wave & 1) * 8 * p.c_t);
-    } else {
-      const u32 at = J < 9 ? voff[J % 9] : voff[J % 9] + 32 - ((flip >> (J % 9) & 1) << 6);
-      dma16_fresh(x.r, x.to + 1024 * J, at, J < 9 ? 0 : 8 * p.c_t);
-    }
+  G9_DEV void fetch(const Rows8& x) const {
+    dma16_fresh(x.r, x.to + 1024 * J, voff[J], 0);
   }
-  static constexpr int kOwn = RB == 4 ? 9 : 18;  // a wave's DMAs of a piece
   template <int J = 0>
-  G9_DEV void fetch_all(const Piece& x, int wave) const {
-    if constexpr (J < kOwn) {
-      fetch<J>(x, wave);
-      fetch_all<J + 1>(x, wave);
+  G9_DEV void fetch_all(const Rows8& x) const {
+    if constexpr (J < 9) {
+      fetch<J>(x);
+      fetch_all<J + 1>(x);
     }
   }
 
@@ -193,127 +245,188 @@ struct Rows {
   }
   G9_DEV void clear() {
     m = kNone, l = 0.f;
-#pragma unroll
-    for (int d = 0; d < kPv; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float x;
-        asm volatile("v_accvgpr_write_b32 %0, 0" : "=a"(x));
-        o[d][i] = x;
-      }
+    each<RB * kPv>([&]<int B>() { each<16>([&]<int E>() { Block<B>::template clear<E>(); }); });
+    asm volatile("s_nop 1");
   }
 
-  // Adds the tile in `stage`, whose first key is k0; TAIL: not every row may read all of it.
-  // The DMAs of piece `next` (RB > 1) are issued between the products: all at once, they
-  // would hold the wave until memory has taken them.
-  template <bool TAIL>
-  G9_DEV void tile(int k0, int stage, const Piece& next, int wave) {
-    const u32 ks = lds + stage * kTile + ak, vs = lds + stage * kTile + av;
-    // Fragments are read kDepth ahead of the product that takes them (the compiler takes
-    // assembly for instructions without a latency, and would read each just before).
+  // The products of tile j's values (VALUES; P in LDS, the tile in stage `vstage`) and of tile
+  // j + 1's scores (SCORES; from key k0 on, stage `kstage`).  The scores come first, in turn
+  // with the values' products that their softmax does not need behind them: alone, they would
+  // wait for LDS (each wave reads the whole tile for them).  The softmax is cut into pieces of
+  // about the 32 cycles that a product takes and goes between the other products.  So do the
+  // DMAs of `next`: all at once, they would hold the wave until memory has taken them.  TAIL:
+  // tiles that not every row may read whole.
+  template <bool SCORES, bool VALUES, bool TAIL>
+  G9_DEV void products(int k0, int kstage, int vstage, const Rows8& next) {
+    constexpr int kK = SCORES ? kQk : 0, kV = VALUES ? 2 * kPv * RB : 0, kAll = kK + kV;
+    constexpr int kDepth = 4;  // K fragments read ahead (the compiler takes assembly for instructions
+                               // without a latency, and would read each just before)
+    const u32 ks = ak + kstage * kTile, vs = av + vstage * kTile;
     const u32 kb[4] = {ks, ks ^ 32, ks ^ 64, ks ^ 96}, vb[4] = {vs, vs ^ 64, vs ^ 32, vs ^ 96};
+    const u32 pb = lds + kP + 16 * (u32)lane_here();
     const auto k_at = [&](int s) { return *(const G9_LDS u32x4*)(uintptr_t)(kb[s & 3] + 128 * (s >> 2)); };
+    // Fragment i: block i % 4 of the values, 16 of the keys.
     const auto v_at = [&](int i) {
       const int at = 16 * kRowBytes * (i / kPv) + 128 * (i % kPv >> 1);
       const u32x2 lo = tr_read(vb[i & 1] + at), hi = tr_read(vb[2 + (i & 1)] + at + 8 * kRowBytes);
       return u32x4{lo.x, lo.y, hi.x, hi.y};
     };
-    u32x4 f[kDepth];
-    // DMA J behind product (2 J + 1) / 2 / kOwn of all.
-    const auto slot = [&]<int S>() {
-      constexpr int kAll = kQk + 2 * kPv, J = (2 * S + 1) * kOwn / (2 * kAll), K = (2 * S + 3) * kOwn / (2 * kAll);
-      if constexpr (RB > 1 && J != K && J < kOwn) fetch<J>(next, wave);
-    };
+    const auto p_at = [&](int rb, int t) { return *(const G9_LDS u32x4*)(uintptr_t)(pb + 1024 * (2 * rb + t)); };
+    const u32 out = VALUES && TAIL ? bad >> (4 * (lane_here() >> 5)) : 0;  // of this lane's keys
+    u32x4 f[kDepth], v[2], pf[RB];
     f32x16 sc;
+    if constexpr (VALUES) {
 #pragma unroll
-    for (int s = 0; s < kDepth; ++s) f[s] = k_at(s);
-    const auto qk_step = [&]<int S>(auto self) {
-      if constexpr (S < kQk) {
-        if constexpr (S == 0)
-          first_score<BF16>(sc, f[0], qf[0]);
-        else
-          score<BF16>(sc, f[S % kDepth], qf[S]);
-        __builtin_amdgcn_sched_barrier(0);
-        f[S % kDepth] = S + kDepth < kQk ? k_at(S + kDepth) : v_at(S + kDepth - kQk);
+      for (int rb = 0; rb < RB; ++rb) pf[rb] = p_at(rb, 0);
+      v[0] = v_at(0), v[1] = v_at(1);
+    }
+    if constexpr (SCORES) {
+#pragma unroll
+      for (int s = 0; s < kDepth; ++s) f[s] = k_at(s);
+    }
+    // DMA J behind product (2 J + 1) / 18 of all.
+    const auto slot = [&]<int S>() {
+      constexpr int J = (2 * S + 1) * 9 / (2 * kAll), K = (2 * S + 3) * 9 / (2 * kAll);
+      static_assert(K - J <= 2);
+      if constexpr (J != K && J < 9) fetch<J>(next);
+      if constexpr (K == J + 2 && K <= 9) fetch<J + 1>(next);
+    };
+    const auto value = [&]<int I>() {
+      constexpr int kFrag = I / RB, kBlock = I % RB, kTime = kFrag / kPv;
+      u32x4& x = v[kFrag & 1];
+      if constexpr (TAIL && kBlock == 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const u32 two = out >> (16 * kTime + 8 * (e / 2) + 2 * (e % 2));
+          x[e] &= (two & 1 ? 0 : 0xffffu) | (two & 2 ? 0 : 0xffff0000u);
+        }
+        asm volatile("s_nop 1" : "+v"(x));
+      }
+      Block<kBlock * kPv + kFrag % kPv>::template product<BF16>(x, pf[kBlock]);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (kFrag == kPv - 1) pf[kBlock] = p_at(kBlock, 1);
+      if constexpr (kBlock == RB - 1 && kFrag + 2 < 2 * kPv) x = v_at(kFrag + 2);
+    };
+    // The softmax: kPieces pieces behind product kLast + 2.
+    constexpr int kPieces = 20, kMix = SCORES && kV > kPieces + 2 ? kV - kPieces - 2 : 0;
+    constexpr int kLast = kK + kMix - 1;  // the last score's product, at the latest
+    constexpr int kSlots = kAll - kLast - 3, kEach = kSlots > 0 ? (kPieces + kSlots - 1) / kSlots : kPieces;
+    Soft<TAIL> soft{k0, kstage};
+    const auto pieces = [&]<int FIRST, int N>() {
+      each<N>([&]<int I>() {
+        if constexpr (FIRST + I < kPieces) piece<TAIL, FIRST + I>(soft, sc);
+      });
+    };
+    const auto step = [&]<int S>(auto self) {
+      // Product S of all.
+      if constexpr (S < kAll) {
+        constexpr int kBefore = SCORES ? (S <= kLast ? S * kK / (kLast + 1) : kK) : 0;
+        constexpr int kBehind = SCORES ? (S < kLast ? (S + 1) * kK / (kLast + 1) : kK) : 0;
+        if constexpr (kBehind > kBefore) {
+          if constexpr (kBefore == 0)
+            first_score<BF16>(sc, f[0], qf[0]);
+          else
+            score<BF16>(sc, f[kBefore % kDepth], qf[kBefore]);
+          __builtin_amdgcn_sched_barrier(0);
+          if constexpr (kBefore + kDepth < kK) f[kBefore % kDepth] = k_at(kBefore + kDepth);
+        } else {
+          value.template operator()<S - kBefore>();
+        }
         slot.template operator()<S>();
+        if constexpr (SCORES && S > kLast + 2) pieces.template operator()<(S - kLast - 3) * kEach, kEach>();
         self.template operator()<S + 1>(self);
       }
     };
-    qk_step.template operator()<0>(qk_step);
-    settle(sc);
-    u32x4 keep[2];  // TAIL: the keys whose values enter the product
-    if constexpr (TAIL) {
-      const int h = lane_here() >> 5;
-      const u32 reads = (u32)node_reads(p, row, k0, keys), bad = special(stage);
-      u32 quiet;  // a NaN that the compiler, told not to mind them, does not see
-      asm("v_mov_b32 %0, 0x7fc00000" : "=v"(quiet));
-      const u32 bits = reads >> (4 * h), nan = (reads & bad) >> (4 * h);
+    step.template operator()<0>(step);
+    if constexpr (SCORES) pieces.template operator()<(kSlots > 0 ? kSlots * kEach : 0), kPieces>();
+    if constexpr (SCORES && TAIL) bad = soft.bad;
+  }
+
+  template <bool TAIL>
+  struct Soft {
+    int k0, stage;
+    u32 bad = 0;
+    float top = 0.f, sum[2] = {0.f, 0.f};
+  };
+  // Piece N of the softmax: the maximum of the scores, the weights one by one.
+  template <bool TAIL, int N>
+  G9_DEV void piece(Soft<TAIL>& x, f32x16& sc) {
+    if constexpr (N == 0) {
+      settle(sc);
+      if constexpr (TAIL) {
+        x.bad = x.k0 + kKeys > whole ? special(x.stage) : 0;
+        const int h = lane_here() >> 5;
+        const u32 reads = (u32)node_reads(p, row, x.k0, keys);
+        u32 quiet;  // a NaN that the compiler, told not to mind them, does not see
+        asm("v_mov_b32 %0, 0x7fc00000" : "=v"(quiet));
+        const u32 bits = reads >> (4 * h), nan = (reads & x.bad) >> (4 * h);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int key = 8 * (i / 4) + i % 4;
-        const float x = __uint_as_float(nan >> key & 1 ? quiet : __float_as_uint(sc[i]));
-        sc[i] = bits >> key & 1 ? x : -__builtin_inff();
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const u32 two = bad >> (4 * h + 16 * (i / 4) + 8 * (i / 2 % 2) + 2 * (i % 2));
-        keep[i / 4][i % 4] = (two & 1 ? 0 : 0xffffu) | (two & 2 ? 0 : 0xffff0000u);
-      }
-    }
-    float top = sc[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) top = __builtin_fmaxf(top, sc[i]);
-    top = xhalf(top, [](float x, float y) { return __builtin_fmaxf(x, y); }) * p.scale_log2;
-    const bool moves = top - m > kLazyThreshold;
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(moves) != 0, 0)) {
-      const float m_new = moves ? top : m;
-      const float alpha = __builtin_amdgcn_exp2f(m - m_new);
-      const bool first = m < kNone * 0.5f;
-      m = m_new;
-      l *= alpha;
-      // A row's first tile moves its maximum, but not its sums, which are zeros.
-      if (__builtin_amdgcn_ballot_w64(moves && !first)) {
-        settle(o);
-#pragma unroll
-        for (int d = 0; d < kPv; ++d) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float x = o[d][i], y;
-            asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %1, %2\n\tv_accvgpr_write_b32 %0, %1"
-                         : "+a"(x), "=&v"(y)
-                         : "v"(alpha));
-            o[d][i] = x;
-          }
+        for (int i = 0; i < 16; ++i) {
+          const int key = 8 * (i / 4) + i % 4;
+          const float y = __uint_as_float(nan >> key & 1 ? quiet : __float_as_uint(sc[i]));
+          sc[i] = bits >> key & 1 ? y : -__builtin_inff();
         }
       }
-    }
-    u32x4 pf[2];
-    float sum[4] = {};
+      x.top = sc[0];
 #pragma unroll
-    for (int i = 0; i < 16; i += 2) {
-      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], p.scale_log2, -m));
-      const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i + 1], p.scale_log2, -m));
-      sum[i / 2 % 2 * 2] += x, sum[i / 2 % 2 * 2 + 1] += y;
-      pf[i / 8][i % 8 / 2] = pack2<BF16>(x, y);
-    }
-    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    ready(pf);
-    const auto pv_step = [&]<int I>(auto self) {
-      if constexpr (I < 2 * kPv) {
-        // Block d of the sums, 16 of the keys at a time: fragment kQk + I.
-        u32x4& v = f[(kQk + I) % kDepth];
-        if constexpr (TAIL) {
-          v &= keep[I / kPv];
-          asm volatile("s_nop 1" : "+v"(v));
-        }
-        product<BF16>(o[I % kPv], v, pf[I / kPv]);
-        __builtin_amdgcn_sched_barrier(0);
-        if constexpr (I + kDepth < 2 * kPv) v = v_at(I + kDepth);
-        slot.template operator()<kQk + I>();
-        self.template operator()<I + 1>(self);
+      for (int i = 1; i < 8; ++i) x.top = __builtin_fmaxf(x.top, sc[i]);
+    } else if constexpr (N == 1) {
+#pragma unroll
+      for (int i = 8; i < 16; ++i) x.top = __builtin_fmaxf(x.top, sc[i]);
+      x.top = xhalf(x.top, [](float a, float b) { return __builtin_fmaxf(a, b); }) * p.scale_log2;
+    } else if constexpr (N == 2) {
+      const bool up = x.top - m > kLazyThreshold;
+      factor = 1.f, moves = false;
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(up) != 0, 0)) {
+        const float m_new = up ? x.top : m;
+        factor = __builtin_amdgcn_exp2f(m - m_new);
+        // A row's first tile moves its maximum, but not its sums, which are zeros.
+        moves = __builtin_amdgcn_ballot_w64(up && m >= kNone * 0.5f) != 0;
+        m = m_new;
+        l *= factor;
       }
-    };
-    pv_step.template operator()<0>(pv_step);
+    } else if constexpr (N < 19) {
+      // Weight N - 3, and what follows from those before it.
+      constexpr int E = N - 3;
+      sc[E] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[E], p.scale_log2, -m));
+      if constexpr (E > 0) x.sum[(E - 1) % 2] += sc[E - 1];
+      if constexpr (E > 1 && E % 2 == 0) weight[(E - 2) / 8][(E - 2) % 8 / 2] = pack2<BF16>(sc[E - 2], sc[E - 1]);
+    } else {
+      weight[1][3] = pack2<BF16>(sc[14], sc[15]);
+      l += x.sum[0] + (x.sum[1] + sc[15]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
+  // The weights to LDS behind a barrier (every wave has read the last tile's), with the
+  // factors of the rows whose maximum moved.
+  G9_DEV void publish() {
+    barrier();
+    if (wave < RB) {
+      const int lane = lane_here();
+      G9_LDS u32x4* const to = (G9_LDS u32x4*)(uintptr_t)(lds + kP + 2048 * wave + 16 * lane);
+      to[0] = weight[0], to[64] = weight[1];
+      *(G9_LDS float*)(uintptr_t)(lds + kFactors + 128 * wave + 4 * (lane & 31)) = factor;
+      *(G9_LDS u32*)(uintptr_t)(lds + kMoved + 4 * wave) = moves;
+    }
+    waitcnt<63, 0>();
+  }
+
+  // Whether a row's maximum moved with the last weights.
+  G9_DEV bool moved() const {
+    const u32x4 x = *(const G9_LDS u32x4*)(uintptr_t)(lds + kMoved);
+    const u32 any = RB == 1 ? x.x : RB == 2 ? x.x | x.y : x.x | x.y | x.z | x.w;
+    return __builtin_amdgcn_readfirstlane((int)any) != 0;
+  }
+  // Then all rows' sums are multiplied by their factors before the weights join them.
+  G9_DEV void rescale() {
+    const u32 at = lds + kFactors + 4 * (lane_here() & 31);
+    settle();
+    each<RB>([&]<int R>() {
+      const float factor = *(const G9_LDS float*)(uintptr_t)(at + 128 * R);
+      each<kPv>([&]<int D>() { each<16>([&]<int E>() { Block<R * kPv + D>::template multiply<E>(factor); }); });
+    });
+    asm volatile("s_nop 1");
   }
 
   // The keys of the tile that hold an infinite or NaN latent.  A weight of 0 would not
@@ -368,89 +481,41 @@ G9_DEV u32x2 scaled(f32x4 x, float inv) {
 G9_DEV bool nothing(float l) { return (__float_as_uint(l) << 1) == 0; }
 G9_DEV float lse_of(float m, float l) { return nothing(l) ? -__builtin_inff() : (m + __builtin_log2f(l)) * kLn2; }
 
-// A block's results, or its sums to slot `slot` of the workspace.  The groups' sums of the
-// same rows (over different keys) are joined in LDS, 256 of the 512 values at a time; every
-// wave takes a share of the values.  Branches of lanes are not nested: nothing may come
-// between the ends of two of them.
+// A block's results, or its sums to slot `slot` of the workspace: the rows' maxima and weights
+// go through LDS from the waves that have them.  Branches of lanes are not nested: nothing
+// may come between the ends of two of them.
 template <bool BF16, int RB, class L>
-G9_DEV void finish_block(const Params& p, const Place& at, int slot, char* smem, int wave, const Rows<BF16, RB>& w) {
-  constexpr int kGroups = 4 / RB, kPitch = 256 + 4, kSums = 32 * kPitch;  // 16 bytes more a row: banks
-  static_assert((4 * kSums + 4 * 64) * 4 <= kLds);
+G9_DEV void finish_block(const Params& p, const Place& at, int slot, Wave4<BF16, RB>& w) {
   const int lane = lane_here(), h = lane >> 5, col = lane & 31;
-  float* const sums = reinterpret_cast<float*>(smem);
-  float* const ml = sums + 4 * kSums;  // maximum and weight of wave w's row r: [w][2][32]
-  const int rb = wave % RB, row = at.block * L::kBlock + 32 * rb + col, node = w.row.node;
-  float m = w.m, l = xhalf(w.l, [](float x, float y) { return x + y; }), f[kGroups];
+  const float l = xhalf(w.l, [](float x, float y) { return x + y; });
   waitcnt<0, 15>();  // the DMAs behind the last step
-  barrier();         // every wave has read its tiles
-  if constexpr (kGroups > 1) {
-    if (h == 0) ml[wave * 64 + col] = m, ml[wave * 64 + 32 + col] = l;
-    __syncthreads();
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) m = __builtin_fmaxf(m, ml[(g * RB + rb) * 64 + col]);
-    l = 0.f;
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      f[g] = __builtin_amdgcn_exp2f(ml[(g * RB + rb) * 64 + col] - m);
-      l += f[g] * ml[(g * RB + rb) * 64 + 32 + col];
-    }
-  }
-  const float inv = nothing(l) ? 0.f : 1.f / l;
-  const Out out = out_of(p, at.r.q0, row, max(node, 0));
-  const auto put = [&](int q, f32x4 x) {
-    if (slot >= 0)
-      *reinterpret_cast<f32x4*>(p.part + part_at<RB>(slot, rb, q) + 4 * lane) = x;
-    else if (node >= 0)
-      *reinterpret_cast<u32x2*>(out.o + 16 * q + 8 * h) = scaled<BF16>(x, inv);
-  };
-  const auto quad = [&](int q) {
-    const f32x16& x = w.o[q / 4];
-    const int r = 4 * (q % 4);
-    return f32x4{sum_of(x, r), sum_of(x, r + 1), sum_of(x, r + 2), sum_of(x, r + 3)};
-  };
-  if constexpr (kGroups == 1) {
+  if (h == 0) *reinterpret_cast<f32x2*>(w.smem + kMl + 256 * w.wave + 8 * col) = f32x2{w.m, l};
+  __syncthreads();  // and every wave has read its tiles
+  settle();
+  each<RB>([&]<int R>() {
+    const f32x2 ml = *reinterpret_cast<const f32x2*>(w.smem + kMl + 256 * R + 8 * col);
+    // Values 8 I + 4 h .. of this wave's 128.
+    const auto quad = [&]<int I>() {
+      using B = Block<R * kPv + I / 4>;
+      constexpr int kFirst = 4 * (I % 4);
+      return f32x4{B::template value<kFirst>(), B::template value<kFirst + 1>(), B::template value<kFirst + 2>(),
+                   B::template value<kFirst + 3>()};
+    };
     if (slot >= 0) {
-#pragma unroll
-      for (int q = 0; q < 64; ++q) {
-        put(q, quad(q));
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      float* const to = p.part + part_at<RB>(slot, R, 16 * w.wave) + 4 * lane;
+      each<16>([&]<int I>() { *reinterpret_cast<f32x4*>(to + 256 * I) = quad.template operator()<I>(); });
+      if (w.wave == R && h == 0) *reinterpret_cast<f32x2*>(p.part + ml_at<RB>(slot, 32 * R + col)) = ml;
     } else {
-#pragma unroll
-      for (int q = 0; q < 64; ++q) {
-        put(q, quad(q));
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      const int row = at.block * L::kBlock + 32 * R + col, node = row_of<L>(p, at, 32 * R + col).node;
+      const Out out = out_of(p, at.r.q0, row, max(node, 0));
+      const float inv = nothing(ml.y) ? 0.f : 1.f / ml.y;
+      if (node >= 0)
+        each<16>([&]<int I>() {
+          *reinterpret_cast<u32x2*>(out.o + 256 * w.wave + 16 * I + 8 * h) = scaled<BF16>(quad.template operator()<I>(), inv);
+        });
+      if (w.wave == R && h == 0 && node >= 0 && out.lse) *out.lse = lse_of(ml.x, ml.y);
     }
-  } else {
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if (half) __syncthreads();
-#pragma unroll
-      for (int q = 0; q < 32; ++q) {
-        *reinterpret_cast<f32x4*>(sums + wave * kSums + col * kPitch + 8 * q + 4 * h) = quad(32 * half + q);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      __syncthreads();
-#pragma unroll 4
-      for (int i = 0; i < 32 / kGroups; ++i) {
-        const int q = wave / RB * (32 / kGroups) + i;
-        f32x4 x = {};
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g)
-          x += f[g] * *reinterpret_cast<const f32x4*>(sums + (g * RB + rb) * kSums + col * kPitch + 8 * q + 4 * h);
-        put(32 * half + q, x);
-      }
-    }
-    __syncthreads();  // the next block's tiles take the sums' place
-  }
-  if (wave / RB == 0) {
-    if (slot >= 0) {
-      if (h == 0) *reinterpret_cast<f32x2*>(p.part + ml_at<RB>(slot, 32 * rb + col)) = f32x2{m, l};
-    } else {
-      if (h == 0 && node >= 0 && out.lse) *out.lse = lse_of(m, l);
-    }
-  }
+  });
 }
 
 // Joins the blocks that are cut.  A block of n parts has the n - 1 workers whose parts
@@ -579,88 +644,75 @@ G9_DEV void join_parts(const Params& p, float* lds) {
 template <bool BF16, int RB>
 G9_DEV void fwd(const Params& p, char* smem) {
   using L = Steps<RB>;
-  using R = Rows<BF16, RB>;
-  constexpr int kAhead = RB - 1;  // steps asked for ahead: the stages of a group but one
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int group = wave / RB;
+  using W = Wave4<BF16, RB>;
   const unsigned worker = my_part();
   Place cur{};
   int left = L::template locate<256>(p, smem, worker, cur);
-  R w(p);
-  w.init(smem, wave);
+  W w(p);
+  w.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  w.init(smem);
   while (left > 0) {
     const int seg = min(left, cur.r.tiles - cur.tile);
     const bool last = cur.tile + seg == cur.r.tiles, from_start = cur.tile == 0;
-    const int first = cur.tile * L::kKeys + group * kKeys;  // this wave's first key
-    const int in_block = 32 * (wave % RB) + (lane_here() & 31);
-    w.row = row_of<L>(p, cur, in_block);
+    const int first = cur.tile * kKeys;  // the part's first key
+    const int in_block = 32 * w.wave + (lane_here() & 31);
+    // This wave has rows.  One that has none (with RB 1 and 2 some never do) forms the first
+    // row's weights all the same, and no one reads them: the others take as long.
+    const bool some = w.wave < RB && cur.block * L::kBlock + 32 * w.wave < cur.r.n * p.group;
+    w.row = row_of<L>(p, cur, some ? in_block : 0);
     w.keys = cur.r.keys;
+    w.whole = min(cur.r.context, cur.r.keys);
     // The pages of 32 steps' tiles, two 16-row pieces each, are held in the lanes: a load in
     // every step would be waited for in it, as scalar loads are behind the next LDS read.
     const int* const table = p.table + cur.b * p.table_stride;
     int held;
     const auto hold = [&](int step) {
-      const int lane = lane_here(), k = first + (step + (lane >> 1)) * L::kKeys + 16 * (lane & 1);
+      const int lane = lane_here(), k = first + (step + (lane >> 1)) * kKeys + 16 * (lane & 1);
       held = k < cur.r.keys ? table[k >> p.shift] : -1;
       waitcnt<0, 15>();
     };
-    // Piece i of a step's tile of this wave's group.
-    const auto piece = [&](int i, int step) {
-      return w.aim(i, group * RB + step % RB, first + step * L::kKeys, step < seg ? cur.r.keys : 0,
-                   __builtin_amdgcn_readlane(held, 2 * (step & 31) + i));
-    };
-    const int mine = RB == 4 ? wave >> 1 : wave & 1;
-    const auto ask = [&](int step) {
-      if constexpr (RB == 1) {
-        w.fetch_all(piece(0, step), wave);
-        w.fetch_all(piece(1, step), wave);
-      } else {
-        w.fetch_all(piece(mine, step), wave);
-      }
+    const auto rows_of = [&](int step) {
+      return w.aim(step & 3, first + step * kKeys, step < seg ? cur.r.keys : 0,
+                   __builtin_amdgcn_readlane(held, 2 * (step & 31) + (w.wave >> 1)));
     };
     hold(0);
-    ask(0);
-    w.load_q(query_of<L>(p, cur, in_block, w.row.node));
-    waitcnt<0, 0>();  // here: a wait of the compiler's for the queries would be one in every step
-#pragma unroll
-    for (int i = 1; i < kAhead; ++i) ask(i);
+    w.fetch_all(rows_of(0));
+    w.load_q(query_of<L>(p, cur, some ? in_block : 0, w.row.node));
     w.clear();
-    // Rows of this wave, tiles that none of them reads.
-    const bool some = cur.block * L::kBlock + 32 * (wave % RB) < cur.r.n * p.group;
-    const int whole = min(cur.r.context, cur.r.keys);  // keys that every row reads
-    const auto steps = [&]<bool TAIL>(int from, int to) {
-#pragma unroll 1
-      for (int j = from; j < to; ++j) {
-        // The step's tile has landed, for every wave that shares it (a wave of RB 1 has its own).
-        waitcnt<(RB == 4 ? 2 * R::kOwn : 0), 15>();
-        typename R::Piece next;
-        if constexpr (RB > 1) {
-          barrier();
-          if (((j + kAhead) & 31) == 0) hold(j + kAhead);
-          next = piece(mine, j + kAhead);
-        } else {
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        const int k0 = first + j * L::kKeys;
-        if (some)
-          w.template tile<TAIL>(k0, group * RB + j % RB, next, wave);
-        else if constexpr (RB > 1)
-          w.fetch_all(next, wave);
-        if constexpr (RB == 1) {
-          waitcnt<63, 0>();
-          __builtin_amdgcn_sched_barrier(0);
-          if (((j + 1) & 31) == 0) hold(j + 1);
-          if (j + 1 < seg) ask(j + 1);
-        }
-      }
+    waitcnt<0, 0>();  // here: a wait of the compiler's for the queries would be one in every step
+    w.fetch_all(rows_of(1));
+    barrier();  // tile 0 has landed
+    w.template products<true, false, true>(first, 0, 0, rows_of(2));
+    w.publish();
+    waitcnt<9, 15>();
+    barrier();  // tile 1 has landed, P and the factors are there
+    // Step j: the values of tile j, the scores and weights of tile j + 1.
+    const auto step = [&]<bool TAIL>(int j) {
+      if (((j + kAhead) & 31) == 0) hold(j + kAhead);
+      w.template products<true, true, TAIL>(first + (j + 1) * kKeys, (j + 1) & 3, j & 3, rows_of(j + kAhead));
+      w.publish();
+      waitcnt<9, 15>();
+      barrier();  // tile j + 2 has landed, P and the factors are there
     };
-    // The steps whose tiles every row reads whole, then the others.
-    const int mid = min(max((whole - cur.tile * L::kKeys) / L::kKeys, 0), seg);
-    steps.template operator()<false>(0, mid);
-    steps.template operator()<true>(mid, seg);
-    settle(w.o);
+    // The steps of tiles that every row reads whole, then the others; the last tile's values.
+    // The loops are left to multiply the sums: in them, that code would cost registers.
+    const int mid = min((w.whole - first) / kKeys - 1, seg - 1);
+    int j = 0;
+    for (;;) {
+      if (__builtin_expect(w.moved(), 0)) w.rescale();
+      if (j < mid) {
+        do step.template operator()<false>(j++);
+        while (j < mid && !w.moved());
+      } else if (j < seg - 1) {
+        step.template operator()<true>(j++);
+      } else {
+        break;
+      }
+    }
+    w.template products<false, true, true>(0, 0, j & 3, rows_of(j + kAhead));
     const int slot = last && from_start ? -1 : (int)(2 * worker + (from_start ? 1 : 0));
-    finish_block<BF16, RB, L>(p, cur, slot, smem, wave, w);
+    finish_block<BF16, RB, L>(p, cur, slot, w);
+    __syncthreads();  // the maxima and weights are read
     left -= seg + L::kLead;
     if (left > 0) cur = L::next_block(p, cur);
   }
@@ -692,7 +744,10 @@ G9_LATENT_KERNEL(f16_q128, false, 4)
 namespace {
 
 // Query rows of a block, by the rows (nodes by heads) that a request of the batch
-// brings on average.
+// brings on average: the fewest that hold them, and 128 above (us with 32, 64 and 128 rows; 64
+// requests of 100 to 8192 tokens, cache cold, by 16 heads 123, 125, 133, 32: 136, 139, 142,
+// 40: 167, 142, 148, 64: 167, 143, 153, 80: 222, 188, 159, 128: 200, 149, 144; 16 requests of
+// 12 nodes by 16 heads 102, 79, 72; but one of 30000 tokens by 128 heads 44, 44, 56).
 enum { Q32, Q64, Q128 };
 int form_of(int64_t B, int64_t T, int64_t H) {
   const int64_t rows = (T + B - 1) / B * H;

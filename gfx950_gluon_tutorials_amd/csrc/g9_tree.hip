@@ -51,6 +51,45 @@ struct Params {
   G9_DEV unsigned long long reads(const Row& r, int k0, int keys) const { return node_reads(*this, r, k0, keys); }
 };
 
+// The row's results, or its sum to slot `slot` of the workspace.  o, m, l as the
+// 32x32 layout leaves them: lane half h has the values 8 r + 4 h + 0..3 of every
+// 32, l is its half of the weight.
+template <bool BF16, int HD, class L>
+G9_DEV void finish(const Params& p, const Place& at, int slot, int row, int node, const f32x16 (&o)[HD / 32], float m,
+                   float l) {
+  const int h = (threadIdx.x & 63) >> 5;
+  const float lt = xhalf(l, [](float x, float y) { return x + y; });
+  if (node < 0) return;
+  if (slot >= 0) {
+    float* const sum = p.part + ((size_t)slot * L::kBlock + row) * HD;
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *reinterpret_cast<f32x4*>(sum + 32 * d + 8 * r + 4 * h) =
+            f32x4{o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]};
+    if (h == 0) {
+      float* const ml = p.part + (size_t)2 * L::kWorkers * L::kBlock * HD + ((size_t)slot * L::kBlock + row) * 2;
+      ml[0] = m, ml[1] = lt;
+    }
+    return;
+  }
+  const int hq = at.hk * p.group + at.block * L::kBlock + row - node * p.group;
+  const long long tok = at.r.q0 + node;
+  // By its bits: comparisons here may take NaN for a number.
+  const bool none = (__float_as_uint(lt) << 1) == 0;
+  const float inv = none ? 0.f : 1.f / lt;
+  char* const orow = p.o + tok * p.o_t + hq * p.o_h;
+#pragma unroll
+  for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      *reinterpret_cast<u32x2*>(orow + (32 * d + 8 * r + 4 * h) * 2) =
+          u32x2{pack2<BF16>(o[d][4 * r] * inv, o[d][4 * r + 1] * inv),
+                pack2<BF16>(o[d][4 * r + 2] * inv, o[d][4 * r + 3] * inv)};
+  if (p.lse && h == 0) p.lse[(long long)hq * p.T + tok] = none ? -__builtin_inff() : (m + __builtin_log2f(lt)) * kLn2;
+}
+
 // A wave's own tiles of up to 8 KB, or a workgroup's of 16 KB.  A block costs a
 // wave nothing beside its tiles that shows (1 to 3 places: 0 to 5% slower); a
 // workgroup it costs as much as 384 keys (us, blocks of 256 rows of head dim 128,
@@ -277,6 +316,106 @@ G9_DEV void wide(const Params& p, char* smem) {
     left -= seg + L::kLead;
     if (left > 0) cur = L::next_block(pe, cur);
     barrier();  // the stages are read: the next block's tiles take them
+  }
+}
+
+// The joined row: with m the largest of the parts' maxima, the sum of 2^(m_i - m)
+// O_i over the sum of 2^(m_i - m) l_i, in the order of the keys.
+template <bool BF16>
+G9_DEV void store4(const Params& p, long long tok, int hq, int c, f32x4 sum, float m, float l) {
+  const bool none = (__float_as_uint(l) << 1) == 0;
+  const float inv = none ? 0.f : 1.f / l;
+  *reinterpret_cast<u32x2*>(p.o + tok * p.o_t + hq * p.o_h + c * 8) =
+      u32x2{pack2<BF16>(sum[0] * inv, sum[1] * inv), pack2<BF16>(sum[2] * inv, sum[3] * inv)};
+  if (p.lse && c == 0) p.lse[(long long)hq * p.T + tok] = none ? -__builtin_inff() : (m + __builtin_log2f(l)) * kLn2;
+}
+
+// Joins the blocks that are cut.  A block of n parts has the n - 1 workers whose
+// parts begin within it, and with each of them a workgroup here (blockIdx.x + 1):
+// they (and gridDim.y times as many) share its rows, so that a workgroup's work
+// is a fraction of a part, however many parts a long request's blocks have.
+template <int HD>
+constexpr int kJoinThreads = 4 * HD;
+template <bool BF16, int HD, class L>
+G9_DEV void join(const Params& p, float* lds) {
+  const unsigned w = blockIdx.x + 1;
+  const Start zero = p.start[0];
+  const unsigned long long total = (unsigned long long)zero.total_hi << 32 | zero.total_lo;
+  const Start st = p.start[w];  // asked for together with worker 0's
+  if (w >= L::workers(total) || st.tile == 0) return;
+  const unsigned long long u0 = L::part_begin(w, total) - (unsigned)st.tile;
+  const unsigned w0 = L::worker_of(u0, total), n = L::worker_of(u0 + st.tiles - 1, total) - w0 + 1;
+  // Worker w0, in whose part the block begins, has it in slot 1, the others in slot 0.
+  const size_t head = (size_t)2 * w0 + 1;
+  const float* const ml = p.part + (size_t)2 * L::kWorkers * L::kBlock * HD;
+  const int row0 = st.block * L::kBlock;
+  const u32 rows = (u32)min((long long)st.n * p.group - row0, (long long)L::kBlock);
+  const u32 share = (w - w0 - 1) * gridDim.y + blockIdx.y, shares = (n - 1) * gridDim.y;
+  const u32 from = share * rows / shares, to = (share + 1) * rows / shares;
+  constexpr unsigned kCols = HD / 4, kLanes = kJoinThreads<HD> / kCols;
+  const unsigned c = threadIdx.x % kCols, lane = threadIdx.x / kCols;
+  f32x4 sum;
+  float m, l;
+  const auto clear = [&] { sum = f32x4{}, m = -3.0e38f, l = 0.f; };
+  const auto add = [&](f32x4 x, float mk, float lk) {
+    const float m_new = __builtin_fmaxf(m, mk);
+    const float f = __builtin_amdgcn_exp2f(m - m_new), g = __builtin_amdgcn_exp2f(mk - m_new);
+    l = l * f + lk * g;
+    sum = sum * f + x * g;
+    m = m_new;
+  };
+  // Adds the row's parts k0, k0 + step, ..., kAtOnce of them asked for together.
+  const auto add_parts = [&]<unsigned kAtOnce>(unsigned in, unsigned k0, unsigned step) {
+    for (unsigned k = k0; k < n; k += kAtOnce * step) {
+      float mk[kAtOnce], lk[kAtOnce];
+      f32x4 x[kAtOnce];
+#pragma unroll
+      for (unsigned e = 0; e < kAtOnce; ++e) {
+        const unsigned i = min(k + e * step, n - 1);
+        const size_t a = (i ? (size_t)2 * (w0 + i) : head) * L::kBlock + in;
+        mk[e] = ml[a * 2], lk[e] = ml[a * 2 + 1];
+        x[e] = *reinterpret_cast<const f32x4*>(p.part + a * HD + 4 * c);
+      }
+#pragma unroll
+      for (unsigned e = 0; e < kAtOnce; ++e)
+        if (k + e * step < n) add(x[e], mk[e], lk[e]);
+    }
+  };
+  const auto store = [&](unsigned in) {
+    const int row = row0 + (int)in, nd = row / p.group;
+    store4<BF16>(p, st.q0 + nd, st.hk * p.group + row - nd * p.group, c, sum, m, l);
+  };
+  // Round trips to memory: a row per 16-byte column group of threads, its parts
+  // eight at a time, or the threads sharing a row's parts, and the row's join in
+  // LDS behind them.
+  const u32 r = to - from;
+  if ((r + kLanes - 1) / kLanes * ((n + 7) / 8) <= 2 * r) {
+    for (unsigned in = from + lane; in < to; in += kLanes) {
+      clear();
+      if (n <= 3)
+        add_parts.template operator()<3>(in, 0, 1);
+      else
+        add_parts.template operator()<8>(in, 0, 1);
+      store(in);
+    }
+    return;
+  }
+  for (unsigned in = from; in < to; ++in) {
+    clear();
+    add_parts.template operator()<8>(in, lane, kLanes);
+    float* const mine = lds + threadIdx.x * 7;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) mine[e] = sum[e];
+    mine[4] = m, mine[5] = l;
+    __syncthreads();
+    if (lane == 0) {
+      for (unsigned i = 1; i < kLanes; ++i) {
+        const float* const o = lds + (i * kCols + c) * 7;
+        add(f32x4{o[0], o[1], o[2], o[3]}, o[4], o[5]);
+      }
+      store(in);
+    }
+    __syncthreads();
   }
 }
 

@@ -351,6 +351,36 @@ def check_text(asm: str) -> list[str]:
     return violations
 
 
+def check_accumulators(asm: str) -> list[str]:
+    """For kernels that keep sums in accumulation registers of their own naming: in a
+    function whose assembly statements name any, no instruction of the compiler's may."""
+    violations = []
+    name, own, found, inside = None, False, [], False
+
+    def close():
+        if own:
+            violations.extend(f"{name}: the compiler's own use of an accumulation register: {t}" for t in found)
+
+    for raw in asm.split("\n"):
+        m = re.match(r"^([A-Za-z_]\w*):", raw)
+        if m:
+            close()
+            name, own, found, inside = m.group(1), False, [], False
+        elif "#ASMSTART" in raw:
+            inside = True
+        elif "#ASMEND" in raw:
+            inside = False
+        elif name and not raw.lstrip().startswith((".", ";")):
+            text = raw.split(";")[0].strip()
+            if _regs(text, "a"):
+                if inside:
+                    own = True
+                else:
+                    found.append(text)
+    close()
+    return violations
+
+
 def resource_table(asm: str) -> list[dict]:
     """Per-kernel register, scratch and LDS use from the code-object metadata
     of an assembly listing (the figures the reference reads from its own

@@ -58,3 +58,13 @@ def test_unrelated_registers_and_comments_are_ignored():
     text = _fn(MFMA32 + "\tv_accvgpr_read_b32 v20, a16 ; reads a16, not a0..a15\n"
                "\t;;#ASMSTART\n\t;;#ASMEND\n\tv_add_u32_e32 v40, 0xa3, v41\n")
     assert isa_check.check_text(text) == []
+
+
+def test_accumulators_of_assembly_are_left_alone():
+    own = "\t;;#ASMSTART\n\tv_mfma_f32_32x32x16_f16 a[0:15], v[0:3], v[4:7], a[0:15]\n\t;;#ASMEND\n"
+    spill = "\tv_accvgpr_write_b32 a7, v9\n"
+    assert isa_check.check_accumulators(_fn(own)) == []
+    assert isa_check.check_accumulators(_fn(spill)) == []  # a kernel without such sums
+    assert len(isa_check.check_accumulators(_fn(own + spill))) == 1
+    assert len(isa_check.check_accumulators(_fn(spill + own) + _fn(own))) == 1
+    assert isa_check.check_accumulators(_fn(own + "\tv_mov_b32 v3, v9 ; not a7\n") + _fn(spill)) == []

@@ -163,6 +163,20 @@ def test_paged_long_contexts(gpu, H, context):
     _check_paged(gpu, "bf16", _paged(gpu, "bf16", context, [1] * len(context), H, 64, H))
 
 
+@pytest.mark.parametrize("H", [16, 64, 128])
+def test_paged_long_parts(gpu, H):
+    """A workgroup's part of more than the 32 tiles whose pages it holds at once.  The
+    requests share their pages."""
+    B, n = 24, 14000
+    a = _paged(gpu, "bf16", [n], [1], H, 64, H)
+    g = torch.Generator().manual_seed(H)
+    a["q"] = (torch.randn(B, H, 576, generator=g) * 0.6).to(torch.bfloat16).to(gpu)
+    a["table"] = np.repeat(a["table"], B, 0)
+    a["context"] = [n - 7 * b for b in range(B)]
+    a["cu"] = _cu([1] * B)
+    _check_paged(gpu, "bf16", a)
+
+
 @pytest.mark.parametrize("qscale", [0.0, 1e-3, 6.0, 40.0])
 @pytest.mark.parametrize("H", [16, 128])
 def test_paged_score_ranges(gpu, qscale, H):
