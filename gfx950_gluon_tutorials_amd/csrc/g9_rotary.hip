@@ -57,7 +57,8 @@ struct RotaryParams {
 };
 
 // A thread has one place within the rows: 16 values that turn (eight pairs), or 8
-// that are copied.  Its angles serve every head of its token that it takes.
+// that are copied.  Its angles serve every head of its token that it takes.  Bound by HBM:
+// 16384 rows of 40 heads of 128 67 us (4.9 TB/s, the rate of a large copy); 64 rows 3.8.
 template <bool BF16, bool INTERLEAVED>
 G9_DEV void rotary(const RotaryParams& p) {
   for (long long u = (long long)blockIdx.x * 256 + threadIdx.x; u < p.units; u += (long long)gridDim.x * 256) {
@@ -118,7 +119,8 @@ struct LatentWriteParams {
 };
 
 // A wave per token: 8 of the latent's 512 values a lane, their squares' sum in fp32
-// across the wave; of the 32 pairs of the key one a lane.
+// across the wave; of the 32 pairs of the key one a lane.  Bound by HBM: 16384 tokens, with
+// c_out and k_out, 12.1-12.8 us (4.5 TB/s); 64 tokens 3.3.
 template <bool BF16, bool INTERLEAVED>
 G9_DEV void write_latent(const LatentWriteParams& p) {
   const int lane = threadIdx.x & 63;

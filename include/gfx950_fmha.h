@@ -203,7 +203,8 @@ int g9_write_latent(const void* c, const void* k_rope, void* cache, const int64_
  * then its rotated part, o (T x H x 512) the weighted latents, which the caller
  * multiplies by the heads' value projections.  score = sm_scale * q . row; requests,
  * nodes, masks and workspace (g9_latent_workspace_size bytes) as in g9_tree_fwd.
- * The cache's tokens at least 576 elements apart.
+ * The cache's tokens at least 576 elements apart.  A row that reads an infinite or NaN
+ * latent gets NaN in all or some of its values; rows that do not read it are as without it.
  */
 int g9_latent_fwd(const void* q, const void* cache, void* o, float* lse, const int32_t* block_table,
                   int64_t table_stride, int64_t width, const int32_t* lengths, const int32_t* cu_q,
