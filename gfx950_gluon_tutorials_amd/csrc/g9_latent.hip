@@ -26,11 +26,11 @@
 // factor goes through LDS, too.
 //
 // Measured (us, kernel and join, inputs partly in the last-level cache): 64 requests of 100 to
-// 8192 tokens by 16 heads 32 + 8: 1.5 a tile, 6.1 TB/s over the loop, but 14 of the 32 go to
-// finding the part, the first loads and the sums' way out; by 128 heads 48 + 18, 2.1 a tile
+// 8192 tokens by 16 heads 32 + 7: 1.5 a tile, 6.1 TB/s over the loop, but 14 of the 32 go to
+// finding the part, the first loads and the sums' way out; by 128 heads 47 + 16, 2.1 a tile
 // (68 MFMAs of 32 cycles are 1.2 at the clock that they leave), 25 outside the loop, much of
 // them and of the join for the 256 KB of sums of a part; 16 trees of 12 nodes by 32 heads
-// 79 + 19; one request of 700 tokens by 16 heads 10 + 6.
+// 78 + 15; one request of 700 tokens by 16 heads 10 + 4.
 #include "../../include/gfx950_fmha.h"
 #include <utility>
 
@@ -548,36 +548,33 @@ G9_DEV void join_parts(const Params& p, float* lds) {
     *reinterpret_cast<u32x2*>(out.o + 16 * q + 8 * h) = scaled<BF16>(x, nothing(l) ? 0.f : 1.f / l);
     if (q == 0 && h == 0 && out.lse) *out.lse = lse_of(m, l);
   };
-  // The sums of U units from u on over the parts k0, k0 + step, ..: first their largest
-  // maximum, then the sums, 16 loads asked for together.
+  // The sums of U units from u on over the parts k0, k0 + step, .., 16 loads and their maxima
+  // and weights asked for together, and what they find scaled to the largest maximum so far.
   const auto sum_parts = [&]<int U>(int u, unsigned k0, unsigned step, f32x4 (&sum)[U], float& m, float& l) {
     constexpr unsigned kAtOnce = 16 / U;
     const int rb = u >> 6, q = u & 63, in = 32 * rb + (lane & 31);
-    const auto ml = [&](unsigned k) {
-      return *reinterpret_cast<const f32x2*>(p.part + ml_at<RB>(slot_of(min(k, n - 1)), in));
-    };
     m = kNone, l = 0.f;
 #pragma unroll
     for (int i = 0; i < U; ++i) sum[i] = f32x4{};
-    for (unsigned k = k0; k < n; k += 8 * step) {
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = ml(k + e * step).x;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (k + e * step < n) m = __builtin_fmaxf(m, x[e]);
-    }
     for (unsigned k = k0; k < n; k += kAtOnce * step) {
       f32x4 x[kAtOnce][U];
       f32x2 v[kAtOnce];
 #pragma unroll
       for (unsigned e = 0; e < kAtOnce; ++e) {
-        const unsigned i = min(k + e * step, n - 1);
-        v[e] = ml(i);
-        const f32x4* const at = reinterpret_cast<const f32x4*>(p.part + part_at<RB>(slot_of(i), rb, q) + 4 * lane);
+        const size_t slot = slot_of(min(k + e * step, n - 1));
+        v[e] = *reinterpret_cast<const f32x2*>(p.part + ml_at<RB>(slot, in));
+        const f32x4* const at = reinterpret_cast<const f32x4*>(p.part + part_at<RB>(slot, rb, q) + 4 * lane);
 #pragma unroll
         for (int j = 0; j < U; ++j) x[e][j] = at[64 * j];
       }
+      float top = m;
+#pragma unroll
+      for (unsigned e = 0; e < kAtOnce; ++e)
+        if (k + e * step < n) top = __builtin_fmaxf(top, v[e].x);
+      const float g = __builtin_amdgcn_exp2f(m - top);
+      m = top, l *= g;
+#pragma unroll
+      for (int j = 0; j < U; ++j) sum[j] *= g;
 #pragma unroll
       for (unsigned e = 0; e < kAtOnce; ++e) {
         if (k + e * step >= n) break;
@@ -600,9 +597,9 @@ G9_DEV void join_parts(const Params& p, float* lds) {
       }
     };
     if (n <= 4)
-      run.template operator()<8>();
-    else
       run.template operator()<4>();
+    else
+      run.template operator()<2>();
     return;
   }
   const auto run = [&]<int U>() {
@@ -665,19 +662,19 @@ G9_DEV void fwd(const Params& p, char* smem) {
     // The pages of 32 steps' tiles, two 16-row pieces each, are held in the lanes: a load in
     // every step would be waited for in it, as scalar loads are behind the next LDS read.
     const int* const table = p.table + cur.b * p.table_stride;
-    int held;
-    const auto hold = [&](int step) {
+    const auto pages = [&](int step) {
       const int lane = lane_here(), k = first + (step + (lane >> 1)) * kKeys + 16 * (lane & 1);
-      held = k < cur.r.keys ? table[k >> p.shift] : -1;
-      waitcnt<0, 15>();
+      return k < cur.r.keys ? table[k >> p.shift] : -1;
     };
+    int held = pages(0);
+    __builtin_amdgcn_sched_barrier(0);  // the queries come behind the pages
     const auto rows_of = [&](int step) {
       return w.aim(step & 3, first + step * kKeys, step < seg ? cur.r.keys : 0,
                    __builtin_amdgcn_readlane(held, 2 * (step & 31) + (w.wave >> 1)));
     };
-    hold(0);
-    w.fetch_all(rows_of(0));
     w.load_q(query_of<L>(p, cur, some ? in_block : 0, w.row.node));
+    __builtin_amdgcn_sched_barrier(0);
+    w.fetch_all(rows_of(0));
     w.clear();
     waitcnt<0, 0>();  // here: a wait of the compiler's for the queries would be one in every step
     w.fetch_all(rows_of(1));
@@ -688,7 +685,10 @@ G9_DEV void fwd(const Params& p, char* smem) {
     barrier();  // tile 1 has landed, P and the factors are there
     // Step j: the values of tile j, the scores and weights of tile j + 1.
     const auto step = [&]<bool TAIL>(int j) {
-      if (((j + kAhead) & 31) == 0) hold(j + kAhead);
+      if (((j + kAhead) & 31) == 0) {
+        held = pages(j + kAhead);
+        waitcnt<0, 15>();
+      }
       w.template products<true, true, TAIL>(first + (j + 1) * kKeys, (j + 1) & 3, j & 3, rows_of(j + kAhead));
       w.publish();
       waitcnt<9, 15>();
@@ -753,6 +753,10 @@ int form_of(int64_t B, int64_t T, int64_t H) {
   const int64_t rows = (T + B - 1) / B * H;
   return rows <= 32 ? Q32 : rows <= 64 ? Q64 : Q128;
 }
+// Workgroups of the join for each worker: the more, the larger a part (us, the join alone: one
+// request by 16 heads with 1 and 2 4.4 and 5.6, 64 requests 6.8 and 6.5; by 128 heads with 2, 4
+// and 8 16.8, 15.6 and 14.2, trees 20, 15.3 and 15.8).
+constexpr unsigned join_shares(int form) { return 1u << form; }
 // The workspace: the sums of 2 x 256 blocks and their (m, l) pairs, then start[].
 size_t start_at(int form) { return (size_t)2 * fa::kWgs * (32 << form) * (512 + 2) * 4; }
 
@@ -819,6 +823,6 @@ extern "C" int g9_latent_fwd(const void* q, const void* cache, void* o, float* l
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int bf16 = dtype == G9_BF16;
   if (hipLaunchKernel(kRun[form][bf16], dim3(fa::kWgs), dim3(256), args, 0, st) != hipSuccess) return G9_ERR_HIP;
-  return launched(hipLaunchKernel(kJoin[form][bf16], dim3(fa::kWgs - 1, 2),
+  return launched(hipLaunchKernel(kJoin[form][bf16], dim3(fa::kWgs - 1, join_shares(form)),
                                   dim3(64 * latent::kJoinWaves), args, 0, st));
 }
