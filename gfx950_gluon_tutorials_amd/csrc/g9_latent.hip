@@ -52,7 +52,11 @@ constexpr int kAhead = 3;               // steps asked for ahead
 // LDS: the stages, P of up to 128 rows, factors of the rows, a word a wave that says
 // whether there are any, then the rows' maxima and weights at the end.
 constexpr int kP = 4 * kTile, kFactors = kP + 8192, kMoved = kFactors + 512, kMl = kMoved + 64, kLds = kMl + 1024;
-constexpr float kNone = -3.0e38f;       // the maximum of a row that has read nothing: finite, weights 0
+constexpr float kNone = -__FLT_MAX__;   // the maximum of a row that has read nothing: finite, weights 0
+// From here on (log2 units) a step of fp32 is 2 and more.  A weight's exponent is its score's exact
+// product with the scale less the rounded maximum: off by half such a step, and far from 0 for the
+// largest score itself.  Then the product is rounded as the maximum is.
+constexpr float kLarge = 16777216.f;
 
 struct Params {
   const char* q;
@@ -167,6 +171,9 @@ G9_DEV int lane_here() {
 // 5, 9, 12 places: 128 heads 70, 68.5, 66, trees 99, 97, 98; 16 heads with 5 and 7: 40.5, 41.5).
 template <int RB>
 using Steps = Line<Params, kKeys, 32 * RB, kWgs, RB == 4 ? 12 : RB == 2 ? 8 : 5>;
+
+// By its bits: comparisons here may take NaN for a number.
+G9_DEV bool nothing(float l) { return (__float_as_uint(l) << 1) == 0; }
 
 // One wave: rows 32 wave .. of the block for the scores, values 128 wave .. for the sums.
 template <bool BF16, int RB>
@@ -311,7 +318,7 @@ struct Wave4 {
     constexpr int kPieces = 20, kMix = SCORES && kV > kPieces + 2 ? kV - kPieces - 2 : 0;
     constexpr int kLast = kK + kMix - 1;  // the last score's product, at the latest
     constexpr int kSlots = kAll - kLast - 3, kEach = kSlots > 0 ? (kPieces + kSlots - 1) / kSlots : kPieces;
-    Soft<TAIL> soft{k0, kstage};
+    Soft<TAIL> soft{k0, kstage, p.scale_log2};
     const auto pieces = [&]<int FIRST, int N>() {
       each<N>([&]<int I>() {
         if constexpr (FIRST + I < kPieces) piece<TAIL, FIRST + I>(soft, sc);
@@ -345,6 +352,7 @@ struct Wave4 {
   template <bool TAIL>
   struct Soft {
     int k0, stage;
+    float scale;  // what is left of it to multiply the scores by
     u32 bad = 0;
     float top = 0.f, sum[2] = {0.f, 0.f};
   };
@@ -381,14 +389,19 @@ struct Wave4 {
         const float m_new = up ? x.top : m;
         factor = __builtin_amdgcn_exp2f(m - m_new);
         // A row's first tile moves its maximum, but not its sums, which are zeros.
-        moves = __builtin_amdgcn_ballot_w64(up && m >= kNone * 0.5f) != 0;
+        moves = __builtin_amdgcn_ballot_w64(up && (m > kNone || !nothing(l))) != 0;
         m = m_new;
         l *= factor;
+      }
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(__builtin_fabsf(m) >= kLarge) != 0, 0)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[i] *= p.scale_log2;
+        x.scale = 1.f;
       }
     } else if constexpr (N < 19) {
       // Weight N - 3, and what follows from those before it.
       constexpr int E = N - 3;
-      sc[E] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[E], p.scale_log2, -m));
+      sc[E] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[E], x.scale, -m));
       if constexpr (E > 0) x.sum[(E - 1) % 2] += sc[E - 1];
       if constexpr (E > 1 && E % 2 == 0) weight[(E - 2) / 8][(E - 2) % 8 / 2] = pack2<BF16>(sc[E - 2], sc[E - 1]);
     } else {
@@ -477,8 +490,6 @@ template <bool BF16>
 G9_DEV u32x2 scaled(f32x4 x, float inv) {
   return u32x2{pack2<BF16>(x[0] * inv, x[1] * inv), pack2<BF16>(x[2] * inv, x[3] * inv)};
 }
-// By its bits: comparisons here may take NaN for a number.
-G9_DEV bool nothing(float l) { return (__float_as_uint(l) << 1) == 0; }
 G9_DEV float lse_of(float m, float l) { return nothing(l) ? -__builtin_inff() : (m + __builtin_log2f(l)) * kLn2; }
 
 // A block's results, or its sums to slot `slot` of the workspace: the rows' maxima and weights

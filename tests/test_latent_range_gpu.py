@@ -1,0 +1,81 @@
+"""latent_attention over the whole range of finite scores, against the float64 oracle.
+
+The query has one value that is not zero, so a score is one exact product; keys come in
+levels, whose scores differ by far more than an exponential can tell from zero.  A row's
+result is then the mean of its highest level's latents, all of weight 2^0."""
+
+import numpy as np
+import pytest
+import torch
+
+from gfx950_gluon_tutorials_amd.attention import latent_attention
+from oracle import latent_ref as L
+
+pytestmark = pytest.mark.gpu
+
+DT = {"fp16": torch.float16, "bf16": torch.bfloat16}
+# Scores (natural log), one for each 32 keys of the beginning and one for the rest.  fp16: by
+# values up to 2^15 and a scale of 2^6.
+RISING = [-1.4e38, -1.1e38, -6e37, -1e30, 1e20, 1.5e38]
+LEVELS = {
+    "bf16": [[-1.4e38, 0.0], [-1.4e38], [-2.3e38], [2.3e38], [0.0, -1.4e38], RISING, RISING[::-1], [-2.2e38, -1.4e38],
+             [-3e9, 5e9, 4e9], [2.0**24, 2.0**25 + 2.0**20]],
+    "fp16": [[-2.0**34, -2.0**33 - 2.0**30], [2.0**28], [-2.0**29 - 2.0**22], [2.0**34, 2.0**33, 2.0**34 + 2.0**26]],
+}
+
+
+def _case(dev, dtype, levels, context, nodes, H, sign, size=16):
+    """Heads of which every second sees the scores negated, where `sign` is -1."""
+    g = torch.Generator().manual_seed(context + H)
+    a, scale = (2.0**60, 1.0) if dtype == "bf16" else (2.0**14, 2.0**6)
+    n = context + nodes
+    per_key = [levels[min(j // 32, len(levels) - 1)] / (a * scale) for j in range(n)]
+    rows = torch.randn(n, 576, generator=g).to(DT[dtype])
+    rows[:, 512] = torch.tensor(per_key, dtype=torch.float64).to(DT[dtype])
+    used = -(-n // size)
+    table = torch.randperm(used + 2, generator=g)[:used]
+    cache = torch.randn(used + 2, size, 576, generator=g).to(DT[dtype])
+    at = torch.arange(n)
+    cache[table[at // size], at % size] = rows
+    q = torch.zeros(nodes, H, 576, dtype=DT[dtype])
+    q[:, 0::2, 512] = a
+    q[:, 1::2, 512] = a * sign
+    assert q.isfinite().all() and cache.isfinite().all()
+    return q.to(dev), cache.to(dev), table[None].int().to(dev), scale
+
+
+def _check(dev, dtype, levels, context, nodes, H, sign):
+    q, cache, table, scale = _case(dev, dtype, levels, context, nodes, H, sign)
+    lse = torch.empty(H, nodes, device=dev)
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)
+    got = latent_attention(q, cache, table, i(context), i(0, nodes), sm_scale=scale, lse=lse)
+    torch.cuda.synchronize()
+    n = lambda t: t.double().cpu().numpy()
+    # The heads are of two kinds.
+    want, lse_want, mag, _ = L.paged(n(q)[:, :2], n(cache), table.cpu().numpy(), [context], [0, nodes], None, scale)
+    kind = np.arange(H) % 2
+    want, lse_want, mag = want[:, kind], lse_want[kind], mag[:, kind]
+    # Weights of 1 and 0 are exact.  Their sum over the keys is fp32, its quotient and two products
+    # are 2^-22 at most; then half a step.  lse: its maximum is a product with the scale by log2 e,
+    # itself rounded twice, a sum, and a product with ln 2, rounded too: seven times 2^-24 at most.
+    h = torch.finfo(DT[dtype]).eps / 2
+    tol = h * np.abs(want) * (1 + h) + ((context + nodes) * 2.0**-24 + 2.0**-22) * (1 + h) * mag
+    tol += 2.0**-25 if dtype == "fp16" else 0
+    off = np.abs(n(got) - want)
+    assert (off <= tol).all(), f"{(off - tol).max():.3g} past its bound, or not finite"
+    assert (np.abs(n(lse) - lse_want) <= 2.0**-21 * np.abs(lse_want) + 1e-6).all()
+
+
+@pytest.mark.parametrize("H,nodes", [(1, 1), (16, 1), (40, 1), (128, 1), (16, 9)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_scores_of_any_finite_size(gpu, dtype, H, nodes):
+    for levels in LEVELS[dtype]:
+        for context in (1, 33, 100, 1000):
+            for sign in (1, -1):
+                _check(gpu, dtype, levels, context, nodes, H, sign)
+
+
+def test_scores_of_any_finite_size_in_many_parts(gpu):
+    for H in (16, 128):
+        for levels in (RISING, RISING[::-1], [-1.4e38, 0.0]):
+            _check(gpu, "bf16", levels, 20000, 1, H, -1)
