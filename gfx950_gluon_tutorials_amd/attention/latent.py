@@ -50,7 +50,8 @@ def write_latent(c: torch.Tensor, k_rope: torch.Tensor, cache: torch.Tensor, slo
     eps) * weight; with ``positions`` and ``freqs`` (32,) the key is turned as by
     ``rotary`` (``interleaved`` and ``scale`` as there).  Both in fp32, rounded once.
     ``c_out`` (T, 512) and ``k_out`` (T, 64), if given, receive every row as the cache
-    does, for the expansion of a prompt's keys and values; they may be c and k_rope.
+    does, for the expansion of a prompt's keys and values; they may be c and k_rope
+    themselves and must not overlap the inputs, each other or the cache otherwise.
 
     Rows whose slot is negative or behind the cache are skipped (in ``c_out`` and
     ``k_out`` they are not); slots must be distinct.  fp16 or bf16; row steps of 16

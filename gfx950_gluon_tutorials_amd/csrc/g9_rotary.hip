@@ -257,6 +257,8 @@ int g9_write_latent(const void* c, const void* k_rope, void* cache, const int64_
   if (!c || !k_rope || !slots || (num_blocks && !cache) || (freqs && !positions)) return G9_ERR_LAYOUT;
   for (const void* q : {c, k_rope, (const void*)cache, weight, (const void*)c_out, (const void*)k_out})
     if (!aligned16(q)) return G9_ERR_LAYOUT;
+  // In place a row's wave reads what it writes; with other steps it would write rows that are not read yet.
+  if (T > 1 && ((c_out == c && out[0] != in[0]) || (k_out == k_rope && out[1] != in[1]))) return G9_ERR_LAYOUT;
   if (((uintptr_t)slots | (uintptr_t)positions | (uintptr_t)freqs) & 7) return G9_ERR_LAYOUT;
   LatentWriteParams p{};
   p.c = static_cast<const char*>(c);

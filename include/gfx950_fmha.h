@@ -71,8 +71,9 @@ int g9_fmha_fwd(const void* q, const void* k, const void* v, void* o, float* lse
  * - Strides are in ELEMENTS with a unit head-dim stride left out: (token, head)
  *   for packed tensors, (block, token, head) for caches.  They are multiples of
  *   8 and not negative; base pointers are 16-byte aligned.  What is written (o,
- *   the caches) must not overlap itself; what is only read may (expanded tensors),
- *   but for g9_tree_fwd's caches.  Offsets are 64-bit throughout.
+ *   the caches) must not overlap itself, nor, but where an entry says so, what is
+ *   read; what is only read may (expanded tensors), but for g9_tree_fwd's caches.
+ *   Offsets are 64-bit throughout.
  * - Lengths, tables and offsets are device data, read when the kernel runs.
  *   Whatever they hold, nothing outside the tensors is touched: negative lengths
  *   count as 0, cu_seqlens are held inside the packed tensor, a table entry
@@ -190,7 +191,8 @@ int g9_rotary(const void* x, void* o, const int64_t* positions, const double* fr
  * weight (512 values; NULL: no norm) replaces c by c / sqrt(mean(c^2) + eps) * weight;
  * freqs (32 values; NULL: no rotation) turns k_rope as g9_rotary does.  c_out (T x
  * 512) and k_out (T x 64), optional, receive every row as the cache would; they may be
- * c and k_rope.
+ * c and k_rope, with the same strides, and must not overlap the inputs, each other or
+ * the cache otherwise.
  */
 int g9_write_latent(const void* c, const void* k_rope, void* cache, const int64_t* slots, const void* weight, float eps,
                     const int64_t* positions, const double* freqs, void* c_out, void* k_out, int64_t T,

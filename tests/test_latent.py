@@ -183,6 +183,13 @@ def test_c_write(kw, code):
     assert _c_write(**kw) == code
 
 
+@pytest.mark.parametrize("kw", [dict(c_out=FAKE), dict(c_out=FAKE, cos=640), dict(k_out=FAKE), dict(k_out=FAKE, kos=584, T=2),
+                                dict(c_out=FAKE, cs=0)])
+def test_c_write_in_place_needs_the_rows_of_the_input(kw):
+    """With other steps a row would land on inputs that are not read yet."""
+    assert _c_write(**kw) == _lib.G9_ERR_LAYOUT
+
+
 def _c_paged(q=FAKE, cache=FAKE, o=FAKE, lse=None, table=FAKE, ts=4, width=4, lengths=FAKE, cu=FAKE, mask=None, words=0, B=2, T=4,
              H=2, blocks=3, size=16, qs=(1152, 576), cs=(9216, 576), os=(1024, 512), scale=1.0, dtype=1, ws=FAKE, wsb=1 << 40):
     return _lib.load().g9_latent_fwd(q, cache, o, lse, table, ts, width, lengths, cu, mask, words, B, T, H, blocks, size,
