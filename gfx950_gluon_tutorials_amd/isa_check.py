@@ -343,9 +343,10 @@ def check_text(asm: str) -> list[str]:
     for n, (i, name) in enumerate(starts):
         end = starts[n + 1][0] if n + 1 < len(starts) else len(lines)
         body = lines[i + 1:end]
+        # To the function's end, not its first s_endpgm: an early return has one of its own.
         for j, l in enumerate(body):
-            if l.strip().startswith("s_endpgm"):
-                body = body[: j + 1]
+            if l.startswith(".Lfunc_end"):
+                body = body[:j]
                 break
         violations += check_function(name, body)
     return violations
