@@ -38,9 +38,9 @@ SOURCE_FLAGS = {s: ["-fno-honor-nans"] for s in ("g9_fmha.hip", "g9_varlen.hip",
 # Sources whose kernels hold almost every register through branches of lanes.  Where two
 # such branches end at once the compiler turns the lanes on again at the outer end only, and
 # has reloaded spilled registers between the two, in some of the lanes: here each
-# branch turns its lanes on again.  The kernels of NO_SPILLS must not spill at all (the build
-# fails if they do), and keep their sums in accumulation registers that the compiler must
-# leave alone (the same).
+# branch turns its lanes on again, and isa_check follows the reloads of every source.
+# The kernels of NO_SPILLS must not spill at all (the build fails if they do), and keep their
+# sums in accumulation registers that the compiler must leave alone (the same).
 for _s in ("g9_latent.hip", "g9_latent_varlen.hip"):
     SOURCE_FLAGS[_s] = SOURCE_FLAGS[_s] + ["-mllvm", "-amdgpu-remove-redundant-endcf=0"]
 NO_SPILLS = {"g9_latent.hip"}

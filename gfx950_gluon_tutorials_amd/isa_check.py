@@ -33,6 +33,12 @@ that the vector unit wrote (``v_readfirstlane``, ``v_readlane``, a compare) may
 be read by a vector-memory instruction ``VMEM_AFTER_VALU_SGPR`` wait states later
 at the earliest.
 
+A fourth scan follows every value that is loaded from scratch memory (a spilled
+register): an instruction that reads it may run in no lane that was off at the load.
+The compiler has reloaded registers between the ends of two branches of lanes, in the
+lanes of the inner one, and used them behind the outer end: the others went on with what
+the register held before.
+
 Usage: ``python -m gfx950_gluon_tutorials_amd.isa_check file.s`` (exit status 1
 on violations), or ``check_text(asm) -> list of violations``.
 """
@@ -329,10 +335,139 @@ def _fixpoint(name: str, blocks, step, merge) -> list[str]:
     return list(seen_violations)
 
 
+# --- reloads of spilled registers under a part of the lanes -------------------------
+
+# Vector instructions that also read their first operand.
+_READS_DST = re.compile(r"v_\w*(?:fmac|_mac_|dot\w*c_|_dpp|_sdwa|swap)")
+_MASK = re.compile(r"s\[(\d+):(\d+)\]|s(\d+)$|vcc|exec")
+
+
+class _Lanes:
+    """The lanes of one reload, followed from there on.
+
+    within: exec lies within the reload's lanes.  masks: scalar registers (and lanes of
+    vector registers that hold spilled ones) whose bits do.  regs: the reloaded
+    registers that have not been written since."""
+
+    __slots__ = ("within", "masks", "regs")
+
+    def __init__(self, within, masks, regs):
+        self.within, self.masks, self.regs = within, masks, regs
+
+    def key(self):
+        return (self.within, frozenset(self.masks), frozenset(self.regs))
+
+    @staticmethod
+    def _names(op: str):
+        m = _MASK.match(op)
+        if not m:
+            return None
+        if op.startswith("vcc"):
+            return ["vcc"]
+        if m.group(3):
+            return [("s", int(m.group(3)))]
+        return [("s", r) for r in range(int(m.group(1)), int(m.group(2)) + 1)] if m.group(1) else None
+
+    def inside(self, op: str) -> bool:
+        if op == "0":
+            return True  # no lane
+        if op == "exec":
+            return self.within
+        names = self._names(op)
+        return names is not None and all(n in self.masks for n in names)
+
+    def assign(self, op: str, inside: bool):
+        if op.startswith("exec"):
+            self.within = inside
+            return
+        for n in self._names(op) or ():
+            (self.masks.add if inside else self.masks.discard)(n)
+
+    def step(self, ins: Instr) -> bool:
+        """Advances over one instruction; True: it reads a reloaded register in other lanes."""
+        mn, parts = ins.mnemonic, ins.text.split(None, 1)
+        ops = [o.strip() for o in parts[1].split(",")] if len(parts) > 1 else []
+        if ins.dst or ins.src:
+            src = ins.src | ins.dst if _READS_DST.match(mn) else ins.src
+            if not self.within and any(r in self.regs for k, r in src if k == "v"):
+                return True
+        if mn.startswith("v_writelane") and len(ops) == 3:
+            key = ("lane", ops[0], ops[2])
+            (self.masks.add if self.inside(ops[1]) else self.masks.discard)(key)
+            return False
+        if mn.startswith("v_readlane") and len(ops) == 3:
+            self.assign(ops[0], ("lane", ops[1], ops[2]) in self.masks)
+            return False
+        for k, r in ins.dst:
+            if k == "v":
+                self.regs.discard(r)
+                self.masks = {m for m in self.masks if m[:2] != ("lane", f"v{r}")}
+        if mn.startswith("v_cmpx"):
+            pass  # exec loses lanes
+        elif mn.startswith("v_cmp"):
+            self.assign(ops[0], self.within)  # zero where a lane is off
+        elif mn.startswith("v_"):
+            for o in ops[:2 if _SCALAR_SECOND.match(mn) else 1]:
+                self.assign(o, False)
+        elif mn.startswith("s_") and ops and not mn.startswith(("s_cmp", "s_bitcmp", "s_set", "s_cbranch")):
+            if "_saveexec_b64" in mn:
+                d, x = ops
+                old, x = self.within, self.inside(x)
+                self.within = {"s_and": old or x, "s_or": old and x, "s_andn2": x, "s_xor": old and x}.get(
+                    mn[:mn.index("_saveexec")], False)
+                self.assign(d, old)
+            else:
+                a = [self.inside(o) for o in ops[1:]]
+                op = mn.rsplit("_", 1)[0]
+                ok = {"s_mov": lambda: a[0], "s_and": lambda: a[0] or a[1], "s_andn2": lambda: a[0],
+                      "s_or": lambda: a[0] and a[1], "s_xor": lambda: a[0] and a[1],
+                      "s_cselect": lambda: a[0] and a[1]}.get(op, lambda: False)()
+                self.assign(ops[0], ok)
+        return False
+
+
+def check_reloads(name: str, blocks) -> list[str]:
+    """A store to scratch counts as a read, also where it stores a tuple of which only some
+    registers hold a value."""
+    violations = []
+    for b, (_, code, _) in enumerate(blocks):
+        for i, load in enumerate(code):
+            if load.mnemonic.startswith("scratch_load"):
+                hit = _follow(blocks, b, i + 1, {r for k, r in load.dst if k == "v"})
+                if hit:
+                    violations.append(f"{name}: line {hit.line + 1}: '{hit.text}' reads a register in lanes that were off when it "
+                                      f"was reloaded at line {load.line + 1}")
+    return violations
+
+
+def _follow(blocks, b: int, i: int, regs: set) -> Instr | None:
+    """The first instruction found that reads `regs`, as loaded before instruction i of block b,
+    in lanes that were off there."""
+    entry: dict[int, _Lanes] = {}
+    work = [(b, i, _Lanes(True, set(), regs))]
+    while work:
+        b, i, st = work.pop()
+        for ins in blocks[b][1][i:]:
+            if st.step(ins):
+                return ins
+            if not st.regs:
+                break
+        if not st.regs:
+            continue
+        for s in blocks[b][2]:
+            old = entry.get(s)
+            new = _Lanes(st.within, set(st.masks), set(st.regs)) if old is None else _Lanes(
+                st.within and old.within, st.masks & old.masks, st.regs | old.regs)
+            if old is None or new.key() != old.key():
+                entry[s] = _Lanes(new.within, set(new.masks), set(new.regs))
+                work.append((s, 0, new))
+    return None
+
+
 def check_function(name: str, lines: list[str]) -> list[str]:
     blocks = _blocks(lines)
     return _fixpoint(name, blocks, _step, _merge) + _fixpoint(
-        name, blocks, _lds_step, _merge_lds) + _fixpoint(name, blocks, _sgpr_step, _merge)
+        name, blocks, _lds_step, _merge_lds) + _fixpoint(name, blocks, _sgpr_step, _merge) + check_reloads(name, blocks)
 
 
 def check_text(asm: str) -> list[str]:
