@@ -6,7 +6,7 @@
 // b cos), in fp32 and rounded once.  The angle is formed in 64 bits: a product in 32
 // would be off by whole radians where n f passes 2^24, and at position 10^5 by
 // 2^-7.  f / 2 pi turns the product into whole turns, which are dropped exactly,
-// and a rest of at most half a turn, which fp32 holds to 2^-25.
+// and a rest of at most half a turn, which fp32 holds to 2^-26.
 #include "../../include/gfx950_fmha.h"
 #include "g9_attn_host.hpp"
 #include "g9_common.hpp"

@@ -23,13 +23,19 @@ def rotate(x, positions, freqs, first=0, interleaved=False, inverse=False, scale
 
 
 def rotate_bound(x, y, positions, freqs, eps, subnormal, first=0, interleaved=False, scale=1.0):
-    """A bound on the error of y = rotate(x): the angle's rest in turns is rounded to
-    fp32 (2^-25 of a turn, 2 pi 2^-25 radians), its 64-bit product twice (2^-52 of
-    it), sine and cosine are good to 2^-23 each, the scale and the sum of two products round
-    four times (2^-24 each): together less than 2^-21 + 2^-52 |n f| of |a| + |b|; then
-    the result is rounded to half a step."""
+    """A bound on the error of y = rotate(x):
+
+    * the angle's rest, at most half a turn, is rounded to fp32: 2^-26 of a turn, 2 pi
+      2^-26 radians;
+    * sine and cosine of it are within 2^-24 (0.88 of it, over every fp32 value up to half
+      a turn, on the card);
+    * the scale as an argument, its product, the product with x and the sum of two such round
+      once each: 4 times 2^-24.  So far 3.92e-7, less than 2^-21 = 4.77e-7, of |a| + |b|;
+    * in 64 bits 1 / 2 pi, its product with f, that with n and the oracle's n f are rounded,
+      2^-53 of the angle each: 2^-51 |n f|;
+    * the result is rounded to half a step."""
     half = len(freqs)
-    e = scale * (2.0**-21 + 2.0**-52 * np.abs(np.asarray(positions, np.float64)[:, None] * freqs))[:, None]
+    e = scale * (2.0**-21 + 2.0**-51 * np.abs(np.asarray(positions, np.float64)[:, None] * freqs))[:, None]
     x, out = np.abs(np.asarray(x, np.float64)), np.zeros(np.shape(x))
     if interleaved:
         ia, ib = first + 2 * np.arange(half), first + 2 * np.arange(half) + 1

@@ -302,3 +302,26 @@ def test_oracle_attention_forms_agree():
     for h in range(H):
         want, w_lse, _, _ = R.masked_attention(q[:, h], keys[:, h], vals[:, h], reads, 0.3)
         assert np.allclose(o[:, h], want) and np.allclose(lse[h], w_lse)
+
+
+def test_rotation_bound_counts_the_roundings():
+    """The angle's 64-bit part, as the kernel forms it, against 60 digits; and the bound's fp32 terms."""
+    import random
+    from fractions import Fraction
+
+    pi = Fraction("3.14159265358979323846264338327950288419716939937510582097494459")
+    inv, rng, top = float(0.15915494309189533577), random.Random(0), 0
+    assert abs(Fraction(inv) * 2 * pi - 1) <= Fraction(1, 2**53)
+    for _ in range(20000):
+        n, f = rng.randrange(1, 2**31), 10.0 ** rng.uniform(-4, 0)
+        t = n * (f * inv)
+        off = abs(Fraction(t) * 2 * pi - Fraction(n) * Fraction(f)) / (Fraction(n) * Fraction(f))
+        top = max(top, off)
+    # Three roundings (the constant's, two products'); with the oracle's own product four.
+    assert 2.0**-53 < top <= 3 * 2.0**-53
+    angle, sine, products = 2 * math.pi * 2.0**-26, 2.0**-24, 4 * 2.0**-24
+    assert angle + sine + products < 2.0**-21
+    x, n, f = np.ones((1, 1, 2)), 2**31, 1.0
+    y = L.rotate(x, [n], [f])
+    bound = L.rotate_bound(x, y, [n], [f], 0.0, 0.0)
+    assert (bound >= 2 * (angle + sine + products + 4 * 2.0**-53 * n * f)).all()
