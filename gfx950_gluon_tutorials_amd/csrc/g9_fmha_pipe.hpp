@@ -713,7 +713,7 @@ struct Pipe : Where<Params, KIND>, SharedKeys<ROPE> {
     }
   }
 
-  // D1 with the shared keys: 24 MFMAs; eight LDS reads go beside the 5th to the 12th, whose
+  // D1 with the shared keys: 24 MFMAs; eight LDS reads go beside the 9th to the 16th, whose
   // registers they take.
   template <int VN, int I = 0>
   G9_DEV static void interleave_shared() {
