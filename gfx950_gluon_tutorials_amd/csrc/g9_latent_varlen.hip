@@ -51,7 +51,17 @@ G9_LATENT_VARLEN_KERNEL(g9_latent_varlen_f16, false)
 // by 32 47.7 and 44.8, 2048 by 24 65 and 64, 1024 by 64 53 and 41, 4096 by 16 146 and 118.
 // Beyond that many rows: 64 x 30 by 32 27 and 82, 500 x 20 behind 500 keys 919 and 1574, 256 x
 // 64 by 16 144 and 203, but 128 x 64 behind 1000 403 and 338, 32 x 200 62 and 43.
+// Behind a longer prefix every block of 32 queries reads it again, from the last-level cache or HBM where
+// there are many K/V heads: then from 20 K rows on only sequences of one block stay with the short
+// form.  With prefixes of 500, 1000, 4000 and 16000 keys: 1 x 192 by 128 32 45 140 619 and 30 41
+// 108 386, 1 x 320 by 128 48 69 226 1027 and 34 52 134 502, 1 x 384 by 64 32 45 119 528 and 32 45 117
+// 399, 4 x 100 by 64 42 74 310 1347 and 27 38 127 457, 16 x 64 by 32 52 92 368 1465 and 44 77 240 873,
+// 64 x 40 by 32 207 378 1413 5692 and 199 315 969 3599.  On the other side of each limit: 8 x 32
+// by 128 53 102 360 1402 and 93 153 487 1780, 10 x 64 by 32 36 58 228 930 and 42 61 222 811, 1 x
+// 128 by 128 18 26 79 365 and 24 34 102 383, 1 x 2048 by 16 56 71 153 476 and 74 86 159 441; without a
+// prefix 4 x 100 by 64 14 and 15, 16 x 64 by 32 14 and 24, 64 x 40 by 32 48 and 85.
 static constexpr int64_t kShortRows = 40 * 1024, kShortQueries = 48;
+static constexpr int64_t kPrefix = 500, kPrefixRows = 20 * 1024, kPrefixHeads = 64;
 
 extern "C" int g9_latent_varlen_fwd(const void* q, const void* k, const void* v, const void* k_rope, void* o, float* lse,
                                     const int32_t* cu_q, const int32_t* cu_k, int64_t B, int64_t T, int64_t TK,
@@ -97,7 +107,8 @@ extern "C" int g9_latent_varlen_fwd(const void* q, const void* k, const void* v,
   void* args[] = {&p};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int64_t group = HQ / HK;
-  const bool few = T * HQ <= kShortRows || T < kShortQueries * B;
+  const bool reread = B * HK >= kPrefixHeads && T * HQ > kPrefixRows && T > 32 * B && TK - T >= kPrefix * B;
+  const bool few = (T * HQ <= kShortRows || T < kShortQueries * B) && !reread;
   if (few) {
     const int64_t blocks = T * group / 32 + (B < T ? B : T);
     if (blocks * HK * 256 > UINT32_MAX) return G9_ERR_SHAPE;  // the threads of a launch
