@@ -105,7 +105,8 @@ def latent_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     fp16 or bf16, any number of heads; block_size a power of two from 16 to 1024.
     Returns ``o``, allocated when not given; rows behind the last request are left as
     they were, a row that reads nothing gives zeros.  ``lse`` (H, T) and the
-    arithmetic as in ``varlen_attention``.  Asynchronous on the current stream;
+    arithmetic as in ``varlen_attention``, but for scores of any finite size.  A call's
+    workspace is 34 to 135 MB, by T / B times H.  Asynchronous on the current stream;
     forward only."""
     sm_scale = float(sm_scale)
     key = ("latent", sm_scale, sig(q), sig(cache), sig(block_table), sig(lengths), sig(cu_seqlens),

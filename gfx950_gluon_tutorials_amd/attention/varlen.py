@@ -32,7 +32,8 @@ def varlen_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     sequence are left as they were.  ``lse``, if given, is a contiguous fp32
     (HQ, T) tensor that receives each query's natural-log log-sum-exp.
     Scores, softmax and sums are fp32, each weight is rounded to the input type for
-    its product with v.  Asynchronous on the current stream; forward only."""
+    its product with v; scaled scores up to 2^26 in magnitude.  Asynchronous on the
+    current stream; forward only."""
     causal, sm_scale = bool(causal), None if sm_scale is None else float(sm_scale)
     key = ("varlen", causal, sm_scale, sig(q), sig(k), sig(v), sig(cu_seqlens), cu_seqlens_k is not None and sig(cu_seqlens_k),
            o is not None and sig(o), lse is not None and sig(lse))

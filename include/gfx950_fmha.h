@@ -68,6 +68,10 @@ int g9_fmha_fwd(const void* q, const void* k, const void* v, void* o, float* lse
  *   to the input type before its product with V, as in g9_fmha_fwd (the matrix unit
  *   takes both alike): up to half a step, 2^-8 (bf16) or 2^-11 (fp16), of the average
  *   of |V|.
+ * - Scaled scores up to 2^26 in magnitude; for g9_latent_fwd any whose product with
+ *   log2(e) is finite.  (A weight's exponent is its score less the row's maximum, which is
+ *   rounded: beyond, that rounding alone can take a weight out of the input type's range,
+ *   and a row becomes zeros, infinite or NaN.)
  * - Strides are in ELEMENTS with a unit head-dim stride left out: (token, head)
  *   for packed tensors, (block, token, head) for caches.  They are multiples of
  *   8 and not negative; base pointers are 16-byte aligned.  What is written (o,
@@ -204,7 +208,9 @@ int g9_write_latent(const void* c, const void* k_rope, void* cache, const int64_
  * The absorbed form: q (T x H x 576) is each head's query times its key projection,
  * then its rotated part, o (T x H x 512) the weighted latents, which the caller
  * multiplies by the heads' value projections.  score = sm_scale * q . row; requests,
- * nodes, masks and workspace (g9_latent_workspace_size bytes) as in g9_tree_fwd.
+ * nodes, masks and workspace (g9_latent_workspace_size bytes: 34, 67 or 135 MB, by the
+ * rows that a request brings on average, T / B rounded up times H, whatever their number:
+ * up to 32, up to 64, more) as in g9_tree_fwd.
  * The cache's tokens at least 576 elements apart.  A row that reads an infinite or NaN
  * latent gets NaN in all or some of its values; rows that do not read it are as without it.
  */
