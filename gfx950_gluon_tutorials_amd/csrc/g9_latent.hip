@@ -25,12 +25,13 @@
 // A row's maximum moves only where a tile passes it by more than 8 (log2 units); then its
 // factor goes through LDS, too.
 //
-// Measured (us, kernel and join, inputs partly in the last-level cache): 64 requests of 100 to
-// 8192 tokens by 16 heads 32 + 7: 1.5 a tile, 6.1 TB/s over the loop, but 14 of the 32 go to
-// finding the part, the first loads and the sums' way out; by 128 heads 47 + 16, 2.1 a tile
-// (68 MFMAs of 32 cycles are 1.2 at the clock that they leave), 25 outside the loop, much of
-// them and of the join for the 256 KB of sums of a part; 16 trees of 12 nodes by 32 heads
-// 78 + 15; one request of 700 tokens by 16 heads 10 + 4.
+// Measured (us; kernel and join under the profiler, and a call among others; inputs partly in
+// the last-level cache): 64 requests of 100 to 8192 tokens (88 K in all) by 16 heads 34-36 + 8 and
+// 37: 1.5 a tile, 6.1 TB/s over the loop, but 14 go to finding the part, the first loads and
+// the sums' way out; by 128 heads 47-49 + 17 and 60, 2.1 a tile (68 MFMAs of 32 cycles are 1.2
+// at the clock that they leave), 25 outside the loop, much of them and of the join for the
+// 256 KB of sums of a part; 16 trees of 12 nodes by 32 heads 79-81 + 16 and, on several cards,
+// 86-95; one request of 700 tokens by 16 heads 11 + 4 and 15.
 #include "../../include/gfx950_fmha.h"
 #include <utility>
 
@@ -168,7 +169,9 @@ G9_DEV int lane_here() {
 
 // RB blocks of 32 rows; a step of the workgroup is a tile.  What a block's beginning and end
 // cost, in tiles, is the line's LEAD (us, the cases above with
-// 5, 9, 12 places: 128 heads 70, 68.5, 66, trees 99, 97, 98; 16 heads with 5 and 7: 40.5, 41.5).
+// 5, 9, 12 places: 128 heads 70, 68.5, 66, trees 99, 97, 98; 16 heads with 5 and 7: 40.5, 41.5;
+// 64 rows with 5, 8, 12: 64 requests of 100 to 8192 by 40 heads 87, 85, 85, by 64 90, 87, 86, 256 of
+// 100 to 2000 by 64 106, 101, 102).
 template <int RB>
 using Steps = Line<Params, kKeys, 32 * RB, kWgs, RB == 4 ? 12 : RB == 2 ? 8 : 5>;
 
@@ -756,9 +759,13 @@ namespace {
 
 // Query rows of a block, by the rows (nodes by heads) that a request of the batch
 // brings on average: the fewest that hold them, and 128 above (us with 32, 64 and 128 rows; 64
-// requests of 100 to 8192 tokens, cache cold, by 16 heads 123, 125, 133, 32: 136, 139, 142,
-// 40: 167, 142, 148, 64: 167, 143, 153, 80: 222, 188, 159, 128: 200, 149, 144; 16 requests of
-// 12 nodes by 16 heads 102, 79, 72; but one of 30000 tokens by 128 heads 44, 44, 56).
+// requests, their lengths spread evenly over 100 to 8192: 265 K tokens, three times the bytes of the
+// case above, and each call behind 1 GiB of writes; by 16 heads 123, 125, 133, 32: 136, 139,
+// 142, 40: 167, 142, 148, 64: 167, 143, 153, 80: 222, 188, 159, 128: 200, 149, 144; 16 requests
+// of 12 nodes by 16 heads 102, 79, 72.  One call behind another: 64 requests by 40 heads 122,
+// 85, 97, by 64 126, 87, 99, 16 of 4 nodes by 16 48, 41, 48, 4 of 8000 to 16000 by 64 34, 32, 41.
+// But a single request takes the fewer rows: 30000 tokens by 128 heads 44, 44, 56, by 64 31,
+// 36, 42, 700 by 64 16, 20, 21).
 enum { Q32, Q64, Q128 };
 int form_of(int64_t B, int64_t T, int64_t H) {
   const int64_t rows = (T + B - 1) / B * H;
@@ -766,7 +773,9 @@ int form_of(int64_t B, int64_t T, int64_t H) {
 }
 // Workgroups of the join for each worker: the more, the larger a part (us, the join alone: one
 // request by 16 heads with 1 and 2 4.4 and 5.6, 64 requests 6.8 and 6.5; by 128 heads with 2, 4
-// and 8 16.8, 15.6 and 14.2, trees 20, 15.3 and 15.8).
+// and 8 16.8, 15.6 and 14.2, trees 20, 15.3 and 15.8; 64 rows with 1, 2 and 4, whole calls: 64
+// requests by 64 heads 87, 87 and 86, 256 of 100 to 2000 102, 101 and 100, 4 of 8000 to 16000 32, 32
+// and 35).
 constexpr unsigned join_shares(int form) { return 1u << form; }
 // The workspace: the sums of 2 x 256 blocks and their (m, l) pairs, then start[].
 size_t start_at(int form) { return (size_t)2 * fa::kWgs * (32 << form) * (512 + 2) * 4; }

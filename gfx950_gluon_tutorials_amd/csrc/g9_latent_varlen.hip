@@ -5,9 +5,12 @@
 // g9_varlen.hip's kernel with 192 values of QK: the pipeline reads the shared keys as
 // chunk columns of their own behind the head's, so that nothing is copied together.
 // Bound by the matrix unit (640 flops a query and key of a head): 16384 causal tokens by 32
-// heads 2.28-2.45 ms on two cards (1.12-1.21 PFLOP/s, of 1.40 for a large matrix product),
-// 12 prompts of 100 to 2500 by 32 heads 336-364 us (0.74-0.80 PFLOP/s: half-empty tiles on the
-// diagonal, start-up); 197 tokens by 16 heads 8 us in the short form.
+// heads 2.28-2.66 ms on several cards (1.03-1.21 PFLOP/s, where a large matrix product has 1.40-1.52).
+// On one of 2.35 ms it is busy for 64% of the cycles, which the power limit holds at 1.77 GHz;
+// a tenth of the waves' time is waits for LDS, and 1% of the products are masked.  12 prompts of 100
+// to 2500 by 32 heads 336-386 us (0.70-0.80 PFLOP/s): busy for 41% at 1.92 GHz, 8% of the products
+// masked; the rest is the beginnings and ends of 1600 workgroups, one a CU at a time.  197
+// tokens by 16 heads 8 us in the short form.
 #include "../../include/gfx950_fmha.h"
 #include "g9_attn_host.hpp"
 #include "g9_packed.hpp"
