@@ -27,11 +27,11 @@
 //
 // Measured (us; kernel and join under the profiler, and a call among others; inputs partly in
 // the last-level cache): 64 requests of 100 to 8192 tokens (88 K in all) by 16 heads 34-36 + 8 and
-// 37: 1.5 a tile, 6.1 TB/s over the loop, but 14 go to finding the part, the first loads and
-// the sums' way out; by 128 heads 47-49 + 17 and 60, 2.1 a tile (68 MFMAs of 32 cycles are 1.2
+// 36-38: 1.5 a tile, 6.1 TB/s over the loop, but 14 go to finding the part, the first loads and
+// the sums' way out; by 128 heads 47-49 + 17 and 58-60, 2.1 a tile (68 MFMAs of 32 cycles are 1.2
 // at the clock that they leave), 25 outside the loop, much of them and of the join for the
 // 256 KB of sums of a part; 16 trees of 12 nodes by 32 heads 79-81 + 16 and, on several cards,
-// 86-95; one request of 700 tokens by 16 heads 11 + 4 and 15.
+// 85-95; one request of 700 tokens by 16 heads 11 + 4 and 15.
 #include "../../include/gfx950_fmha.h"
 #include <utility>
 
@@ -396,10 +396,13 @@ struct Wave4 {
         m = m_new;
         l *= factor;
       }
-      if (__builtin_expect(__builtin_amdgcn_ballot_w64(__builtin_fabsf(m) >= kLarge) != 0, 0)) {
+      const bool large = __builtin_fabsf(m) >= kLarge;
+      if (__builtin_expect(__builtin_amdgcn_ballot_w64(large) != 0, 0)) {
+        // The other rows' products are by 1: their weights stay those of their own scores.
+        const float by = large ? p.scale_log2 : 1.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sc[i] *= p.scale_log2;
-        x.scale = 1.f;
+        for (int i = 0; i < 16; ++i) sc[i] *= by;
+        x.scale = large ? 1.f : p.scale_log2;
       }
     } else if constexpr (N < 19) {
       // Weight N - 3, and what follows from those before it.

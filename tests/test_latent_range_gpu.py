@@ -83,6 +83,21 @@ def test_scores_of_any_finite_size_in_many_parts(gpu):
             _check(gpu, "bf16", levels, 20000, 1, H, -1)
 
 
+@pytest.mark.parametrize("H", [16, 64, 128])
+def test_large_scores_leave_the_other_rows_as_they_are(gpu, H):
+    """Rows of one wave: the others' bits do not depend on them."""
+    g = torch.Generator().manual_seed(H)
+    cache = torch.randn(70, 16, 576, generator=g).bfloat16().to(gpu)
+    q = (torch.randn(1, H, 576, generator=g) * 0.6).bfloat16().to(gpu)
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device=gpu)
+    run = lambda: latent_attention(q, cache, torch.arange(70, dtype=torch.int32, device=gpu)[None], i(1000), i(0, 1), sm_scale=192**-0.5)
+    clean = run().clone()
+    for size in (2.0**40, 2.0**100, float("inf")):
+        q[:, 3::32] = size
+        got, rest = run(), torch.arange(H) % 32 != 3
+        assert torch.equal(got[:, rest], clean[:, rest]) and got[:, 3::32].isfinite().all() == (size < float("inf"))
+
+
 # --- the packed forms and the paged cache of keys and values --------------------------------
 
 UP_TO_2_26 = [[2.0**26], [-2.0**26], [-2.0**26, -2.0**26 + 2.0**20], [2.0**26, 2.0**25 + 2.0**22, 2.0**26],
